@@ -1,0 +1,523 @@
+// Scaled embedding lookup, and its gradient by sorted tokens.
+//
+//   y[r, :]      = scale * table[ids[r], :]
+//   dtable[v, :] = scale * sum of g[r, :] over the positions r with ids[r] = v, in the order of r
+//
+// An id outside [0, vocab) gives a row of zeros and no gradient; positions that hold `padding` give no gradient.
+//
+// The gradient sorts (token, position) pairs with a stable radix sort, so the positions of a token lie together in their
+// order and every sum is taken in one fixed order: no atomics, the same bits in every run.  The sorted list is cut in
+// tiles of a few positions; a block walks its tile and keeps the running sum of the present token.  Tokens that lie
+// inside one tile are written at once.  A token that crosses tiles leaves the sum of each tile as a partial row, and
+// join_tokens adds those in order, so a token that fills half of the batch costs no more than its bytes.
+#include <cuda_runtime.h>
+#include <cooperative_groups.h>
+#include <stdint.h>
+
+#include "launch.cuh"
+#include "scratch.h"
+#include "smem_limit.h"
+
+#define TSB_OK 0
+#define TSB_ERR_ARG 1
+#define TSB_ERR_UNSUPPORTED 2
+#define TSB_ERR_LAUNCH 3
+#define TSB_ERR_OOM 5
+
+namespace {
+
+namespace cg = cooperative_groups;
+using tsb_launch::load;
+
+int launch_status(cudaError_t e) {
+  if (e == cudaSuccess) e = cudaGetLastError();
+  else cudaGetLastError();
+  return e == cudaSuccess ? TSB_OK : TSB_ERR_LAUNCH | ((int)e << 8);
+}
+
+// ------------------------------------------------------------------------------------------------ lookup
+// T: float4 where rows are whole 16-byte pieces, float otherwise.  U pieces in flight per thread.
+template <class T> __device__ __forceinline__ T zero();
+template <> __device__ __forceinline__ float zero<float>() { return 0.f; }
+template <> __device__ __forceinline__ float4 zero<float4>() { return make_float4(0.f, 0.f, 0.f, 0.f); }
+__device__ __forceinline__ float times(float v, float s) { return v * s; }
+__device__ __forceinline__ float4 times(float4 v, float s) { return make_float4(v.x * s, v.y * s, v.z * s, v.w * s); }
+__device__ __forceinline__ float plus(float a, float b) { return a + b; }
+__device__ __forceinline__ float4 plus(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
+
+template <class T, int U>
+__global__ void __launch_bounds__(256) scaled_lookup(const T* table, const float* ids, T* __restrict__ y, long long pieces,
+                                                     long long vocab, unsigned dim, float scale) {
+  tsb_launch::enter();
+  const long long i = blockIdx.x * (256ll * U) + threadIdx.x;
+  T v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const long long j = i + u * 256;
+    v[u] = zero<T>();
+    if (j < pieces) {
+      const long long r = (pieces >> 32) == 0 ? (long long)((unsigned)j / dim) : j / dim;
+      const long long id = (long long)load(ids + r);
+      if (id >= 0 && id < vocab) v[u] = times(load(table + id * dim + (j - r * dim)), scale);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (i + u * 256 < pieces) y[i + u * 256] = v[u];
+}
+
+// ------------------------------------------------------------------------------------------------ sort
+// Keys are token ids, `vocab` for positions that give no gradient (they end up last).  What fills the last tile behind
+// position n has all bits set, so it stays behind everything in every pass.  Digits of up to 8 bits, the lowest first.  A position's rank among equal digits is counted in the order of the positions: lanes by match.any, the
+// rounds of a warp by a running count, warps and blocks by prefix sums.
+constexpr int SORT_THREADS = 1024, SORT_ITEMS = 4, SORT_TILE = SORT_THREADS * SORT_ITEMS, SORT_WARPS = SORT_THREADS / 32;
+constexpr int DIGITS = 256, MAX_CLUSTER = 8;
+constexpr unsigned FILL = 0xffffffffu;
+static_assert(SORT_TILE == 4096, "the launcher and the scratch layout use it");
+
+struct SortShared {
+  unsigned counts[SORT_WARPS][DIGITS];       // running counts of each warp, then what lies before it
+  unsigned total[DIGITS];                    // of this block (read by the others of the cluster)
+  unsigned base[DIGITS];                     // where this block's first position of a digit goes
+  unsigned scan[8];
+};
+
+__device__ __forceinline__ unsigned key_of(const float* ids, long long r, long long n, unsigned vocab, long long padding) {
+  if (r >= n) return FILL;
+  const long long id = (long long)load(ids + r);
+  return id >= 0 && id < (long long)vocab && id != padding ? (unsigned)id : vocab;
+}
+
+// rank[i]: positions of the same digit before item i in this warp (items of a warp lie 32 apart, lane by lane)
+__device__ __forceinline__ void rank_items(const unsigned (&key)[SORT_ITEMS], int shift, unsigned mask, unsigned* count,
+                                           unsigned (&rank)[SORT_ITEMS]) {
+  const unsigned lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < SORT_ITEMS; ++i) {
+    const unsigned d = (key[i] >> shift) & mask;
+    const unsigned same = __match_any_sync(0xffffffffu, d);
+    const unsigned before = __popc(same & ((1u << lane) - 1));
+    const unsigned old = count[d];
+    __syncwarp();
+    if (before == 0) count[d] = old + __popc(same);
+    __syncwarp();
+    rank[i] = old + before;
+  }
+}
+
+__device__ __forceinline__ void clear_counts(SortShared& s) {
+  for (int i = threadIdx.x; i < SORT_WARPS * DIGITS; i += SORT_THREADS) (&s.counts[0][0])[i] = 0;
+}
+
+// Per digit: what lies before each warp, and the block's total.
+__device__ __forceinline__ void scan_warps(SortShared& s) {
+  if (threadIdx.x < DIGITS) {
+    unsigned sum = 0;
+#pragma unroll 8
+    for (int w = 0; w < SORT_WARPS; ++w) {
+      const unsigned c = s.counts[w][threadIdx.x];
+      s.counts[w][threadIdx.x] = sum;
+      sum += c;
+    }
+    s.total[threadIdx.x] = sum;
+  }
+}
+
+// Exclusive prefix sum of one value of each of the first 256 threads (all threads call it).
+__device__ __forceinline__ unsigned scan_digits(SortShared& s, unsigned v) {
+  const unsigned lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  unsigned sum = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned up = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += up;
+  }
+  if (w < 8 && lane == 31) s.scan[w] = sum;
+  __syncthreads();
+  unsigned before = 0;
+  for (unsigned k = 0; k < w && k < 8; ++k) before += s.scan[k];
+  return before + sum - v;
+}
+
+// Up to 32768 positions: one cluster of up to eight blocks holds them all in shared memory and trades them through
+// distributed shared memory, one launch for all digits.  The other clusters of the grid fill the table's gradient with
+// zeros meanwhile, which takes longer than the sort for a table of any size.
+__global__ void __launch_bounds__(SORT_THREADS) sort_cluster(const float* ids, long long n, unsigned vocab, long long padding,
+                                                             int bits, int passes, unsigned* __restrict__ out_key,
+                                                             unsigned* __restrict__ out_pos, float* __restrict__ dtable,
+                                                             long long cells, bool aligned) {
+  tsb_launch::enter();
+  extern __shared__ uint4 raw[];
+  cg::cluster_group cluster = cg::this_cluster();
+  const unsigned size = cluster.num_blocks(), me = cluster.block_rank();
+  if (blockIdx.x >= size) {
+    const long long step = (long long)(gridDim.x - size) * SORT_THREADS;
+    long long i = (long long)(blockIdx.x - size) * SORT_THREADS + threadIdx.x;
+    if (aligned) {
+      for (long long j = i; j < cells / 4; j += step) reinterpret_cast<float4*>(dtable)[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      i += cells / 4 * 4;
+    }
+    for (; i < cells; i += step) dtable[i] = 0.f;
+    return;
+  }
+  SortShared& s = *reinterpret_cast<SortShared*>(raw);
+  unsigned* keys = reinterpret_cast<unsigned*>(&s + 1);
+  unsigned* poss = keys + SORT_TILE;
+  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = warp * (32 * SORT_ITEMS) + lane;
+  const int step = (bits + passes - 1) / passes;
+  unsigned key[SORT_ITEMS], pos[SORT_ITEMS], rank[SORT_ITEMS];
+#pragma unroll
+  for (int i = 0; i < SORT_ITEMS; ++i) {
+    pos[i] = me * SORT_TILE + at + i * 32;
+    key[i] = key_of(ids, pos[i], n, vocab, padding);
+  }
+  for (int p = 0; p < passes; ++p) {
+    const int shift = p * step;
+    const unsigned mask = (1u << step) - 1;
+    clear_counts(s);
+    __syncthreads();
+    rank_items(key, shift, mask, s.counts[warp], rank);
+    __syncthreads();
+    scan_warps(s);
+    cluster.sync();                          // totals are there, and every item is in registers
+    unsigned all = 0, mine = 0;
+    if (threadIdx.x < DIGITS) {
+      for (unsigned b = 0; b < size; ++b) {
+        const unsigned c = *cluster.map_shared_rank(&s.total[threadIdx.x], b);
+        if (b < me) mine += c;
+        all += c;
+      }
+    }
+    const unsigned before = scan_digits(s, all);
+    if (threadIdx.x < DIGITS) s.base[threadIdx.x] = before + mine;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < SORT_ITEMS; ++i) {
+      const unsigned d = (key[i] >> shift) & mask;
+      const unsigned to = s.base[d] + s.counts[warp][d] + rank[i];
+      *cluster.map_shared_rank(&keys[to % SORT_TILE], to / SORT_TILE) = key[i];
+      *cluster.map_shared_rank(&poss[to % SORT_TILE], to / SORT_TILE) = pos[i];
+    }
+    cluster.sync();
+#pragma unroll
+    for (int i = 0; i < SORT_ITEMS; ++i) {
+      key[i] = keys[at + i * 32];
+      pos[i] = poss[at + i * 32];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < SORT_ITEMS; ++i) {
+    const unsigned to = me * SORT_TILE + at + i * 32;
+    if (to < n) {
+      out_key[to] = key[i];
+      out_pos[to] = pos[i];
+    }
+  }
+}
+
+// More positions: per digit a histogram of every tile, their prefix sums, and the scatter.
+__device__ __forceinline__ void load_items(const float* ids, const unsigned* in_key, const unsigned* in_pos, long long n,
+                                           unsigned vocab, long long padding, unsigned (&key)[SORT_ITEMS],
+                                           unsigned (&pos)[SORT_ITEMS]) {
+  const long long at = blockIdx.x * (long long)SORT_TILE + (threadIdx.x >> 5) * (32 * SORT_ITEMS) + (threadIdx.x & 31);
+#pragma unroll
+  for (int i = 0; i < SORT_ITEMS; ++i) {
+    const long long r = at + i * 32;
+    pos[i] = (unsigned)r;
+    if (!in_key) key[i] = key_of(ids, r, n, vocab, padding);
+    else if (r < n) key[i] = load(in_key + r), pos[i] = load(in_pos + r);
+    else key[i] = FILL;
+  }
+}
+
+__global__ void __launch_bounds__(SORT_THREADS) tile_histogram(const float* ids, const unsigned* in_key, long long n,
+                                                               unsigned vocab, long long padding, int shift, unsigned mask,
+                                                               unsigned* __restrict__ hist, unsigned tiles) {
+  tsb_launch::enter();
+  __shared__ unsigned count[DIGITS];
+  if (threadIdx.x < DIGITS) count[threadIdx.x] = 0;
+  __syncthreads();
+  const long long at = blockIdx.x * (long long)SORT_TILE;
+#pragma unroll
+  for (int i = 0; i < SORT_ITEMS; ++i) {
+    const long long r = at + i * SORT_THREADS + threadIdx.x;
+    const unsigned k = in_key ? (r < n ? load(in_key + r) : FILL) : key_of(ids, r, n, vocab, padding);
+    atomicAdd(&count[(k >> shift) & mask], 1u);        // whole numbers: any order gives the same sums
+  }
+  __syncthreads();
+  if (threadIdx.x < DIGITS) hist[(size_t)threadIdx.x * tiles + blockIdx.x] = count[threadIdx.x];
+}
+
+__global__ void __launch_bounds__(1024) scan_histogram(unsigned* hist, unsigned entries) {
+  tsb_launch::enter();
+  __shared__ unsigned sums[32];
+  __shared__ unsigned carry;
+  if (threadIdx.x == 0) carry = 0;
+  __syncthreads();
+  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (unsigned begin = 0; begin < entries; begin += 4096) {          // (a digit has `tiles` entries, 256 digits)
+    const unsigned i = begin + threadIdx.x * 4;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (i < entries) v = *reinterpret_cast<const uint4*>(hist + i);   // entries is a multiple of 256
+    const unsigned own = v.x + v.y + v.z + v.w;
+    unsigned sum = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    if (lane == 31) sums[warp] = sum;
+    __syncthreads();
+    unsigned before = carry, block = 0;
+    for (unsigned w = 0; w < 32; ++w) {
+      if (w < warp) before += sums[w];
+      block += sums[w];
+    }
+    before += sum - own;
+    if (i < entries)
+      *reinterpret_cast<uint4*>(hist + i) = make_uint4(before, before + v.x, before + v.x + v.y, before + v.x + v.y + v.z);
+    __syncthreads();
+    if (threadIdx.x == 0) carry += block;
+    __syncthreads();
+  }
+}
+
+__global__ void __launch_bounds__(SORT_THREADS) scatter_tiles(const float* ids, const unsigned* in_key, const unsigned* in_pos,
+                                                              long long n, unsigned vocab, long long padding, int shift,
+                                                              unsigned mask, const unsigned* hist, unsigned tiles,
+                                                              unsigned* __restrict__ out_key, unsigned* __restrict__ out_pos) {
+  tsb_launch::enter();
+  extern __shared__ uint4 raw[];
+  SortShared& s = *reinterpret_cast<SortShared*>(raw);
+  unsigned key[SORT_ITEMS], pos[SORT_ITEMS], rank[SORT_ITEMS];
+  load_items(ids, in_key, in_pos, n, vocab, padding, key, pos);
+  clear_counts(s);
+  __syncthreads();
+  const unsigned warp = threadIdx.x >> 5;
+  rank_items(key, shift, mask, s.counts[warp], rank);
+  __syncthreads();
+  scan_warps(s);
+  if (threadIdx.x < DIGITS) s.base[threadIdx.x] = load(hist + (size_t)threadIdx.x * tiles + blockIdx.x);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < SORT_ITEMS; ++i) {
+    const unsigned d = (key[i] >> shift) & mask;
+    const unsigned to = s.base[d] + s.counts[warp][d] + rank[i];
+    if (to < n) {                            // (what fills the last tile is behind all of them)
+      out_key[to] = key[i];
+      out_pos[to] = pos[i];
+    }
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) fill_zero(T* __restrict__ y, long long n) {
+  tsb_launch::enter();
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) y[i] = zero<T>();
+}
+
+// ------------------------------------------------------------------------------------------------ sums
+// Block (tile, column slice): positions [tile * size, ...) of the sorted list, one column piece per thread.  BATCH rows in
+// flight.  part[2 * tile]: what belongs to a token of an earlier tile; part[2 * tile + 1]: the token that goes on.
+constexpr int BATCH = 8, SUM_THREADS = 128, MAX_TILE = 64;
+
+template <class T>
+__global__ void __launch_bounds__(SUM_THREADS) sum_tiles(const T* g, const unsigned* key, const unsigned* pos, long long n,
+                                                         unsigned vocab, unsigned dim, float scale, int size,
+                                                         T* __restrict__ dtable, T* __restrict__ part) {
+  tsb_launch::enter();
+  __shared__ unsigned k[MAX_TILE + 2], p[MAX_TILE];
+  const long long begin = blockIdx.x * (long long)size;
+  const int count = (int)(n - begin < size ? n - begin : size);
+  for (int i = threadIdx.x; i < count + 2; i += SUM_THREADS) {
+    const long long at = begin + i - 1;
+    k[i] = at >= 0 && at < n ? load(key + at) : vocab;
+    if (i >= 1 && i <= count) p[i - 1] = load(pos + at);
+  }
+  __syncthreads();
+  if (k[1] == vocab) return;                 // nothing but positions without a gradient from here on
+  const unsigned c = blockIdx.y * SUM_THREADS + threadIdx.x;
+  if (c >= dim) return;
+  const T* row = g + c;
+  const bool goes_on = begin + count < n && k[count + 1] == k[count];
+  T acc = zero<T>();
+  bool first = k[0] == k[1];                 // the present token began in an earlier tile
+  for (int i = 0; i < count; i += BATCH) {
+    T v[BATCH];
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u)
+      if (i + u < count && k[i + u + 1] != vocab) v[u] = load(row + (size_t)p[i + u] * dim);
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const int j = i + u;
+      if (j >= count || k[j + 1] == vocab) break;
+      acc = plus(acc, v[u]);
+      if (j + 1 < count ? k[j + 2] != k[j + 1] : true) {              // the last one of its token, in this tile at least
+        if (first) part[(size_t)(2 * blockIdx.x) * dim + c] = acc;
+        else if (j + 1 == count && goes_on) part[(size_t)(2 * blockIdx.x + 1) * dim + c] = acc;
+        else dtable[(size_t)k[j + 1] * dim + c] = times(acc, scale);
+        acc = zero<T>();
+        first = false;
+      }
+    }
+  }
+}
+
+// Block (tile, column slice) of 32 x 8 threads: the token that begins in the tile and goes on.  Its partial rows are
+// taken by eight groups of threads, group j the rows j, j + 8, ..., and the groups are added in their order.
+template <class T>
+__global__ void __launch_bounds__(256) join_tokens(const T* part, const unsigned* key, long long n, unsigned vocab, unsigned dim,
+                                                   float scale, int size, unsigned tiles, T* __restrict__ dtable) {
+  tsb_launch::enter();
+  __shared__ T sums[8][32];
+  const unsigned tile = blockIdx.x;
+  const long long begin = tile * (long long)size, end = begin + size;
+  if (end >= n) return;
+  const unsigned token = load(key + end - 1);
+  if (token == vocab || load(key + end) != token) return;
+  if (begin > 0 && load(key + begin - 1) == token) return;             // it began earlier
+  // the last tile that holds the token
+  unsigned lo = tile + 1, hi = tiles - 1;
+  while (lo < hi) {
+    const unsigned mid = lo + (hi - lo + 1) / 2;
+    if (load(key + (long long)mid * size) == token) lo = mid;
+    else hi = mid - 1;
+  }
+  const unsigned rows = lo - tile + 1;                                 // partial rows: its tail, then the heads
+  const unsigned c = blockIdx.y * 32 + threadIdx.x, group = threadIdx.y;
+  T acc = zero<T>();
+  if (c < dim) {
+    for (unsigned r = group; r < rows; r += 8 * BATCH) {
+      T v[BATCH];
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const unsigned q = r + u * 8;
+        if (q < rows) v[u] = load(part + (size_t)(q == 0 ? 2 * tile + 1 : 2 * (tile + q)) * dim + c);
+      }
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u)
+        if (r + u * 8 < rows) acc = plus(acc, v[u]);
+    }
+  }
+  sums[group][threadIdx.x] = acc;
+  __syncthreads();
+  if (group == 0 && c < dim) {
+#pragma unroll
+    for (int j = 1; j < 8; ++j) acc = plus(acc, sums[j][threadIdx.x]);
+    dtable[(size_t)token * dim + c] = times(acc, scale);
+  }
+}
+
+int bits_of(long long v) {
+  int b = 1;
+  while (b < 32 && (v >> b)) ++b;
+  return b;
+}
+
+template <class T>
+int sums(const T* g, const unsigned* key, const unsigned* pos, long long n, unsigned vocab, unsigned dim, float scale, int size,
+         unsigned tiles, T* dtable, T* part, cudaStream_t st) {
+  cudaError_t e = tsb_launch::launch(sum_tiles<T>, dim3(tiles, (dim + SUM_THREADS - 1) / SUM_THREADS), dim3(SUM_THREADS), 0, st,
+                                     g, key, pos, n, vocab, dim, scale, size, dtable, part);
+  if (e == cudaSuccess && tiles > 1)
+    e = tsb_launch::launch(join_tokens<T>, dim3(tiles - 1, (dim + 31) / 32), dim3(32, 8), 0, st, part, key, n, vocab, dim, scale,
+                           size, tiles, dtable);
+  return launch_status(e);
+}
+
+constexpr long long MAX_TOKENS = 1ll << 30, MAX_VOCAB = 1ll << 24, MAX_DIM = 1ll << 20;     // (ids are whole numbers in fp32)
+
+}  // namespace
+
+extern "C" {
+
+int tsb_embedding_scaled(const float* table, const float* ids, float* y, long long n, long long vocab, long long dim,
+                         float scale, void* stream) {
+  if (n < 0 || vocab <= 0 || dim <= 0 || dim > MAX_DIM || n > MAX_TOKENS || vocab > MAX_VOCAB) return TSB_ERR_ARG;
+  if (n == 0) return TSB_OK;
+  if (!table || !ids || !y) return TSB_ERR_ARG;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool v4 = dim % 4 == 0 && ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(y)) & 15) == 0;
+  const long long pieces = v4 ? n * (dim / 4) : n * dim;
+  const long long blocks = (pieces + 1023) / 1024;
+  if (blocks > INT32_MAX) return TSB_ERR_ARG;
+  if (v4)
+    return launch_status(tsb_launch::launch(scaled_lookup<float4, 4>, dim3((unsigned)blocks), dim3(256), 0, st,
+                                            reinterpret_cast<const float4*>(table), ids, reinterpret_cast<float4*>(y), pieces,
+                                            vocab, (unsigned)(dim / 4), scale));
+  return launch_status(tsb_launch::launch(scaled_lookup<float, 4>, dim3((unsigned)blocks), dim3(256), 0, st, table, ids, y,
+                                          pieces, vocab, (unsigned)dim, scale));
+}
+
+// Scratch of a gradient: sorted keys and positions (twice, and the histograms, above one cluster's share), partial rows.
+int tsb_embedding_sorted_grad(const float* g, const float* ids, float* dtable, long long n, long long vocab, long long dim,
+                              float scale, long long padding, void* stream) {
+  if (n < 0 || vocab <= 0 || dim <= 0 || dim > MAX_DIM || n > MAX_TOKENS || vocab > MAX_VOCAB) return TSB_ERR_ARG;
+  if (!dtable || (n && (!g || !ids))) return TSB_ERR_ARG;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const long long cells = vocab * dim;
+  const bool out16 = (reinterpret_cast<uintptr_t>(dtable) & 15) == 0;
+  const bool v4 = dim % 4 == 0 && out16 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
+  const bool cluster_sort = n <= (long long)MAX_CLUSTER * SORT_TILE;
+  if (n == 0 || !cluster_sort) {
+    const cudaError_t e =
+        out16 && cells % 4 == 0
+            ? tsb_launch::launch(fill_zero<float4>, dim3(148 * 8), dim3(256), 0, st, reinterpret_cast<float4*>(dtable), cells / 4)
+            : tsb_launch::launch(fill_zero<float>, dim3(148 * 8), dim3(256), 0, st, dtable, cells);
+    if (e != cudaSuccess || n == 0) return launch_status(e);
+  }
+  const int size = n <= 16384 ? 16 : MAX_TILE;
+  const unsigned tiles = (unsigned)((n + size - 1) / size);
+  const unsigned sort_tiles = (unsigned)((n + SORT_TILE - 1) / SORT_TILE);
+  const size_t list = ((size_t)n * 4 + 255) / 256 * 256;
+  const size_t hist_bytes = cluster_sort ? 0 : (size_t)DIGITS * sort_tiles * 4;
+  const size_t part_bytes = (size_t)2 * tiles * dim * 4;
+  char* base = static_cast<char*>(tsb_scratch::get(st, tsb_scratch::EMBED_SORT, list * (cluster_sort ? 2 : 4) + hist_bytes + part_bytes));
+  if (!base) return TSB_ERR_OOM;
+  unsigned* key[2] = {reinterpret_cast<unsigned*>(base), nullptr};
+  unsigned* pos[2] = {reinterpret_cast<unsigned*>(base + list), nullptr};
+  char* rest = base + 2 * list;
+  const int bits = bits_of(vocab), passes = (bits + 7) / 8, step = (bits + passes - 1) / passes;
+  int last = 0;
+  if (cluster_sort) {
+    unsigned blocks = 1;
+    while (blocks < sort_tiles) blocks *= 2;
+    // zeros: 64 KB a block, in whole clusters, as many as the chip takes beside the sort
+    long long fillers = (cells * 4 + 65535) / 65536;
+    if (fillers > 148) fillers = 148;
+    fillers = (fillers + blocks - 1) / blocks * blocks;
+    const int smem = (int)sizeof(SortShared) + SORT_TILE * 8;
+    static tsb_launch::SmemLimit limit;
+    cudaError_t e = limit.raise(sort_cluster, smem);
+    if (e == cudaSuccess)
+      e = tsb_launch::launch_cluster(blocks, sort_cluster, dim3(blocks + (unsigned)fillers), dim3(SORT_THREADS), smem, st, ids, n,
+                                     (unsigned)vocab, padding, bits, passes, key[0], pos[0], dtable, cells, out16);
+    if (e != cudaSuccess) return launch_status(e);
+  } else {
+    key[1] = reinterpret_cast<unsigned*>(rest);
+    pos[1] = reinterpret_cast<unsigned*>(rest + list);
+    unsigned* hist = reinterpret_cast<unsigned*>(rest + 2 * list);
+    rest += 2 * list + hist_bytes;
+    const unsigned mask = (1u << step) - 1;
+    for (int p = 0; p < passes; ++p) {
+      const unsigned* in_key = p ? key[(p + 1) & 1] : nullptr;
+      const unsigned* in_pos = p ? pos[(p + 1) & 1] : nullptr;
+      last = p & 1;
+      cudaError_t e = tsb_launch::launch(tile_histogram, dim3(sort_tiles), dim3(SORT_THREADS), 0, st, ids, in_key, n,
+                                         (unsigned)vocab, padding, p * step, mask, hist, sort_tiles);
+      if (e == cudaSuccess)
+        e = tsb_launch::launch(scan_histogram, dim3(1), dim3(1024), 0, st, hist, DIGITS * sort_tiles);
+      if (e == cudaSuccess)
+        e = tsb_launch::launch(scatter_tiles, dim3(sort_tiles), dim3(SORT_THREADS), sizeof(SortShared), st, ids, in_key, in_pos, n,
+                               (unsigned)vocab, padding, p * step, mask, hist, sort_tiles, key[last], pos[last]);
+      if (e != cudaSuccess) return launch_status(e);
+    }
+  }
+  if (v4)
+    return sums(reinterpret_cast<const float4*>(g), key[last], pos[last], n, (unsigned)vocab, (unsigned)(dim / 4), scale, size,
+                tiles, reinterpret_cast<float4*>(dtable), reinterpret_cast<float4*>(rest), st);
+  return sums(g, key[last], pos[last], n, (unsigned)vocab, (unsigned)dim, scale, size, tiles, dtable,
+              reinterpret_cast<float*>(rest), st);
+}
+
+}  // extern "C"

@@ -10,6 +10,7 @@ There is no fallback: on a CUDA context a missing library is an error.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 from ctypes import c_void_p, c_int, c_int64, c_float
@@ -309,6 +310,53 @@ def embedding_grad(g, idx, dtable, stream):
     _check(lib().tsb_embedding_grad(_p(g), _p(idx), _p(dtable), c_int64(_numel(idx.shape)),
                                     c_int64(dtable.shape[0]), c_int64(dtable.shape[1]), _s(stream)),
            "embedding_grad")
+
+
+def _dense_rows(what, *arrs):
+    for a in arrs:
+        if not a.is_contiguous():
+            raise ValueError("%s: an array of shape %s with strides %s is not row-major" % (what, a.shape, a.strides))
+
+
+def _on_device(arr):
+    """The device of ``arr`` as the current one: launches and the library's scratch belong to that."""
+    import torch
+    if arr.is_cuda and torch.cuda.current_device() != arr.ctx.device_id:
+        return torch.cuda.device(arr.ctx.device_id)
+    return contextlib.nullcontext()
+
+
+def scaled_embedding(table, idx, y, scale, stream):
+    _dense_rows("scaled_embedding", table, idx, y)
+    with _on_device(table):
+        _check(lib().tsb_embedding_scaled(_p(table), _p(idx), _p(y), c_int64(_numel(idx.shape)), c_int64(table.shape[0]),
+                                          c_int64(table.shape[1]), c_float(scale), _s(stream)), "scaled_embedding")
+
+
+def scaled_embedding_grad(g, idx, dtable, scale, padding_id, stream):
+    """dtable: all of it is written.  ``padding_id``: an id without a gradient, or None."""
+    _dense_rows("scaled_embedding_grad", g, idx, dtable)
+    with _on_device(g):
+        _check(lib().tsb_embedding_sorted_grad(_p(g), _p(idx), _p(dtable), c_int64(_numel(idx.shape)), c_int64(dtable.shape[0]),
+                                               c_int64(dtable.shape[1]), c_float(scale),
+                                               c_int64(-1 if padding_id is None else padding_id), _s(stream)),
+               "scaled_embedding_grad")
+
+
+def token_score(logits, ids, out, top, stream):
+    _dense_rows("token_log_prob", logits, ids, out)
+    rows, cols = logits.shape
+    with _on_device(logits):
+        _check(lib().tsb_token_score(_p(logits), _p(ids), _p(out), c_int64(rows), c_int64(cols), c_int(top), _s(stream)),
+               "token_log_prob")
+
+
+def token_score_grad(logits, ids, out, g, dx, stream):
+    _dense_rows("token_log_prob_gradient", logits, ids, out, g, dx)
+    rows, cols = logits.shape
+    with _on_device(logits):
+        _check(lib().tsb_token_score_grad(_p(logits), _p(ids), _p(out), _p(g), _p(dx), c_int64(rows), c_int64(cols),
+                                          c_int((out.shape[1] - 3) // 2), _s(stream)), "token_log_prob_gradient")
 
 
 def dropout(x, y, keep_prob, seed, stream, step_dev=0, offset=0):

@@ -221,6 +221,122 @@ class SoftmaxCrossEntropyGradientOp(Op):
         return 6.0 * np.prod(out)
 
 
+MAX_ALTERNATIVES = 32
+
+
+class TokenLogProbOp(Op):
+    """What a language model says about given tokens, from one pass over its ``logits`` [rows, vocab]: a row of
+    ``3 + 2 * top_k`` numbers
+
+        log p(id), entropy of p, log-sum-exp of the logits, log p of the ``top_k`` likeliest tokens (falling), their ids
+
+    with p the soft-max of the row.  ``ids``: one whole number a row, in any shape; one outside [0, vocab) means no token and
+    gives 0.  Logits of -inf are tokens that cannot be said.  A row that has no other logit has log-sum-exp and log
+    probabilities of -inf, no entropy and no gradient.  Of equal logits the one with the lower id comes first; a NaN makes its
+    row's numbers NaN and is not among the likeliest (id -1 where fewer than ``top_k`` logits are numbers).  Gradients reach
+    the logits from every column but the ids."""
+    name = "TokenLogProb"
+
+    def __call__(self, logits, ids, top_k=0):
+        top_k = int(top_k)
+        assert 0 <= top_k <= MAX_ALTERNATIVES, "top_k is 0 to %d, not %d" % (MAX_ALTERNATIVES, top_k)
+        return Op.__call__(self, logits, ids, top_k=top_k)
+
+    def np_compute(self, node, iv):
+        x, top = iv[0].astype(np.float64), node.attrs["top_k"]
+        ids = iv[1].reshape(-1).astype(np.int64)
+        with np.errstate(invalid="ignore", divide="ignore"):
+            m = x.max(1, keepdims=True)
+            empty = (x == -np.inf).all(1)
+            u = x - np.where(empty[:, None], 0, m)
+            e = np.exp(u)
+            z = e.sum(1)
+            lse = np.where(empty, 0, m[:, 0]) + np.log(z)
+            h = np.log(z) - np.where(e == 0, 0, e * u).sum(1) / z
+            out = np.empty((x.shape[0], 3 + 2 * top))
+            given = (ids >= 0) & (ids < x.shape[1])
+            own = x[np.arange(len(ids)), np.where(given, ids, 0)] - lse
+            out[:, 0] = np.where(given, np.where(empty, -np.inf, own), 0)
+            out[:, 1] = np.where(empty, 0, h)
+            out[:, 2] = lse
+            cols = np.argsort(-x, axis=1, kind="stable")[:, :top]          # (NaN last)
+            best = np.take_along_axis(x, cols, 1)
+            out[:, 3:3 + top] = np.where(empty[:, None], -np.inf, best - lse[:, None])
+            out[:, 3 + top:] = np.where(np.isnan(best), -1, cols)
+        return out.astype(np.float32)
+
+    def gpu_compute(self, node, iv, out, stream):
+        G.token_score(iv[0], iv[1], out, node.attrs["top_k"], stream)
+
+    def gradient(self, node, g):
+        return [token_log_prob_gradient_op(node.inputs[0], node.inputs[1], node, g), None]
+
+    def infer_shape(self, node, s):
+        assert len(s[0]) == 2 and np.prod(s[1], dtype=np.int64) == s[0][0], \
+            "logits are [rows, vocab] with one id a row, not %s with %s" % (tuple(s[0]), tuple(s[1]))
+        assert node.attrs["top_k"] <= s[0][1], "%d alternatives of %d tokens" % (node.attrs["top_k"], s[0][1])
+        return (s[0][0], 3 + 2 * node.attrs["top_k"])
+
+    def flops(self, node, s, out):
+        return 8.0 * np.prod(s[0])
+
+
+class TokenLogProbGradientOp(Op):
+    """``sum_i w_i (1[c = id_i] - p_c) + w_lse p_c - w_H p_c (log p_c + H)``: w is the gradient ``g`` of a
+    :class:`TokenLogProbOp`'s result ``out``, i its given token and the likeliest ones."""
+    name = "TokenLogProbGradient"
+
+    def __call__(self, logits, ids, out, g):
+        return Op.__call__(self, logits, ids, out, g)
+
+    def np_compute(self, node, iv):
+        x, ids, out, g = iv[0].astype(np.float64), iv[1].reshape(-1).astype(np.int64), iv[2], iv[3].astype(np.float64)
+        top, rows = (out.shape[1] - 3) // 2, np.arange(x.shape[0])
+        with np.errstate(invalid="ignore"):
+            m = x.max(1, keepdims=True)
+            empty = (x == -np.inf).all(1)
+            e = np.exp(x - np.where(empty[:, None], 0, m))
+            z = np.where(empty, 1, e.sum(1))[:, None]
+            p, logs = e / z, x - np.where(empty[:, None], 0, m) - np.log(z)
+            h = -np.where(p == 0, 0, p * logs).sum(1, keepdims=True)
+            dx = g[:, 2:3] * p - g[:, 1:2] * np.where(p == 0, 0, p * (logs + h))
+            given = (ids >= 0) & (ids < x.shape[1])
+            for j in range(top + 1):
+                col = np.where(given, ids, -1) if j == 0 else out[:, 2 + top + j].astype(np.int64)
+                w = np.where(col >= 0, g[:, 0] if j == 0 else g[:, 2 + j], 0)
+                dx -= w[:, None] * p
+                dx[rows, np.maximum(col, 0)] += w
+            dx[empty] = 0
+        return dx.astype(np.float32)
+
+    def gpu_compute(self, node, iv, out, stream):
+        G.token_score_grad(iv[0], iv[1], iv[2], iv[3], out, stream)
+
+    def gradient(self, node, g):
+        raise NotImplementedError
+
+    def infer_shape(self, node, s):
+        assert len(s[0]) == 2 and np.prod(s[1], dtype=np.int64) == s[0][0], \
+            "logits are [rows, vocab] with one id a row, not %s with %s" % (tuple(s[0]), tuple(s[1]))
+        assert tuple(s[2]) == tuple(s[3]) and len(s[2]) == 2 and s[2][0] == s[0][0] and s[2][1] >= 3 and s[2][1] % 2, \
+            "results %s and gradients %s do not belong to logits %s" % (tuple(s[2]), tuple(s[3]), tuple(s[0]))
+        return tuple(s[0])
+
+    def flops(self, node, s, out):
+        return 8.0 * np.prod(out)
+
+
+_tlp, _tlpg = TokenLogProbOp(), TokenLogProbGradientOp()
+
+
+def token_log_prob_op(logits, ids, top_k=0):
+    return _tlp(logits, ids, top_k)
+
+
+def token_log_prob_gradient_op(logits, ids, node, g):
+    return _tlpg(logits, ids, node, g)
+
+
 _sm, _ce, _ceg = SoftmaxOp(), SoftmaxCrossEntropyOp(), SoftmaxCrossEntropyGradientOp()
 _smg = SoftmaxGradientOp()
 

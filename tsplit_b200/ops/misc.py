@@ -190,6 +190,75 @@ def embedding_lookup_gradient_op(vectors, index, embedding):
     return _embg(vectors, index, embedding)
 
 
+class ScaledEmbeddingOp(Op):
+    """``scale * table[ids]``: the lookup and the scale of a Transformer's token embedding in one kernel.  ``ids``: whole
+    numbers of any shape, ``table`` [vocab, dim], result ``ids.shape + (dim,)``.  An id outside [0, vocab) gives a row of
+    zeros and no gradient; ``padding_id`` is looked up like any other but gives no gradient."""
+    name = "ScaledEmbedding"
+
+    def __call__(self, table, ids, scale=1.0, padding_id=None):
+        return Op.__call__(self, table, ids, scale=float(scale), padding_id=None if padding_id is None else int(padding_id))
+
+    def np_compute(self, node, iv):
+        table, ids = iv[0], iv[1].astype(np.int64)
+        known = (ids >= 0) & (ids < table.shape[0])
+        rows = table[np.where(known, ids, 0)] * np.float32(node.attrs["scale"])
+        return np.where(known[..., None], rows, np.float32(0)).astype(np.float32)
+
+    def gpu_compute(self, node, iv, out, stream):
+        G.scaled_embedding(iv[0], iv[1], out, node.attrs["scale"], stream)
+
+    def gradient(self, node, g):
+        table, ids = node.inputs
+        return [scaled_embedding_gradient_op(g, ids, table, node.attrs["scale"], node.attrs["padding_id"]), None]
+
+    def infer_shape(self, node, s):
+        assert len(s[0]) == 2, "an embedding table is [vocab, dim], not %s" % (tuple(s[0]),)
+        return tuple(s[1]) + (s[0][1],)
+
+
+class ScaledEmbeddingGradientOp(Op):
+    """Gradient of the table: row v is ``scale`` times the sum of the ``vectors`` at the positions that hold v, taken in the
+    order of the positions (the ids are sorted on the device), so two runs give the same bits."""
+    name = "ScaledEmbeddingGradient"
+
+    def __call__(self, vectors, ids, table, scale=1.0, padding_id=None):
+        return Op.__call__(self, vectors, ids, table, scale=float(scale),
+                           padding_id=None if padding_id is None else int(padding_id))
+
+    def np_compute(self, node, iv):
+        vectors, ids, table = iv
+        flat, pad = ids.reshape(-1).astype(np.int64), node.attrs["padding_id"]
+        known = (flat >= 0) & (flat < table.shape[0])
+        if pad is not None:
+            known &= flat != pad
+        out = np.zeros(table.shape, dtype=np.float64)
+        np.add.at(out, flat[known], vectors.reshape(-1, table.shape[1])[known])
+        return (out * np.float32(node.attrs["scale"])).astype(np.float32)
+
+    def gpu_compute(self, node, iv, out, stream):
+        G.scaled_embedding_grad(iv[0], iv[1], out, node.attrs["scale"], node.attrs["padding_id"], stream)
+
+    def gradient(self, node, g):
+        raise NotImplementedError
+
+    def infer_shape(self, node, s):
+        assert len(s[2]) == 2 and tuple(s[0]) == tuple(s[1]) + (s[2][1],), \
+            "gradients %s do not belong to ids %s of a table %s" % (tuple(s[0]), tuple(s[1]), tuple(s[2]))
+        return tuple(s[2])
+
+
+_semb, _sembg = ScaledEmbeddingOp(), ScaledEmbeddingGradientOp()
+
+
+def scaled_embedding_op(embedding, index, scale=1.0, padding_id=None):
+    return _semb(embedding, index, scale, padding_id)
+
+
+def scaled_embedding_gradient_op(vectors, index, embedding, scale=1.0, padding_id=None):
+    return _sembg(vectors, index, embedding, scale, padding_id)
+
+
 # -- dropout ---------------------------------------------------------------------------
 def philox_like_mask(shape, keep_prob, seed, offset=0):
     """Host twin of the device mask generator: element i is kept when
