@@ -1,0 +1,253 @@
+"""Attention across to an encoder's states: the NumPy path and the kernels against the definition in 64 bits, at lengths,
+head layouts and masks where they can go wrong."""
+import numpy as np
+import pytest
+
+from tsplit_b200 import ndarray, gpu_ops as ad
+
+#: a pair of bf16 pieces keeps a number to 2^-18, the product of the low pieces that is left out is another 2^-18
+PIECE = 2.0 ** -18
+
+
+@pytest.fixture(params=[pytest.param("cpu"), pytest.param("gpu", marks=pytest.mark.gpu)])
+def ctx(request):
+    return None if request.param == "cpu" else ndarray.gpu(0)
+
+
+def definition(q, kv, key, scale, g):
+    """(y, dq, dkv) and bounds of what pieces of 2^-18 and fp32 sums may be off, element by element."""
+    n, tq, h, d = q.shape
+    tk, s = kv.shape[1], kv.shape[3]
+    out = [np.zeros(a.shape) for a in (q, q, kv)]
+    tol = [np.zeros(a.shape) for a in (q, q, kv)]
+    for b in range(n):
+        kept = np.arange(tk) if key is None else np.flatnonzero(key[b] != 0)
+        if not len(kept):
+            continue
+        for j in range(h):
+            t = j // (h // s)
+            qq, k, v, gg = (a.astype(np.float64) for a in (q[b, :, j], kv[b, kept, 0, t], kv[b, kept, 1, t], g[b, :, j]))
+            x = qq @ k.T * scale
+            p = np.exp(x - x.max(1, keepdims=True))
+            p /= p.sum(1, keepdims=True)
+            y = p @ v
+            dp, dot = gg @ v.T, (gg * y).sum(1, keepdims=True)
+            ds = p * (dp - dot) * scale
+            out[0][b, :, j], out[1][b, :, j] = y, ds @ k
+            out[2][b, kept, 0, t] += ds.T @ qq
+            out[2][b, kept, 1, t] += p.T @ gg
+            # a product is off by three times PIECE of the sum of its terms' sizes (either factor, what is left out), and
+            # by a truncation a step of its sum; a score's error e makes p off by a factor of e (its normaliser by no more)
+            step = 3 * PIECE + d * 2.0 ** -23
+            e = (np.abs(qq) @ np.abs(k).T * abs(scale)) * step + 2.0 ** -22 * (4 + np.abs(x))
+            rel = 2 * e.max(1, keepdims=True) + len(kept) * 2.0 ** -24
+            long = 3 * PIECE + 300 * 2.0 ** -23
+            dy = rel * (p @ np.abs(v)) + long * (p @ np.abs(v))
+            tol[0][b, :, j] = dy
+            ddp = np.abs(gg) @ np.abs(v).T * step
+            ddot = (np.abs(gg) * dy).sum(1, keepdims=True) + d * 2.0 ** -23 * (np.abs(gg) * np.abs(y)).sum(1, keepdims=True)
+            dds = abs(scale) * p * (ddp + ddot) + rel * np.abs(ds)
+            tol[1][b, :, j] = dds @ np.abs(k) + long * (np.abs(ds) @ np.abs(k))
+            tol[2][b, kept, 0, t] += dds.T @ np.abs(qq) + long * (np.abs(ds).T @ np.abs(qq))
+            tol[2][b, kept, 1, t] += (rel * p).T @ np.abs(gg) + long * (p.T @ np.abs(gg))
+    return out, tol
+
+
+def graph(masked, scale):
+    def build():
+        q, kv, key, g = (ad.Variable(v) for v in ("q", "kv", "key", "g"))
+        y = ad.cross_attention_op(q, kv, key if masked else None, scale=scale)
+        names = {"q": q, "kv": kv, "g": g}
+        if masked:
+            names["key"] = key
+        return names, [y] + ad.cross_attention_gradient_op(y, g)
+    return build
+
+
+def evaluate(build, feeds, ctx, **kw):
+    names, nodes = build()
+    ex = ad.Executor(nodes, ctx=ctx, **kw)
+    return [np.asarray(o).astype(np.float64) for o in ex.run({names[k]: v for k, v in feeds.items()}, convert_to_numpy_ret_vals=True)]
+
+
+def case(n, tq, tk, h, s, d, mask="tail", seed=0, spread=1.0):
+    r = np.random.default_rng([n, tq, tk, h, s, d, seed])
+    f = {"q": r.standard_normal((n, tq, h, d), np.float32) * np.float32(spread), "kv": r.standard_normal((n, tk, 2, s, d), np.float32),
+         "g": r.standard_normal((n, tq, h, d), np.float32)}
+    if mask:
+        key = r.integers(1, 9, (n, tk)).astype(np.float32)
+        if mask == "tail":                                        # the last sentence is padding all through
+            for b in range(n):
+                key[b, tk - tk * b // max(1, n - 1):] = 0
+        elif mask == "holes":
+            key[r.random((n, tk)) < 0.6] = 0
+        elif mask == "head":
+            key[:, :tk - 1] = 0
+        f["key"] = key
+    return f
+
+
+def check(f, ctx, scale=None, **kw):
+    got = evaluate(graph("key" in f, scale), f, ctx, **kw)
+    want, tol = definition(f["q"], f["kv"], f.get("key"), scale if scale is not None else f["q"].shape[3] ** -0.5, f["g"])
+    for name, a, b, t in zip(("y", "dq", "dkv"), got, want, tol):
+        assert a.shape == b.shape and np.isfinite(a).all(), name
+        worst = np.unravel_index(np.argmax(np.abs(a - b) - t), a.shape)
+        assert np.all(np.abs(a - b) <= t + 1e-37), "%s at %s: %r for %r, tolerance %r" % (name, worst, a[worst], b[worst], t[worst])
+        assert not a[t == 0].any(), name                            # what is masked has no result and no gradient at all
+    return got
+
+
+@pytest.mark.parametrize("n,tq,tk,h,s,d", [(1, 1, 1, 1, 1, 1), (2, 1, 5, 2, 2, 8), (2, 3, 40, 4, 2, 32), (1, 8, 130, 2, 2, 64), (2, 9, 33, 2, 2, 64),
+                                           (3, 30, 37, 4, 4, 32), (1, 128, 128, 1, 1, 64), (2, 129, 127, 2, 1, 64), (1, 70, 300, 3, 1, 20),
+                                           (2, 17, 129, 2, 2, 128), (1, 140, 260, 2, 1, 100), (1, 33, 65, 2, 2, 69), (1, 20, 64, 1, 1, 3)])
+@pytest.mark.parametrize("mask", [None, "tail", "holes", "head"])
+def test_attention_and_its_gradients(n, tq, tk, h, s, d, mask, ctx):
+    check(case(n, tq, tk, h, s, d, mask), ctx)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,tq,tk,h,s,d", [(4, 255, 256, 8, 8, 64), (1, 600, 1100, 4, 1, 64), (1, 500, 1030, 4, 2, 128), (2, 1, 3000, 8, 2, 128),
+                                           (1, 2, 5000, 4, 1, 64), (70, 1, 40, 2, 2, 32), (3, 385, 513, 2, 2, 96), (1, 1300, 200, 2, 1, 64),
+                                           (5, 10, 700, 1, 1, 128)])
+@pytest.mark.parametrize("mask", [None, "tail", "holes"])
+def test_longer_attention(n, tq, tk, h, s, d, mask):
+    check(case(n, tq, tk, h, s, d, mask), ndarray.gpu(0))
+
+
+@pytest.mark.parametrize("tq", [1, 40])
+@pytest.mark.parametrize("spread,scale", [(8.0, None), (1.0, 0.0), (1.0, -0.3), (3.0, 1.0)])
+def test_attention_scales_and_peaks(tq, spread, scale, ctx):
+    check(case(2, tq, 150, 2, 1, 64, "holes", spread=spread), ctx, scale=scale)
+
+
+@pytest.mark.parametrize("tq", [1, 33])
+@pytest.mark.parametrize("what", [np.nan, np.inf, np.finfo(np.float32).max])
+def test_what_masked_states_hold_does_not_matter(tq, what, ctx):
+    f = case(3, tq, 200, 2, 2, 64, "holes")
+    f["key"][1] = 0
+    clean = [a.copy() for a in check(f, ctx)]
+    f["kv"][f["key"] == 0] = what
+    for a, b in zip(evaluate(graph(True, None), f, ctx), clean):
+        assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("n,tq,tk", [(0, 4, 5), (2, 0, 5), (2, 4, 0), (2, 20, 0)])
+def test_empty_attention(n, tq, tk, ctx):
+    y, dq, dkv = evaluate(graph(True, None), case(n, tq, tk, 2, 2, 16, None) | {"key": np.ones((n, tk), np.float32)}, ctx)
+    assert y.shape == dq.shape == (n, tq, 2, 16) and dkv.shape == (n, tk, 2, 2, 16)
+    assert not y.any() and not dq.any() and not dkv.any()
+
+
+def test_gradients_by_differences():
+    """The NumPy gradients against central differences of the definition."""
+    f = case(2, 3, 7, 4, 2, 5, "holes")
+    f["key"][0] = 1
+    _, dq, dkv = evaluate(graph(True, 0.7), f, None)
+    def loss(**kw):
+        a = {**f, **kw}
+        return (definition(a["q"], a["kv"], a["key"], 0.7, a["g"])[0][0] * a["g"]).sum()
+    h = 1e-5
+    for name, got in (("q", dq), ("kv", dkv)):
+        for at in list(np.ndindex(*got.shape))[::7]:
+            up, down = f[name].astype(np.float64), f[name].astype(np.float64)
+            up[at] += h
+            down[at] -= h
+            assert abs((loss(**{name: up}) - loss(**{name: down})) / (2 * h) - got[at]) <= 1e-5
+
+
+def test_attention_in_a_training_graph(ctx):
+    """Projections around it, and every gradient through ``ad.gradients``, against the same from separate operators."""
+    n, tq, tk, h, d = 2, 11, 9, 2, 16
+    r = np.random.default_rng(3)
+    feeds = {"x": r.standard_normal((n * tq, 8), np.float32), "e": r.standard_normal((n * tk, 8), np.float32),
+             "wq": r.standard_normal((8, h * d), np.float32) * 0.3, "wkv": r.standard_normal((8, 2 * h * d), np.float32) * 0.3,
+             "key": (np.arange(n * tk).reshape(n, tk) % 4).astype(np.float32), "w": r.standard_normal((n, tq, h, d), np.float32)}
+
+    def build(fused):
+        def make():
+            v = {k: ad.Variable(k) for k in feeds}
+            q = ad.array_reshape_op(ad.matmul_op(v["x"], v["wq"]), (n, tq, h, d))
+            kv = ad.array_reshape_op(ad.matmul_op(v["e"], v["wkv"]), (n, tk, 2, h, d))
+            if fused:
+                y = ad.cross_attention_op(q, kv, v["key"])
+            else:
+                flat = ad.matmul_op(v["e"], v["wkv"])
+                k, val = (ad.array_reshape_op(ad.slice_op(flat, (0, i * h * d), (n * tk, h * d)), (n, tk, h, d)) for i in (0, 1))
+                p = ad.masked_softmax_op(ad.batch_matmul_op(q, k, trans_B=True, heads_A=True, heads_B=True), v["key"], scale=d ** -0.5)
+                y = ad.batch_matmul_op(p, val, heads_B=True, heads_out=True)
+            loss = ad.reduce_sum_op(ad.mul_op(y, v["w"]), [0, 1, 2, 3])
+            return v, [y] + ad.gradients(loss, [v["wq"], v["wkv"], v["x"], v["e"]])
+        return make
+    one, parts = evaluate(build(True), feeds, ctx), evaluate(build(False), feeds, None)
+    for a, b in zip(one, parts):
+        # the projections around it take ten bits of each factor on the GPU
+        assert np.allclose(a, b, rtol=0, atol=(2e-5 if ctx is None else 0.02) * np.abs(b).max())
+
+
+def test_attention_refuses(ctx):
+    shapes = {"q": (2, 3, 4, 8), "kv": (2, 5, 2, 2, 8), "key": (2, 5), "g": (2, 3, 4, 8)}
+    for change in [{"q": (2, 3, 32)}, {"kv": (2, 5, 2, 8)}, {"kv": (2, 5, 3, 2, 8)}, {"kv": (1, 5, 2, 2, 8)}, {"kv": (2, 5, 2, 3, 8)},
+                   {"kv": (2, 5, 2, 2, 4)}, {"key": (2, 4)}, {"g": (2, 3, 4, 4)}, {"q": (2, 3, 4, 129), "kv": (2, 5, 2, 2, 129), "g": (2, 3, 4, 129)}]:
+        with pytest.raises(AssertionError):
+            evaluate(graph(True, None), {k: np.ones(v, np.float32) for k, v in {**shapes, **change}.items()}, ctx)
+
+
+def test_attention_refuses_what_is_not_row_major():
+    import torch
+    from tsplit_b200.ops import _gpu as G
+    cpu = ndarray.cpu(0)
+    q = ndarray.NDArray(torch.zeros(2, 8, 4, 3).permute(0, 3, 2, 1), cpu)                 # (2, 3, 4, 8)
+    ok, kv, rows = ndarray.empty((2, 3, 4, 8)), ndarray.empty((2, 5, 2, 2, 8)), ndarray.empty((2, 4, 3))
+    sizes = (2, 3, 5, 4, 2, 8)
+    for call in [lambda: G.cross_attention(q, kv, None, ok, rows, sizes, 1.0, None), lambda: G.cross_attention_dots(ok, q, rows, None),
+                 lambda: G.cross_attention_grad_q(ok, kv, None, rows, q, rows, ok, sizes, 1.0, None),
+                 lambda: G.cross_attention_grad_kv(q, kv, None, rows, ok, rows, kv, sizes, 1.0, None)]:
+        with pytest.raises(ValueError, match="row-major"):
+            call()
+
+
+@pytest.mark.gpu
+def test_attention_has_the_same_bits_every_time_in_a_captured_step():
+    """Replays of one graph, another executor's in between on its own stream."""
+    a, b = case(2, 150, 300, 4, 2, 64, "holes"), case(3, 1, 900, 4, 4, 128, "holes")
+    first, ex = {}, {}
+    for k, f in (("a", a), ("b", b)):
+        names, nodes = graph(True, None)()
+        ex[k] = (ad.Executor(nodes, ctx=ndarray.gpu(0), use_graph=True), {names[x]: v for x, v in f.items()})
+    for _ in range(5):
+        for k in ("a", "b"):
+            got = ex[k][0].run(ex[k][1], convert_to_numpy_ret_vals=True)
+            if k not in first:
+                first[k] = [x.copy() for x in got]
+            for x, y in zip(got, first[k]):
+                assert np.array_equal(x, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tq", [1, 20])
+def test_attention_of_arrays_that_begin_anywhere(tq):
+    """Arrays 4 bytes off a 16-byte boundary take the loads of single numbers, with the same results."""
+    import torch
+    from tsplit_b200.ops import _gpu as G
+    from tsplit_b200.stream import create_stream_handle
+    ctx = ndarray.gpu(0)
+    st = create_stream_handle(ctx)
+    f = case(2, tq, 100, 2, 1, 64, "holes")
+    sizes, got = (2, tq, 100, 2, 1, 64), []
+    for off in (0, 1):
+        def at(v):
+            t = torch.empty(v.size + 8, device="cuda")[off:off + v.size].view(v.shape)
+            return ndarray.from_tensor(t.copy_(torch.from_numpy(v)), ctx)
+        q, kv, key, g = (at(f[k]) for k in ("q", "kv", "key", "g"))
+        y, dq, dkv, lse, dots = at(f["q"] * 0), at(f["q"] * 0), at(f["kv"] * 0), at(np.zeros((2, 2, tq), np.float32)), at(np.zeros((2, 2, tq), np.float32))
+        torch.cuda.synchronize()
+        G.cross_attention(q, kv, key, y, lse, sizes, 0.125, st)
+        G.cross_attention_dots(g, y, dots, st)
+        G.cross_attention_grad_q(q, kv, key, lse, g, dots, dq, sizes, 0.125, st)
+        G.cross_attention_grad_kv(q, kv, key, lse, g, dots, dkv, sizes, 0.125, st)
+        st.sync()
+        got.append([a.asnumpy() for a in (y, dq, dkv)])
+    want, tol = definition(f["q"], f["kv"], f["key"], 0.125, f["g"])
+    for a, b, w, t in zip(got[0], got[1], want, tol):
+        assert np.all(np.abs(a - w) <= t + 1e-37) and np.all(np.abs(b - w) <= t + 1e-37)

@@ -19,6 +19,7 @@ from ..ops.shape import (array_reshape_op, array_reshape_gradient_op, transpose_
                          slice_gradient_op, concat_op, concat_gradient_op, pad_op, pad_gradient_op,
                          broadcastto_op, broadcast_shape_op, broadcasttoTF_op, add_broadcast_op, reduce_sum_op,
                          reducesumaxiszero_op)
+from ..ops.attention import cross_attention_op, cross_attention_gradient_op
 from ..ops.loss import (softmax_func, softmax_op, softmax_gradient_op, softmaxcrossentropy_op,
                         softmaxcrossentropy_gradient_op, masked_softmax_op, masked_softmax_gradient_op,
                         token_log_prob_op, token_log_prob_gradient_op)

@@ -359,6 +359,38 @@ def token_score_grad(logits, ids, out, g, dx, stream):
                                           c_int((out.shape[1] - 3) // 2), _s(stream)), "token_log_prob_gradient")
 
 
+def cross_attention(q, kv, key, y, lse, sizes, scale, stream):
+    """``sizes``: (N, Tq, Tk, heads, heads of the states, d).  ``lse`` [N, heads, Tq] is written for the gradients."""
+    _dense_rows("cross_attention", q, kv, y, lse, *([key] if key is not None else []))
+    with _on_device(q):
+        _check(lib().tsb_cross_attention(_p(q), _p(kv), c_void_p(key.ptr if key is not None else 0), _p(y), _p(lse),
+                                         *[c_int(s) for s in sizes], c_float(scale), _s(stream)), "cross_attention")
+
+
+def cross_attention_dots(g, y, dots, stream):
+    _dense_rows("cross_attention_gradient", g, y, dots)
+    n, tq, h, d = g.shape
+    with _on_device(g):
+        _check(lib().tsb_cross_attention_dots(_p(g), _p(y), _p(dots), c_int(n), c_int(tq), c_int(h), c_int(d), _s(stream)),
+               "cross_attention_gradient")
+
+
+def cross_attention_grad_q(q, kv, key, lse, g, dots, dq, sizes, scale, stream):
+    _dense_rows("cross_attention_gradient", q, kv, lse, g, dots, dq, *([key] if key is not None else []))
+    with _on_device(q):
+        _check(lib().tsb_cross_attention_grad_q(_p(q), _p(kv), c_void_p(key.ptr if key is not None else 0), _p(lse), _p(g), _p(dots),
+                                                _p(dq), *[c_int(s) for s in sizes], c_float(scale), _s(stream)),
+               "cross_attention_gradient")
+
+
+def cross_attention_grad_kv(q, kv, key, lse, g, dots, dkv, sizes, scale, stream):
+    _dense_rows("cross_attention_gradient", q, kv, lse, g, dots, dkv, *([key] if key is not None else []))
+    with _on_device(q):
+        _check(lib().tsb_cross_attention_grad_kv(_p(q), _p(kv), c_void_p(key.ptr if key is not None else 0), _p(lse), _p(g), _p(dots),
+                                                 _p(dkv), *[c_int(s) for s in sizes], c_float(scale), _s(stream)),
+               "cross_attention_gradient")
+
+
 def dropout(x, y, keep_prob, seed, stream, step_dev=0, offset=0):
     """``step_dev``: device address of the executor's step counter (0 = ``seed`` is already step-mixed);
     ``offset``: index of ``x``'s first element in the whole tensor when ``x`` is a batch piece of it."""

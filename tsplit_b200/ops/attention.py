@@ -1,0 +1,202 @@
+"""Attention across to an encoder's states, as one operator with its gradients.
+
+The reference's example builds it from batched products, a scale, a padding mask and a soft-max
+(``examples/transformer.py:117-171``) and keeps the scores; here they never leave the chip
+(``csrc/kernels/cross_attention.cu``), forward or backward, and the products keep the accuracy of fp32.
+"""
+from __future__ import annotations
+
+import numpy as np
+
+from ..graph import Op
+from . import _gpu as G
+
+MAX_HEAD_DIM = 128
+
+
+def _sizes(q, kv, key=None):
+    """(N, Tq, Tk, heads, heads of the states, d) of shapes that belong together."""
+    assert len(q) == 4 and len(kv) == 5 and kv[2] == 2, \
+        "queries are [N, Tq, heads, d] and states [N, Tk, 2, heads, d], not %s and %s" % (tuple(q), tuple(kv))
+    n, tq, h, d = q
+    assert kv[0] == n and kv[4] == d and kv[3] > 0 and h % kv[3] == 0, "queries %s do not fit states %s" % (tuple(q), tuple(kv))
+    assert 0 < d <= MAX_HEAD_DIM, "a head has 1 to %d columns, not %d" % (MAX_HEAD_DIM, d)
+    assert key is None or tuple(key) == (n, kv[1]), "key tokens are [N, Tk] = %s, not %s" % ((n, kv[1]), tuple(key))
+    return n, tq, kv[1], h, kv[3], d
+
+
+def _heads(x, shared):
+    """[N, T, heads, d] -> [N, shared, heads / shared, T, d] in 64 bits."""
+    n, t, h, d = x.shape
+    return x.astype(np.float64).reshape(n, t, shared, h // shared, d).transpose(0, 2, 3, 1, 4)
+
+
+def _back(x):
+    n, s, r, t, d = x.shape
+    return x.transpose(0, 3, 1, 2, 4).reshape(n, t, s * r, d)
+
+
+def _probabilities(q, kv, key, scale):
+    """(P, q, k, v) in 64 bits, a row without keys all zero; what is masked is taken out whatever it holds."""
+    s = kv.shape[3]
+    k, v = _heads(kv[:, :, 0], s), _heads(kv[:, :, 1], s)
+    q = _heads(q, s)
+    keep = np.ones((kv.shape[0], kv.shape[1]), bool) if key is None else key != 0
+    at = keep[:, None, None, :, None]
+    k, v = np.where(at, k, 0), np.where(at, v, 0)
+    x = np.where(keep[:, None, None, None, :], q @ np.swapaxes(k, 3, 4) * scale, -np.inf)
+    m = x.max(axis=4, keepdims=True, initial=-np.inf)
+    p = np.exp(x - np.where(np.isneginf(m), 0, m))
+    z = p.sum(axis=4, keepdims=True)
+    return p / np.where(z == 0, 1, z), q, k, v
+
+
+class CrossAttentionOp(Op):
+    """``softmax(scale * q k^T) v`` of queries [N, Tq, heads, d] over an encoder's states [N, Tk, 2, shared, d], keys and values
+    of one projection; ``heads / shared`` consecutive query heads read each head of the states.  ``key_tokens`` [N, Tk]: states
+    whose token is 0 are padding and take no part, whatever they hold; a query that has none left gives 0 and no gradient.
+    ``scale`` defaults to ``d ** -0.5``.  Up to eight queries of a head of the states (single tokens) take a path of their own."""
+    name = "CrossAttention"
+
+    def __call__(self, q, kv, key_tokens=None, scale=None):
+        node = Op.__call__(self, *([q, kv] + ([key_tokens] if key_tokens is not None else [])),
+                           scale=None if scale is None else float(scale))
+        node.state = {}
+        return node
+
+    @staticmethod
+    def scale_of(node, d):
+        return node.attrs["scale"] if node.attrs["scale"] is not None else float(d) ** -0.5
+
+    def np_compute(self, node, iv):
+        p, _, _, v = _probabilities(iv[0], iv[1], iv[2] if len(iv) > 2 else None, self.scale_of(node, iv[0].shape[3]))
+        return _back(p @ v).astype(np.float32)
+
+    def gpu_compute(self, node, iv, out, stream):
+        sizes = _sizes(iv[0].shape, iv[1].shape, iv[2].shape if len(iv) > 2 else None)
+        n, tq, _, h, _, d = sizes
+        st = node.state
+        if "lse" not in st or st["lse"].shape != (n, h, tq) or st["lse"].ctx != iv[0].ctx:
+            st["lse"] = _rows((n, h, tq), iv[0].ctx)
+        G.cross_attention(iv[0], iv[1], iv[2] if len(iv) > 2 else None, out, st["lse"], sizes, self.scale_of(node, d), stream)
+
+    def gradient(self, node, g):
+        return cross_attention_gradient_op(node, g) + [None] * (len(node.inputs) - 2)
+
+    def infer_shape(self, node, s):
+        _sizes(s[0], s[1], s[2] if len(s) > 2 else None)
+        return tuple(s[0])
+
+    def flops(self, node, s, out):
+        return 4.0 * np.prod(s[0]) * s[1][1]
+
+
+def _rows(shape, ctx):
+    from .. import ndarray
+    return ndarray.empty(shape, ctx, use_pool=False)
+
+
+class CrossAttentionDotsOp(Op):
+    """``sum(g * y)`` over a head's row: [N, Tq, heads, d] -> [N, heads, Tq], what both gradients subtract from dP."""
+    name = "CrossAttentionDots"
+
+    def __call__(self, g, y):
+        return Op.__call__(self, g, y)
+
+    def np_compute(self, node, iv):
+        return (iv[0].astype(np.float64) * iv[1]).sum(3).transpose(0, 2, 1).astype(np.float32)
+
+    def gpu_compute(self, node, iv, out, stream):
+        G.cross_attention_dots(iv[0], iv[1], out, stream)
+
+    def gradient(self, node, g):
+        raise NotImplementedError
+
+    def infer_shape(self, node, s):
+        assert tuple(s[0]) == tuple(s[1]) and len(s[0]) == 4, "gradient %s of a result %s" % (tuple(s[0]), tuple(s[1]))
+        n, tq, h, _ = s[0]
+        return (n, h, tq)
+
+    def flops(self, node, s, out):
+        return 2.0 * np.prod(s[0])
+
+
+class _CrossAttentionGradient(Op):
+    def __call__(self, g, dots, forward):
+        return Op.__call__(self, g, dots, *(list(forward.inputs) + [forward]), scale=forward.attrs["scale"], fwd=forward)
+
+    @staticmethod
+    def _parts(iv):
+        """g, dots, q, kv, key tokens or None (the last input, the forward result, is there to be computed first)"""
+        return iv[0], iv[1], iv[2], iv[3], iv[4] if len(iv) > 5 else None
+
+    def _ds(self, node, iv):
+        g, dots, q, kv, key = self._parts(iv)
+        scale = CrossAttentionOp.scale_of(node, q.shape[3])
+        p, q, k, v = _probabilities(q, kv, key, scale)
+        g = _heads(g, kv.shape[3])
+        n, s, r, tq, _ = g.shape
+        ds = p * (g @ np.swapaxes(v, 3, 4) - dots.astype(np.float64).reshape(n, s, r, tq, 1)) * scale
+        return ds, p, g, q, k
+
+    def gpu_compute(self, node, iv, out, stream):
+        g, dots, q, kv, key = self._parts(iv)
+        sizes = _sizes(q.shape, kv.shape, key.shape if key is not None else None)
+        lse = node.attrs["fwd"].state.get("lse")
+        assert lse is not None and lse.shape == (sizes[0], sizes[3], sizes[1]), \
+            "the gradient of a cross attention needs its forward pass on the same device first"
+        self._launch(q, kv, key, lse, g, dots, out, sizes, CrossAttentionOp.scale_of(node, sizes[5]), stream)
+
+    def gradient(self, node, g):
+        raise NotImplementedError
+
+    def _check(self, s):
+        n, tq, tk, h, shared, d = _sizes(s[2], s[3], s[4] if len(s) > 5 else None)
+        assert tuple(s[0]) == tuple(s[2]) and tuple(s[1]) == (n, h, tq), \
+            "gradient %s of a result %s" % (tuple(s[0]), tuple(s[2]))
+
+
+class CrossAttentionGradQueryOp(_CrossAttentionGradient):
+    name = "CrossAttentionGradQuery"
+    _launch = staticmethod(G.cross_attention_grad_q)
+
+    def np_compute(self, node, iv):
+        ds, _, _, _, k = self._ds(node, iv)
+        return _back(ds @ k).astype(np.float32)
+
+    def infer_shape(self, node, s):
+        self._check(s)
+        return tuple(s[2])
+
+    def flops(self, node, s, out):
+        return 6.0 * np.prod(s[2]) * s[3][1]
+
+
+class CrossAttentionGradStatesOp(_CrossAttentionGradient):
+    name = "CrossAttentionGradStates"
+    _launch = staticmethod(G.cross_attention_grad_kv)
+
+    def np_compute(self, node, iv):
+        ds, p, g, q, _ = self._ds(node, iv)
+        dk, dv = ((np.swapaxes(a, 3, 4) @ b).sum(2, keepdims=True) for a, b in ((ds, q), (p, g)))
+        return np.stack([_back(dk), _back(dv)], 2).astype(np.float32)
+
+    def infer_shape(self, node, s):
+        self._check(s)
+        return tuple(s[3])
+
+    def flops(self, node, s, out):
+        return 8.0 * np.prod(s[2]) * s[3][1]
+
+
+_ca, _cad, _cagq, _cagkv = CrossAttentionOp(), CrossAttentionDotsOp(), CrossAttentionGradQueryOp(), CrossAttentionGradStatesOp()
+
+
+def cross_attention_op(q, kv, key_tokens=None, scale=None):
+    return _ca(q, kv, key_tokens, scale)
+
+
+def cross_attention_gradient_op(node, g):
+    """[gradient of the queries, gradient of the states] of a :func:`cross_attention_op` ``node`` whose result has ``g``."""
+    dots = _cad(g, node)
+    return [_cagq(g, dots, node), _cagkv(g, dots, node)]
