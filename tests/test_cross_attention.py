@@ -5,8 +5,11 @@ import pytest
 
 from tsplit_b200 import ndarray, gpu_ops as ad
 
-#: a pair of bf16 pieces keeps a number to 2^-18, the product of the low pieces that is left out is another 2^-18
-PIECE = 2.0 ** -18
+#: a pair of fp16 pieces keeps a number to 2^-22, the product of the low pieces that is left out is another 2^-22
+PIECE = 2.0 ** -22
+#: fp16 ends at 2^-25 (half of its last step): of a tile whose largest number is at least 2^13, of dS whose bound
+#: d (2 max|g|) (2 max|v|) + max|dot| is at least 2^14, of P whose 1 is 2^14
+TILE, LAST = 2.0 ** -38, 2.0 ** -39
 
 
 @pytest.fixture(params=[pytest.param("cpu"), pytest.param("gpu", marks=pytest.mark.gpu)])
@@ -15,7 +18,7 @@ def ctx(request):
 
 
 def definition(q, kv, key, scale, g):
-    """(y, dq, dkv) and bounds of what pieces of 2^-18 and fp32 sums may be off, element by element."""
+    """(y, dq, dkv) and bounds of what pieces of 2^-22 and fp32 sums may be off, element by element."""
     n, tq, h, d = q.shape
     tk, s = kv.shape[1], kv.shape[3]
     out = [np.zeros(a.shape) for a in (q, q, kv)]
@@ -39,17 +42,19 @@ def definition(q, kv, key, scale, g):
             # a product is off by three times PIECE of the sum of its terms' sizes (either factor, what is left out), and
             # by a truncation a step of its sum; a score's error e makes p off by a factor of e (its normaliser by no more)
             step = 3 * PIECE + d * 2.0 ** -23
+            aq, ak, av, ag = (np.abs(a).max(initial=0) for a in (qq, k, v, gg))
             e = (np.abs(qq) @ np.abs(k).T * abs(scale)) * step + 2.0 ** -22 * (4 + np.abs(x))
+            e += abs(scale) * TILE * (aq * np.abs(k).sum(1)[None, :] + ak * np.abs(qq).sum(1)[:, None])
             rel = 2 * e.max(1, keepdims=True) + len(kept) * 2.0 ** -24
-            long = 3 * PIECE + 300 * 2.0 ** -23
-            dy = rel * (p @ np.abs(v)) + long * (p @ np.abs(v))
+            long = 3 * PIECE + 100 * 2.0 ** -23                   # 24 steps a tile, and up to 80 tiles
+            dy = rel * (p @ np.abs(v)) + long * (p @ np.abs(v)) + LAST * np.abs(v).sum(0) + TILE * av
             tol[0][b, :, j] = dy
-            ddp = np.abs(gg) @ np.abs(v).T * step
+            ddp = np.abs(gg) @ np.abs(v).T * step + TILE * (ag * np.abs(v).sum(1)[None, :] + av * np.abs(gg).sum(1)[:, None])
             ddot = (np.abs(gg) * dy).sum(1, keepdims=True) + d * 2.0 ** -23 * (np.abs(gg) * np.abs(y)).sum(1, keepdims=True)
-            dds = abs(scale) * p * (ddp + ddot) + rel * np.abs(ds)
-            tol[1][b, :, j] = dds @ np.abs(k) + long * (np.abs(ds) @ np.abs(k))
-            tol[2][b, kept, 0, t] += dds.T @ np.abs(qq) + long * (np.abs(ds).T @ np.abs(qq))
-            tol[2][b, kept, 1, t] += (rel * p).T @ np.abs(gg) + long * (p.T @ np.abs(gg))
+            dds = abs(scale) * p * (ddp + ddot) + rel * np.abs(ds) + abs(scale) * LAST * (4 * d * ag * av + np.abs(dot).max(initial=0))
+            tol[1][b, :, j] = dds @ np.abs(k) + long * (np.abs(ds) @ np.abs(k)) + TILE * ak * np.abs(ds).sum(1, keepdims=True)
+            tol[2][b, kept, 0, t] += dds.T @ np.abs(qq) + long * (np.abs(ds).T @ np.abs(qq)) + TILE * aq * np.abs(ds).sum(0)[:, None]
+            tol[2][b, kept, 1, t] += (rel * p + LAST).T @ np.abs(gg) + long * (p.T @ np.abs(gg)) + TILE * ag * p.sum(0)[:, None]
     return out, tol
 
 
@@ -94,7 +99,7 @@ def check(f, ctx, scale=None, **kw):
         assert a.shape == b.shape and np.isfinite(a).all(), name
         worst = np.unravel_index(np.argmax(np.abs(a - b) - t), a.shape)
         assert np.all(np.abs(a - b) <= t + 1e-37), "%s at %s: %r for %r, tolerance %r" % (name, worst, a[worst], b[worst], t[worst])
-        assert not a[t == 0].any(), name                            # what is masked has no result and no gradient at all
+        assert not a[t == 0].any(), name                           # what is masked has no result and no gradient at all
     return got
 
 
@@ -119,6 +124,26 @@ def test_longer_attention(n, tq, tk, h, s, d, mask):
 @pytest.mark.parametrize("spread,scale", [(8.0, None), (1.0, 0.0), (1.0, -0.3), (3.0, 1.0)])
 def test_attention_scales_and_peaks(tq, spread, scale, ctx):
     check(case(2, tq, 150, 2, 1, 64, "holes", spread=spread), ctx, scale=scale)
+
+
+@pytest.mark.parametrize("tq", [1, 150])
+@pytest.mark.parametrize("sizes", [(1e-3, 1e-6, 1e-12), (1e-20, 1e18, 1e-9), (30.0, 3e5, 1e20), (1.0, 1e-30, 1e30)])
+def test_attention_of_small_and_large_numbers(tq, sizes, ctx):
+    """Queries, states and gradients far from 1: pieces of 16 bits have to be scaled."""
+    f = case(2, tq, 260, 2, 1, 64, "holes")
+    for k, v in zip(("q", "kv", "g"), sizes):
+        f[k] = f[k] * np.float32(v)
+    check(f, ctx, scale=1.0 / (8 * sizes[0] * sizes[1]))
+
+
+@pytest.mark.parametrize("tq", [1, 150])
+def test_attention_of_rows_of_unequal_size(tq, ctx):
+    """Rows whose sizes differ by up to 2^12, side by side in a tile."""
+    f = case(2, tq, 300, 4, 2, 64, "holes")
+    r = np.random.default_rng(2)
+    for k in ("q", "kv", "g"):
+        f[k] *= 2.0 ** -r.integers(0, 13, f[k].shape[:2] + (1,) * (f[k].ndim - 2)).astype(np.float32)
+    check(f, ctx)
 
 
 @pytest.mark.parametrize("tq", [1, 33])

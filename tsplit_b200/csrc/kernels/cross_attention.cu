@@ -7,17 +7,19 @@
 // A key that is out takes no part, whatever its row holds (it is not read).  A query without any key has y = 0 and no
 // gradient.  The scores never leave the chip: the backward kernels compute them again from the rows' log-sum-exp.
 //
-// Products run on tcgen05 with fp32 accuracy in mind.  An fp32 operand is split into two bf16 numbers, x = hi + lo with
-// |x - hi - lo| <= 2^-18 |x|, and a product is three: hi hi + hi lo + lo hi.  That is 1.5 times the tensor time of one TF32
-// product, which keeps 2^-11, takes the room of fp32, and bf16 tiles can be read in both directions (K-major and MN-major)
-// from one copy in shared memory.  Loader warps split what they load; P and dS are split by the threads that compute them
-// and go to tensor memory, from where they are the A operand of the next product.  Tensor-memory sums run over 256 rows at
-// most, then they are added up in registers (tcgen05 sums in fp32 but does not round to nearest).
+// Products run on tcgen05 with the accuracy of fp32.  An operand tile is scaled by a power of two that brings its largest
+// number to [2^13, 2^14) and split into two fp16 numbers, x = hi + lo, |x - hi - lo| <= 2^-22 |x| (or 2^-38 of the tile's
+// largest, where fp16 ends); a product is three: hi hi + hi lo + lo hi.  That takes 1.5 times the tensor time of one TF32
+// product, which keeps 2^-11, and the room of fp32, and 16-bit tiles can be read in both directions (K-major and MN-major)
+// from one copy in shared memory.  (Two bf16 numbers need no scale but keep 2^-17, three need six products.)  Loader
+// warps find the scale and split what they load; P and dS are split by the threads that compute them and go to tensor
+// memory, from where they are the A operand of the next product: P is at most 2^14, dS is scaled by a bound of its own.  What
+// a tile adds to y, dq, dk or dv is read from tensor memory and added in registers with the tile's scale.
 //
 // Scores are kept in units of log 2 (q is scaled by scale * log2(e) as it is loaded), so that an exponential is one ex2.
 #include <cuda_runtime.h>
 #include <cooperative_groups.h>
-#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <stdint.h>
 
 #include "launch.cuh"
@@ -44,75 +46,123 @@ struct Problem {
 };
 
 // ------------------------------------------------------------------------------------------------ pieces
-__device__ __forceinline__ uint32_t pack_bf16(float low, float high) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
-  return r;
-}
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pack_bf16(a, b);
-  lo = pack_bf16(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
+// e with |x| 2^e in [2^top, 2^(top+1)), kept where 2^e and 2^-e are normal numbers (0 and tiny x: the largest)
+__device__ __forceinline__ int exponent_to(uint32_t bits_of_abs, int top) {
+  return min(top + 127 - (int)(bits_of_abs >> 23), 126);
+}
+constexpr int TOP = 13;                      // of a tile's largest number
+constexpr float LARGEST = 16384.f;           // and what that is below, 2^(TOP+1); P is scaled by it too
 
 // A tile of ROWS x D numbers in shared memory: the plane of the hi pieces, then that of the lo pieces; a plane is D / 64
-// chunks of [ROWS][64] bf16 whose rows of 128 bytes are swizzled (16-byte unit u of row r lies at u ^ (r & 7)).
+// chunks of [ROWS][64] halves whose rows of 128 bytes are swizzled (16-byte unit u of row r lies at u ^ (r & 7)).
 template <int D, int ROWS> struct Tile {
   static constexpr int CHUNK = ROWS * 128, PLANE = ROWS * D * 2, BYTES = 2 * PLANE;
 };
 
+// What loaders share: the largest number of a tile, by warp, twice, since a tile's may still be read when the next one's
+// are written.
+struct LoaderShared {
+  uint32_t largest[2][8];
+};
+
 // Loads `rows` rows of d numbers, `stride` apart, times `mult`; zeros for the rest of the tile and for rows whose token is
-// 0.  `ready` is called between the first loads and the first store; false: give up.
+// 0.  `ready` is called between the loads and the first store; when it fails for one of the THREADS, which all call this, all
+// give up (false).  *unit: what a number in shared memory has to be multiplied by.
 template <int D, int ROWS, int THREADS, class Ready>
-__device__ __forceinline__ bool load_tile(char* tile, int t, const float* base, long long stride, int rows, const Problem& p,
-                                          const float* tokens, float mult, Ready ready) {
-  using L = Tile<D, ROWS>;
-  constexpr int UNITS = D / 8, BATCH = 4, TRIPS = ROWS * UNITS / THREADS;
-  static_assert(ROWS * UNITS % THREADS == 0 && TRIPS % BATCH == 0, "whole batches");
-#pragma unroll 1
-  for (int b = 0; b < TRIPS; b += BATCH) {
-    float v[BATCH][8];
+__device__ __forceinline__ bool load_tile(char* tile, int plane, int chunk, int t, const float* base, long long stride, int rows,
+                                          const Problem& p, const float* tokens, float mult, LoaderShared& sh, int& turn,
+                                          float* unit, Ready ready) {
+  constexpr int UNITS = D / 8, TRIPS = ROWS * UNITS / THREADS;
+  static_assert(ROWS * UNITS % THREADS == 0 && TRIPS <= 8, "a thread keeps up to 64 numbers");
+  float v[TRIPS][8];
 #pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-      const int i = t + (b + u) * THREADS, row = i / UNITS, c = i % UNITS * 8;
-      const bool in = row < rows && (!tokens || load(tokens + row) != 0.f);
-      const float* src = base + row * stride + c;
-      if (p.vec) {
-        float4 w = make_float4(0.f, 0.f, 0.f, 0.f), x = w;
-        if (in && c < p.d) w = load(reinterpret_cast<const float4*>(src));
-        if (in && c + 4 < p.d) x = load(reinterpret_cast<const float4*>(src + 4));
-        v[u][0] = w.x; v[u][1] = w.y; v[u][2] = w.z; v[u][3] = w.w;
-        v[u][4] = x.x; v[u][5] = x.y; v[u][6] = x.z; v[u][7] = x.w;
-      } else {
+  for (int u = 0; u < TRIPS; ++u) {
+    const int i = t + u * THREADS, row = i / UNITS, c = i % UNITS * 8;
+    const bool in = row < rows && (!tokens || load(tokens + row) != 0.f);
+    const float* src = base + row * stride + c;
+    if (p.vec) {
+      float4 w = make_float4(0.f, 0.f, 0.f, 0.f), x = w;
+      if (in && c < p.d) w = load(reinterpret_cast<const float4*>(src));
+      if (in && c + 4 < p.d) x = load(reinterpret_cast<const float4*>(src + 4));
+      v[u][0] = w.x; v[u][1] = w.y; v[u][2] = w.z; v[u][3] = w.w;
+      v[u][4] = x.x; v[u][5] = x.y; v[u][6] = x.z; v[u][7] = x.w;
+    } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[u][k] = in && c + k < p.d ? load(src + k) : 0.f;
-      }
+      for (int k = 0; k < 8; ++k) v[u][k] = in && c + k < p.d ? load(src + k) : 0.f;
     }
-    if (b == 0 && !ready()) return false;
+  }
+  const bool ok = ready();
+  uint32_t most = 0;
 #pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-      const int i = t + (b + u) * THREADS, row = i / UNITS, unit = i % UNITS;
-      char* to = tile + unit / 8 * L::CHUNK + row * 128 + (((unit & 7) ^ (row & 7)) << 4);
-      uint4 hi, lo;
-      split2(v[u][0] * mult, v[u][1] * mult, hi.x, lo.x);
-      split2(v[u][2] * mult, v[u][3] * mult, hi.y, lo.y);
-      split2(v[u][4] * mult, v[u][5] * mult, hi.z, lo.z);
-      split2(v[u][6] * mult, v[u][7] * mult, hi.w, lo.w);
-      *reinterpret_cast<uint4*>(to) = hi;
-      *reinterpret_cast<uint4*>(to + L::PLANE) = lo;
+  for (int u = 0; u < TRIPS; ++u)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      v[u][k] *= mult;
+      most = max(most, __float_as_uint(v[u][k]) & 0x7fffffffu);
     }
+  most = __reduce_max_sync(ALL, most);
+  uint32_t* slots = sh.largest[turn & 1];
+  ++turn;
+  if ((t & 31) == 0) slots[t >> 5] = most;
+  uint32_t failed;
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.u32 p, %1, 0;\n"
+      "barrier.cta.red.or.pred q, 1, %2, p;\n"
+      "selp.u32 %0, 1, 0, q;\n"
+      "}\n"
+      : "=r"(failed)
+      : "r"(ok ? 0u : 1u), "n"(THREADS)
+      : "memory");
+  if (failed) return false;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) most = max(most, slots[w]);
+  const int e = exponent_to(most, TOP);
+  const float scale = power_of_two(e);
+  if (t == 0) *unit = power_of_two(-e);
+#pragma unroll
+  for (int u = 0; u < TRIPS; ++u) {
+    const int i = t + u * THREADS, row = i / UNITS, at = i % UNITS;
+    char* to = tile + at / 8 * chunk + row * 128 + (((at & 7) ^ (row & 7)) << 4);
+    uint4 hi, lo;
+    split2(v[u][0] * scale, v[u][1] * scale, hi.x, lo.x);
+    split2(v[u][2] * scale, v[u][3] * scale, hi.y, lo.y);
+    split2(v[u][4] * scale, v[u][5] * scale, hi.z, lo.z);
+    split2(v[u][6] * scale, v[u][7] * scale, hi.w, lo.w);
+    *reinterpret_cast<uint4*>(to) = hi;
+    *reinterpret_cast<uint4*>(to + plane) = lo;
   }
   fence_proxy_async();
   return true;
 }
+// A tile of its own.
+template <int D, int ROWS, int THREADS, class Ready>
+__device__ __forceinline__ bool load_whole(char* tile, int t, const float* base, long long stride, int rows, const Problem& p,
+                                           const float* tokens, float mult, LoaderShared& sh, int& turn, float* unit, Ready ready) {
+  return load_tile<D, ROWS, THREADS>(tile, Tile<D, ROWS>::PLANE, Tile<D, ROWS>::CHUNK, t, base, stride, rows, p, tokens, mult, sh, turn,
+                                     unit, ready);
+}
+
+template <int R> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int R> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 
 // ------------------------------------------------------------------------------------------------ products
-__host__ __device__ constexpr uint32_t idesc_bf16(int n, int b_mn_major) {      // M = 128, D fp32, A K-major
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+__host__ __device__ constexpr uint32_t idesc_f16(int n, int b_mn_major) {      // M = 128, D fp32, A and B fp16, A K-major
+  return (1u << 4) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
 __device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -147,22 +197,22 @@ __device__ __forceinline__ void product_of_rows(uint32_t to, uint32_t a, uint32_
     const uint32_t ao = (k / 4 * LA::CHUNK + k % 4 * 32) >> 4, bo = (k / 4 * LB::CHUNK + k % 4 * 32) >> 4;
     const uint64_t ah = smem_desc_join(DESC_HI, al + ao), bh = smem_desc_join(DESC_HI, bl + bo);
     const uint64_t a2 = smem_desc_join(DESC_HI, al + ao + (LA::PLANE >> 4)), b2 = smem_desc_join(DESC_HI, bl + bo + (LB::PLANE >> 4));
-    mma_smem(to, ah, bh, idesc_bf16(ROWS_B, 0), k > 0);
-    mma_smem(to, ah, b2, idesc_bf16(ROWS_B, 0), 1);
-    mma_smem(to, a2, bh, idesc_bf16(ROWS_B, 0), 1);
+    mma_smem(to, ah, bh, idesc_f16(ROWS_B, 0), k > 0);
+    mma_smem(to, ah, b2, idesc_f16(ROWS_B, 0), 1);
+    mma_smem(to, a2, bh, idesc_f16(ROWS_B, 0), 1);
   }
 }
-// D [128 x D] (+)= A B, A [128 x ROWS] in tensor memory: 16 columns for every 16 of its, hi pieces in the first eight.
+// D [128 x D] = A B, A [128 x ROWS] in tensor memory: 16 columns for every 16 of its, hi pieces in the first eight.
 template <int D, int ROWS>
-__device__ __forceinline__ void product_with_columns(uint32_t to, uint32_t a, uint32_t b, bool accumulate) {
+__device__ __forceinline__ void product_with_columns(uint32_t to, uint32_t a, uint32_t b) {
   using L = Tile<D, ROWS>;
   const uint32_t bl = smem_desc_lo(b, L::CHUNK);
 #pragma unroll
   for (int k = 0; k < ROWS / 16; ++k) {
     const uint64_t bh = smem_desc_join(DESC_HI, bl + (k * 2048 >> 4)), b2 = smem_desc_join(DESC_HI, bl + ((k * 2048 + L::PLANE) >> 4));
-    mma_tmem(to, a + 16 * k, bh, idesc_bf16(D, 1), accumulate || k > 0);
-    mma_tmem(to, a + 16 * k, b2, idesc_bf16(D, 1), 1);
-    mma_tmem(to, a + 16 * k + 8, bh, idesc_bf16(D, 1), 1);
+    mma_tmem(to, a + 16 * k, bh, idesc_f16(D, 1), k > 0);
+    mma_tmem(to, a + 16 * k, b2, idesc_f16(D, 1), 1);
+    mma_tmem(to, a + 16 * k + 8, bh, idesc_f16(D, 1), 1);
   }
 }
 
@@ -217,9 +267,11 @@ __device__ __forceinline__ void drain(uint64_t* bar) {
   }
 }
 
+// The tiles begin at a multiple of 1024 bytes, behind the barriers.
 template <class Barriers>
 __device__ __forceinline__ char* dynamic_tiles(Barriers*& bars) {
   extern __shared__ char raw[];
+  static_assert(sizeof(Barriers) <= 1024, "one kilobyte is kept for them");
   char* at = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);
   bars = reinterpret_cast<Barriers*>(at);
   return at + 1024;
@@ -240,61 +292,66 @@ __device__ __forceinline__ void store_row(float* to, const float (&v)[COUNT], fl
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// A block takes 128 queries of a head.  Warps 0 to 3: soft-max, a row per thread; 4 to 7: loaders; 8: issues the products.
-// Two tiles of scores are in tensor memory, so S of the next tile runs while a thread works on this one; P takes the place
-// of its S.  y of a tile is added to the registers (rescaled to the new maximum there) while the next tile's P is computed.
+// A block takes 128 queries of a head and tiles of 128 keys.  Warps 0 to 3: soft-max, a row per thread; 4 to 11: loaders; 12
+// issues the products.  Two tiles of scores are in tensor memory, so S of the next tile runs while a thread works on this
+// one; P takes the place of its S.  y of a tile is added to the registers (rescaled to the new maximum there) while the next
+// tile's P is computed.
+constexpr int THREADS = 512;                 // of every block here: 128 registers a thread at first, traded below
 template <int D> struct ForwardShape {
   static constexpr int STAGES = D == 64 ? 2 : 1;
   using L = Tile<D, 128>;
   static constexpr int SMEM = 2048 + L::BYTES * (1 + 2 * STAGES);
 };
-struct ForwardBarriers {
+struct ForwardShared {
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], drained;
+  float q_unit, k_unit[4], v_unit[4];        // (the loaders may be three tiles ahead of who reads them)
+  LoaderShared loaders;
   uint32_t tmem;
 };
 
 template <int D>
-__global__ void __launch_bounds__(288, 1) attend(const Problem p) {
+__global__ void __launch_bounds__(THREADS, 1) attend(const Problem p) {
   using Shape = ForwardShape<D>;
   using L = typename Shape::L;
   constexpr int STAGES = Shape::STAGES;
-  ForwardBarriers* bar;
+  ForwardShared* bar;
   char* q_tile = dynamic_tiles(bar);
   char* k_tile = q_tile + L::BYTES;
   char* v_tile = k_tile + STAGES * L::BYTES;
   const int warp = __shfl_sync(ALL, threadIdx.x >> 5, 0);
   if (threadIdx.x == 0) {
-    mbar_init(&bar->q_full, 128);
+    mbar_init(&bar->q_full, 256);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar->k_full[i], 128);
+      mbar_init(&bar->k_full[i], 256);
       mbar_init(&bar->k_empty[i], 1);
-      mbar_init(&bar->v_full[i], 128);
+      mbar_init(&bar->v_full[i], 256);
       mbar_init(&bar->v_empty[i], 1);
-      mbar_init(&bar->s_full[i], 1);
+      mbar_init(&bar->s_full[i], 2);
       mbar_init(&bar->p_full[i], 128);
-      mbar_init(&bar->o_full[i], 1);
+      mbar_init(&bar->o_full[i], 2);
     }
     mbar_init(&bar->drained, 1);
     fence_barrier_init();
   }
-  if (warp == 8) {
+  if (warp == 12) {
     tmem_alloc(&bar->tmem, TMEM_COLUMNS);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bar->tmem;
+  const uint32_t tmem = bar->tmem;             // S 0 and 128, y 256 and 384
   tsb_launch::enter();
 
   const int qt = blockIdx.x % p.qtiles, h = blockIdx.x / p.qtiles % p.heads, n = blockIdx.x / p.qtiles / p.heads;
   const int shared = h / (p.heads / p.shared), q0 = qt * 128;
   const float* tokens = p.key ? p.key + (long long)n * p.tk : nullptr;
-  const int keys = keys_in(tokens, p.tk), tiles = (keys + 127) / 128;
+  const int tiles = (keys_in(tokens, p.tk) + 127) / 128;
   const long long kv_row = 2ll * p.shared * p.d, q_row = (long long)p.heads * p.d;
   const float* k_base = p.kv + (long long)n * p.tk * kv_row + (long long)shared * p.d;
 
   if (warp < 4) {
+    more_registers<232>();
     float acc[D], m = NEG_INF, l = 0.f, before = 1.f;
 #pragma unroll
     for (int c = 0; c < D; ++c) acc[c] = 0.f;
@@ -303,13 +360,14 @@ __global__ void __launch_bounds__(288, 1) attend(const Problem p) {
     auto add_tile = [&](int j, float factor) {
       if (!mbar_wait(&bar->o_full[j & 1], (j >> 1) & 1, p.status, 0x301)) return false;
       tc_fence_after();
+      const float unit = bar->v_unit[j & 3];
 #pragma unroll
       for (int c = 0; c < D; c += 16) {
         float o[16];
         tmem_ld16(mine + 256 + (j & 1) * 128 + c, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[c + i] = acc[c + i] * factor + o[i];
+        for (int i = 0; i < 16; ++i) acc[c + i] = acc[c + i] * factor + o[i] * unit;
       }
       return true;
     };
@@ -320,16 +378,23 @@ __global__ void __launch_bounds__(288, 1) attend(const Problem p) {
       if (!mbar_wait(&bar->s_full[j & 1], (j >> 1) & 1, p.status, 0x302)) { ok = false; break; }
       tc_fence_after();
       const uint32_t at = mine + (j & 1) * 128;
-      float top = m;
+      const float unit = bar->q_unit * bar->k_unit[j & 3];
+      float most = NEG_INF;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         float s[32];
         tmem_ld_32x32(at + 32 * w, s);
         tmem_ld_wait();
+        if (in[w] == ALL) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) top = fmaxf(top, (in[w] >> i) & 1 ? s[i] : NEG_INF);
+          for (int i = 0; i < 32; ++i) most = fmaxf(most, s[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) most = fmaxf(most, (in[w] >> i) & 1 ? s[i] : NEG_INF);
+        }
       }
-      const float ref = top == NEG_INF ? 0.f : top, factor = exp2_fast(m - ref);
+      const float top = fmaxf(m, most == NEG_INF ? NEG_INF : most * unit), ref = top == NEG_INF ? 0.f : top;
+      const float factor = exp2_fast(m - ref), shift = TOP + 1 - ref;
       float sum = 0.f;
 #pragma unroll
       for (int w = 0; w < 8; ++w) {
@@ -339,7 +404,8 @@ __global__ void __launch_bounds__(288, 1) attend(const Problem p) {
         const unsigned mask = in[w / 2] >> (w % 2 * 16);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          s[i] = (mask >> i) & 1 ? exp2_fast(s[i] - ref) : 0.f;
+          s[i] = exp2_fast(s[i] * unit + shift);
+          if (in[w / 2] != ALL) s[i] = (mask >> i) & 1 ? s[i] : 0.f;
           sum += s[i];
         }
         tmem_st_pieces(at + 16 * w, s);
@@ -357,58 +423,66 @@ __global__ void __launch_bounds__(288, 1) attend(const Problem p) {
     if (ok && t < p.tq) {
       store_row(p.y + ((long long)n * p.tq + t) * q_row + (long long)h * p.d, acc, l > 0.f ? 1.f / l : 0.f, p.d, p.vec);
       // (a row without keys: exp2(S - inf) = 0 in the backward pass)
-      p.lse[((long long)n * p.heads + h) * p.tq + t] = l > 0.f ? m + log2f(l) : -NEG_INF;
+      p.lse[((long long)n * p.heads + h) * p.tq + t] = l > 0.f ? m - (TOP + 1) + log2f(l) : -NEG_INF;
     }
-  } else if (warp < 8) {
+  } else if (warp < 12) {
+    fewer_registers<104>();
     const int t = threadIdx.x - 128;
+    int turn = 0;
     if (tiles > 0) {
-      load_tile<D, 128, 128>(q_tile, t, p.q + ((long long)n * p.tq + q0) * q_row + (long long)h * p.d, q_row, p.tq - q0, p,
-                             nullptr, p.scale * LOG2E, [] { return true; });
+      load_whole<D, 128, 256>(q_tile, t, p.q + ((long long)n * p.tq + q0) * q_row + (long long)h * p.d, q_row, p.tq - q0, p, nullptr,
+                              p.scale * LOG2E, bar->loaders, turn, &bar->q_unit, [] { return true; });
       mbar_arrive(&bar->q_full);
     }
     for (int j = 0; j < tiles; ++j) {
       const int s = j % STAGES, ph = j / STAGES & 1;
       const float* base = k_base + (long long)j * 128 * kv_row;
       const float* tok = tokens ? tokens + j * 128 : nullptr;
-      if (!load_tile<D, 128, 128>(k_tile + s * L::BYTES, t, base, kv_row, p.tk - j * 128, p, tok, 1.f,
-                                  [&] { return mbar_wait(&bar->k_empty[s], ph ^ 1, p.status, 0x303); }))
+      if (!load_whole<D, 128, 256>(k_tile + s * L::BYTES, t, base, kv_row, p.tk - j * 128, p, tok, 1.f, bar->loaders, turn,
+                                   &bar->k_unit[j & 3], [&] { return mbar_wait(&bar->k_empty[s], ph ^ 1, p.status, 0x303); }))
         break;
       mbar_arrive(&bar->k_full[s]);
-      if (!load_tile<D, 128, 128>(v_tile + s * L::BYTES, t, base + (long long)p.shared * p.d, kv_row, p.tk - j * 128, p, tok, 1.f,
-                                  [&] { return mbar_wait(&bar->v_empty[s], ph ^ 1, p.status, 0x304); }))
+      if (!load_whole<D, 128, 256>(v_tile + s * L::BYTES, t, base + (long long)p.shared * p.d, kv_row, p.tk - j * 128, p, tok, 1.f,
+                                   bar->loaders, turn, &bar->v_unit[j & 3],
+                                   [&] { return mbar_wait(&bar->v_empty[s], ph ^ 1, p.status, 0x304); }))
         break;
       mbar_arrive(&bar->v_full[s]);
     }
-  } else if (elect_one()) {
-    const uint32_t qa = smem_u32(q_tile), ka = smem_u32(k_tile), va = smem_u32(v_tile);
-    bool ok = tiles == 0 || mbar_wait(&bar->q_full, 0, p.status, 0x305);
-    auto scores = [&](int j) {
-      const int s = j % STAGES;
-      if (!mbar_wait(&bar->k_full[s], j / STAGES & 1, p.status, 0x306)) return false;
-      tc_fence_after();
-      product_of_rows<D, 128, 128>(tmem + (j & 1) * 128, qa, ka + s * L::BYTES);
-      umma_commit(&bar->s_full[j & 1]);
-      umma_commit(&bar->k_empty[s]);
-      return true;
-    };
-    for (int j = 0; j < 2 && j < tiles && ok; ++j) ok = scores(j);
-    for (int j = 0; j < tiles && ok; ++j) {
-      const int s = j % STAGES;
-      if (!(ok = mbar_wait(&bar->v_full[s], j / STAGES & 1, p.status, 0x307))) break;
-      if (!(ok = mbar_wait(&bar->p_full[j & 1], (j >> 1) & 1, p.status, 0x308))) break;
-      tc_fence_after();
-      product_with_columns<D, 128>(tmem + 256 + (j & 1) * 128, tmem + (j & 1) * 128, va + s * L::BYTES, false);
-      umma_commit(&bar->o_full[j & 1]);
-      umma_commit(&bar->v_empty[s]);
-      if (j + 2 < tiles) ok = scores(j + 2);
+  } else {
+    fewer_registers<72>();
+    if (warp == 12 && elect_one()) {
+      const uint32_t qa = smem_u32(q_tile), ka = smem_u32(k_tile), va = smem_u32(v_tile);
+      bool ok = tiles == 0 || mbar_wait(&bar->q_full, 0, p.status, 0x305);
+      auto scores = [&](int j) {
+        const int s = j % STAGES;
+        if (!mbar_wait(&bar->k_full[s], j / STAGES & 1, p.status, 0x306)) return false;
+        tc_fence_after();
+        product_of_rows<D, 128, 128>(tmem + (j & 1) * 128, qa, ka + s * L::BYTES);
+        umma_commit(&bar->s_full[j & 1]);
+        mbar_arrive(&bar->s_full[j & 1]);      // (what the loaders wrote is seen through this one)
+        umma_commit(&bar->k_empty[s]);
+        return true;
+      };
+      for (int j = 0; j < 2 && j < tiles && ok; ++j) ok = scores(j);
+      for (int j = 0; j < tiles && ok; ++j) {
+        const int s = j % STAGES;
+        if (!(ok = mbar_wait(&bar->v_full[s], j / STAGES & 1, p.status, 0x307))) break;
+        if (!(ok = mbar_wait(&bar->p_full[j & 1], (j >> 1) & 1, p.status, 0x308))) break;
+        tc_fence_after();
+        product_with_columns<D, 128>(tmem + 256 + (j & 1) * 128, tmem + (j & 1) * 128, va + s * L::BYTES);
+        umma_commit(&bar->o_full[j & 1]);
+        mbar_arrive(&bar->o_full[j & 1]);
+        umma_commit(&bar->v_empty[s]);
+        if (j + 2 < tiles) ok = scores(j + 2);
+      }
+      if (!ok) drain(&bar->drained);
     }
-    if (!ok) drain(&bar->drained);
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tmem, TMEM_COLUMNS);
+  if (warp == 12) tmem_dealloc(tmem, TMEM_COLUMNS);
 }
 
 // ------------------------------------------------------------------------------------------------ gradients
@@ -439,48 +513,55 @@ __global__ void __launch_bounds__(256) row_dots(const float* g, const float* y, 
   }
 }
 
-// dq: a block takes 128 queries of a head, tiles of 64 keys; the same roles.  dS takes the place of its S; dq of four
-// tiles is summed in tensor memory.
+// A bound of |dP - dot| over a tile: e with (d |g| |v| + |dot|) 2^e below 2^15 (units: what 2^14 of a tile stands for).
+__device__ __forceinline__ int exponent_of_ds(int d, float g_unit, float v_unit, float dot) {
+  const float most = (float)d * (LARGEST * g_unit) * (LARGEST * v_unit) + fabsf(dot);
+  return exponent_to(__float_as_uint(most), TOP + 1);
+}
+
+// dq: a block takes 128 queries of a head and tiles of 64 keys; the same roles.  dS takes the place of its S.
 template <int D> struct QueryShape {
-  static constexpr int K_STAGES = D == 64 ? 3 : 2, V_STAGES = D == 64 ? 3 : 1, GROUP = 4;
+  static constexpr int K_STAGES = D == 64 ? 3 : 2, V_STAGES = D == 64 ? 3 : 1;
   using LQ = Tile<D, 128>;
   using LK = Tile<D, 64>;
   static constexpr int SMEM = 2048 + 2 * LQ::BYTES + (K_STAGES + V_STAGES) * LK::BYTES;
 };
-struct QueryBarriers {
+struct QueryShared {
   uint64_t q_full, k_full[3], k_empty[3], v_full[3], v_empty[3], s_full[2], ds_full[2], dq_full[2], drained;
+  float q_unit, g_unit, k_unit[8], v_unit[8];  // (the loaders may be four tiles ahead of who reads them)
+  LoaderShared loaders;
   uint32_t tmem;
 };
 
 template <int D>
-__global__ void __launch_bounds__(288, 1) grad_of_queries(const Problem p) {
+__global__ void __launch_bounds__(THREADS, 1) grad_of_queries(const Problem p) {
   using Shape = QueryShape<D>;
   using LQ = typename Shape::LQ;
   using LK = typename Shape::LK;
-  constexpr int KS = Shape::K_STAGES, VS = Shape::V_STAGES, GROUP = Shape::GROUP;
-  QueryBarriers* bar;
+  constexpr int KS = Shape::K_STAGES, VS = Shape::V_STAGES;
+  QueryShared* bar;
   char* q_tile = dynamic_tiles(bar);
   char* g_tile = q_tile + LQ::BYTES;
   char* k_tile = g_tile + LQ::BYTES;
   char* v_tile = k_tile + KS * LK::BYTES;
   const int warp = __shfl_sync(ALL, threadIdx.x >> 5, 0);
   if (threadIdx.x == 0) {
-    mbar_init(&bar->q_full, 128);
+    mbar_init(&bar->q_full, 256);
     for (int i = 0; i < 3; ++i) {
-      mbar_init(&bar->k_full[i], 128);
+      mbar_init(&bar->k_full[i], 256);
       mbar_init(&bar->k_empty[i], 1);
-      mbar_init(&bar->v_full[i], 128);
+      mbar_init(&bar->v_full[i], 256);
       mbar_init(&bar->v_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar->s_full[i], 1);
+      mbar_init(&bar->s_full[i], 2);
       mbar_init(&bar->ds_full[i], 128);
       mbar_init(&bar->dq_full[i], 1);
     }
     mbar_init(&bar->drained, 1);
     fence_barrier_init();
   }
-  if (warp == 8) {
+  if (warp == 12) {
     tmem_alloc(&bar->tmem, TMEM_COLUMNS);
     tmem_relinquish();
   }
@@ -499,7 +580,8 @@ __global__ void __launch_bounds__(288, 1) grad_of_queries(const Problem p) {
   const long long q_at = ((long long)n * p.tq + q0) * q_row + (long long)h * p.d;
 
   if (warp < 4) {
-    float acc[D];
+    more_registers<232>();
+    float acc[D], before = 0.f;
 #pragma unroll
     for (int c = 0; c < D; ++c) acc[c] = 0.f;
     const uint32_t mine = tmem + ((uint32_t)warp << 21);
@@ -507,16 +589,16 @@ __global__ void __launch_bounds__(288, 1) grad_of_queries(const Problem p) {
     const long long at_row = ((long long)n * p.heads + h) * p.tq + t;
     const float lse = t < p.tq ? load(p.lse + at_row) : -NEG_INF, dot = t < p.tq ? load(p.dot + at_row) : 0.f;
     bool ok = true;
-    auto add_group = [&](int k) {
-      if (!mbar_wait(&bar->dq_full[k & 1], (k >> 1) & 1, p.status, 0x311)) return false;
+    auto add_tile = [&](int j, float unit) {
+      if (!mbar_wait(&bar->dq_full[j & 1], (j >> 1) & 1, p.status, 0x311)) return false;
       tc_fence_after();
 #pragma unroll
       for (int c = 0; c < D; c += 16) {
         float o[16];
-        tmem_ld16(mine + 256 + (k & 1) * 128 + c, o);
+        tmem_ld16(mine + 256 + (j & 1) * 128 + c, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[c + i] += o[i];
+        for (int i = 0; i < 16; ++i) acc[c + i] += o[i] * unit;
       }
       return true;
     };
@@ -525,6 +607,9 @@ __global__ void __launch_bounds__(288, 1) grad_of_queries(const Problem p) {
       if (!mbar_wait(&bar->s_full[j & 1], (j >> 1) & 1, p.status, 0x312)) { ok = false; break; }
       tc_fence_after();
       const uint32_t at = mine + (j & 1) * 64;
+      const float k_unit = bar->k_unit[j & 7], v_unit = bar->v_unit[j & 7], g_unit = bar->g_unit;
+      const int e = exponent_of_ds(p.d, g_unit, v_unit, dot);
+      const float s_unit = bar->q_unit * k_unit, dp_unit = g_unit * v_unit, shift = (float)e - lse;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         float s[16], dp[16];
@@ -533,106 +618,117 @@ __global__ void __launch_bounds__(288, 1) grad_of_queries(const Problem p) {
         tmem_ld_wait();
         const unsigned mask = in[w / 2] >> (w % 2 * 16);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = (mask >> i) & 1 ? exp2_fast(s[i] - lse) * (dp[i] - dot) : 0.f;
+        for (int i = 0; i < 16; ++i) {
+          s[i] = exp2_fast(s[i] * s_unit + shift) * (dp[i] * dp_unit - dot);
+          if (in[w / 2] != ALL) s[i] = (mask >> i) & 1 ? s[i] : 0.f;
+        }
         tmem_st_pieces(at + 16 * w, s);
       }
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&bar->ds_full[j & 1]);
-      if (j && j % GROUP == 0 && !(ok = add_group(j / GROUP - 1))) break;
+      if (j > 0 && !(ok = add_tile(j - 1, before))) break;
+      before = k_unit * power_of_two(-e);
     }
-    if (ok && tiles > 0) ok = add_group((tiles - 1) / GROUP);
+    if (ok && tiles > 0) ok = add_tile(tiles - 1, before);
     if (ok && t < p.tq) store_row(p.dq + q_at + (long long)threadIdx.x * q_row, acc, p.scale, p.d, p.vec);
-  } else if (warp < 8) {
+  } else if (warp < 12) {
+    fewer_registers<104>();
     const int t = threadIdx.x - 128;
+    int turn = 0;
     if (tiles > 0) {
-      load_tile<D, 128, 128>(q_tile, t, p.q + q_at, q_row, p.tq - q0, p, nullptr, p.scale * LOG2E, [] { return true; });
-      load_tile<D, 128, 128>(g_tile, t, p.g + q_at, q_row, p.tq - q0, p, nullptr, 1.f, [] { return true; });
+      load_whole<D, 128, 256>(q_tile, t, p.q + q_at, q_row, p.tq - q0, p, nullptr, p.scale * LOG2E, bar->loaders, turn, &bar->q_unit,
+                              [] { return true; });
+      load_whole<D, 128, 256>(g_tile, t, p.g + q_at, q_row, p.tq - q0, p, nullptr, 1.f, bar->loaders, turn, &bar->g_unit,
+                              [] { return true; });
       mbar_arrive(&bar->q_full);
     }
     for (int j = 0; j < tiles; ++j) {
       const int ks = j % KS, vs = j % VS;
       const float* base = k_base + (long long)j * 64 * kv_row;
       const float* tok = tokens ? tokens + j * 64 : nullptr;
-      if (!load_tile<D, 64, 128>(k_tile + ks * LK::BYTES, t, base, kv_row, p.tk - j * 64, p, tok, 1.f,
-                                 [&] { return mbar_wait(&bar->k_empty[ks], (j / KS & 1) ^ 1, p.status, 0x313); }))
+      if (!load_whole<D, 64, 256>(k_tile + ks * LK::BYTES, t, base, kv_row, p.tk - j * 64, p, tok, 1.f, bar->loaders, turn,
+                                  &bar->k_unit[j & 7], [&] { return mbar_wait(&bar->k_empty[ks], (j / KS & 1) ^ 1, p.status, 0x313); }))
         break;
       mbar_arrive(&bar->k_full[ks]);
-      if (!load_tile<D, 64, 128>(v_tile + vs * LK::BYTES, t, base + (long long)p.shared * p.d, kv_row, p.tk - j * 64, p, tok, 1.f,
-                                 [&] { return mbar_wait(&bar->v_empty[vs], (j / VS & 1) ^ 1, p.status, 0x314); }))
+      if (!load_whole<D, 64, 256>(v_tile + vs * LK::BYTES, t, base + (long long)p.shared * p.d, kv_row, p.tk - j * 64, p, tok, 1.f,
+                                  bar->loaders, turn, &bar->v_unit[j & 7],
+                                  [&] { return mbar_wait(&bar->v_empty[vs], (j / VS & 1) ^ 1, p.status, 0x314); }))
         break;
       mbar_arrive(&bar->v_full[vs]);
     }
-  } else if (elect_one()) {
-    const uint32_t qa = smem_u32(q_tile), ga = smem_u32(g_tile), ka = smem_u32(k_tile), va = smem_u32(v_tile);
-    bool ok = tiles == 0 || mbar_wait(&bar->q_full, 0, p.status, 0x315);
-    auto scores = [&](int j) {
-      const int ks = j % KS, vs = j % VS;
-      if (!mbar_wait(&bar->k_full[ks], j / KS & 1, p.status, 0x316)) return false;
-      tc_fence_after();
-      product_of_rows<D, 128, 64>(tmem + (j & 1) * 64, qa, ka + ks * LK::BYTES);
-      if (!mbar_wait(&bar->v_full[vs], j / VS & 1, p.status, 0x317)) return false;
-      tc_fence_after();
-      product_of_rows<D, 128, 64>(tmem + 128 + (j & 1) * 64, ga, va + vs * LK::BYTES);
-      umma_commit(&bar->s_full[j & 1]);
-      umma_commit(&bar->v_empty[vs]);
-      return true;
-    };
-    // (with two stages of keys, the third tile of scores waits for the first one's dq anyway)
-    for (int j = 0; j < 2 && j < tiles && ok; ++j) ok = scores(j);
-    for (int j = 0; j < tiles && ok; ++j) {
-      if (!(ok = mbar_wait(&bar->ds_full[j & 1], (j >> 1) & 1, p.status, 0x318))) break;
-      tc_fence_after();
-      const int k = j / GROUP;
-      product_with_columns<D, 64>(tmem + 256 + (k & 1) * 128, tmem + (j & 1) * 64, ka + j % KS * LK::BYTES, j % GROUP != 0);
-      umma_commit(&bar->k_empty[j % KS]);
-      if (j % GROUP == GROUP - 1 || j == tiles - 1) umma_commit(&bar->dq_full[k & 1]);
-      if (j + 2 < tiles) ok = scores(j + 2);
+  } else {
+    fewer_registers<72>();
+    if (warp == 12 && elect_one()) {
+      const uint32_t qa = smem_u32(q_tile), ga = smem_u32(g_tile), ka = smem_u32(k_tile), va = smem_u32(v_tile);
+      bool ok = tiles == 0 || mbar_wait(&bar->q_full, 0, p.status, 0x315);
+      auto scores = [&](int j) {
+        const int ks = j % KS, vs = j % VS;
+        if (!mbar_wait(&bar->k_full[ks], j / KS & 1, p.status, 0x316)) return false;
+        tc_fence_after();
+        product_of_rows<D, 128, 64>(tmem + (j & 1) * 64, qa, ka + ks * LK::BYTES);
+        if (!mbar_wait(&bar->v_full[vs], j / VS & 1, p.status, 0x317)) return false;
+        tc_fence_after();
+        product_of_rows<D, 128, 64>(tmem + 128 + (j & 1) * 64, ga, va + vs * LK::BYTES);
+        umma_commit(&bar->s_full[j & 1]);
+        mbar_arrive(&bar->s_full[j & 1]);      // (what the loaders wrote is seen through this one)
+        umma_commit(&bar->v_empty[vs]);
+        return true;
+      };
+      for (int j = 0; j < 2 && j < tiles && ok; ++j) ok = scores(j);
+      for (int j = 0; j < tiles && ok; ++j) {
+        if (!(ok = mbar_wait(&bar->ds_full[j & 1], (j >> 1) & 1, p.status, 0x318))) break;
+        tc_fence_after();
+        product_with_columns<D, 64>(tmem + 256 + (j & 1) * 128, tmem + (j & 1) * 64, ka + j % KS * LK::BYTES);
+        umma_commit(&bar->k_empty[j % KS]);
+        umma_commit(&bar->dq_full[j & 1]);
+        if (j + 2 < tiles) ok = scores(j + 2);
+      }
+      if (!ok) drain(&bar->drained);
     }
-    if (!ok) drain(&bar->drained);
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tmem, TMEM_COLUMNS);
+  if (warp == 12) tmem_dealloc(tmem, TMEM_COLUMNS);
 }
 
-// dk and dv: a block takes 128 keys of a shared head, tiles of 64 queries of every head that reads it.  S^T and dP^T have
+// dk and dv: a block takes 128 keys of a shared head and tiles of 64 queries of every head that reads it.  S^T and dP^T have
 // the keys as rows, so P^T and dS^T are A operands as they lie.  Warps 0 to 3 take the first 32 queries of a tile and add up
-// dv, 4 to 7 the others and dk; 8 and 9 load; 10 issues.
+// dv, 4 to 7 the others and dk; 8 to 11 load; 12 issues.  Tiles of queries and of gradients share a ring of slots: q, g, q, g.
 template <int D> struct StateShape {
-  static constexpr int STAGES = D == 64 ? 3 : 1, GROUP = 4;
+  static constexpr int SLOTS = D == 64 ? 6 : 3;
   using LK = Tile<D, 128>;
   using LQ = Tile<D, 64>;
-  static constexpr int SMEM = 2048 + 2 * LK::BYTES + 2 * STAGES * LQ::BYTES;
+  static constexpr int SMEM = 2048 + 2 * LK::BYTES + SLOTS * LQ::BYTES;
 };
-struct StateBarriers {
-  uint64_t k_full, q_full[3], q_empty[3], s_full[2], ds_full[2], sum_full, sum_empty, drained;
+struct StateShared {
+  uint64_t k_full, full[6], empty[6], s_full[2], ds_full[2], sum_full, sum_empty, drained;
+  float k_unit[2], v_unit[2], unit[6];         // (two of the keys' and values': a thread of the loaders keeps 64 numbers)
+  LoaderShared loaders;
   uint32_t tmem;
 };
 
 template <int D>
-__global__ void __launch_bounds__(352, 1) grad_of_states(const Problem p) {
+__global__ void __launch_bounds__(THREADS, 1) grad_of_states(const Problem p) {
   using Shape = StateShape<D>;
   using LQ = typename Shape::LQ;
   using LK = typename Shape::LK;
-  constexpr int STAGES = Shape::STAGES, GROUP = Shape::GROUP;
-  StateBarriers* bar;
+  constexpr int SLOTS = Shape::SLOTS, PART = 128 * 64 / D;                     // rows of a part of the keys' tile
+  StateShared* bar;
   char* k_tile = dynamic_tiles(bar);
   char* v_tile = k_tile + LK::BYTES;
-  char* q_tile = v_tile + LK::BYTES;
-  char* g_tile = q_tile + STAGES * LQ::BYTES;
-  __shared__ float2 rows[8][64];               // {lse, dot} of a tile's queries, a copy for each warp
+  char* ring = v_tile + LK::BYTES;
   const int warp = __shfl_sync(ALL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(&bar->k_full, 64);
-    for (int i = 0; i < 3; ++i) {
-      mbar_init(&bar->q_full[i], 64);
-      mbar_init(&bar->q_empty[i], 1);
+    mbar_init(&bar->k_full, 128);
+    for (int i = 0; i < 6; ++i) {
+      mbar_init(&bar->full[i], 128);
+      mbar_init(&bar->empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar->s_full[i], 1);
+      mbar_init(&bar->s_full[i], 2);
       mbar_init(&bar->ds_full[i], 256);
     }
     mbar_init(&bar->sum_full, 1);
@@ -640,7 +736,7 @@ __global__ void __launch_bounds__(352, 1) grad_of_states(const Problem p) {
     mbar_init(&bar->drained, 1);
     fence_barrier_init();
   }
-  if (warp == 10) {
+  if (warp == 12) {
     tmem_alloc(&bar->tmem, TMEM_COLUMNS);
     tmem_relinquish();
   }
@@ -659,22 +755,44 @@ __global__ void __launch_bounds__(352, 1) grad_of_states(const Problem p) {
   const int tiles = __syncthreads_or(mine_in) ? p.qtiles * per : 0;
 
   if (warp < 8) {
+    more_registers<184>();
     float acc[D];
 #pragma unroll
     for (int c = 0; c < D; ++c) acc[c] = 0.f;
     const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);
     const int half = warp >> 2, row = threadIdx.x & 127;
+    float before = 0.f;
     bool ok = true;
+    auto add_tile = [&](int j, float unit) {
+      if (!mbar_wait(&bar->sum_full, j & 1, p.status, 0x322)) return false;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < D; c += 16) {
+        float o[16];
+        tmem_ld16(mine + 256 + half * 128 + c, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[c + i] += o[i] * unit;
+      }
+      tc_fence_before();
+      mbar_arrive(&bar->sum_empty);
+      return true;
+    };
     for (int j = 0; j < tiles; ++j) {
-      const int h = shared * per + j / p.qtiles, t0 = j % p.qtiles * 64 + half * 32;
-      const long long at_row = ((long long)n * p.heads + h) * p.tq + t0 + lane;
-      const bool there = t0 + lane < p.tq;
-      __syncwarp();
-      rows[warp][lane] = make_float2(there ? load(p.lse + at_row) : -NEG_INF, there ? load(p.dot + at_row) : 0.f);
-      __syncwarp();
+      // a lane has the log-sum-exp and the dot of one of this half's queries, and the other half's dot for the bound
+      const int h = shared * per + j / p.qtiles, t0 = j % p.qtiles * 64, t = t0 + half * 32 + lane, other = t0 + (half ^ 1) * 32 + lane;
+      const long long at_head = ((long long)n * p.heads + h) * p.tq;
+      const float lse = t < p.tq ? load(p.lse + at_head + t) : -NEG_INF, dot = t < p.tq ? load(p.dot + at_head + t) : 0.f;
+      const float dot2 = other < p.tq ? load(p.dot + at_head + other) : 0.f;
+      const float most = __uint_as_float(__reduce_max_sync(ALL, max(__float_as_uint(fabsf(dot)), __float_as_uint(fabsf(dot2)))));
       if (!mbar_wait(&bar->s_full[j & 1], (j >> 1) & 1, p.status, 0x321)) { ok = false; break; }
       tc_fence_after();
       const uint32_t at = mine + (j & 1) * 64 + half * 32;
+      const float k_unit = bar->k_unit[row / PART], v_unit = bar->v_unit[row / PART];
+      const float q_unit = bar->unit[2 * j % SLOTS], g_unit = bar->unit[(2 * j + 1) % SLOTS];
+      const int e = exponent_of_ds(p.d, g_unit, v_unit, most);
+      // p = 2^14 P, then dS = p (dP - dot) 2^(e - 14)
+      const float s_unit = q_unit * k_unit, f = power_of_two(max(e - TOP - 1, -126)), dp_unit = g_unit * v_unit * f;
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         float s[16], dp[16];
@@ -683,9 +801,8 @@ __global__ void __launch_bounds__(352, 1) grad_of_states(const Problem p) {
         tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float2 r = rows[warp][16 * w + i];
-          s[i] = exp2_fast(s[i] - r.x);
-          dp[i] = s[i] * (dp[i] - r.y);
+          s[i] = exp2_fast(s[i] * s_unit + (TOP + 1 - __shfl_sync(ALL, lse, 16 * w + i)));
+          dp[i] = s[i] * (dp[i] * dp_unit - __shfl_sync(ALL, dot, 16 * w + i) * f);
         }
         tmem_st_pieces(at + 16 * w, s);
         tmem_st_pieces(at + 128 + 16 * w, dp);
@@ -693,21 +810,10 @@ __global__ void __launch_bounds__(352, 1) grad_of_states(const Problem p) {
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&bar->ds_full[j & 1]);
-      if (j % GROUP == GROUP - 1 || j == tiles - 1) {
-        if (!mbar_wait(&bar->sum_full, j / GROUP & 1, p.status, 0x322)) { ok = false; break; }
-        tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < D; c += 16) {
-          float o[16];
-          tmem_ld16(mine + 256 + half * 128 + c, o);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[c + i] += o[i];
-        }
-        tc_fence_before();
-        mbar_arrive(&bar->sum_empty);
-      }
+      if (j > 0 && !(ok = add_tile(j - 1, before))) break;
+      before = half ? q_unit * power_of_two(-e) : g_unit * (1.f / LARGEST);
     }
+    if (ok && tiles > 0) ok = add_tile(tiles - 1, before);
     if (ok && k0 + row < p.tk) {
       const bool in = !tokens || load(tokens + k0 + row) != 0.f;
       float* to = p.dkv + k_at + row * kv_row + (half ? 0 : (long long)p.shared * p.d);
@@ -716,55 +822,75 @@ __global__ void __launch_bounds__(352, 1) grad_of_states(const Problem p) {
         for (int c = 0; c < D; ++c) acc[c] = 0.f;
       store_row(to, acc, half ? LN2 : 1.f, p.d, p.vec);          // (q was loaded times scale * log2(e))
     }
-  } else if (warp < 10) {
+  } else if (warp < 12) {
+    fewer_registers<104>();
     const int t = threadIdx.x - 256;
+    int turn = 0;
     if (tiles > 0) {
-      const float* tok = tokens ? tokens + k0 : nullptr;
-      load_tile<D, 128, 64>(k_tile, t, p.kv + k_at, kv_row, p.tk - k0, p, tok, 1.f, [] { return true; });
-      load_tile<D, 128, 64>(v_tile, t, p.kv + k_at + (long long)p.shared * p.d, kv_row, p.tk - k0, p, tok, 1.f, [] { return true; });
+      for (int part = 0; part < 128 / PART; ++part) {
+        const float* tok = tokens ? tokens + k0 + part * PART : nullptr;
+        const float* base = p.kv + k_at + part * PART * kv_row;
+        load_tile<D, PART, 128>(k_tile + part * PART * 128, LK::PLANE, LK::CHUNK, t, base, kv_row, p.tk - k0 - part * PART, p, tok, 1.f,
+                                bar->loaders, turn, &bar->k_unit[part], [] { return true; });
+        load_tile<D, PART, 128>(v_tile + part * PART * 128, LK::PLANE, LK::CHUNK, t, base + (long long)p.shared * p.d, kv_row,
+                                p.tk - k0 - part * PART, p, tok, 1.f, bar->loaders, turn, &bar->v_unit[part], [] { return true; });
+      }
       mbar_arrive(&bar->k_full);
     }
-    for (int j = 0; j < tiles; ++j) {
-      const int s = j % STAGES, h = shared * per + j / p.qtiles, t0 = j % p.qtiles * 64;
+    for (int i = 0; i < 2 * tiles; ++i) {
+      const int s = i % SLOTS, j = i / 2, h = shared * per + j / p.qtiles, t0 = j % p.qtiles * 64;
       const long long at = ((long long)n * p.tq + t0) * q_row + (long long)h * p.d;
-      if (!load_tile<D, 64, 64>(q_tile + s * LQ::BYTES, t, p.q + at, q_row, p.tq - t0, p, nullptr, p.scale * LOG2E,
-                                [&] { return mbar_wait(&bar->q_empty[s], (j / STAGES & 1) ^ 1, p.status, 0x323); }))
+      if (!load_whole<D, 64, 128>(ring + s * LQ::BYTES, t, (i & 1 ? p.g : p.q) + at, q_row, p.tq - t0, p, nullptr,
+                                  i & 1 ? 1.f : p.scale * LOG2E, bar->loaders, turn, &bar->unit[s],
+                                  [&] { return mbar_wait(&bar->empty[s], (i / SLOTS & 1) ^ 1, p.status, 0x323); }))
         break;
-      if (!load_tile<D, 64, 64>(g_tile + s * LQ::BYTES, t, p.g + at, q_row, p.tq - t0, p, nullptr, 1.f, [] { return true; })) break;
-      mbar_arrive(&bar->q_full[s]);
+      mbar_arrive(&bar->full[s]);
     }
-  } else if (elect_one()) {
-    const uint32_t qa = smem_u32(q_tile), ga = smem_u32(g_tile), ka = smem_u32(k_tile), va = smem_u32(v_tile);
-    bool ok = tiles == 0 || mbar_wait(&bar->k_full, 0, p.status, 0x324);
-    constexpr int AHEAD = STAGES > 1 ? 2 : 1;
-    auto scores = [&](int j) {
-      const int s = j % STAGES;
-      if (!mbar_wait(&bar->q_full[s], j / STAGES & 1, p.status, 0x325)) return false;
-      tc_fence_after();
-      product_of_rows<D, 128, 64>(tmem + (j & 1) * 64, ka, qa + s * LQ::BYTES);
-      product_of_rows<D, 128, 64>(tmem + 128 + (j & 1) * 64, va, ga + s * LQ::BYTES);
-      umma_commit(&bar->s_full[j & 1]);
-      return true;
-    };
-    for (int j = 0; j < AHEAD && j < tiles && ok; ++j) ok = scores(j);
-    for (int j = 0; j < tiles && ok; ++j) {
-      const int s = j % STAGES;
-      if (!(ok = mbar_wait(&bar->ds_full[j & 1], (j >> 1) & 1, p.status, 0x326))) break;
-      if (j && j % GROUP == 0 && !(ok = mbar_wait(&bar->sum_empty, (j / GROUP - 1) & 1, p.status, 0x327))) break;
-      tc_fence_after();
-      product_with_columns<D, 64>(tmem + 256, tmem + (j & 1) * 64, ga + s * LQ::BYTES, j % GROUP != 0);
-      product_with_columns<D, 64>(tmem + 384, tmem + 128 + (j & 1) * 64, qa + s * LQ::BYTES, j % GROUP != 0);
-      umma_commit(&bar->q_empty[s]);
-      if (j % GROUP == GROUP - 1 || j == tiles - 1) umma_commit(&bar->sum_full);
-      if (j + AHEAD < tiles) ok = scores(j + AHEAD);
+  } else {
+    fewer_registers<40>();
+    if (warp == 12 && elect_one()) {
+      const uint32_t ra = smem_u32(ring), ka = smem_u32(k_tile), va = smem_u32(v_tile);
+      bool ok = tiles == 0 || mbar_wait(&bar->k_full, 0, p.status, 0x324);
+      // S^T and dP^T of tile j: the second half of it commits
+      auto half_of_scores = [&](int j, int half) {
+        const int i = 2 * j + half, s = i % SLOTS;
+        if (!mbar_wait(&bar->full[s], i / SLOTS & 1, p.status, 0x325)) return false;
+        tc_fence_after();
+        product_of_rows<D, 128, 64>(tmem + half * 128 + (j & 1) * 64, half ? va : ka, ra + s * LQ::BYTES);
+        if (half) {
+          umma_commit(&bar->s_full[j & 1]);
+          mbar_arrive(&bar->s_full[j & 1]);    // (what the loaders wrote is seen through this one)
+        }
+        return true;
+      };
+      // With six slots the scores of two tiles are under way; with three there is room for the next tile's queries only
+      constexpr bool WIDE = SLOTS == 6;
+      for (int i = 0; i < (WIDE ? 4 : 2) && i < 2 * tiles && ok; ++i) ok = half_of_scores(i / 2, i & 1);
+      for (int j = 0; j < tiles && ok; ++j) {
+        if (!WIDE && j + 1 < tiles && !(ok = half_of_scores(j + 1, 0))) break;
+        if (!(ok = mbar_wait(&bar->ds_full[j & 1], (j >> 1) & 1, p.status, 0x326))) break;
+        if (j > 0 && !(ok = mbar_wait(&bar->sum_empty, (j - 1) & 1, p.status, 0x327))) break;
+        tc_fence_after();
+        const int qs = 2 * j % SLOTS, gs = (2 * j + 1) % SLOTS;
+        product_with_columns<D, 64>(tmem + 384, tmem + 128 + (j & 1) * 64, ra + qs * LQ::BYTES);
+        umma_commit(&bar->empty[qs]);
+        product_with_columns<D, 64>(tmem + 256, tmem + (j & 1) * 64, ra + gs * LQ::BYTES);
+        umma_commit(&bar->empty[gs]);
+        umma_commit(&bar->sum_full);
+        if (WIDE) {
+          if (j + 2 < tiles) ok = half_of_scores(j + 2, 0) && half_of_scores(j + 2, 1);
+        } else if (j + 1 < tiles) {
+          ok = half_of_scores(j + 1, 1);
+        }
+      }
+      if (!ok) drain(&bar->drained);
     }
-    if (!ok) drain(&bar->drained);
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 10) tmem_dealloc(tmem, TMEM_COLUMNS);
+  if (warp == 12) tmem_dealloc(tmem, TMEM_COLUMNS);
 }
 
 // ------------------------------------------------------------------------------------------------ single tokens
@@ -942,13 +1068,13 @@ bool describe(Problem& p, int n, int tq, int tk, int heads, int shared, int d, f
   return true;
 }
 
-template <class K> int run(K kernel, const Problem& p, long long blocks, int threads, int smem, cudaStream_t st, tsb_launch::SmemLimit& limit) {
+template <class K> int run(K kernel, const Problem& p, long long blocks, int smem, cudaStream_t st, tsb_launch::SmemLimit& limit) {
   if (blocks > INT32_MAX) return TSB_ERR_ARG;
   Problem q = p;
   q.status = tsb_host::status_word(st);
   if (!q.status) return TSB_ERR_LAUNCH;
   cudaError_t e = limit.raise(kernel, smem);
-  if (e == cudaSuccess) e = tsb_launch::launch(kernel, dim3((unsigned)blocks), dim3(threads), smem, st, q);
+  if (e == cudaSuccess) e = tsb_launch::launch(kernel, dim3((unsigned)blocks), dim3(THREADS), smem, st, q);
   return launched(e);
 }
 
@@ -988,8 +1114,8 @@ int tsb_cross_attention(const float* q, const float* kv, const float* key, float
   p.qtiles = (tq + 127) / 128;
   const long long blocks = (long long)n * heads * p.qtiles;
   static tsb_launch::SmemLimit limit64, limit128;
-  if (d <= 64) return run(attend<64>, p, blocks, 288, ForwardShape<64>::SMEM, st, limit64);
-  return run(attend<128>, p, blocks, 288, ForwardShape<128>::SMEM, st, limit128);
+  if (d <= 64) return run(attend<64>, p, blocks, ForwardShape<64>::SMEM, st, limit64);
+  return run(attend<128>, p, blocks, ForwardShape<128>::SMEM, st, limit128);
 }
 
 // dot [N, H, Tq]: the sum of g y over a head's row of both, [N, Tq, H, d].
@@ -1021,8 +1147,8 @@ int tsb_cross_attention_grad_q(const float* q, const float* kv, const float* key
   p.qtiles = (tq + 127) / 128;
   const long long blocks = (long long)n * heads * p.qtiles;
   static tsb_launch::SmemLimit limit64, limit128;
-  if (d <= 64) return run(grad_of_queries<64>, p, blocks, 288, QueryShape<64>::SMEM, st, limit64);
-  return run(grad_of_queries<128>, p, blocks, 288, QueryShape<128>::SMEM, st, limit128);
+  if (d <= 64) return run(grad_of_queries<64>, p, blocks, QueryShape<64>::SMEM, st, limit64);
+  return run(grad_of_queries<128>, p, blocks, QueryShape<128>::SMEM, st, limit128);
 }
 
 int tsb_cross_attention_grad_kv(const float* q, const float* kv, const float* key, const float* lse, const float* g, const float* dot,
@@ -1041,8 +1167,8 @@ int tsb_cross_attention_grad_kv(const float* q, const float* kv, const float* ke
   const long long blocks = (long long)n * shared * p.ktiles;
   if ((long long)p.qtiles * (heads / shared) > INT32_MAX) return TSB_ERR_ARG;
   static tsb_launch::SmemLimit limit64, limit128;
-  if (d <= 64) return run(grad_of_states<64>, p, blocks, 352, StateShape<64>::SMEM, st, limit64);
-  return run(grad_of_states<128>, p, blocks, 352, StateShape<128>::SMEM, st, limit128);
+  if (d <= 64) return run(grad_of_states<64>, p, blocks, StateShape<64>::SMEM, st, limit64);
+  return run(grad_of_states<128>, p, blocks, StateShape<128>::SMEM, st, limit128);
 }
 
 }  // extern "C"
