@@ -223,11 +223,12 @@ def test_attention_refuses_what_is_not_row_major():
     from tsplit_b200.ops import _gpu as G
     cpu = ndarray.cpu(0)
     q = ndarray.NDArray(torch.zeros(2, 8, 4, 3).permute(0, 3, 2, 1), cpu)                 # (2, 3, 4, 8)
-    ok, kv, rows = ndarray.empty((2, 3, 4, 8)), ndarray.empty((2, 5, 2, 2, 8)), ndarray.empty((2, 4, 3))
+    ok, kv, rows, flat = ndarray.empty((2, 3, 4, 8)), ndarray.empty((2, 5, 2, 2, 8)), ndarray.empty((2, 4, 3)), ndarray.empty((64,))
     sizes = (2, 3, 5, 4, 2, 8)
-    for call in [lambda: G.cross_attention(q, kv, None, ok, rows, sizes, 1.0, None), lambda: G.cross_attention_dots(ok, q, rows, None),
-                 lambda: G.cross_attention_grad_q(ok, kv, None, rows, q, rows, ok, sizes, 1.0, None),
-                 lambda: G.cross_attention_grad_kv(q, kv, None, rows, ok, rows, kv, sizes, 1.0, None)]:
+    for call in [lambda: G.cross_attention(q, kv, None, ok, rows, sizes, 1.0, None),
+                 lambda: G.cross_attention_prepare(ok, kv, None, q, ok, flat, sizes, 1.0, None),
+                 lambda: G.cross_attention_grad_q(flat, None, rows, q, sizes, 1.0, None),
+                 lambda: G.cross_attention_grad_kv(flat, None, q, kv, sizes, 1.0, None)]:
         with pytest.raises(ValueError, match="row-major"):
             call()
 
@@ -254,7 +255,7 @@ def test_attention_has_the_same_bits_every_time_in_a_captured_step():
 def test_attention_of_arrays_that_begin_anywhere(tq):
     """Arrays 4 bytes off a 16-byte boundary take the loads of single numbers, with the same results."""
     import torch
-    from tsplit_b200.ops import _gpu as G
+    from tsplit_b200.ops import _gpu as G, attention as A
     from tsplit_b200.stream import create_stream_handle
     ctx = ndarray.gpu(0)
     st = create_stream_handle(ctx)
@@ -265,14 +266,34 @@ def test_attention_of_arrays_that_begin_anywhere(tq):
             t = torch.empty(v.size + 8, device="cuda")[off:off + v.size].view(v.shape)
             return ndarray.from_tensor(t.copy_(torch.from_numpy(v)), ctx)
         q, kv, key, g = (at(f[k]) for k in ("q", "kv", "key", "g"))
-        y, dq, dkv, lse, dots = at(f["q"] * 0), at(f["q"] * 0), at(f["kv"] * 0), at(np.zeros((2, 2, tq), np.float32)), at(np.zeros((2, 2, tq), np.float32))
+        y, dq, dkv, lse = at(f["q"] * 0), at(f["q"] * 0), at(f["kv"] * 0), at(np.zeros((2, 2, tq), np.float32))
+        flat = ndarray.empty((A._prepared_floats(*sizes),), ctx, use_pool=False)
         torch.cuda.synchronize()
         G.cross_attention(q, kv, key, y, lse, sizes, 0.125, st)
-        G.cross_attention_dots(g, y, dots, st)
-        G.cross_attention_grad_q(q, kv, key, lse, g, dots, dq, sizes, 0.125, st)
-        G.cross_attention_grad_kv(q, kv, key, lse, g, dots, dkv, sizes, 0.125, st)
+        G.cross_attention_prepare(q, kv, key, g, y, flat, sizes, 0.125, st)
+        G.cross_attention_grad_q(flat, key, lse, dq, sizes, 0.125, st)
+        G.cross_attention_grad_kv(flat, key, lse, dkv, sizes, 0.125, st)
         st.sync()
         got.append([a.asnumpy() for a in (y, dq, dkv)])
     want, tol = definition(f["q"], f["kv"], f["key"], 0.125, f["g"])
     for a, b, w, t in zip(got[0], got[1], want, tol):
         assert np.all(np.abs(a - w) <= t + 1e-37) and np.all(np.abs(b - w) <= t + 1e-37)
+
+
+def test_room_for_the_gradients_operands_is_checked():
+    """A flat array that is too short, or off a 16-byte boundary, is refused before anything is launched."""
+    import ctypes
+    from tsplit_b200 import _base
+    from tsplit_b200.ops import attention as A
+    if not _base.have("libtsplit_kernels.so"):
+        pytest.skip("the kernel library is not built")
+    lib = _base._load("libtsplit_kernels.so")
+    sizes = (2, 3, 5, 4, 2, 8)
+    some, need, p, i, f = ctypes.c_void_p(1 << 20), 4 * A._prepared_floats(*sizes), ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+    for at, have in [(1 << 20, need - 16), (0, need), ((1 << 20) + 4, need)]:
+        at, have, rest = p(at), ctypes.c_int64(have), [i(s) for s in sizes] + [f(1.0), p(0)]
+        assert lib.tsb_cross_attention_prepare(some, some, p(0), some, some, at, have, *rest) == 1
+        assert lib.tsb_cross_attention_grad_q(at, have, p(0), some, some, *rest) == 1
+        assert lib.tsb_cross_attention_grad_kv(at, have, p(0), some, some, *rest) == 1
+    for bad in [(2, 3, 5, 4, 3, 8), (2, 3, 5, 4, 2, 129), (2, 3, 5, 4, 2, 0), (-1, 3, 5, 4, 2, 8), (2, 3, 5, 0, 2, 8)]:
+        assert lib.tsb_cross_attention(some, some, p(0), some, some, *[i(s) for s in bad], f(1.0), p(0)) == 1

@@ -11,10 +11,11 @@
 // number to [2^13, 2^14) and split into two fp16 numbers, x = hi + lo, |x - hi - lo| <= 2^-22 |x| (or 2^-38 of the tile's
 // largest, where fp16 ends); a product is three: hi hi + hi lo + lo hi.  That takes 1.5 times the tensor time of one TF32
 // product, which keeps 2^-11, and the room of fp32, and 16-bit tiles can be read in both directions (K-major and MN-major)
-// from one copy in shared memory.  (Two bf16 numbers need no scale but keep 2^-17, three need six products.)  Loader
-// warps find the scale and split what they load; P and dS are split by the threads that compute them and go to tensor
-// memory, from where they are the A operand of the next product: P is at most 2^14, dS is scaled by a bound of its own.  What
-// a tile adds to y, dq, dk or dv is read from tensor memory and added in registers with the tile's scale.
+// from one copy in shared memory.  (Two bf16 numbers need no scale but keep 2^-17, three need six products.)  A kernel
+// before splits every operand once, in tiles of 128 rows that lie in memory as they will in shared memory, so the kernels
+// that multiply load them by bulk copies.  P and dS are split by the threads that compute them and go to tensor memory, from
+// where they are the A operand of the next product: P is at most 2^14, dS is scaled by a bound of its own.  What a tile adds
+// to y, dq, dk or dv is read from tensor memory and added in registers with the tile's scale.
 //
 // Scores are kept in units of log 2 (q is scaled by scale * log2(e) as it is loaded), so that an exponential is one ex2.
 #include <cuda_runtime.h>
@@ -23,6 +24,7 @@
 #include <stdint.h>
 
 #include "launch.cuh"
+#include "scratch.h"
 #include "smem_limit.h"
 #include "tc_common.cuh"
 
@@ -35,9 +37,16 @@ using tsb_launch::load;
 constexpr float NEG_INF = -__builtin_huge_valf(), LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr unsigned ALL = 0xffffffffu;
 
+// Tiles of pieces, [n][head][tile], and what a number of each tile stands for.
+struct Pieces {
+  const char* tiles;
+  const float* units;
+};
+
 struct Problem {
-  const float *q, *kv, *key, *g, *dot;
+  const float *q, *kv, *key, *dot;
   float *y, *lse, *dq, *dkv;
+  Pieces qp, kp, vp, gp;
   int n, tq, tk, heads, shared, d;
   float scale;
   int qtiles, ktiles;
@@ -72,93 +81,126 @@ template <int D, int ROWS> struct Tile {
   static constexpr int CHUNK = ROWS * 128, PLANE = ROWS * D * 2, BYTES = 2 * PLANE;
 };
 
-// What loaders share: the largest number of a tile, by warp, twice, since a tile's may still be read when the next one's
-// are written.
-struct LoaderShared {
-  uint32_t largest[2][8];
+// One operand to split: rows of d numbers of [n][t][head].
+struct Source {
+  const float* x;
+  const float* with;                         // an array like x: dots[n, head, t] = sum of x with over a row; or null
+  const float* tokens;                       // [n][t], a row whose token is 0 counts as zeros and is not read; or null
+  float* dots;
+  char* tiles;
+  float* units;
+  long long batch, row, head;                // strides
+  int rows, heads, count;                    // rows of a batch; tiles of a head
+  float mult;
+};
+struct Sources {
+  Source s[4];
+  int first[5];                              // block where each begins
+  int d;
+  bool vec;
 };
 
-// Loads `rows` rows of d numbers, `stride` apart, times `mult`; zeros for the rest of the tile and for rows whose token is
-// 0.  `ready` is called between the loads and the first store; when it fails for one of the THREADS, which all call this, all
-// give up (false).  *unit: what a number in shared memory has to be multiplied by.
-template <int D, int ROWS, int THREADS, class Ready>
-__device__ __forceinline__ bool load_tile(char* tile, int plane, int chunk, int t, const float* base, long long stride, int rows,
-                                          const Problem& p, const float* tokens, float mult, LoaderShared& sh, int& turn,
-                                          float* unit, Ready ready) {
-  constexpr int UNITS = D / 8, TRIPS = ROWS * UNITS / THREADS;
-  static_assert(ROWS * UNITS % THREADS == 0 && TRIPS <= 8, "a thread keeps up to 64 numbers");
+// A block splits a tile of 128 rows.
+template <int D>
+__global__ void __launch_bounds__(256) split_tiles(const Sources all) {
+  tsb_launch::enter();
+  using L = Tile<D, 128>;
+  constexpr int UNITS = D / 8, TRIPS = 128 * UNITS / 256;
+  __shared__ uint32_t largest[8];
+  int which = 0;
+  while ((int)blockIdx.x >= all.first[which + 1]) ++which;
+  const Source& s = all.s[which];
+  const int b = blockIdx.x - all.first[which], tile = b % s.count, h = b / s.count % s.heads, n = b / s.count / s.heads;
+  const int rows = s.rows - tile * 128, d = all.d;
+  const long long at = n * s.batch + (long long)tile * 128 * s.row + h * s.head;
+  const float* tokens = s.tokens ? s.tokens + (long long)n * s.rows + tile * 128 : nullptr;
   float v[TRIPS][8];
-#pragma unroll
-  for (int u = 0; u < TRIPS; ++u) {
-    const int i = t + u * THREADS, row = i / UNITS, c = i % UNITS * 8;
-    const bool in = row < rows && (!tokens || load(tokens + row) != 0.f);
-    const float* src = base + row * stride + c;
-    if (p.vec) {
+  auto get = [&](const float* base, int row, int c, bool in, float (&to)[8]) {
+    const float* src = base + at + row * s.row + c;
+    if (all.vec) {
       float4 w = make_float4(0.f, 0.f, 0.f, 0.f), x = w;
-      if (in && c < p.d) w = load(reinterpret_cast<const float4*>(src));
-      if (in && c + 4 < p.d) x = load(reinterpret_cast<const float4*>(src + 4));
-      v[u][0] = w.x; v[u][1] = w.y; v[u][2] = w.z; v[u][3] = w.w;
-      v[u][4] = x.x; v[u][5] = x.y; v[u][6] = x.z; v[u][7] = x.w;
+      if (in && c < d) w = load(reinterpret_cast<const float4*>(src));
+      if (in && c + 4 < d) x = load(reinterpret_cast<const float4*>(src + 4));
+      to[0] = w.x; to[1] = w.y; to[2] = w.z; to[3] = w.w;
+      to[4] = x.x; to[5] = x.y; to[6] = x.z; to[7] = x.w;
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[u][k] = in && c + k < p.d ? load(src + k) : 0.f;
+      for (int k = 0; k < 8; ++k) to[k] = in && c + k < d ? load(src + k) : 0.f;
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < TRIPS; ++u) {
+    const int i = threadIdx.x + u * 256, row = i / UNITS;
+    get(s.x, row, i % UNITS * 8, row < rows && (!tokens || load(tokens + row) != 0.f), v[u]);
+  }
+  if (s.with) {
+#pragma unroll
+    for (int u = 0; u < TRIPS; ++u) {
+      const int i = threadIdx.x + u * 256, row = i / UNITS;
+      float w[8], sum = 0.f;
+      get(s.with, row, i % UNITS * 8, row < rows, w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += v[u][k] * w[k];
+#pragma unroll
+      for (int o = UNITS / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(ALL, sum, o);
+      if (row < rows && i % UNITS == 0) s.dots[((long long)n * s.heads + h) * s.rows + tile * 128 + row] = sum;
     }
   }
-  const bool ok = ready();
   uint32_t most = 0;
 #pragma unroll
   for (int u = 0; u < TRIPS; ++u)
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      v[u][k] *= mult;
+      v[u][k] *= s.mult;
       most = max(most, __float_as_uint(v[u][k]) & 0x7fffffffu);
     }
   most = __reduce_max_sync(ALL, most);
-  uint32_t* slots = sh.largest[turn & 1];
-  ++turn;
-  if ((t & 31) == 0) slots[t >> 5] = most;
-  uint32_t failed;
-  asm volatile(
-      "{\n"
-      ".reg .pred p, q;\n"
-      "setp.ne.u32 p, %1, 0;\n"
-      "barrier.cta.red.or.pred q, 1, %2, p;\n"
-      "selp.u32 %0, 1, 0, q;\n"
-      "}\n"
-      : "=r"(failed)
-      : "r"(ok ? 0u : 1u), "n"(THREADS)
-      : "memory");
-  if (failed) return false;
+  if ((threadIdx.x & 31) == 0) largest[threadIdx.x >> 5] = most;
+  __syncthreads();
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) most = max(most, slots[w]);
+  for (int w = 0; w < 8; ++w) most = max(most, largest[w]);
   const int e = exponent_to(most, TOP);
   const float scale = power_of_two(e);
-  if (t == 0) *unit = power_of_two(-e);
+  if (threadIdx.x == 0) s.units[b] = power_of_two(-e);
+  char* out = s.tiles + (size_t)b * L::BYTES;
 #pragma unroll
   for (int u = 0; u < TRIPS; ++u) {
-    const int i = t + u * THREADS, row = i / UNITS, at = i % UNITS;
-    char* to = tile + at / 8 * chunk + row * 128 + (((at & 7) ^ (row & 7)) << 4);
+    const int i = threadIdx.x + u * 256, row = i / UNITS, c = i % UNITS;
+    char* to = out + c / 8 * L::CHUNK + row * 128 + (((c & 7) ^ (row & 7)) << 4);
     uint4 hi, lo;
     split2(v[u][0] * scale, v[u][1] * scale, hi.x, lo.x);
     split2(v[u][2] * scale, v[u][3] * scale, hi.y, lo.y);
     split2(v[u][4] * scale, v[u][5] * scale, hi.z, lo.z);
     split2(v[u][6] * scale, v[u][7] * scale, hi.w, lo.w);
     *reinterpret_cast<uint4*>(to) = hi;
-    *reinterpret_cast<uint4*>(to + plane) = lo;
+    *reinterpret_cast<uint4*>(to + L::PLANE) = lo;
   }
-  fence_proxy_async();
-  return true;
-}
-// A tile of its own.
-template <int D, int ROWS, int THREADS, class Ready>
-__device__ __forceinline__ bool load_whole(char* tile, int t, const float* base, long long stride, int rows, const Problem& p,
-                                           const float* tokens, float mult, LoaderShared& sh, int& turn, float* unit, Ready ready) {
-  return load_tile<D, ROWS, THREADS>(tile, Tile<D, ROWS>::PLANE, Tile<D, ROWS>::CHUNK, t, base, stride, rows, p, tokens, mult, sh, turn,
-                                     unit, ready);
 }
 
-template <int R> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
-template <int R> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
+// Copies of tiles into shared memory by the copy engine; `full` gets their bytes.  Both sides are multiples of 16 bytes.
+__device__ __forceinline__ void bulk_copy(char* to, const char* from, uint32_t bytes, uint64_t* full) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(to)), "l"(from),
+               "r"(bytes), "r"(smem_u32(full))
+               : "memory");
+}
+template <int D>
+__device__ __forceinline__ void copy_tile(char* to, const Pieces& p, long long tile, uint64_t* full) {
+  mbar_expect_tx(full, Tile<D, 128>::BYTES);
+  bulk_copy(to, p.tiles + tile * Tile<D, 128>::BYTES, Tile<D, 128>::BYTES, full);
+}
+// The first or the last 64 rows of a tile, as a tile of 64 rows.
+template <int D>
+__device__ __forceinline__ void copy_half(char* to, const Pieces& p, long long tile, int half, uint64_t* full) {
+  using L = Tile<D, 128>;
+  using H = Tile<D, 64>;
+  mbar_expect_tx(full, H::BYTES);
+#pragma unroll
+  for (int plane = 0; plane < 2; ++plane)
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c)
+      bulk_copy(to + plane * H::PLANE + c * H::CHUNK, p.tiles + tile * L::BYTES + plane * L::PLANE + c * L::CHUNK + half * H::CHUNK,
+                H::CHUNK, full);
+}
 
 // ------------------------------------------------------------------------------------------------ products
 __host__ __device__ constexpr uint32_t idesc_f16(int n, int b_mn_major) {      // M = 128, D fp32, A and B fp16, A K-major
@@ -292,11 +334,10 @@ __device__ __forceinline__ void store_row(float* to, const float (&v)[COUNT], fl
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// A block takes 128 queries of a head and tiles of 128 keys.  Warps 0 to 3: soft-max, a row per thread; 4 to 11: loaders; 12
-// issues the products.  Two tiles of scores are in tensor memory, so S of the next tile runs while a thread works on this
+// A block takes 128 queries of a head and tiles of 128 keys.  Warps 0 to 3: soft-max, a row per thread; 4: copies; 5 issues
+// the products.  Two tiles of scores are in tensor memory, so S of the next tile runs while a thread works on this
 // one; P takes the place of its S.  y of a tile is added to the registers (rescaled to the new maximum there) while the next
 // tile's P is computed.
-constexpr int THREADS = 512;                 // of every block here: 128 registers a thread at first, traded below
 template <int D> struct ForwardShape {
   static constexpr int STAGES = D == 64 ? 2 : 1;
   using L = Tile<D, 128>;
@@ -304,13 +345,11 @@ template <int D> struct ForwardShape {
 };
 struct ForwardShared {
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], drained;
-  float q_unit, k_unit[4], v_unit[4];        // (the loaders may be three tiles ahead of who reads them)
-  LoaderShared loaders;
   uint32_t tmem;
 };
 
 template <int D>
-__global__ void __launch_bounds__(THREADS, 1) attend(const Problem p) {
+__global__ void __launch_bounds__(192, 1) attend(const Problem p) {
   using Shape = ForwardShape<D>;
   using L = typename Shape::L;
   constexpr int STAGES = Shape::STAGES;
@@ -320,20 +359,20 @@ __global__ void __launch_bounds__(THREADS, 1) attend(const Problem p) {
   char* v_tile = k_tile + STAGES * L::BYTES;
   const int warp = __shfl_sync(ALL, threadIdx.x >> 5, 0);
   if (threadIdx.x == 0) {
-    mbar_init(&bar->q_full, 256);
+    mbar_init(&bar->q_full, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar->k_full[i], 256);
+      mbar_init(&bar->k_full[i], 1);
       mbar_init(&bar->k_empty[i], 1);
-      mbar_init(&bar->v_full[i], 256);
+      mbar_init(&bar->v_full[i], 1);
       mbar_init(&bar->v_empty[i], 1);
-      mbar_init(&bar->s_full[i], 2);
+      mbar_init(&bar->s_full[i], 1);
       mbar_init(&bar->p_full[i], 128);
-      mbar_init(&bar->o_full[i], 2);
+      mbar_init(&bar->o_full[i], 1);
     }
     mbar_init(&bar->drained, 1);
     fence_barrier_init();
   }
-  if (warp == 12) {
+  if (warp == 5) {
     tmem_alloc(&bar->tmem, TMEM_COLUMNS);
     tmem_relinquish();
   }
@@ -347,20 +386,19 @@ __global__ void __launch_bounds__(THREADS, 1) attend(const Problem p) {
   const int shared = h / (p.heads / p.shared), q0 = qt * 128;
   const float* tokens = p.key ? p.key + (long long)n * p.tk : nullptr;
   const int tiles = (keys_in(tokens, p.tk) + 127) / 128;
-  const long long kv_row = 2ll * p.shared * p.d, q_row = (long long)p.heads * p.d;
-  const float* k_base = p.kv + (long long)n * p.tk * kv_row + (long long)shared * p.d;
+  const long long q_row = (long long)p.heads * p.d;
+  const long long q_at = ((long long)n * p.heads + h) * p.qtiles + qt, k_at = ((long long)n * p.shared + shared) * p.ktiles;
 
   if (warp < 4) {
-    more_registers<232>();
-    float acc[D], m = NEG_INF, l = 0.f, before = 1.f;
+    float acc[D], m = NEG_INF, l = 0.f, before = 1.f, v_unit = 0.f;
+    const float q_unit = load(p.qp.units + q_at);
 #pragma unroll
     for (int c = 0; c < D; ++c) acc[c] = 0.f;
     const uint32_t mine = tmem + ((uint32_t)warp << 21);         // this warp's 32 lanes
     bool ok = true;
-    auto add_tile = [&](int j, float factor) {
+    auto add_tile = [&](int j, float factor, float unit) {
       if (!mbar_wait(&bar->o_full[j & 1], (j >> 1) & 1, p.status, 0x301)) return false;
       tc_fence_after();
-      const float unit = bar->v_unit[j & 3];
 #pragma unroll
       for (int c = 0; c < D; c += 16) {
         float o[16];
@@ -375,10 +413,10 @@ __global__ void __launch_bounds__(THREADS, 1) attend(const Problem p) {
       unsigned in[4];
 #pragma unroll
       for (int w = 0; w < 4; ++w) in[w] = keys_mask(tokens, j * 128 + w * 32, p.tk);
+      const float unit = q_unit * load(p.kp.units + k_at + j), next_unit = load(p.vp.units + k_at + j);
       if (!mbar_wait(&bar->s_full[j & 1], (j >> 1) & 1, p.status, 0x302)) { ok = false; break; }
       tc_fence_after();
       const uint32_t at = mine + (j & 1) * 128;
-      const float unit = bar->q_unit * bar->k_unit[j & 3];
       float most = NEG_INF;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -415,42 +453,30 @@ __global__ void __launch_bounds__(THREADS, 1) attend(const Problem p) {
       mbar_arrive(&bar->p_full[j & 1]);
       l = l * factor + sum;
       m = top;
-      if (j > 0 && !(ok = add_tile(j - 1, before))) break;
+      if (j > 0 && !(ok = add_tile(j - 1, before, v_unit))) break;
       before = factor;
+      v_unit = next_unit;
     }
-    if (ok && tiles > 0) ok = add_tile(tiles - 1, before);
+    if (ok && tiles > 0) ok = add_tile(tiles - 1, before, v_unit);
     const int t = q0 + threadIdx.x;
     if (ok && t < p.tq) {
       store_row(p.y + ((long long)n * p.tq + t) * q_row + (long long)h * p.d, acc, l > 0.f ? 1.f / l : 0.f, p.d, p.vec);
       // (a row without keys: exp2(S - inf) = 0 in the backward pass)
       p.lse[((long long)n * p.heads + h) * p.tq + t] = l > 0.f ? m - (TOP + 1) + log2f(l) : -NEG_INF;
     }
-  } else if (warp < 12) {
-    fewer_registers<104>();
-    const int t = threadIdx.x - 128;
-    int turn = 0;
-    if (tiles > 0) {
-      load_whole<D, 128, 256>(q_tile, t, p.q + ((long long)n * p.tq + q0) * q_row + (long long)h * p.d, q_row, p.tq - q0, p, nullptr,
-                              p.scale * LOG2E, bar->loaders, turn, &bar->q_unit, [] { return true; });
-      mbar_arrive(&bar->q_full);
-    }
-    for (int j = 0; j < tiles; ++j) {
-      const int s = j % STAGES, ph = j / STAGES & 1;
-      const float* base = k_base + (long long)j * 128 * kv_row;
-      const float* tok = tokens ? tokens + j * 128 : nullptr;
-      if (!load_whole<D, 128, 256>(k_tile + s * L::BYTES, t, base, kv_row, p.tk - j * 128, p, tok, 1.f, bar->loaders, turn,
-                                   &bar->k_unit[j & 3], [&] { return mbar_wait(&bar->k_empty[s], ph ^ 1, p.status, 0x303); }))
-        break;
-      mbar_arrive(&bar->k_full[s]);
-      if (!load_whole<D, 128, 256>(v_tile + s * L::BYTES, t, base + (long long)p.shared * p.d, kv_row, p.tk - j * 128, p, tok, 1.f,
-                                   bar->loaders, turn, &bar->v_unit[j & 3],
-                                   [&] { return mbar_wait(&bar->v_empty[s], ph ^ 1, p.status, 0x304); }))
-        break;
-      mbar_arrive(&bar->v_full[s]);
+  } else if (warp == 4) {
+    if (elect_one() && tiles > 0) {
+      copy_tile<D>(q_tile, p.qp, q_at, &bar->q_full);
+      for (int j = 0; j < tiles; ++j) {
+        const int s = j % STAGES, ph = j / STAGES & 1;
+        if (!mbar_wait(&bar->k_empty[s], ph ^ 1, p.status, 0x303)) break;
+        copy_tile<D>(k_tile + s * L::BYTES, p.kp, k_at + j, &bar->k_full[s]);
+        if (!mbar_wait(&bar->v_empty[s], ph ^ 1, p.status, 0x304)) break;
+        copy_tile<D>(v_tile + s * L::BYTES, p.vp, k_at + j, &bar->v_full[s]);
+      }
     }
   } else {
-    fewer_registers<72>();
-    if (warp == 12 && elect_one()) {
+    if (elect_one()) {
       const uint32_t qa = smem_u32(q_tile), ka = smem_u32(k_tile), va = smem_u32(v_tile);
       bool ok = tiles == 0 || mbar_wait(&bar->q_full, 0, p.status, 0x305);
       auto scores = [&](int j) {
@@ -459,7 +485,6 @@ __global__ void __launch_bounds__(THREADS, 1) attend(const Problem p) {
         tc_fence_after();
         product_of_rows<D, 128, 128>(tmem + (j & 1) * 128, qa, ka + s * L::BYTES);
         umma_commit(&bar->s_full[j & 1]);
-        mbar_arrive(&bar->s_full[j & 1]);      // (what the loaders wrote is seen through this one)
         umma_commit(&bar->k_empty[s]);
         return true;
       };
@@ -471,7 +496,6 @@ __global__ void __launch_bounds__(THREADS, 1) attend(const Problem p) {
         tc_fence_after();
         product_with_columns<D, 128>(tmem + 256 + (j & 1) * 128, tmem + (j & 1) * 128, va + s * L::BYTES);
         umma_commit(&bar->o_full[j & 1]);
-        mbar_arrive(&bar->o_full[j & 1]);
         umma_commit(&bar->v_empty[s]);
         if (j + 2 < tiles) ok = scores(j + 2);
       }
@@ -482,37 +506,10 @@ __global__ void __launch_bounds__(THREADS, 1) attend(const Problem p) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(tmem, TMEM_COLUMNS);
+  if (warp == 5) tmem_dealloc(tmem, TMEM_COLUMNS);
 }
 
 // ------------------------------------------------------------------------------------------------ gradients
-// dot[n, h, t] = sum over c of dy y: a group of LANES threads a row.
-template <int LANES>
-__global__ void __launch_bounds__(256) row_dots(const float* g, const float* y, float* __restrict__ dot, long long rows, int tq,
-                                                int heads, int d, bool vec) {
-  tsb_launch::enter();
-  const long long r = (blockIdx.x * 256ll + threadIdx.x) / LANES;
-  const int lane = threadIdx.x % LANES;
-  float sum = 0.f;
-  if (r < rows) {
-    const float *a = g + r * d, *b = y + r * d;
-    if (vec) {
-      if (lane * 4 < d) {
-        const float4 u = load(reinterpret_cast<const float4*>(a) + lane), v = load(reinterpret_cast<const float4*>(b) + lane);
-        sum = u.x * v.x + u.y * v.y + u.z * v.z + u.w * v.w;
-      }
-    } else {
-      for (int c = lane; c < d; c += LANES) sum += load(a + c) * load(b + c);
-    }
-  }
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(ALL, sum, o);
-  if (r < rows && lane == 0) {
-    const long long nt = r / heads, h = r % heads, n = nt / tq, t = nt % tq;
-    dot[(n * heads + h) * tq + t] = sum;
-  }
-}
-
 // A bound of |dP - dot| over a tile: e with (d |g| |v| + |dot|) 2^e below 2^15 (units: what 2^14 of a tile stands for).
 __device__ __forceinline__ int exponent_of_ds(int d, float g_unit, float v_unit, float dot) {
   const float most = (float)d * (LARGEST * g_unit) * (LARGEST * v_unit) + fabsf(dot);
@@ -527,14 +524,12 @@ template <int D> struct QueryShape {
   static constexpr int SMEM = 2048 + 2 * LQ::BYTES + (K_STAGES + V_STAGES) * LK::BYTES;
 };
 struct QueryShared {
-  uint64_t q_full, k_full[3], k_empty[3], v_full[3], v_empty[3], s_full[2], ds_full[2], dq_full[2], drained;
-  float q_unit, g_unit, k_unit[8], v_unit[8];  // (the loaders may be four tiles ahead of who reads them)
-  LoaderShared loaders;
+  uint64_t q_full, g_full, k_full[3], k_empty[3], v_full[3], v_empty[3], s_full[2], ds_full[2], dq_full[2], drained;
   uint32_t tmem;
 };
 
 template <int D>
-__global__ void __launch_bounds__(THREADS, 1) grad_of_queries(const Problem p) {
+__global__ void __launch_bounds__(192, 1) grad_of_queries(const Problem p) {
   using Shape = QueryShape<D>;
   using LQ = typename Shape::LQ;
   using LK = typename Shape::LK;
@@ -546,22 +541,23 @@ __global__ void __launch_bounds__(THREADS, 1) grad_of_queries(const Problem p) {
   char* v_tile = k_tile + KS * LK::BYTES;
   const int warp = __shfl_sync(ALL, threadIdx.x >> 5, 0);
   if (threadIdx.x == 0) {
-    mbar_init(&bar->q_full, 256);
+    mbar_init(&bar->q_full, 1);
+    mbar_init(&bar->g_full, 1);
     for (int i = 0; i < 3; ++i) {
-      mbar_init(&bar->k_full[i], 256);
+      mbar_init(&bar->k_full[i], 1);
       mbar_init(&bar->k_empty[i], 1);
-      mbar_init(&bar->v_full[i], 256);
+      mbar_init(&bar->v_full[i], 1);
       mbar_init(&bar->v_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar->s_full[i], 2);
+      mbar_init(&bar->s_full[i], 1);
       mbar_init(&bar->ds_full[i], 128);
       mbar_init(&bar->dq_full[i], 1);
     }
     mbar_init(&bar->drained, 1);
     fence_barrier_init();
   }
-  if (warp == 12) {
+  if (warp == 5) {
     tmem_alloc(&bar->tmem, TMEM_COLUMNS);
     tmem_relinquish();
   }
@@ -575,12 +571,10 @@ __global__ void __launch_bounds__(THREADS, 1) grad_of_queries(const Problem p) {
   const int shared = h / (p.heads / p.shared), q0 = qt * 128;
   const float* tokens = p.key ? p.key + (long long)n * p.tk : nullptr;
   const int tiles = (keys_in(tokens, p.tk) + 63) / 64;
-  const long long kv_row = 2ll * p.shared * p.d, q_row = (long long)p.heads * p.d;
-  const float* k_base = p.kv + (long long)n * p.tk * kv_row + (long long)shared * p.d;
-  const long long q_at = ((long long)n * p.tq + q0) * q_row + (long long)h * p.d;
+  const long long q_row = (long long)p.heads * p.d;
+  const long long q_at = ((long long)n * p.heads + h) * p.qtiles + qt, k_at = ((long long)n * p.shared + shared) * p.ktiles;
 
   if (warp < 4) {
-    more_registers<232>();
     float acc[D], before = 0.f;
 #pragma unroll
     for (int c = 0; c < D; ++c) acc[c] = 0.f;
@@ -588,6 +582,7 @@ __global__ void __launch_bounds__(THREADS, 1) grad_of_queries(const Problem p) {
     const int t = q0 + threadIdx.x;
     const long long at_row = ((long long)n * p.heads + h) * p.tq + t;
     const float lse = t < p.tq ? load(p.lse + at_row) : -NEG_INF, dot = t < p.tq ? load(p.dot + at_row) : 0.f;
+    const float q_unit = load(p.qp.units + q_at), g_unit = load(p.gp.units + q_at);
     bool ok = true;
     auto add_tile = [&](int j, float unit) {
       if (!mbar_wait(&bar->dq_full[j & 1], (j >> 1) & 1, p.status, 0x311)) return false;
@@ -604,12 +599,12 @@ __global__ void __launch_bounds__(THREADS, 1) grad_of_queries(const Problem p) {
     };
     for (int j = 0; j < tiles; ++j) {
       const unsigned in[2] = {keys_mask(tokens, j * 64, p.tk), keys_mask(tokens, j * 64 + 32, p.tk)};
+      const float k_unit = load(p.kp.units + k_at + j / 2), v_unit = load(p.vp.units + k_at + j / 2);
+      const int e = exponent_of_ds(p.d, g_unit, v_unit, dot);
+      const float s_unit = q_unit * k_unit, dp_unit = g_unit * v_unit, shift = (float)e - lse;
       if (!mbar_wait(&bar->s_full[j & 1], (j >> 1) & 1, p.status, 0x312)) { ok = false; break; }
       tc_fence_after();
       const uint32_t at = mine + (j & 1) * 64;
-      const float k_unit = bar->k_unit[j & 7], v_unit = bar->v_unit[j & 7], g_unit = bar->g_unit;
-      const int e = exponent_of_ds(p.d, g_unit, v_unit, dot);
-      const float s_unit = bar->q_unit * k_unit, dp_unit = g_unit * v_unit, shift = (float)e - lse;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         float s[16], dp[16];
@@ -631,37 +626,23 @@ __global__ void __launch_bounds__(THREADS, 1) grad_of_queries(const Problem p) {
       before = k_unit * power_of_two(-e);
     }
     if (ok && tiles > 0) ok = add_tile(tiles - 1, before);
-    if (ok && t < p.tq) store_row(p.dq + q_at + (long long)threadIdx.x * q_row, acc, p.scale, p.d, p.vec);
-  } else if (warp < 12) {
-    fewer_registers<104>();
-    const int t = threadIdx.x - 128;
-    int turn = 0;
-    if (tiles > 0) {
-      load_whole<D, 128, 256>(q_tile, t, p.q + q_at, q_row, p.tq - q0, p, nullptr, p.scale * LOG2E, bar->loaders, turn, &bar->q_unit,
-                              [] { return true; });
-      load_whole<D, 128, 256>(g_tile, t, p.g + q_at, q_row, p.tq - q0, p, nullptr, 1.f, bar->loaders, turn, &bar->g_unit,
-                              [] { return true; });
-      mbar_arrive(&bar->q_full);
-    }
-    for (int j = 0; j < tiles; ++j) {
-      const int ks = j % KS, vs = j % VS;
-      const float* base = k_base + (long long)j * 64 * kv_row;
-      const float* tok = tokens ? tokens + j * 64 : nullptr;
-      if (!load_whole<D, 64, 256>(k_tile + ks * LK::BYTES, t, base, kv_row, p.tk - j * 64, p, tok, 1.f, bar->loaders, turn,
-                                  &bar->k_unit[j & 7], [&] { return mbar_wait(&bar->k_empty[ks], (j / KS & 1) ^ 1, p.status, 0x313); }))
-        break;
-      mbar_arrive(&bar->k_full[ks]);
-      if (!load_whole<D, 64, 256>(v_tile + vs * LK::BYTES, t, base + (long long)p.shared * p.d, kv_row, p.tk - j * 64, p, tok, 1.f,
-                                  bar->loaders, turn, &bar->v_unit[j & 7],
-                                  [&] { return mbar_wait(&bar->v_empty[vs], (j / VS & 1) ^ 1, p.status, 0x314); }))
-        break;
-      mbar_arrive(&bar->v_full[vs]);
+    if (ok && t < p.tq) store_row(p.dq + ((long long)n * p.tq + t) * q_row + (long long)h * p.d, acc, p.scale, p.d, p.vec);
+  } else if (warp == 4) {
+    if (elect_one() && tiles > 0) {
+      copy_tile<D>(q_tile, p.qp, q_at, &bar->q_full);
+      copy_tile<D>(g_tile, p.gp, q_at, &bar->g_full);
+      for (int j = 0; j < tiles; ++j) {
+        const int ks = j % KS, vs = j % VS;
+        if (!mbar_wait(&bar->k_empty[ks], (j / KS & 1) ^ 1, p.status, 0x313)) break;
+        copy_half<D>(k_tile + ks * LK::BYTES, p.kp, k_at + j / 2, j & 1, &bar->k_full[ks]);
+        if (!mbar_wait(&bar->v_empty[vs], (j / VS & 1) ^ 1, p.status, 0x314)) break;
+        copy_half<D>(v_tile + vs * LK::BYTES, p.vp, k_at + j / 2, j & 1, &bar->v_full[vs]);
+      }
     }
   } else {
-    fewer_registers<72>();
-    if (warp == 12 && elect_one()) {
+    if (elect_one()) {
       const uint32_t qa = smem_u32(q_tile), ga = smem_u32(g_tile), ka = smem_u32(k_tile), va = smem_u32(v_tile);
-      bool ok = tiles == 0 || mbar_wait(&bar->q_full, 0, p.status, 0x315);
+      bool ok = tiles == 0 || (mbar_wait(&bar->q_full, 0, p.status, 0x315) && mbar_wait(&bar->g_full, 0, p.status, 0x315));
       auto scores = [&](int j) {
         const int ks = j % KS, vs = j % VS;
         if (!mbar_wait(&bar->k_full[ks], j / KS & 1, p.status, 0x316)) return false;
@@ -671,7 +652,6 @@ __global__ void __launch_bounds__(THREADS, 1) grad_of_queries(const Problem p) {
         tc_fence_after();
         product_of_rows<D, 128, 64>(tmem + 128 + (j & 1) * 64, ga, va + vs * LK::BYTES);
         umma_commit(&bar->s_full[j & 1]);
-        mbar_arrive(&bar->s_full[j & 1]);      // (what the loaders wrote is seen through this one)
         umma_commit(&bar->v_empty[vs]);
         return true;
       };
@@ -691,12 +671,12 @@ __global__ void __launch_bounds__(THREADS, 1) grad_of_queries(const Problem p) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(tmem, TMEM_COLUMNS);
+  if (warp == 5) tmem_dealloc(tmem, TMEM_COLUMNS);
 }
 
 // dk and dv: a block takes 128 keys of a shared head and tiles of 64 queries of every head that reads it.  S^T and dP^T have
 // the keys as rows, so P^T and dS^T are A operands as they lie.  Warps 0 to 3 take the first 32 queries of a tile and add up
-// dv, 4 to 7 the others and dk; 8 to 11 load; 12 issues.  Tiles of queries and of gradients share a ring of slots: q, g, q, g.
+// dv, 4 to 7 the others and dk; 8 copies; 9 issues.  Tiles of queries and of gradients share a ring of slots: q, g, q, g.
 template <int D> struct StateShape {
   static constexpr int SLOTS = D == 64 ? 6 : 3;
   using LK = Tile<D, 128>;
@@ -704,31 +684,30 @@ template <int D> struct StateShape {
   static constexpr int SMEM = 2048 + 2 * LK::BYTES + SLOTS * LQ::BYTES;
 };
 struct StateShared {
-  uint64_t k_full, full[6], empty[6], s_full[2], ds_full[2], sum_full, sum_empty, drained;
-  float k_unit[2], v_unit[2], unit[6];         // (two of the keys' and values': a thread of the loaders keeps 64 numbers)
-  LoaderShared loaders;
+  uint64_t k_full, v_full, full[6], empty[6], s_full[2], ds_full[2], sum_full, sum_empty, drained;
   uint32_t tmem;
 };
 
 template <int D>
-__global__ void __launch_bounds__(THREADS, 1) grad_of_states(const Problem p) {
+__global__ void __launch_bounds__(320, 1) grad_of_states(const Problem p) {
   using Shape = StateShape<D>;
   using LQ = typename Shape::LQ;
   using LK = typename Shape::LK;
-  constexpr int SLOTS = Shape::SLOTS, PART = 128 * 64 / D;                     // rows of a part of the keys' tile
+  constexpr int SLOTS = Shape::SLOTS;
   StateShared* bar;
   char* k_tile = dynamic_tiles(bar);
   char* v_tile = k_tile + LK::BYTES;
   char* ring = v_tile + LK::BYTES;
   const int warp = __shfl_sync(ALL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(&bar->k_full, 128);
+    mbar_init(&bar->k_full, 1);
+    mbar_init(&bar->v_full, 1);
     for (int i = 0; i < 6; ++i) {
-      mbar_init(&bar->full[i], 128);
+      mbar_init(&bar->full[i], 1);
       mbar_init(&bar->empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar->s_full[i], 2);
+      mbar_init(&bar->s_full[i], 1);
       mbar_init(&bar->ds_full[i], 256);
     }
     mbar_init(&bar->sum_full, 1);
@@ -736,7 +715,7 @@ __global__ void __launch_bounds__(THREADS, 1) grad_of_states(const Problem p) {
     mbar_init(&bar->drained, 1);
     fence_barrier_init();
   }
-  if (warp == 12) {
+  if (warp == 9) {
     tmem_alloc(&bar->tmem, TMEM_COLUMNS);
     tmem_relinquish();
   }
@@ -749,18 +728,17 @@ __global__ void __launch_bounds__(THREADS, 1) grad_of_states(const Problem p) {
   const int kt = blockIdx.x % p.ktiles, shared = blockIdx.x / p.ktiles % p.shared, n = blockIdx.x / p.ktiles / p.shared;
   const int k0 = kt * 128, per = p.heads / p.shared;
   const float* tokens = p.key ? p.key + (long long)n * p.tk : nullptr;
-  const long long kv_row = 2ll * p.shared * p.d, q_row = (long long)p.heads * p.d;
-  const long long k_at = ((long long)n * p.tk + k0) * kv_row + (long long)shared * p.d;
+  const long long kv_row = 2ll * p.shared * p.d, k_at = ((long long)n * p.shared + shared) * p.ktiles + kt;
   const bool mine_in = threadIdx.x < 128 && k0 + (int)threadIdx.x < p.tk && (!tokens || load(tokens + k0 + threadIdx.x) != 0.f);
-  const int tiles = __syncthreads_or(mine_in) ? p.qtiles * per : 0;
+  const int halves = (p.tq + 63) / 64, tiles = __syncthreads_or(mine_in) ? halves * per : 0;
 
   if (warp < 8) {
-    more_registers<184>();
     float acc[D];
 #pragma unroll
     for (int c = 0; c < D; ++c) acc[c] = 0.f;
     const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);
     const int half = warp >> 2, row = threadIdx.x & 127;
+    const float k_unit = load(p.kp.units + k_at), v_unit = load(p.vp.units + k_at);
     float before = 0.f;
     bool ok = true;
     auto add_tile = [&](int j, float unit) {
@@ -780,16 +758,16 @@ __global__ void __launch_bounds__(THREADS, 1) grad_of_states(const Problem p) {
     };
     for (int j = 0; j < tiles; ++j) {
       // a lane has the log-sum-exp and the dot of one of this half's queries, and the other half's dot for the bound
-      const int h = shared * per + j / p.qtiles, t0 = j % p.qtiles * 64, t = t0 + half * 32 + lane, other = t0 + (half ^ 1) * 32 + lane;
+      const int h = shared * per + j / halves, t0 = j % halves * 64, t = t0 + half * 32 + lane, other = t0 + (half ^ 1) * 32 + lane;
       const long long at_head = ((long long)n * p.heads + h) * p.tq;
       const float lse = t < p.tq ? load(p.lse + at_head + t) : -NEG_INF, dot = t < p.tq ? load(p.dot + at_head + t) : 0.f;
       const float dot2 = other < p.tq ? load(p.dot + at_head + other) : 0.f;
       const float most = __uint_as_float(__reduce_max_sync(ALL, max(__float_as_uint(fabsf(dot)), __float_as_uint(fabsf(dot2)))));
+      const long long q_at = ((long long)n * p.heads + h) * p.qtiles + t0 / 128;
+      const float q_unit = load(p.qp.units + q_at), g_unit = load(p.gp.units + q_at);
       if (!mbar_wait(&bar->s_full[j & 1], (j >> 1) & 1, p.status, 0x321)) { ok = false; break; }
       tc_fence_after();
       const uint32_t at = mine + (j & 1) * 64 + half * 32;
-      const float k_unit = bar->k_unit[row / PART], v_unit = bar->v_unit[row / PART];
-      const float q_unit = bar->unit[2 * j % SLOTS], g_unit = bar->unit[(2 * j + 1) % SLOTS];
       const int e = exponent_of_ds(p.d, g_unit, v_unit, most);
       // p = 2^14 P, then dS = p (dP - dot) 2^(e - 14)
       const float s_unit = q_unit * k_unit, f = power_of_two(max(e - TOP - 1, -126)), dp_unit = g_unit * v_unit * f;
@@ -816,41 +794,27 @@ __global__ void __launch_bounds__(THREADS, 1) grad_of_states(const Problem p) {
     if (ok && tiles > 0) ok = add_tile(tiles - 1, before);
     if (ok && k0 + row < p.tk) {
       const bool in = !tokens || load(tokens + k0 + row) != 0.f;
-      float* to = p.dkv + k_at + row * kv_row + (half ? 0 : (long long)p.shared * p.d);
+      float* to = p.dkv + ((long long)n * p.tk + k0 + row) * kv_row + (long long)shared * p.d + (half ? 0 : (long long)p.shared * p.d);
       if (!in)
 #pragma unroll
         for (int c = 0; c < D; ++c) acc[c] = 0.f;
       store_row(to, acc, half ? LN2 : 1.f, p.d, p.vec);          // (q was loaded times scale * log2(e))
     }
-  } else if (warp < 12) {
-    fewer_registers<104>();
-    const int t = threadIdx.x - 256;
-    int turn = 0;
-    if (tiles > 0) {
-      for (int part = 0; part < 128 / PART; ++part) {
-        const float* tok = tokens ? tokens + k0 + part * PART : nullptr;
-        const float* base = p.kv + k_at + part * PART * kv_row;
-        load_tile<D, PART, 128>(k_tile + part * PART * 128, LK::PLANE, LK::CHUNK, t, base, kv_row, p.tk - k0 - part * PART, p, tok, 1.f,
-                                bar->loaders, turn, &bar->k_unit[part], [] { return true; });
-        load_tile<D, PART, 128>(v_tile + part * PART * 128, LK::PLANE, LK::CHUNK, t, base + (long long)p.shared * p.d, kv_row,
-                                p.tk - k0 - part * PART, p, tok, 1.f, bar->loaders, turn, &bar->v_unit[part], [] { return true; });
+  } else if (warp == 8) {
+    if (elect_one() && tiles > 0) {
+      copy_tile<D>(k_tile, p.kp, k_at, &bar->k_full);
+      copy_tile<D>(v_tile, p.vp, k_at, &bar->v_full);
+      for (int i = 0; i < 2 * tiles; ++i) {
+        const int s = i % SLOTS, j = i / 2, h = shared * per + j / halves, t0 = j % halves * 64;
+        if (!mbar_wait(&bar->empty[s], (i / SLOTS & 1) ^ 1, p.status, 0x323)) break;
+        copy_half<D>(ring + s * LQ::BYTES, i & 1 ? p.gp : p.qp, ((long long)n * p.heads + h) * p.qtiles + t0 / 128, t0 / 64 & 1,
+                     &bar->full[s]);
       }
-      mbar_arrive(&bar->k_full);
-    }
-    for (int i = 0; i < 2 * tiles; ++i) {
-      const int s = i % SLOTS, j = i / 2, h = shared * per + j / p.qtiles, t0 = j % p.qtiles * 64;
-      const long long at = ((long long)n * p.tq + t0) * q_row + (long long)h * p.d;
-      if (!load_whole<D, 64, 128>(ring + s * LQ::BYTES, t, (i & 1 ? p.g : p.q) + at, q_row, p.tq - t0, p, nullptr,
-                                  i & 1 ? 1.f : p.scale * LOG2E, bar->loaders, turn, &bar->unit[s],
-                                  [&] { return mbar_wait(&bar->empty[s], (i / SLOTS & 1) ^ 1, p.status, 0x323); }))
-        break;
-      mbar_arrive(&bar->full[s]);
     }
   } else {
-    fewer_registers<40>();
-    if (warp == 12 && elect_one()) {
+    if (elect_one()) {
       const uint32_t ra = smem_u32(ring), ka = smem_u32(k_tile), va = smem_u32(v_tile);
-      bool ok = tiles == 0 || mbar_wait(&bar->k_full, 0, p.status, 0x324);
+      bool ok = tiles == 0 || (mbar_wait(&bar->k_full, 0, p.status, 0x324) && mbar_wait(&bar->v_full, 0, p.status, 0x324));
       // S^T and dP^T of tile j: the second half of it commits
       auto half_of_scores = [&](int j, int half) {
         const int i = 2 * j + half, s = i % SLOTS;
@@ -859,7 +823,6 @@ __global__ void __launch_bounds__(THREADS, 1) grad_of_states(const Problem p) {
         product_of_rows<D, 128, 64>(tmem + half * 128 + (j & 1) * 64, half ? va : ka, ra + s * LQ::BYTES);
         if (half) {
           umma_commit(&bar->s_full[j & 1]);
-          mbar_arrive(&bar->s_full[j & 1]);    // (what the loaders wrote is seen through this one)
         }
         return true;
       };
@@ -890,7 +853,7 @@ __global__ void __launch_bounds__(THREADS, 1) grad_of_states(const Problem p) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(tmem, TMEM_COLUMNS);
+  if (warp == 9) tmem_dealloc(tmem, TMEM_COLUMNS);
 }
 
 // ------------------------------------------------------------------------------------------------ single tokens
@@ -1064,18 +1027,89 @@ bool describe(Problem& p, int n, int tq, int tk, int heads, int shared, int d, f
   p.q = q; p.kv = kv; p.key = key;
   p.n = n; p.tq = tq; p.tk = tk; p.heads = heads; p.shared = shared; p.d = d;
   p.scale = scale;
+  p.qtiles = (tq + 127) / 128;
+  p.ktiles = (tk + 127) / 128;
   p.vec = d % 4 == 0 && (bits & 15) == 0;
   return true;
 }
 
-template <class K> int run(K kernel, const Problem& p, long long blocks, int smem, cudaStream_t st, tsb_launch::SmemLimit& limit) {
+template <class K>
+int run(K kernel, const Problem& p, long long blocks, int threads, int smem, cudaStream_t st, tsb_launch::SmemLimit& limit) {
   if (blocks > INT32_MAX) return TSB_ERR_ARG;
   Problem q = p;
   q.status = tsb_host::status_word(st);
   if (!q.status) return TSB_ERR_LAUNCH;
   cudaError_t e = limit.raise(kernel, smem);
-  if (e == cudaSuccess) e = tsb_launch::launch(kernel, dim3((unsigned)blocks), dim3(THREADS), smem, st, q);
+  if (e == cudaSuccess) e = tsb_launch::launch(kernel, dim3((unsigned)blocks), dim3(threads), smem, st, q);
   return launched(e);
+}
+
+// Where the pieces of q, k, v and g lie in one buffer, behind them the units and the dots.
+struct Layout {
+  size_t tiles[4], units[4], dots, bytes;
+  Layout(int n, int tq, int tk, int heads, int shared, int d, bool with_g) {
+    const size_t tile = d <= 64 ? Tile<64, 128>::BYTES : Tile<128, 128>::BYTES;
+    const size_t q = (size_t)n * heads * ((tq + 127) / 128), k = (size_t)n * shared * ((tk + 127) / 128);
+    const size_t count[4] = {q, k, k, with_g ? q : 0};
+    bytes = 0;
+    for (int i = 0; i < 4; ++i) {
+      tiles[i] = bytes;
+      bytes += count[i] * tile;
+    }
+    for (int i = 0; i < 4; ++i) {
+      units[i] = bytes;
+      bytes += count[i] * 4;
+    }
+    dots = bytes;
+    if (with_g) bytes += (size_t)n * heads * tq * 4;
+    bytes = (bytes + 15) / 16 * 16;
+  }
+  Pieces of(const char* base, int i) const { return {base + tiles[i], reinterpret_cast<const float*>(base + units[i])}; }
+};
+bool fits(const void* prepared, long long have, const Layout& at) {
+  return prepared && (reinterpret_cast<uintptr_t>(prepared) & 15) == 0 && have >= (long long)at.bytes;
+}
+void use(Problem& p, const Layout& at, const char* base) {
+  p.qp = at.of(base, 0);
+  p.kp = at.of(base, 1);
+  p.vp = at.of(base, 2);
+  p.gp = at.of(base, 3);
+  p.dot = reinterpret_cast<const float*>(base + at.dots);
+}
+
+// Splits q, k and v, and g (with the dots) where it is given.
+int split(const Problem& p, const float* g, const float* y, const Layout& at, char* base, cudaStream_t st) {
+  Sources all = {};
+  all.d = p.d;
+  all.vec = p.vec;
+  const float* from[4] = {p.q, p.kv, p.kv ? p.kv + (long long)p.shared * p.d : nullptr, g};
+  long long blocks = 0;
+  for (int i = 0; i < 4; ++i) {
+    Source& s = all.s[i];
+    const bool state = i == 1 || i == 2;
+    s.x = from[i];
+    s.rows = state ? p.tk : p.tq;
+    s.heads = state ? p.shared : p.heads;
+    s.count = (s.rows + 127) / 128;
+    s.row = state ? 2ll * p.shared * p.d : (long long)p.heads * p.d;
+    s.batch = s.rows * s.row;
+    s.head = p.d;
+    s.mult = i == 0 ? p.scale * LOG2E : 1.f;
+    s.tokens = state ? p.key : nullptr;
+    s.tiles = base + at.tiles[i];
+    s.units = reinterpret_cast<float*>(base + at.units[i]);
+    if (i == 3) {
+      s.with = y;
+      s.dots = reinterpret_cast<float*>(base + at.dots);
+    }
+    all.first[i] = (int)blocks;
+    if (i < 3 || g) blocks += (long long)p.n * s.heads * s.count;
+    if (blocks > INT32_MAX) return TSB_ERR_ARG;
+  }
+  all.first[4] = (int)blocks;
+  if (blocks == 0) return TSB_OK;
+  return launched(p.d <= 64 ? tsb_launch::launch(split_tiles<64>, dim3((unsigned)blocks), dim3(256), 0, st, all)
+                            : tsb_launch::launch(split_tiles<128>, dim3((unsigned)blocks), dim3(256), 0, st, all));
 }
 
 template <int LANES, int ROWS> int run_few(const Problem& p, cudaStream_t st) {
@@ -1111,64 +1145,63 @@ int tsb_cross_attention(const float* q, const float* kv, const float* key, float
   p.lse = lse;
   const long long rows = (long long)(heads / shared) * tq;
   if (rows <= FEW_ROWS) return d <= 32 ? few<8>(p, (int)rows, st) : d <= 64 ? few<16>(p, (int)rows, st) : few<32>(p, (int)rows, st);
-  p.qtiles = (tq + 127) / 128;
+  const Layout at(n, tq, tk, heads, shared, d, false);
+  char* pieces = static_cast<char*>(tsb_scratch::get(st, tsb_scratch::ATTENTION_PIECES, at.bytes));
+  if (!pieces) return TSB_ERR_OOM;
+  use(p, at, pieces);
+  const int rc = split(p, nullptr, nullptr, at, pieces, st);
+  if (rc) return rc;
   const long long blocks = (long long)n * heads * p.qtiles;
   static tsb_launch::SmemLimit limit64, limit128;
-  if (d <= 64) return run(attend<64>, p, blocks, ForwardShape<64>::SMEM, st, limit64);
-  return run(attend<128>, p, blocks, ForwardShape<128>::SMEM, st, limit128);
+  if (d <= 64) return run(attend<64>, p, blocks, 192, ForwardShape<64>::SMEM, st, limit64);
+  return run(attend<128>, p, blocks, 192, ForwardShape<128>::SMEM, st, limit128);
 }
 
-// dot [N, H, Tq]: the sum of g y over a head's row of both, [N, Tq, H, d].
-int tsb_cross_attention_dots(const float* g, const float* y, float* dot, int n, int tq, int heads, int d, void* stream) {
+// The pieces of q, kv and g, and the sums of g y over a head's row, for both gradients.  prepared: `have` bytes on a
+// 16-byte boundary, as many as Layout says.
+int tsb_cross_attention_prepare(const float* q, const float* kv, const float* key, const float* g, const float* y, void* prepared,
+                                long long have, int n, int tq, int tk, int heads, int shared, int d, float scale, void* stream) {
   Problem p;
-  if (!describe(p, n, tq, 0, heads, heads, d, 1.f, g, y, nullptr)) return TSB_ERR_ARG;
-  if (n == 0 || tq == 0) return TSB_OK;
-  if (!g || !y || !dot) return TSB_ERR_ARG;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const long long rows = (long long)n * tq * heads;
-  const int lanes = d <= 32 ? 8 : d <= 64 ? 16 : 32;
-  const long long blocks = (rows * lanes + 255) / 256;
-  if (blocks > INT32_MAX) return TSB_ERR_ARG;
-  auto kernel = lanes == 8 ? row_dots<8> : lanes == 16 ? row_dots<16> : row_dots<32>;
-  return launched(tsb_launch::launch(kernel, dim3((unsigned)blocks), dim3(256), 0, st, g, y, dot, rows, tq, heads, d, p.vec));
+  if (!describe(p, n, tq, tk, heads, shared, d, scale, q, kv, key, g, y)) return TSB_ERR_ARG;
+  if (n == 0) return TSB_OK;
+  const Layout at(n, tq, tk, heads, shared, d, true);
+  if ((tq && (!q || !g || !y)) || (tk && !kv) || !fits(prepared, have, at)) return TSB_ERR_ARG;
+  return split(p, g, y, at, static_cast<char*>(prepared), static_cast<cudaStream_t>(stream));
 }
 
-int tsb_cross_attention_grad_q(const float* q, const float* kv, const float* key, const float* lse, const float* g, const float* dot,
-                               float* dq, int n, int tq, int tk, int heads, int shared, int d, float scale, void* stream) {
+int tsb_cross_attention_grad_q(const void* prepared, long long have, const float* key, const float* lse, float* dq, int n, int tq, int tk, int heads,
+                               int shared, int d, float scale, void* stream) {
   Problem p;
-  if (!describe(p, n, tq, tk, heads, shared, d, scale, q, kv, key, g, dq)) return TSB_ERR_ARG;
+  if (!describe(p, n, tq, tk, heads, shared, d, scale, nullptr, nullptr, key, dq)) return TSB_ERR_ARG;
   if (n == 0 || tq == 0) return TSB_OK;
-  if (!q || !lse || !g || !dot || !dq || (tk && !kv)) return TSB_ERR_ARG;
+  const Layout at(n, tq, tk, heads, shared, d, true);
+  if (!lse || !dq || !fits(prepared, have, at)) return TSB_ERR_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  use(p, at, static_cast<const char*>(prepared));
   p.lse = const_cast<float*>(lse);
-  p.g = g;
-  p.dot = dot;
   p.dq = dq;
-  p.qtiles = (tq + 127) / 128;
   const long long blocks = (long long)n * heads * p.qtiles;
   static tsb_launch::SmemLimit limit64, limit128;
-  if (d <= 64) return run(grad_of_queries<64>, p, blocks, QueryShape<64>::SMEM, st, limit64);
-  return run(grad_of_queries<128>, p, blocks, QueryShape<128>::SMEM, st, limit128);
+  if (d <= 64) return run(grad_of_queries<64>, p, blocks, 192, QueryShape<64>::SMEM, st, limit64);
+  return run(grad_of_queries<128>, p, blocks, 192, QueryShape<128>::SMEM, st, limit128);
 }
 
-int tsb_cross_attention_grad_kv(const float* q, const float* kv, const float* key, const float* lse, const float* g, const float* dot,
-                                float* dkv, int n, int tq, int tk, int heads, int shared, int d, float scale, void* stream) {
+int tsb_cross_attention_grad_kv(const void* prepared, long long have, const float* key, const float* lse, float* dkv, int n, int tq, int tk, int heads,
+                                int shared, int d, float scale, void* stream) {
   Problem p;
-  if (!describe(p, n, tq, tk, heads, shared, d, scale, q, kv, key, g, dkv)) return TSB_ERR_ARG;
+  if (!describe(p, n, tq, tk, heads, shared, d, scale, nullptr, nullptr, key, dkv)) return TSB_ERR_ARG;
   if (n == 0 || tk == 0) return TSB_OK;
-  if (!kv || !dkv || (tq && (!q || !lse || !g || !dot))) return TSB_ERR_ARG;
+  const Layout at(n, tq, tk, heads, shared, d, true);
+  if (!dkv || (tq && !lse) || !fits(prepared, have, at)) return TSB_ERR_ARG;
+  if ((long long)((tq + 63) / 64) * (heads / shared) > INT32_MAX / 2) return TSB_ERR_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  use(p, at, static_cast<const char*>(prepared));
   p.lse = const_cast<float*>(lse);
-  p.g = g;
-  p.dot = dot;
   p.dkv = dkv;
-  p.qtiles = (tq + 63) / 64;
-  p.ktiles = (tk + 127) / 128;
   const long long blocks = (long long)n * shared * p.ktiles;
-  if ((long long)p.qtiles * (heads / shared) > INT32_MAX) return TSB_ERR_ARG;
   static tsb_launch::SmemLimit limit64, limit128;
-  if (d <= 64) return run(grad_of_states<64>, p, blocks, StateShape<64>::SMEM, st, limit64);
-  return run(grad_of_states<128>, p, blocks, StateShape<128>::SMEM, st, limit128);
+  if (d <= 64) return run(grad_of_states<64>, p, blocks, 320, StateShape<64>::SMEM, st, limit64);
+  return run(grad_of_states<128>, p, blocks, 320, StateShape<128>::SMEM, st, limit128);
 }
 
 }  // extern "C"

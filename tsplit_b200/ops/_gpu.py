@@ -367,27 +367,28 @@ def cross_attention(q, kv, key, y, lse, sizes, scale, stream):
                                          *[c_int(s) for s in sizes], c_float(scale), _s(stream)), "cross_attention")
 
 
-def cross_attention_dots(g, y, dots, stream):
-    _dense_rows("cross_attention_gradient", g, y, dots)
-    n, tq, h, d = g.shape
-    with _on_device(g):
-        _check(lib().tsb_cross_attention_dots(_p(g), _p(y), _p(dots), c_int(n), c_int(tq), c_int(h), c_int(d), _s(stream)),
+def cross_attention_prepare(q, kv, key, g, y, prepared, sizes, scale, stream):
+    """What both gradients read, into the flat array ``prepared``."""
+    _dense_rows("cross_attention_gradient", q, kv, g, y, prepared, *([key] if key is not None else []))
+    with _on_device(q):
+        _check(lib().tsb_cross_attention_prepare(_p(q), _p(kv), c_void_p(key.ptr if key is not None else 0), _p(g), _p(y), _p(prepared),
+                                                 c_int64(prepared.nbytes), *[c_int(s) for s in sizes], c_float(scale), _s(stream)),
                "cross_attention_gradient")
 
 
-def cross_attention_grad_q(q, kv, key, lse, g, dots, dq, sizes, scale, stream):
-    _dense_rows("cross_attention_gradient", q, kv, lse, g, dots, dq, *([key] if key is not None else []))
-    with _on_device(q):
-        _check(lib().tsb_cross_attention_grad_q(_p(q), _p(kv), c_void_p(key.ptr if key is not None else 0), _p(lse), _p(g), _p(dots),
-                                                _p(dq), *[c_int(s) for s in sizes], c_float(scale), _s(stream)),
+def cross_attention_grad_q(prepared, key, lse, dq, sizes, scale, stream):
+    _dense_rows("cross_attention_gradient", prepared, lse, dq, *([key] if key is not None else []))
+    with _on_device(dq):
+        _check(lib().tsb_cross_attention_grad_q(_p(prepared), c_int64(prepared.nbytes), c_void_p(key.ptr if key is not None else 0),
+                                                _p(lse), _p(dq), *[c_int(s) for s in sizes], c_float(scale), _s(stream)),
                "cross_attention_gradient")
 
 
-def cross_attention_grad_kv(q, kv, key, lse, g, dots, dkv, sizes, scale, stream):
-    _dense_rows("cross_attention_gradient", q, kv, lse, g, dots, dkv, *([key] if key is not None else []))
-    with _on_device(q):
-        _check(lib().tsb_cross_attention_grad_kv(_p(q), _p(kv), c_void_p(key.ptr if key is not None else 0), _p(lse), _p(g), _p(dots),
-                                                 _p(dkv), *[c_int(s) for s in sizes], c_float(scale), _s(stream)),
+def cross_attention_grad_kv(prepared, key, lse, dkv, sizes, scale, stream):
+    _dense_rows("cross_attention_gradient", prepared, lse, dkv, *([key] if key is not None else []))
+    with _on_device(dkv):
+        _check(lib().tsb_cross_attention_grad_kv(_p(prepared), c_int64(prepared.nbytes), c_void_p(key.ptr if key is not None else 0),
+                                                 _p(lse), _p(dkv), *[c_int(s) for s in sizes], c_float(scale), _s(stream)),
                "cross_attention_gradient")
 
 

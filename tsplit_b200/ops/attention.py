@@ -96,64 +96,68 @@ def _rows(shape, ctx):
     return ndarray.empty(shape, ctx, use_pool=False)
 
 
-class CrossAttentionDotsOp(Op):
-    """``sum(g * y)`` over a head's row: [N, Tq, heads, d] -> [N, heads, Tq], what both gradients subtract from dP."""
-    name = "CrossAttentionDots"
+def _prepared_floats(n, tq, tk, h, shared, d):
+    """Length of what the gradients read: tiles of 128 rows and 64 or 128 columns of q, k, v and g, one number for each, and
+    one for every row of g."""
+    q, k, columns = n * h * (-(-tq // 128)), n * shared * (-(-tk // 128)), 64 if d <= 64 else 128
+    return -(-((2 * q + 2 * k) * (128 * columns + 1) + n * h * tq) // 4) * 4
 
-    def __call__(self, g, y):
-        return Op.__call__(self, g, y)
+
+class CrossAttentionPrepareOp(Op):
+    """Operands of both gradients as the tensor cores take them, and ``sum(g * y)`` over every row: a flat array that only the
+    kernels read."""
+    name = "CrossAttentionPrepare"
+
+    def __call__(self, g, forward):
+        return Op.__call__(self, g, forward, *forward.inputs, scale=forward.attrs["scale"])
 
     def np_compute(self, node, iv):
-        return (iv[0].astype(np.float64) * iv[1]).sum(3).transpose(0, 2, 1).astype(np.float32)
+        return np.zeros(self.infer_shape(node, [v.shape for v in iv]), np.float32)
 
     def gpu_compute(self, node, iv, out, stream):
-        G.cross_attention_dots(iv[0], iv[1], out, stream)
+        g, y, q, kv = iv[:4]
+        key = iv[4] if len(iv) > 4 else None
+        sizes = _sizes(q.shape, kv.shape, key.shape if key is not None else None)
+        G.cross_attention_prepare(q, kv, key, g, y, out, sizes, CrossAttentionOp.scale_of(node, sizes[5]), stream)
 
     def gradient(self, node, g):
         raise NotImplementedError
 
     def infer_shape(self, node, s):
-        assert tuple(s[0]) == tuple(s[1]) and len(s[0]) == 4, "gradient %s of a result %s" % (tuple(s[0]), tuple(s[1]))
-        n, tq, h, _ = s[0]
-        return (n, h, tq)
+        assert tuple(s[0]) == tuple(s[1]) == tuple(s[2]), "gradient %s of a result %s" % (tuple(s[0]), tuple(s[1]))
+        return (_prepared_floats(*_sizes(s[2], s[3], s[4] if len(s) > 4 else None)),)
 
     def flops(self, node, s, out):
-        return 2.0 * np.prod(s[0])
+        return 8.0 * np.prod(out)
 
 
 class _CrossAttentionGradient(Op):
-    def __call__(self, g, dots, forward):
-        return Op.__call__(self, g, dots, *(list(forward.inputs) + [forward]), scale=forward.attrs["scale"], fwd=forward)
-
-    @staticmethod
-    def _parts(iv):
-        """g, dots, q, kv, key tokens or None (the last input, the forward result, is there to be computed first)"""
-        return iv[0], iv[1], iv[2], iv[3], iv[4] if len(iv) > 5 else None
+    def __call__(self, prepared, g, forward):
+        return Op.__call__(self, prepared, g, *forward.inputs, scale=forward.attrs["scale"], fwd=forward)
 
     def _ds(self, node, iv):
-        g, dots, q, kv, key = self._parts(iv)
-        scale = CrossAttentionOp.scale_of(node, q.shape[3])
-        p, q, k, v = _probabilities(q, kv, key, scale)
+        g, q, kv, key = iv[1], iv[2], iv[3], iv[4] if len(iv) > 4 else None
+        p, q, k, v = _probabilities(q, kv, key, CrossAttentionOp.scale_of(node, q.shape[3]))
         g = _heads(g, kv.shape[3])
-        n, s, r, tq, _ = g.shape
-        ds = p * (g @ np.swapaxes(v, 3, 4) - dots.astype(np.float64).reshape(n, s, r, tq, 1)) * scale
+        dp = g @ np.swapaxes(v, 3, 4)
+        ds = p * (dp - (dp * p).sum(4, keepdims=True)) * CrossAttentionOp.scale_of(node, kv.shape[4])
         return ds, p, g, q, k
 
     def gpu_compute(self, node, iv, out, stream):
-        g, dots, q, kv, key = self._parts(iv)
-        sizes = _sizes(q.shape, kv.shape, key.shape if key is not None else None)
+        key = iv[4] if len(iv) > 4 else None
+        sizes = _sizes(iv[2].shape, iv[3].shape, key.shape if key is not None else None)
         lse = node.attrs["fwd"].state.get("lse")
-        assert lse is not None and lse.shape == (sizes[0], sizes[3], sizes[1]), \
+        assert lse is not None and lse.shape == (sizes[0], sizes[3], sizes[1]) and lse.ctx == out.ctx, \
             "the gradient of a cross attention needs its forward pass on the same device first"
-        self._launch(q, kv, key, lse, g, dots, out, sizes, CrossAttentionOp.scale_of(node, sizes[5]), stream)
+        self._launch(iv[0], key, lse, out, sizes, CrossAttentionOp.scale_of(node, sizes[5]), stream)
 
     def gradient(self, node, g):
         raise NotImplementedError
 
     def _check(self, s):
-        n, tq, tk, h, shared, d = _sizes(s[2], s[3], s[4] if len(s) > 5 else None)
-        assert tuple(s[0]) == tuple(s[2]) and tuple(s[1]) == (n, h, tq), \
-            "gradient %s of a result %s" % (tuple(s[0]), tuple(s[2]))
+        sizes = _sizes(s[2], s[3], s[4] if len(s) > 4 else None)
+        assert tuple(s[1]) == tuple(s[2]) and tuple(s[0]) == (_prepared_floats(*sizes),), \
+            "gradient %s of a result %s" % (tuple(s[1]), tuple(s[2]))
 
 
 class CrossAttentionGradQueryOp(_CrossAttentionGradient):
@@ -189,7 +193,7 @@ class CrossAttentionGradStatesOp(_CrossAttentionGradient):
         return 8.0 * np.prod(s[2]) * s[3][1]
 
 
-_ca, _cad, _cagq, _cagkv = CrossAttentionOp(), CrossAttentionDotsOp(), CrossAttentionGradQueryOp(), CrossAttentionGradStatesOp()
+_ca, _cap, _cagq, _cagkv = CrossAttentionOp(), CrossAttentionPrepareOp(), CrossAttentionGradQueryOp(), CrossAttentionGradStatesOp()
 
 
 def cross_attention_op(q, kv, key_tokens=None, scale=None):
@@ -198,5 +202,5 @@ def cross_attention_op(q, kv, key_tokens=None, scale=None):
 
 def cross_attention_gradient_op(node, g):
     """[gradient of the queries, gradient of the states] of a :func:`cross_attention_op` ``node`` whose result has ``g``."""
-    dots = _cad(g, node)
-    return [_cagq(g, dots, node), _cagkv(g, dots, node)]
+    prepared = _cap(g, node)
+    return [_cagq(prepared, g, node), _cagkv(prepared, g, node)]
