@@ -266,7 +266,7 @@ def test_attention_of_arrays_that_begin_anywhere(tq):
             t = torch.empty(v.size + 8, device="cuda")[off:off + v.size].view(v.shape)
             return ndarray.from_tensor(t.copy_(torch.from_numpy(v)), ctx)
         q, kv, key, g = (at(f[k]) for k in ("q", "kv", "key", "g"))
-        y, dq, dkv, lse = at(f["q"] * 0), at(f["q"] * 0), at(f["kv"] * 0), at(np.zeros((2, 2, tq), np.float32))
+        y, dq, dkv, lse = at(f["q"] * 0), at(f["q"] * 0), at(f["kv"] * 0), ndarray.empty((2, 2, 128), ctx, use_pool=False)
         flat = ndarray.empty((A._prepared_floats(*sizes),), ctx, use_pool=False)
         torch.cuda.synchronize()
         G.cross_attention(q, kv, key, y, lse, sizes, 0.125, st)

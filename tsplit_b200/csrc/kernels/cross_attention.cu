@@ -19,7 +19,6 @@
 //
 // Scores are kept in units of log 2 (q is scaled by scale * log2(e) as it is loaded), so that an exponential is one ex2.
 #include <cuda_runtime.h>
-#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
 
@@ -30,7 +29,6 @@
 
 namespace {
 
-namespace cg = cooperative_groups;
 using namespace tsb;
 using tsb_launch::load;
 
@@ -84,7 +82,7 @@ template <int D, int ROWS> struct Tile {
 // One operand to split: rows of d numbers of [n][t][head].
 struct Source {
   const float* x;
-  const float* with;                         // an array like x: dots[n, head, t] = sum of x with over a row; or null
+  const float* with;                         // an array like x: dots[n, head, tile, row] = sum of x with over a row; or null
   const float* tokens;                       // [n][t], a row whose token is 0 counts as zeros and is not read; or null
   float* dots;
   char* tiles;
@@ -143,7 +141,7 @@ __global__ void __launch_bounds__(256) split_tiles(const Sources all) {
       for (int k = 0; k < 8; ++k) sum += v[u][k] * w[k];
 #pragma unroll
       for (int o = UNITS / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(ALL, sum, o);
-      if (row < rows && i % UNITS == 0) s.dots[((long long)n * s.heads + h) * s.rows + tile * 128 + row] = sum;
+      if (i % UNITS == 0) s.dots[(size_t)b * 128 + row] = sum;
     }
   }
   uint32_t most = 0;
@@ -188,12 +186,12 @@ __device__ __forceinline__ void copy_tile(char* to, const Pieces& p, long long t
   mbar_expect_tx(full, Tile<D, 128>::BYTES);
   bulk_copy(to, p.tiles + tile * Tile<D, 128>::BYTES, Tile<D, 128>::BYTES, full);
 }
-// The first or the last 64 rows of a tile, as a tile of 64 rows.
+// The first or the last 64 rows of a tile, as a tile of 64 rows; `more` bytes are to come to the same barrier.
 template <int D>
-__device__ __forceinline__ void copy_half(char* to, const Pieces& p, long long tile, int half, uint64_t* full) {
+__device__ __forceinline__ void copy_half(char* to, const Pieces& p, long long tile, int half, uint64_t* full, int more = 0) {
   using L = Tile<D, 128>;
   using H = Tile<D, 64>;
-  mbar_expect_tx(full, H::BYTES);
+  mbar_expect_tx(full, H::BYTES + more);
 #pragma unroll
   for (int plane = 0; plane < 2; ++plane)
 #pragma unroll
@@ -258,27 +256,65 @@ __device__ __forceinline__ void product_with_columns(uint32_t to, uint32_t a, ui
   }
 }
 
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, float* v) {
-  uint32_t* r = reinterpret_cast<uint32_t*>(v);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(addr)
-      : "memory");
+// Loads from tensor memory run behind what the thread does until tmem_ld_wait; tmem_arrived then names the registers, so
+// that nothing that reads them is moved before the wait.
+__device__ __forceinline__ void tmem_begin(uint32_t addr, float (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+               "%14, %15}, [%16];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+                 "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
+                 "=f"(v[14]), "=f"(v[15])
+               : "r"(addr)
+               : "memory");
 }
-// 16 numbers of a row as hi pieces in eight columns and lo pieces in the next eight
-__device__ __forceinline__ void tmem_st_pieces(uint32_t addr, const float (&v)[16]) {
-  uint32_t r[16];
+__device__ __forceinline__ void tmem_begin(uint32_t addr, float (&v)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+               "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+                 "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
+                 "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]),
+                 "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]),
+                 "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+               : "r"(addr)
+               : "memory");
+}
+template <int COUNT> __device__ __forceinline__ void tmem_arrived(float (&v)[COUNT]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) split2(v[2 * i], v[2 * i + 1], r[i], r[8 + i]);
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
-      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
-      : "memory");
+  for (int i = 0; i < COUNT; ++i) asm volatile("" : "+f"(v[i]));
+}
+// Numbers of a row, 16 at a time, as hi pieces in eight columns and lo pieces in the next eight
+template <int COUNT> __device__ __forceinline__ void tmem_st_pieces(uint32_t addr, const float (&v)[COUNT]) {
+#pragma unroll
+  for (int c = 0; c < COUNT; c += 16) {
+    uint32_t r[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) split2(v[c + 2 * i], v[c + 2 * i + 1], r[i], r[8 + i]);
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+          "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr + c)
+        : "memory");
+  }
+}
+// acc = acc times + what the tensor memory holds from addr on, times unit
+template <bool TIMES, int COUNT>
+__device__ __forceinline__ void add_columns(uint32_t addr, float (&acc)[COUNT], int first, int count, float times, float unit) {
+#pragma unroll
+  for (int c = 0; c < COUNT; c += 64) {
+    if (c < first || c >= first + count) continue;
+    float v[32], w[32];
+    tmem_begin(addr + c, v);
+    tmem_begin(addr + c + 32, w);
+    tmem_ld_wait();
+    tmem_arrived(v);
+    tmem_arrived(w);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      acc[c + i] = (TIMES ? acc[c + i] * times : acc[c + i]) + v[i] * unit;
+      acc[c + 32 + i] = (TIMES ? acc[c + 32 + i] * times : acc[c + 32 + i]) + w[i] * unit;
+    }
+  }
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -299,8 +335,6 @@ __device__ __forceinline__ unsigned keys_mask(const float* tokens, int first, in
   return __ballot_sync(ALL, k < tk && (!tokens || load(tokens + k) != 0.f));
 }
 
-constexpr int TMEM_COLUMNS = 512;
-
 // After a wait that ran out: the products that were issued still use shared and tensor memory.
 __device__ __forceinline__ void drain(uint64_t* bar) {
   umma_commit(bar);
@@ -309,15 +343,18 @@ __device__ __forceinline__ void drain(uint64_t* bar) {
   }
 }
 
-// The tiles begin at a multiple of 1024 bytes, behind the barriers.
-template <class Barriers>
-__device__ __forceinline__ char* dynamic_tiles(Barriers*& bars) {
-  extern __shared__ char raw[];
-  static_assert(sizeof(Barriers) <= 1024, "one kilobyte is kept for them");
-  char* at = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);
-  bars = reinterpret_cast<Barriers*>(at);
-  return at + 1024;
+// Shared memory: tiles from a multiple of 1024 bytes on, and 1024 bytes of barriers behind them.
+constexpr int CONTROL = 1024;
+extern __shared__ __align__(1024) char tiles_of_block[];
+template <class Control> __device__ __forceinline__ Control* control_at(int bytes_of_tiles) {
+  static_assert(sizeof(Control) <= CONTROL, "one kilobyte is kept for it");
+  return reinterpret_cast<Control*>(tiles_of_block + bytes_of_tiles);
 }
+
+// Blocks of up to 64 columns: two to an SM, so that one's products run while the other computes its soft-max or begins or
+// ends.  They have 256 threads; of the 128 registers a thread, the four warps that compute take 200 and the rest 56.
+template <int R> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int R> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 
 // Writes the d first numbers of a row.
 template <int COUNT>
@@ -335,51 +372,50 @@ __device__ __forceinline__ void store_row(float* to, const float (&v)[COUNT], fl
 
 // ------------------------------------------------------------------------------------------------ forward
 // A block takes 128 queries of a head and tiles of 128 keys.  Warps 0 to 3: soft-max, a row per thread; 4: copies; 5 issues
-// the products.  Two tiles of scores are in tensor memory, so S of the next tile runs while a thread works on this
-// one; P takes the place of its S.  y of a tile is added to the registers (rescaled to the new maximum there) while the next
-// tile's P is computed.
+// the products.  P takes the place of its S.  With 128 columns a block has an SM to itself and two tiles of scores in tensor
+// memory: S of the next tile runs while a thread works on this one, and y of a tile is added to the registers while the next
+// tile's product runs.
 template <int D> struct ForwardShape {
-  static constexpr int STAGES = D == 64 ? 2 : 1;
+  static constexpr bool TWO = D == 64;       // blocks to an SM
+  static constexpr int BUFFERS = TWO ? 1 : 2, BLOCK = TWO ? 256 : 192, COLUMNS = TWO ? 256 : 512, Y_AT = 128 * BUFFERS;
   using L = Tile<D, 128>;
-  static constexpr int SMEM = 2048 + L::BYTES * (1 + 2 * STAGES);
+  static constexpr int TILES = 3 * L::BYTES, SMEM = TILES + CONTROL;
 };
-struct ForwardShared {
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], drained;
+struct ForwardControl {
+  uint64_t q_full, k_full, k_empty, v_full, v_empty, s_full[2], p_full[2], y_full[2], drained;
   uint32_t tmem;
 };
 
 template <int D>
-__global__ void __launch_bounds__(192, 1) attend(const Problem p) {
+__global__ void __launch_bounds__(ForwardShape<D>::BLOCK, ForwardShape<D>::TWO ? 2 : 1) attend(const Problem p) {
   using Shape = ForwardShape<D>;
   using L = typename Shape::L;
-  constexpr int STAGES = Shape::STAGES;
-  ForwardShared* bar;
-  char* q_tile = dynamic_tiles(bar);
-  char* k_tile = q_tile + L::BYTES;
-  char* v_tile = k_tile + STAGES * L::BYTES;
+  constexpr int BUFFERS = Shape::BUFFERS, Y_AT = Shape::Y_AT;
+  char *const q_tile = tiles_of_block, *const k_tile = q_tile + L::BYTES, *const v_tile = k_tile + L::BYTES;
+  ForwardControl* bar = control_at<ForwardControl>(Shape::TILES);
   const int warp = __shfl_sync(ALL, threadIdx.x >> 5, 0);
   if (threadIdx.x == 0) {
     mbar_init(&bar->q_full, 1);
+    mbar_init(&bar->k_full, 1);
+    mbar_init(&bar->k_empty, 1);
+    mbar_init(&bar->v_full, 1);
+    mbar_init(&bar->v_empty, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar->k_full[i], 1);
-      mbar_init(&bar->k_empty[i], 1);
-      mbar_init(&bar->v_full[i], 1);
-      mbar_init(&bar->v_empty[i], 1);
       mbar_init(&bar->s_full[i], 1);
       mbar_init(&bar->p_full[i], 128);
-      mbar_init(&bar->o_full[i], 1);
+      mbar_init(&bar->y_full[i], 1);
     }
     mbar_init(&bar->drained, 1);
     fence_barrier_init();
   }
   if (warp == 5) {
-    tmem_alloc(&bar->tmem, TMEM_COLUMNS);
+    tmem_alloc(&bar->tmem, Shape::COLUMNS);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bar->tmem;             // S 0 and 128, y 256 and 384
+  const uint32_t tmem = bar->tmem;
   tsb_launch::enter();
 
   const int qt = blockIdx.x % p.qtiles, h = blockIdx.x / p.qtiles % p.heads, n = blockIdx.x / p.qtiles / p.heads;
@@ -390,114 +426,118 @@ __global__ void __launch_bounds__(192, 1) attend(const Problem p) {
   const long long q_at = ((long long)n * p.heads + h) * p.qtiles + qt, k_at = ((long long)n * p.shared + shared) * p.ktiles;
 
   if (warp < 4) {
+    if (Shape::TWO) more_registers<200>();
     float acc[D], m = NEG_INF, l = 0.f, before = 1.f, v_unit = 0.f;
     const float q_unit = load(p.qp.units + q_at);
 #pragma unroll
     for (int c = 0; c < D; ++c) acc[c] = 0.f;
     const uint32_t mine = tmem + ((uint32_t)warp << 21);         // this warp's 32 lanes
     bool ok = true;
-    auto add_tile = [&](int j, float factor, float unit) {
-      if (!mbar_wait(&bar->o_full[j & 1], (j >> 1) & 1, p.status, 0x301)) return false;
+    auto add_tile = [&](int j) {                                 // before: from the maximum then to the one that tile j has
+      const int b = j % BUFFERS;
+      if (!mbar_wait(&bar->y_full[b], j / BUFFERS & 1, p.status, 0x301)) return false;
       tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < D; c += 16) {
-        float o[16];
-        tmem_ld16(mine + 256 + (j & 1) * 128 + c, o);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[c + i] = acc[c + i] * factor + o[i] * unit;
-      }
+      add_columns<true>(mine + Y_AT + b * 128, acc, 0, D, before, v_unit);
       return true;
     };
     for (int j = 0; j < tiles; ++j) {
+      const int b = j % BUFFERS;
       unsigned in[4];
 #pragma unroll
       for (int w = 0; w < 4; ++w) in[w] = keys_mask(tokens, j * 128 + w * 32, p.tk);
       const float unit = q_unit * load(p.kp.units + k_at + j), next_unit = load(p.vp.units + k_at + j);
-      if (!mbar_wait(&bar->s_full[j & 1], (j >> 1) & 1, p.status, 0x302)) { ok = false; break; }
+      if (!mbar_wait(&bar->s_full[b], j / BUFFERS & 1, p.status, 0x302)) { ok = false; break; }
       tc_fence_after();
-      const uint32_t at = mine + (j & 1) * 128;
-      float most = NEG_INF;
+      if (BUFFERS == 1 && j > 0 && !(ok = add_tile(j - 1))) break;             // (its product ran before S)
+      const uint32_t at = mine + b * 128;
+      float part[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};     // (four chains: a thread has few others to wait behind)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        float s[32];
-        tmem_ld_32x32(at + 32 * w, s);
+      for (int w = 0; w < 4; w += 2) {
+        float s[2][32];
+        tmem_begin(at + 32 * w, s[0]);
+        tmem_begin(at + 32 * w + 32, s[1]);
         tmem_ld_wait();
-        if (in[w] == ALL) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) most = fmaxf(most, s[i]);
-        } else {
+        for (int k = 0; k < 2; ++k) {
+          tmem_arrived(s[k]);
+          if (in[w + k] == ALL) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) most = fmaxf(most, (in[w] >> i) & 1 ? s[i] : NEG_INF);
+            for (int i = 0; i < 32; ++i) part[i & 3] = fmaxf(part[i & 3], s[k][i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) part[i & 3] = fmaxf(part[i & 3], (in[w + k] >> i) & 1 ? s[k][i] : NEG_INF);
+          }
         }
       }
+      const float most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
       const float top = fmaxf(m, most == NEG_INF ? NEG_INF : most * unit), ref = top == NEG_INF ? 0.f : top;
       const float factor = exp2_fast(m - ref), shift = TOP + 1 - ref;
-      float sum = 0.f;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f}, s[2][32];
+      tmem_begin(at, s[0]);
 #pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        float s[16];
-        tmem_ld16(at + 16 * w, s);
+      for (int w = 0; w < 4; ++w) {
+        float(&v)[32] = s[w & 1];
         tmem_ld_wait();
-        const unsigned mask = in[w / 2] >> (w % 2 * 16);
+        tmem_arrived(v);
+        if (w < 3) tmem_begin(at + 32 * w + 32, s[(w + 1) & 1]);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[i] = exp2_fast(s[i] * unit + shift);
-          if (in[w / 2] != ALL) s[i] = (mask >> i) & 1 ? s[i] : 0.f;
-          sum += s[i];
+        for (int i = 0; i < 32; ++i) v[i] = exp2_fast(v[i] * unit + shift);
+        if (in[w] != ALL) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = (in[w] >> i) & 1 ? v[i] : 0.f;
         }
-        tmem_st_pieces(at + 16 * w, s);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) sum[i & 3] += v[i];
+        tmem_st_pieces(at + 32 * w, v);
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&bar->p_full[j & 1]);
-      l = l * factor + sum;
+      mbar_arrive(&bar->p_full[b]);
+      l = l * factor + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
       m = top;
-      if (j > 0 && !(ok = add_tile(j - 1, before, v_unit))) break;
+      if (BUFFERS == 2 && j > 0 && !(ok = add_tile(j - 1))) break;
       before = factor;
       v_unit = next_unit;
     }
-    if (ok && tiles > 0) ok = add_tile(tiles - 1, before, v_unit);
+    if (ok && tiles > 0) ok = add_tile(tiles - 1);
     const int t = q0 + threadIdx.x;
-    if (ok && t < p.tq) {
-      store_row(p.y + ((long long)n * p.tq + t) * q_row + (long long)h * p.d, acc, l > 0.f ? 1.f / l : 0.f, p.d, p.vec);
-      // (a row without keys: exp2(S - inf) = 0 in the backward pass)
-      p.lse[((long long)n * p.heads + h) * p.tq + t] = l > 0.f ? m - (TOP + 1) + log2f(l) : -NEG_INF;
-    }
-  } else if (warp == 4) {
-    if (elect_one() && tiles > 0) {
-      copy_tile<D>(q_tile, p.qp, q_at, &bar->q_full);
-      for (int j = 0; j < tiles; ++j) {
-        const int s = j % STAGES, ph = j / STAGES & 1;
-        if (!mbar_wait(&bar->k_empty[s], ph ^ 1, p.status, 0x303)) break;
-        copy_tile<D>(k_tile + s * L::BYTES, p.kp, k_at + j, &bar->k_full[s]);
-        if (!mbar_wait(&bar->v_empty[s], ph ^ 1, p.status, 0x304)) break;
-        copy_tile<D>(v_tile + s * L::BYTES, p.vp, k_at + j, &bar->v_full[s]);
-      }
+    if (ok) {
+      if (t < p.tq) store_row(p.y + ((long long)n * p.tq + t) * q_row + (long long)h * p.d, acc, l > 0.f ? 1.f / l : 0.f, p.d, p.vec);
+      // (a row without keys, or behind the last one: exp2(S - inf) = 0 in the backward pass)
+      p.lse[q_at * 128 + threadIdx.x] = l > 0.f && t < p.tq ? m - (TOP + 1) + log2f(l) : -NEG_INF;
     }
   } else {
-    if (elect_one()) {
+    if (Shape::TWO) fewer_registers<56>();
+    if (warp == 4 && elect_one() && tiles > 0) {
+      copy_tile<D>(q_tile, p.qp, q_at, &bar->q_full);
+      for (int j = 0; j < tiles; ++j) {
+        if (!mbar_wait(&bar->k_empty, (j & 1) ^ 1, p.status, 0x303)) break;
+        copy_tile<D>(k_tile, p.kp, k_at + j, &bar->k_full);
+        if (!mbar_wait(&bar->v_empty, (j & 1) ^ 1, p.status, 0x304)) break;
+        copy_tile<D>(v_tile, p.vp, k_at + j, &bar->v_full);
+      }
+    }
+    if (warp == 5 && elect_one() && tiles > 0) {
       const uint32_t qa = smem_u32(q_tile), ka = smem_u32(k_tile), va = smem_u32(v_tile);
-      bool ok = tiles == 0 || mbar_wait(&bar->q_full, 0, p.status, 0x305);
+      bool ok = mbar_wait(&bar->q_full, 0, p.status, 0x305);
       auto scores = [&](int j) {
-        const int s = j % STAGES;
-        if (!mbar_wait(&bar->k_full[s], j / STAGES & 1, p.status, 0x306)) return false;
+        if (!mbar_wait(&bar->k_full, j & 1, p.status, 0x306)) return false;
         tc_fence_after();
-        product_of_rows<D, 128, 128>(tmem + (j & 1) * 128, qa, ka + s * L::BYTES);
-        umma_commit(&bar->s_full[j & 1]);
-        umma_commit(&bar->k_empty[s]);
+        product_of_rows<D, 128, 128>(tmem + j % BUFFERS * 128, qa, ka);
+        umma_commit(&bar->s_full[j % BUFFERS]);
+        umma_commit(&bar->k_empty);
         return true;
       };
-      for (int j = 0; j < 2 && j < tiles && ok; ++j) ok = scores(j);
+      for (int j = 0; j < BUFFERS && j < tiles && ok; ++j) ok = scores(j);
       for (int j = 0; j < tiles && ok; ++j) {
-        const int s = j % STAGES;
-        if (!(ok = mbar_wait(&bar->v_full[s], j / STAGES & 1, p.status, 0x307))) break;
-        if (!(ok = mbar_wait(&bar->p_full[j & 1], (j >> 1) & 1, p.status, 0x308))) break;
+        const int b = j % BUFFERS;
+        if (!(ok = mbar_wait(&bar->v_full, j & 1, p.status, 0x307))) break;
+        if (!(ok = mbar_wait(&bar->p_full[b], j / BUFFERS & 1, p.status, 0x308))) break;
         tc_fence_after();
-        product_with_columns<D, 128>(tmem + 256 + (j & 1) * 128, tmem + (j & 1) * 128, va + s * L::BYTES);
-        umma_commit(&bar->o_full[j & 1]);
-        umma_commit(&bar->v_empty[s]);
-        if (j + 2 < tiles) ok = scores(j + 2);
+        product_with_columns<D, 128>(tmem + Y_AT + b * 128, tmem + b * 128, va);
+        umma_commit(&bar->y_full[b]);
+        umma_commit(&bar->v_empty);
+        if (j + BUFFERS < tiles) ok = scores(j + BUFFERS);
       }
       if (!ok) drain(&bar->drained);
     }
@@ -506,7 +546,7 @@ __global__ void __launch_bounds__(192, 1) attend(const Problem p) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) tmem_dealloc(tmem, TMEM_COLUMNS);
+  if (warp == 5) tmem_dealloc(tmem, Shape::COLUMNS);
 }
 
 // ------------------------------------------------------------------------------------------------ gradients
@@ -518,38 +558,36 @@ __device__ __forceinline__ int exponent_of_ds(int d, float g_unit, float v_unit,
 
 // dq: a block takes 128 queries of a head and tiles of 64 keys; the same roles.  dS takes the place of its S.
 template <int D> struct QueryShape {
-  static constexpr int K_STAGES = D == 64 ? 3 : 2, V_STAGES = D == 64 ? 3 : 1;
+  static constexpr bool TWO = D == 64;
+  static constexpr int BUFFERS = TWO ? 1 : 2, BLOCK = TWO ? 256 : 192, COLUMNS = TWO ? 256 : 512;
+  static constexpr int DP_AT = 64 * BUFFERS, DQ_AT = 128 * BUFFERS;
   using LQ = Tile<D, 128>;
   using LK = Tile<D, 64>;
-  static constexpr int SMEM = 2048 + 2 * LQ::BYTES + (K_STAGES + V_STAGES) * LK::BYTES;
+  static constexpr int TILES = 2 * LQ::BYTES + 3 * LK::BYTES, SMEM = TILES + CONTROL;       // two of keys, one of values
 };
-struct QueryShared {
-  uint64_t q_full, g_full, k_full[3], k_empty[3], v_full[3], v_empty[3], s_full[2], ds_full[2], dq_full[2], drained;
+struct QueryControl {
+  uint64_t q_full, g_full, k_full[2], k_empty[2], v_full, v_empty, s_full[2], ds_full[2], dq_full[2], drained;
   uint32_t tmem;
 };
 
 template <int D>
-__global__ void __launch_bounds__(192, 1) grad_of_queries(const Problem p) {
+__global__ void __launch_bounds__(QueryShape<D>::BLOCK, QueryShape<D>::TWO ? 2 : 1) grad_of_queries(const Problem p) {
   using Shape = QueryShape<D>;
   using LQ = typename Shape::LQ;
   using LK = typename Shape::LK;
-  constexpr int KS = Shape::K_STAGES, VS = Shape::V_STAGES;
-  QueryShared* bar;
-  char* q_tile = dynamic_tiles(bar);
-  char* g_tile = q_tile + LQ::BYTES;
-  char* k_tile = g_tile + LQ::BYTES;
-  char* v_tile = k_tile + KS * LK::BYTES;
+  constexpr int BUFFERS = Shape::BUFFERS, DP_AT = Shape::DP_AT, DQ_AT = Shape::DQ_AT;
+  char *const q_tile = tiles_of_block, *const g_tile = q_tile + LQ::BYTES, *const k_tile = g_tile + LQ::BYTES;
+  char* const v_tile = k_tile + 2 * LK::BYTES;
+  QueryControl* bar = control_at<QueryControl>(Shape::TILES);
   const int warp = __shfl_sync(ALL, threadIdx.x >> 5, 0);
   if (threadIdx.x == 0) {
     mbar_init(&bar->q_full, 1);
     mbar_init(&bar->g_full, 1);
-    for (int i = 0; i < 3; ++i) {
+    mbar_init(&bar->v_full, 1);
+    mbar_init(&bar->v_empty, 1);
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&bar->k_full[i], 1);
       mbar_init(&bar->k_empty[i], 1);
-      mbar_init(&bar->v_full[i], 1);
-      mbar_init(&bar->v_empty[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
       mbar_init(&bar->s_full[i], 1);
       mbar_init(&bar->ds_full[i], 128);
       mbar_init(&bar->dq_full[i], 1);
@@ -558,13 +596,13 @@ __global__ void __launch_bounds__(192, 1) grad_of_queries(const Problem p) {
     fence_barrier_init();
   }
   if (warp == 5) {
-    tmem_alloc(&bar->tmem, TMEM_COLUMNS);
+    tmem_alloc(&bar->tmem, Shape::COLUMNS);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bar->tmem;             // S 0 and 64, dP 128 and 192, dq 256 and 384
+  const uint32_t tmem = bar->tmem;
   tsb_launch::enter();
 
   const int qt = blockIdx.x % p.qtiles, h = blockIdx.x / p.qtiles % p.heads, n = blockIdx.x / p.qtiles / p.heads;
@@ -575,94 +613,101 @@ __global__ void __launch_bounds__(192, 1) grad_of_queries(const Problem p) {
   const long long q_at = ((long long)n * p.heads + h) * p.qtiles + qt, k_at = ((long long)n * p.shared + shared) * p.ktiles;
 
   if (warp < 4) {
+    if (Shape::TWO) more_registers<200>();
     float acc[D], before = 0.f;
 #pragma unroll
     for (int c = 0; c < D; ++c) acc[c] = 0.f;
     const uint32_t mine = tmem + ((uint32_t)warp << 21);
-    const int t = q0 + threadIdx.x;
-    const long long at_row = ((long long)n * p.heads + h) * p.tq + t;
-    const float lse = t < p.tq ? load(p.lse + at_row) : -NEG_INF, dot = t < p.tq ? load(p.dot + at_row) : 0.f;
+    const float lse = load(p.lse + q_at * 128 + threadIdx.x), dot = load(p.dot + q_at * 128 + threadIdx.x);
     const float q_unit = load(p.qp.units + q_at), g_unit = load(p.gp.units + q_at);
     bool ok = true;
-    auto add_tile = [&](int j, float unit) {
-      if (!mbar_wait(&bar->dq_full[j & 1], (j >> 1) & 1, p.status, 0x311)) return false;
+    auto add_tile = [&](int j) {
+      const int b = j % BUFFERS;
+      if (!mbar_wait(&bar->dq_full[b], j / BUFFERS & 1, p.status, 0x311)) return false;
       tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < D; c += 16) {
-        float o[16];
-        tmem_ld16(mine + 256 + (j & 1) * 128 + c, o);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[c + i] += o[i] * unit;
-      }
+      add_columns<false>(mine + DQ_AT + b * 128, acc, 0, D, 1.f, before);
       return true;
     };
     for (int j = 0; j < tiles; ++j) {
+      const int b = j % BUFFERS;
       const unsigned in[2] = {keys_mask(tokens, j * 64, p.tk), keys_mask(tokens, j * 64 + 32, p.tk)};
       const float k_unit = load(p.kp.units + k_at + j / 2), v_unit = load(p.vp.units + k_at + j / 2);
       const int e = exponent_of_ds(p.d, g_unit, v_unit, dot);
       const float s_unit = q_unit * k_unit, dp_unit = g_unit * v_unit, shift = (float)e - lse;
-      if (!mbar_wait(&bar->s_full[j & 1], (j >> 1) & 1, p.status, 0x312)) { ok = false; break; }
+      if (!mbar_wait(&bar->s_full[b], j / BUFFERS & 1, p.status, 0x312)) { ok = false; break; }
       tc_fence_after();
-      const uint32_t at = mine + (j & 1) * 64;
+      if (BUFFERS == 1 && j > 0 && !(ok = add_tile(j - 1))) break;
+      const uint32_t at = mine + b * 64;
+      float s[2][16], dp[2][16];
+      tmem_begin(at, s[0]);
+      tmem_begin(at + DP_AT, dp[0]);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        float s[16], dp[16];
-        tmem_ld16(at + 16 * w, s);
-        tmem_ld16(at + 128 + 16 * w, dp);
+        float(&v)[16] = s[w & 1];
+        float(&x)[16] = dp[w & 1];
         tmem_ld_wait();
-        const unsigned mask = in[w / 2] >> (w % 2 * 16);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[i] = exp2_fast(s[i] * s_unit + shift) * (dp[i] * dp_unit - dot);
-          if (in[w / 2] != ALL) s[i] = (mask >> i) & 1 ? s[i] : 0.f;
+        tmem_arrived(v);
+        tmem_arrived(x);
+        if (w < 3) {
+          tmem_begin(at + 16 * w + 16, s[(w + 1) & 1]);
+          tmem_begin(at + DP_AT + 16 * w + 16, dp[(w + 1) & 1]);
         }
-        tmem_st_pieces(at + 16 * w, s);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = exp2_fast(v[i] * s_unit + shift) * (x[i] * dp_unit - dot);
+        if (in[w / 2] != ALL) {
+          const unsigned mask = in[w / 2] >> (w % 2 * 16);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = (mask >> i) & 1 ? v[i] : 0.f;
+        }
+        tmem_st_pieces(at + 16 * w, v);
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&bar->ds_full[j & 1]);
-      if (j > 0 && !(ok = add_tile(j - 1, before))) break;
+      mbar_arrive(&bar->ds_full[b]);
+      if (BUFFERS == 2 && j > 0 && !(ok = add_tile(j - 1))) break;
       before = k_unit * power_of_two(-e);
     }
-    if (ok && tiles > 0) ok = add_tile(tiles - 1, before);
+    if (ok && tiles > 0) ok = add_tile(tiles - 1);
+    const int t = q0 + threadIdx.x;
     if (ok && t < p.tq) store_row(p.dq + ((long long)n * p.tq + t) * q_row + (long long)h * p.d, acc, p.scale, p.d, p.vec);
-  } else if (warp == 4) {
-    if (elect_one() && tiles > 0) {
+  } else {
+    if (Shape::TWO) fewer_registers<56>();
+    if (warp == 4 && elect_one() && tiles > 0) {
       copy_tile<D>(q_tile, p.qp, q_at, &bar->q_full);
-      copy_tile<D>(g_tile, p.gp, q_at, &bar->g_full);
       for (int j = 0; j < tiles; ++j) {
-        const int ks = j % KS, vs = j % VS;
-        if (!mbar_wait(&bar->k_empty[ks], (j / KS & 1) ^ 1, p.status, 0x313)) break;
-        copy_half<D>(k_tile + ks * LK::BYTES, p.kp, k_at + j / 2, j & 1, &bar->k_full[ks]);
-        if (!mbar_wait(&bar->v_empty[vs], (j / VS & 1) ^ 1, p.status, 0x314)) break;
-        copy_half<D>(v_tile + vs * LK::BYTES, p.vp, k_at + j / 2, j & 1, &bar->v_full[vs]);
+        const int s = j & 1;
+        if (!mbar_wait(&bar->k_empty[s], (j >> 1 & 1) ^ 1, p.status, 0x313)) break;
+        copy_half<D>(k_tile + s * LK::BYTES, p.kp, k_at + j / 2, j & 1, &bar->k_full[s]);
+        if (j == 0) copy_tile<D>(g_tile, p.gp, q_at, &bar->g_full);
+        if (!mbar_wait(&bar->v_empty, (j & 1) ^ 1, p.status, 0x314)) break;
+        copy_half<D>(v_tile, p.vp, k_at + j / 2, j & 1, &bar->v_full);
       }
     }
-  } else {
-    if (elect_one()) {
+    if (warp == 5 && elect_one() && tiles > 0) {
       const uint32_t qa = smem_u32(q_tile), ga = smem_u32(g_tile), ka = smem_u32(k_tile), va = smem_u32(v_tile);
-      bool ok = tiles == 0 || (mbar_wait(&bar->q_full, 0, p.status, 0x315) && mbar_wait(&bar->g_full, 0, p.status, 0x315));
+      bool ok = mbar_wait(&bar->q_full, 0, p.status, 0x315);
       auto scores = [&](int j) {
-        const int ks = j % KS, vs = j % VS;
-        if (!mbar_wait(&bar->k_full[ks], j / KS & 1, p.status, 0x316)) return false;
+        const int s = j & 1, b = j % BUFFERS;
+        if (!mbar_wait(&bar->k_full[s], j >> 1 & 1, p.status, 0x316)) return false;
         tc_fence_after();
-        product_of_rows<D, 128, 64>(tmem + (j & 1) * 64, qa, ka + ks * LK::BYTES);
-        if (!mbar_wait(&bar->v_full[vs], j / VS & 1, p.status, 0x317)) return false;
+        product_of_rows<D, 128, 64>(tmem + b * 64, qa, ka + s * LK::BYTES);
+        if (j == 0 && !mbar_wait(&bar->g_full, 0, p.status, 0x315)) return false;
+        if (!mbar_wait(&bar->v_full, j & 1, p.status, 0x317)) return false;
         tc_fence_after();
-        product_of_rows<D, 128, 64>(tmem + 128 + (j & 1) * 64, ga, va + vs * LK::BYTES);
-        umma_commit(&bar->s_full[j & 1]);
-        umma_commit(&bar->v_empty[vs]);
+        product_of_rows<D, 128, 64>(tmem + DP_AT + b * 64, ga, va);
+        umma_commit(&bar->s_full[b]);
+        umma_commit(&bar->v_empty);
         return true;
       };
-      for (int j = 0; j < 2 && j < tiles && ok; ++j) ok = scores(j);
+      for (int j = 0; j < BUFFERS && j < tiles && ok; ++j) ok = scores(j);
       for (int j = 0; j < tiles && ok; ++j) {
-        if (!(ok = mbar_wait(&bar->ds_full[j & 1], (j >> 1) & 1, p.status, 0x318))) break;
+        const int b = j % BUFFERS;
+        if (!(ok = mbar_wait(&bar->ds_full[b], j / BUFFERS & 1, p.status, 0x318))) break;
         tc_fence_after();
-        product_with_columns<D, 64>(tmem + 256 + (j & 1) * 128, tmem + (j & 1) * 64, ka + j % KS * LK::BYTES);
-        umma_commit(&bar->k_empty[j % KS]);
-        umma_commit(&bar->dq_full[j & 1]);
-        if (j + 2 < tiles) ok = scores(j + 2);
+        product_with_columns<D, 64>(tmem + DQ_AT + b * 128, tmem + b * 64, ka + (j & 1) * LK::BYTES);
+        umma_commit(&bar->k_empty[j & 1]);
+        umma_commit(&bar->dq_full[b]);
+        if (j + BUFFERS < tiles) ok = scores(j + BUFFERS);
       }
       if (!ok) drain(&bar->drained);
     }
@@ -671,38 +716,42 @@ __global__ void __launch_bounds__(192, 1) grad_of_queries(const Problem p) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) tmem_dealloc(tmem, TMEM_COLUMNS);
+  if (warp == 5) tmem_dealloc(tmem, Shape::COLUMNS);
 }
 
 // dk and dv: a block takes 128 keys of a shared head and tiles of 64 queries of every head that reads it.  S^T and dP^T have
-// the keys as rows, so P^T and dS^T are A operands as they lie.  Warps 0 to 3 take the first 32 queries of a tile and add up
-// dv, 4 to 7 the others and dk; 8 copies; 9 issues.  Tiles of queries and of gradients share a ring of slots: q, g, q, g.
+// the keys as rows, so P^T and dS^T are A operands as they lie.  Halves of the tiles of queries and of gradients share a ring
+// of slots (q, g, q, g, ...), each with its rows' log-sum-exps or dots.  Warps 0 to 3 take the first 32 queries of a tile and
+// add up dv, 4 to 7 the others and dk; 8: copies; 9 issues.  Two tiles of S^T and dP^T are in tensor memory.  (Two blocks of
+// four such warps to an SM, as above, took 516 us in place of 397 for 4 x 2048 x 2048, 16 heads of 64: the two sums leave a
+// thread no registers.)
 template <int D> struct StateShape {
-  static constexpr int SLOTS = D == 64 ? 6 : 3;
+  static constexpr int BLOCK = 384, DP_AT = 128, DV_AT = 256, DK_AT = 384, SLOTS = D == 64 ? 6 : 3;
   using LK = Tile<D, 128>;
   using LQ = Tile<D, 64>;
-  static constexpr int SMEM = 2048 + 2 * LK::BYTES + SLOTS * LQ::BYTES;
+  static constexpr int TILES = 2 * LK::BYTES + SLOTS * LQ::BYTES, SMEM = TILES + CONTROL + (SLOTS - 3) * 256;
 };
-struct StateShared {
-  uint64_t k_full, v_full, full[6], empty[6], s_full[2], ds_full[2], sum_full, sum_empty, drained;
+struct StateControl {
+  uint64_t k_full, v_full, full[6], empty[6], s_full[2], ds_full[2], sum_full, drained;
   uint32_t tmem;
 };
+constexpr int ROWS_AT = 256;                   // of the slots' log-sum-exps and dots, behind the barriers
+static_assert(sizeof(StateControl) <= ROWS_AT && ROWS_AT + 3 * 256 <= CONTROL, "");
 
 template <int D>
-__global__ void __launch_bounds__(320, 1) grad_of_states(const Problem p) {
+__global__ void __launch_bounds__(StateShape<D>::BLOCK, 1) grad_of_states(const Problem p) {
   using Shape = StateShape<D>;
   using LQ = typename Shape::LQ;
   using LK = typename Shape::LK;
-  constexpr int SLOTS = Shape::SLOTS;
-  StateShared* bar;
-  char* k_tile = dynamic_tiles(bar);
-  char* v_tile = k_tile + LK::BYTES;
-  char* ring = v_tile + LK::BYTES;
+  constexpr int SLOTS = Shape::SLOTS, DP_AT = Shape::DP_AT;
+  char *const k_tile = tiles_of_block, *const v_tile = k_tile + LK::BYTES, *const ring = v_tile + LK::BYTES;
+  StateControl* bar = control_at<StateControl>(Shape::TILES);
+  float* const rows = reinterpret_cast<float*>(reinterpret_cast<char*>(bar) + ROWS_AT);        // [SLOTS][64]
   const int warp = __shfl_sync(ALL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(&bar->k_full, 1);
     mbar_init(&bar->v_full, 1);
-    for (int i = 0; i < 6; ++i) {
+    for (int i = 0; i < SLOTS; ++i) {
       mbar_init(&bar->full[i], 1);
       mbar_init(&bar->empty[i], 1);
     }
@@ -711,133 +760,140 @@ __global__ void __launch_bounds__(320, 1) grad_of_states(const Problem p) {
       mbar_init(&bar->ds_full[i], 256);
     }
     mbar_init(&bar->sum_full, 1);
-    mbar_init(&bar->sum_empty, 256);
     mbar_init(&bar->drained, 1);
     fence_barrier_init();
   }
   if (warp == 9) {
-    tmem_alloc(&bar->tmem, TMEM_COLUMNS);
+    tmem_alloc(&bar->tmem, 512);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bar->tmem;             // S^T 0 and 64, dP^T 128 and 192, dv 256, dk 384
+  const uint32_t tmem = bar->tmem;
   tsb_launch::enter();
 
   const int kt = blockIdx.x % p.ktiles, shared = blockIdx.x / p.ktiles % p.shared, n = blockIdx.x / p.ktiles / p.shared;
-  const int k0 = kt * 128, per = p.heads / p.shared;
+  const int k0 = kt * 128, per = p.heads / p.shared, halves = (p.tq + 63) / 64;
   const float* tokens = p.key ? p.key + (long long)n * p.tk : nullptr;
   const long long kv_row = 2ll * p.shared * p.d, k_at = ((long long)n * p.shared + shared) * p.ktiles + kt;
+  const long long q_at = ((long long)n * p.heads + shared * per) * p.qtiles;                // of the first head that reads it
   const bool mine_in = threadIdx.x < 128 && k0 + (int)threadIdx.x < p.tk && (!tokens || load(tokens + k0 + threadIdx.x) != 0.f);
-  const int halves = (p.tq + 63) / 64, tiles = __syncthreads_or(mine_in) ? halves * per : 0;
+  const int tiles = __syncthreads_or(mine_in) ? halves * per : 0;
+  auto tile_of = [&](int j) { return q_at + (long long)(j / halves) * p.qtiles + j % halves / 2; };
 
   if (warp < 8) {
-    float acc[D];
+    more_registers<208>();
+    float acc[D], before = 0.f;
 #pragma unroll
     for (int c = 0; c < D; ++c) acc[c] = 0.f;
     const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);
     const int half = warp >> 2, row = threadIdx.x & 127;
     const float k_unit = load(p.kp.units + k_at), v_unit = load(p.vp.units + k_at);
-    float before = 0.f;
     bool ok = true;
-    auto add_tile = [&](int j, float unit) {
+    auto add_tile = [&](int j) {
       if (!mbar_wait(&bar->sum_full, j & 1, p.status, 0x322)) return false;
       tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < D; c += 16) {
-        float o[16];
-        tmem_ld16(mine + 256 + half * 128 + c, o);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[c + i] += o[i] * unit;
-      }
-      tc_fence_before();
-      mbar_arrive(&bar->sum_empty);
+      add_columns<false>(mine + (half ? Shape::DK_AT : Shape::DV_AT), acc, 0, D, 1.f, before);
       return true;
     };
     for (int j = 0; j < tiles; ++j) {
-      // a lane has the log-sum-exp and the dot of one of this half's queries, and the other half's dot for the bound
-      const int h = shared * per + j / halves, t0 = j % halves * 64, t = t0 + half * 32 + lane, other = t0 + (half ^ 1) * 32 + lane;
-      const long long at_head = ((long long)n * p.heads + h) * p.tq;
-      const float lse = t < p.tq ? load(p.lse + at_head + t) : -NEG_INF, dot = t < p.tq ? load(p.dot + at_head + t) : 0.f;
-      const float dot2 = other < p.tq ? load(p.dot + at_head + other) : 0.f;
-      const float most = __uint_as_float(__reduce_max_sync(ALL, max(__float_as_uint(fabsf(dot)), __float_as_uint(fabsf(dot2)))));
-      const long long q_at = ((long long)n * p.heads + h) * p.qtiles + t0 / 128;
-      const float q_unit = load(p.qp.units + q_at), g_unit = load(p.gp.units + q_at);
-      if (!mbar_wait(&bar->s_full[j & 1], (j >> 1) & 1, p.status, 0x321)) { ok = false; break; }
-      tc_fence_after();
-      const uint32_t at = mine + (j & 1) * 64 + half * 32;
-      const int e = exponent_of_ds(p.d, g_unit, v_unit, most);
+      const int b = j & 1, qs = 2 * j % SLOTS, gs = (2 * j + 1) % SLOTS;
+      const long long t = tile_of(j);
+      const float q_unit = load(p.qp.units + t), g_unit = load(p.gp.units + t);
+      if (!mbar_wait(&bar->full[gs], (2 * j + 1) / SLOTS & 1, p.status, 0x321)) { ok = false; break; }
+      if (!mbar_wait(&bar->full[qs], 2 * j / SLOTS & 1, p.status, 0x321)) { ok = false; break; }
+      const float *const lse = rows + qs * 64, *const dots = rows + gs * 64;
+      const uint32_t largest = max(__float_as_uint(fabsf(dots[lane])), __float_as_uint(fabsf(dots[lane + 32])));
+      const int e = exponent_of_ds(p.d, g_unit, v_unit, __uint_as_float(__reduce_max_sync(ALL, largest)));
       // p = 2^14 P, then dS = p (dP - dot) 2^(e - 14)
       const float s_unit = q_unit * k_unit, f = power_of_two(max(e - TOP - 1, -126)), dp_unit = g_unit * v_unit * f;
+      if (!mbar_wait(&bar->s_full[b], j >> 1 & 1, p.status, 0x321)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t at = mine + b * 64 + half * 32;
+      float s[2][16], dp[2][16];
+      tmem_begin(at, s[0]);
+      tmem_begin(at + DP_AT, dp[0]);
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        float s[16], dp[16];
-        tmem_ld16(at + 16 * w, s);
-        tmem_ld16(at + 128 + 16 * w, dp);
+        float(&v)[16] = s[w & 1];
+        float(&x)[16] = dp[w & 1];
         tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[i] = exp2_fast(s[i] * s_unit + (TOP + 1 - __shfl_sync(ALL, lse, 16 * w + i)));
-          dp[i] = s[i] * (dp[i] * dp_unit - __shfl_sync(ALL, dot, 16 * w + i) * f);
+        tmem_arrived(v);
+        tmem_arrived(x);
+        if (w + 1 < 2) {
+          tmem_begin(at + 16 * w + 16, s[(w + 1) & 1]);
+          tmem_begin(at + DP_AT + 16 * w + 16, dp[(w + 1) & 1]);
         }
-        tmem_st_pieces(at + 16 * w, s);
-        tmem_st_pieces(at + 128 + 16 * w, dp);
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const float4 a = *reinterpret_cast<const float4*>(lse + half * 32 + 16 * w + i);
+          const float4 c = *reinterpret_cast<const float4*>(dots + half * 32 + 16 * w + i);
+          const float as[4] = {a.x, a.y, a.z, a.w}, cs[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            v[i + k] = exp2_fast(v[i + k] * s_unit + (TOP + 1 - as[k]));
+            x[i + k] = v[i + k] * (x[i + k] * dp_unit - cs[k] * f);
+          }
+        }
+        tmem_st_pieces(at + 16 * w, v);
+        tmem_st_pieces(at + DP_AT + 16 * w, x);
       }
       tmem_st_wait();
+      if (j > 0 && !(ok = add_tile(j - 1))) break;
       tc_fence_before();
-      mbar_arrive(&bar->ds_full[j & 1]);
-      if (j > 0 && !(ok = add_tile(j - 1, before))) break;
+      mbar_arrive(&bar->ds_full[b]);                              // (the sums of the tile before are in registers by now)
       before = half ? q_unit * power_of_two(-e) : g_unit * (1.f / LARGEST);
     }
-    if (ok && tiles > 0) ok = add_tile(tiles - 1, before);
+    if (ok && tiles > 0) ok = add_tile(tiles - 1);
     if (ok && k0 + row < p.tk) {
       const bool in = !tokens || load(tokens + k0 + row) != 0.f;
-      float* to = p.dkv + ((long long)n * p.tk + k0 + row) * kv_row + (long long)shared * p.d + (half ? 0 : (long long)p.shared * p.d);
+      float* to = p.dkv + ((long long)n * p.tk + k0 + row) * kv_row + (long long)shared * p.d;
       if (!in)
 #pragma unroll
         for (int c = 0; c < D; ++c) acc[c] = 0.f;
-      store_row(to, acc, half ? LN2 : 1.f, p.d, p.vec);          // (q was loaded times scale * log2(e))
-    }
-  } else if (warp == 8) {
-    if (elect_one() && tiles > 0) {
-      copy_tile<D>(k_tile, p.kp, k_at, &bar->k_full);
-      copy_tile<D>(v_tile, p.vp, k_at, &bar->v_full);
-      for (int i = 0; i < 2 * tiles; ++i) {
-        const int s = i % SLOTS, j = i / 2, h = shared * per + j / halves, t0 = j % halves * 64;
-        if (!mbar_wait(&bar->empty[s], (i / SLOTS & 1) ^ 1, p.status, 0x323)) break;
-        copy_half<D>(ring + s * LQ::BYTES, i & 1 ? p.gp : p.qp, ((long long)n * p.heads + h) * p.qtiles + t0 / 128, t0 / 64 & 1,
-                     &bar->full[s]);
-      }
+      // (q was scaled by scale * log2(e))
+      store_row(half ? to : to + (long long)p.shared * p.d, acc, half ? LN2 : 1.f, p.d, p.vec);
     }
   } else {
-    if (elect_one()) {
+    fewer_registers<88>();
+    if (warp == 8 && elect_one() && tiles > 0) {
+      copy_tile<D>(k_tile, p.kp, k_at, &bar->k_full);
+      for (int i = 0; i < 2 * tiles; ++i) {
+        const int s = i % SLOTS, j = i / 2;
+        const long long t = tile_of(j);
+        const int h = j % halves % 2;
+        if (!mbar_wait(&bar->empty[s], (i / SLOTS & 1) ^ 1, p.status, 0x323)) break;
+        copy_half<D>(ring + s * LQ::BYTES, i & 1 ? p.gp : p.qp, t, h, &bar->full[s], 256);
+        bulk_copy(reinterpret_cast<char*>(rows + s * 64), reinterpret_cast<const char*>((i & 1 ? p.dot : p.lse) + t * 128 + h * 64), 256,
+                  &bar->full[s]);
+        if (i == 0) copy_tile<D>(v_tile, p.vp, k_at, &bar->v_full);
+      }
+    }
+    if (warp == 9 && elect_one() && tiles > 0) {
       const uint32_t ra = smem_u32(ring), ka = smem_u32(k_tile), va = smem_u32(v_tile);
-      bool ok = tiles == 0 || (mbar_wait(&bar->k_full, 0, p.status, 0x324) && mbar_wait(&bar->v_full, 0, p.status, 0x324));
-      // S^T and dP^T of tile j: the second half of it commits
+      bool ok = mbar_wait(&bar->k_full, 0, p.status, 0x324);
+      // S^T or dP^T of tile j; the latter commits both
       auto half_of_scores = [&](int j, int half) {
-        const int i = 2 * j + half, s = i % SLOTS;
+        const int i = 2 * j + half, s = i % SLOTS, b = j & 1;
+        if (i == 1 && !mbar_wait(&bar->v_full, 0, p.status, 0x324)) return false;
         if (!mbar_wait(&bar->full[s], i / SLOTS & 1, p.status, 0x325)) return false;
         tc_fence_after();
-        product_of_rows<D, 128, 64>(tmem + half * 128 + (j & 1) * 64, half ? va : ka, ra + s * LQ::BYTES);
-        if (half) {
-          umma_commit(&bar->s_full[j & 1]);
-        }
+        product_of_rows<D, 128, 64>(tmem + half * DP_AT + b * 64, half ? va : ka, ra + s * LQ::BYTES);
+        if (half) umma_commit(&bar->s_full[b]);
         return true;
       };
       // With six slots the scores of two tiles are under way; with three there is room for the next tile's queries only
       constexpr bool WIDE = SLOTS == 6;
       for (int i = 0; i < (WIDE ? 4 : 2) && i < 2 * tiles && ok; ++i) ok = half_of_scores(i / 2, i & 1);
       for (int j = 0; j < tiles && ok; ++j) {
+        const int b = j & 1, qs = 2 * j % SLOTS, gs = (2 * j + 1) % SLOTS;
         if (!WIDE && j + 1 < tiles && !(ok = half_of_scores(j + 1, 0))) break;
-        if (!(ok = mbar_wait(&bar->ds_full[j & 1], (j >> 1) & 1, p.status, 0x326))) break;
-        if (j > 0 && !(ok = mbar_wait(&bar->sum_empty, (j - 1) & 1, p.status, 0x327))) break;
+        if (!(ok = mbar_wait(&bar->ds_full[b], j >> 1 & 1, p.status, 0x326))) break;
         tc_fence_after();
-        const int qs = 2 * j % SLOTS, gs = (2 * j + 1) % SLOTS;
-        product_with_columns<D, 64>(tmem + 384, tmem + 128 + (j & 1) * 64, ra + qs * LQ::BYTES);
+        product_with_columns<D, 64>(tmem + Shape::DK_AT, tmem + DP_AT + b * 64, ra + qs * LQ::BYTES);
         umma_commit(&bar->empty[qs]);
-        product_with_columns<D, 64>(tmem + 256, tmem + (j & 1) * 64, ra + gs * LQ::BYTES);
+        product_with_columns<D, 64>(tmem + Shape::DV_AT, tmem + b * 64, ra + gs * LQ::BYTES);
         umma_commit(&bar->empty[gs]);
         umma_commit(&bar->sum_full);
         if (WIDE) {
@@ -853,155 +909,230 @@ __global__ void __launch_bounds__(320, 1) grad_of_states(const Problem p) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 9) tmem_dealloc(tmem, TMEM_COLUMNS);
+  if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
 // ------------------------------------------------------------------------------------------------ single tokens
 // Up to ROWS queries that read one shared head (H / G heads x Tq tokens): bound by reading keys and values once, so plain
-// fp32.  LANES threads take a key (four numbers each), so a warp takes 32 / LANES keys at a time and BATCH times that are in
-// flight; each such group keeps a soft-max of its own for every row, joined at the end: in the warp by shuffles, in the
-// block through shared memory, and over the blocks of a cluster that share a long sentence through distributed shared memory.
-constexpr int FEW_WARPS = 8;
-template <int LANES, int ROWS> struct FewShared {
-  float m[FEW_WARPS][ROWS], l[FEW_WARPS][ROWS];
-  float o[FEW_WARPS][ROWS][LANES * 4];
+// fp32.  A group of D / 4 threads takes four keys at a time, four columns a thread, and keeps a soft-max of its own; a thread
+// reads from shared memory only what it had copied there itself, three such steps deep, so nobody waits for anybody until
+// the end.  The 4 x ROWS dots of a step are added up over the group by halves: a thread sends half of its sums and keeps the
+// other half, until each holds one score, computes one exponential, and hands it to the others.  At the end the groups of a
+// block join through shared memory.  A long sentence is shared by as many blocks as leave two to every SM, and join_parts adds
+// up what they found (clusters of 8 or 16 that join through distributed shared memory do not spread over all SMs: 97 and 81 us
+// for the states below, 16 heads).
+// (4 x 16384 x 4 x 128 states, four rows each: registers and an all-reduce for every dot 182 us; tiles that the block shares,
+// with three barriers 136, with one 156.)
+constexpr int FEW_WARPS = 8, FEW_STAGES = 3, STEP = 4;
+template <int D, int ROWS> struct FewShape {
+  static constexpr int LANES = D / 4, GROUPS = FEW_WARPS * 32 / LANES, KEYS = GROUPS * STEP;
+  static constexpr int HELD = STEP * ROWS > LANES ? STEP * ROWS / LANES : 1;       // scores a thread ends up with, rows of one key
+  static constexpr int APART = LANES * HELD / (STEP * ROWS);                       // threads from one of these to the next
+  static constexpr int RING = FEW_STAGES * 2 * STEP * FEW_WARPS * 32 * 4;
+  // the ring, in its place later y of the groups [GROUPS][ROWS][D]; their maxima and sums
+  static constexpr int FLOATS = RING + 2 * GROUPS * ROWS;
+  static_assert(GROUPS * ROWS * D <= RING, "the sums of the groups take the place of the ring");
 };
 
-template <int LANES, int ROWS, int BATCH>
-__global__ void __launch_bounds__(FEW_WARPS * 32) attend_few(const Problem p, int split) {
+// 16 bytes, or zeros where nothing is to be read; `vec`: both sides on 16-byte boundaries
+__device__ __forceinline__ void copy_piece(float* to, const float* from, int count, bool vec) {
+  if (vec) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(count > 0 ? 16 : 0) : "memory");
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(to + k)), "l"(count > k ? from + k : from), "r"(count > k ? 4 : 0)
+                   : "memory");
+  }
+}
+
+// Cell i of the rows [ROWS][D] that read a shared head: y, and the row's log-sum-exp with its first column.
+template <int D> __device__ __forceinline__ void store_cell(const Problem& p, int n, int shared, int i, float top, float total, float sum) {
+  const int r = i / D, c = i % D, per = p.heads / p.shared, t = r / per, h = shared * per + r % per;
+  if (t >= p.tq) return;
+  if (c < p.d) p.y[(((long long)n * p.tq + t) * p.heads + h) * p.d + c] = total > 0.f ? sum / total : 0.f;
+  if (c == 0) p.lse[((long long)n * p.heads + h) * 128 + t] = total > 0.f ? top + log2f(total) : -NEG_INF;
+}
+
+template <int D, int ROWS>
+__global__ void __launch_bounds__(FEW_WARPS * 32, 2) attend_few(const Problem p, int split, float* __restrict__ parts) {
   tsb_launch::enter();
-  __shared__ FewShared<LANES, ROWS> s;
-  constexpr int GROUPS = 32 / LANES;
+  using S = FewShape<D, ROWS>;
+  constexpr int LANES = S::LANES, GROUPS = S::GROUPS, KEYS = S::KEYS, HELD = S::HELD, THREADS = FEW_WARPS * 32;
+  float* const ring = reinterpret_cast<float*>(tiles_of_block);
+  float *const maxima = ring + S::RING, *const totals = maxima + GROUPS * ROWS;
   const int part = blockIdx.x % split, shared = blockIdx.x / split % p.shared, n = blockIdx.x / split / p.shared;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / LANES, c = lane % LANES * 4;
+  const int tid = threadIdx.x, group = tid / LANES, c = tid % LANES * 4, base = tid & 31 & ~(LANES - 1);
   const int per = p.heads / p.shared, rows = per * p.tq;
   const float* tokens = p.key ? p.key + (long long)n * p.tk : nullptr;
-  const long long kv_row = 2ll * p.shared * p.d, q_row = (long long)p.heads * p.d;
+  const long long kv_row = 2ll * p.shared * p.d, q_row = (long long)p.heads * p.d, values = (long long)p.shared * p.d;
   const float* k_base = p.kv + (long long)n * p.tk * kv_row + (long long)shared * p.d + c;
-  auto four = [&](const float* at, bool in) {
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (!in || c >= p.d) return v;
-    if (p.vec) return load(reinterpret_cast<const float4*>(at));
-    v.x = load(at);
-    if (c + 1 < p.d) v.y = load(at + 1);
-    if (c + 2 < p.d) v.z = load(at + 2);
-    if (c + 3 < p.d) v.w = load(at + 3);
-    return v;
-  };
   float4 q[ROWS], o[ROWS];
-  float m[ROWS], l[ROWS];
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) {           // row r: query r / per of head r % per
-    q[r] = four(p.q + ((long long)n * p.tq + r / per) * q_row + (long long)(shared * per + r % per) * p.d + c, r < rows);
-    const float f = p.scale * LOG2E;
-    q[r] = make_float4(q[r].x * f, q[r].y * f, q[r].z * f, q[r].w * f);
+  for (int r = 0; r < ROWS; ++r) {                     // row r: query r / per of head r % per
+    const float* at = p.q + ((long long)n * p.tq + r / per) * q_row + (long long)(shared * per + r % per) * p.d + c;
+    float x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = r < rows && c + k < p.d ? load(at + k) * (p.scale * LOG2E) : 0.f;
+    q[r] = make_float4(x[0], x[1], x[2], x[3]);
     o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-    m[r] = NEG_INF;
-    l[r] = 0.f;
   }
-  const int share = (p.tk + split - 1) / split, begin = part * share, end = min(begin + share, p.tk);
-  constexpr int STEP = FEW_WARPS * GROUPS;
-  for (int first = begin; first < end; first += STEP * BATCH) {
-    float4 k[BATCH], v[BATCH];
-    bool in[BATCH];
+  // (rows behind the last query, of the one tile of each head: see attend)
+  for (int i = part * THREADS + tid; i < per * 128; i += split * THREADS)
+    if (i % 128 >= p.tq) p.lse[((long long)n * p.heads + shared * per + i / 128) * 128 + i % 128] = -NEG_INF;
+
+  const int share = (p.tk + split - 1) / split, begin = min(part * share, p.tk), end = min(begin + share, p.tk);
+  const int count = (end - begin + KEYS - 1) / KEYS;
+  float token[STEP];                                   // of the step that is copied next, read a step ahead
+  auto read_tokens = [&](int j) {
 #pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-      const int t = first + u * STEP + warp * GROUPS + group;
-      in[u] = t < end && (!tokens || load(tokens + t) != 0.f);
-      k[u] = four(k_base + t * kv_row, in[u]);
-      v[u] = four(k_base + t * kv_row + (long long)p.shared * p.d, in[u]);
+    for (int u = 0; u < STEP; ++u) {
+      const int t = begin + j * KEYS + group * STEP + u;
+      token[u] = t < end ? (tokens ? load(tokens + t) : 1.f) : 0.f;
+    }
+  };
+  unsigned in[FEW_STAGES] = {};                        // which of the four keys are in, of this step and those behind it
+  auto copy = [&](int j) {
+    unsigned mask = 0;
+    if (j < count) {
+      float* const to = ring + (j % FEW_STAGES * 2 * STEP * THREADS + tid) * 4;
+      const float* const from = k_base + (begin + j * KEYS + group * STEP) * kv_row;
+#pragma unroll
+      for (int u = 0; u < STEP; ++u) {
+        const bool is = token[u] != 0.f;
+        const int numbers = is ? p.d - c : 0;
+        mask |= (unsigned)is << u;
+        copy_piece(to + u * THREADS * 4, numbers > 0 ? from + u * kv_row : p.kv, numbers, p.vec);
+        copy_piece(to + (STEP + u) * THREADS * 4, numbers > 0 ? from + u * kv_row + values : p.kv, numbers, p.vec);
+      }
+      read_tokens(j + 1);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    return mask;
+  };
+  read_tokens(0);
+#pragma unroll
+  for (int j = 0; j < FEW_STAGES - 1; ++j) in[j] = copy(j);
+  // This thread's scores: of key `u` of a step, rows r0 to r0 + HELD - 1
+  const int place = (tid & (LANES - 1)) / S::APART, u = place / (ROWS / HELD), r0 = place % (ROWS / HELD) * HELD;
+  float m[HELD], l[HELD];
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) m[i] = NEG_INF, l[i] = 0.f;
+  for (int j = 0; j < count; ++j) {
+    in[FEW_STAGES - 1] = copy(j + FEW_STAGES - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(FEW_STAGES - 1) : "memory");
+    const float4* const at = reinterpret_cast<const float4*>(ring) + j % FEW_STAGES * 2 * STEP * THREADS + tid;
+    float x[STEP * ROWS];
+#pragma unroll
+    for (int k = 0; k < STEP; ++k) {
+      const float4 v = at[k * THREADS];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) x[k * ROWS + r] = q[r].x * v.x + q[r].y * v.y + q[r].z * v.z + q[r].w * v.w;
+    }
+#pragma unroll
+    for (int off = LANES / 2, left = STEP * ROWS; off > 0; off >>= 1) {
+      if (left > 1) {
+        left /= 2;
+#pragma unroll
+        for (int i = 0; i < STEP * ROWS / 2; ++i) {
+          if (i >= left) break;
+          const bool upper = tid & off;
+          const float send = upper ? x[i] : x[i + left], keep = upper ? x[i + left] : x[i];
+          x[i] = keep + __shfl_xor_sync(ALL, send, off);
+        }
+      } else {
+        x[0] += __shfl_xor_sync(ALL, x[0], off);
+      }
+    }
+    float factor[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+      if (!(in[0] >> u & 1)) x[i] = NEG_INF;
+      float top = fmaxf(x[i], __shfl_xor_sync(ALL, x[i], LANES / 2));              // (the two highest places tell the key)
+      top = fmaxf(m[i], fmaxf(top, __shfl_xor_sync(ALL, top, LANES / 4)));
+      const float ref = top == NEG_INF ? 0.f : top;
+      factor[i] = exp2_fast(m[i] - ref);
+      x[i] = exp2_fast(x[i] - ref);
+      l[i] = l[i] * factor[i] + x[i];
+      m[i] = top;
     }
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      float x[BATCH], top = m[r];
+      const float f = __shfl_sync(ALL, factor[r % HELD], base + r / HELD * S::APART);
+      o[r] = make_float4(o[r].x * f, o[r].y * f, o[r].z * f, o[r].w * f);
+    }
 #pragma unroll
-      for (int u = 0; u < BATCH; ++u) {
-        float d = q[r].x * k[u].x + q[r].y * k[u].y + q[r].z * k[u].z + q[r].w * k[u].w;
+    for (int k = 0; k < STEP; ++k) {
+      const float4 v = at[(STEP + k) * THREADS];
 #pragma unroll
-        for (int off = LANES / 2; off > 0; off >>= 1) d += __shfl_xor_sync(ALL, d, off);
-        x[u] = in[u] ? d : NEG_INF;
-        top = fmaxf(top, x[u]);
-      }
-      const float ref = top == NEG_INF ? 0.f : top, factor = exp2_fast(m[r] - ref);
-      m[r] = top;
-      l[r] *= factor;
-      o[r] = make_float4(o[r].x * factor, o[r].y * factor, o[r].z * factor, o[r].w * factor);
-#pragma unroll
-      for (int u = 0; u < BATCH; ++u) {
-        const float e = in[u] ? exp2_fast(x[u] - ref) : 0.f;
-        l[r] += e;
-        o[r].x += e * v[u].x; o[r].y += e * v[u].y; o[r].z += e * v[u].z; o[r].w += e * v[u].w;
+      for (int r = 0; r < ROWS; ++r) {
+        const float e = __shfl_sync(ALL, x[r % HELD], base + (k * (ROWS / HELD) + r / HELD) * S::APART);
+        o[r].x += e * v.x; o[r].y += e * v.y; o[r].z += e * v.z; o[r].w += e * v.w;
       }
     }
-  }
-  // the groups of a warp, then the warps
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-#pragma unroll
-    for (int off = LANES; off < 32; off <<= 1) {
-      const float m2 = __shfl_xor_sync(ALL, m[r], off), l2 = __shfl_xor_sync(ALL, l[r], off);
-      const float4 o2 = make_float4(__shfl_xor_sync(ALL, o[r].x, off), __shfl_xor_sync(ALL, o[r].y, off),
-                                    __shfl_xor_sync(ALL, o[r].z, off), __shfl_xor_sync(ALL, o[r].w, off));
-      const float top = fmaxf(m[r], m2), ref = top == NEG_INF ? 0.f : top;
-      const float a = exp2_fast(m[r] - ref), b = exp2_fast(m2 - ref);
-      m[r] = top;
-      l[r] = l[r] * a + l2 * b;
-      o[r] = make_float4(o[r].x * a + o2.x * b, o[r].y * a + o2.y * b, o[r].z * a + o2.z * b, o[r].w * a + o2.w * b);
-    }
-    if (group == 0) {
-      *reinterpret_cast<float4*>(&s.o[warp][r][c]) = o[r];
-      if (lane == 0) s.m[warp][r] = m[r], s.l[warp][r] = l[r];
-    }
+    for (int i = 0; i < FEW_STAGES - 1; ++i) in[i] = in[i + 1];
   }
+  // the groups of the block
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) {
+    l[i] += __shfl_xor_sync(ALL, l[i], LANES / 2);
+    l[i] += __shfl_xor_sync(ALL, l[i], LANES / 4);
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  constexpr int CELLS = ROWS * LANES * 4;
-  for (int i = threadIdx.x; i < CELLS; i += FEW_WARPS * 32) {        // (a thread reads and writes its own cells of o)
-    const int r = i / (LANES * 4), col = i % (LANES * 4);
-    float top = NEG_INF, lsum = 0.f, sum = 0.f;
-    for (int w = 0; w < FEW_WARPS; ++w) top = fmaxf(top, s.m[w][r]);
-    const float ref = top == NEG_INF ? 0.f : top;
-    for (int w = 0; w < FEW_WARPS; ++w) {
-      const float f = exp2_fast(s.m[w][r] - ref);
-      lsum += s.l[w][r] * f;
-      sum += s.o[w][r][col] * f;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) *reinterpret_cast<float4*>(ring + (group * ROWS + r) * D + c) = o[r];
+  if (u == 0 && (tid & (LANES - 1)) % S::APART == 0)
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+      maxima[group * ROWS + r0 + i] = m[i];
+      totals[group * ROWS + r0 + i] = l[i];
     }
-    s.o[0][r][col] = sum;
+  __syncthreads();
+  constexpr int CELLS = ROWS * D;
+  for (int i = tid; i < CELLS; i += THREADS) {
+    const int r = i / D;
+    float top = NEG_INF, total = 0.f, sum = 0.f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) top = fmaxf(top, maxima[g * ROWS + r]);
+    const float ref = top == NEG_INF ? 0.f : top;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      const float f = exp2_fast(maxima[g * ROWS + r] - ref);
+      total += totals[g * ROWS + r] * f;
+      sum += ring[g * CELLS + i] * f;
+    }
     if (split == 1) {
-      if (r < rows && col < p.d)
-        p.y[((long long)n * p.tq + r / per) * q_row + (long long)(shared * per + r % per) * p.d + col] = lsum > 0.f ? sum / lsum : 0.f;
-      if (r < rows && col == 0)
-        p.lse[((long long)n * p.heads + shared * per + r % per) * p.tq + r / per] = lsum > 0.f ? top + log2f(lsum) : -NEG_INF;
+      store_cell<D>(p, n, shared, i, top, total, sum);
+    } else {
+      float* const to = parts + (long long)blockIdx.x * ROWS * (D + 2);
+      to[i] = sum;
+      if (i % D == 0) to[CELLS + 2 * r] = top, to[CELLS + 2 * r + 1] = total;
     }
   }
-  if (split == 1) return;
-  __syncthreads();                                                   // all have read the warps' m and l
-  if (threadIdx.x < ROWS) {
-    float top = NEG_INF, lsum = 0.f;
-    for (int w = 0; w < FEW_WARPS; ++w) top = fmaxf(top, s.m[w][threadIdx.x]);
+}
+
+// A block per sentence and shared head: the parts of its keys, in their order.
+template <int D, int ROWS>
+__global__ void __launch_bounds__(256) join_parts(const Problem p, int split, const float* parts) {
+  tsb_launch::enter();
+  constexpr int CELLS = ROWS * D;
+  const float* const from = parts + (long long)blockIdx.x * split * ROWS * (D + 2);
+  for (int i = threadIdx.x; i < CELLS; i += 256) {
+    const int r = i / D;
+    float top = NEG_INF, total = 0.f, sum = 0.f;
+    for (int b = 0; b < split; ++b) top = fmaxf(top, load(from + b * ROWS * (D + 2) + CELLS + 2 * r));
     const float ref = top == NEG_INF ? 0.f : top;
-    for (int w = 0; w < FEW_WARPS; ++w) lsum += s.l[w][threadIdx.x] * exp2_fast(s.m[w][threadIdx.x] - ref);
-    s.m[0][threadIdx.x] = top;
-    s.l[0][threadIdx.x] = lsum;
-  }
-  cg::cluster_group cluster = cg::this_cluster();
-  cluster.sync();
-  // every block joins a share of the cells
-  for (int i = part * FEW_WARPS * 32 + threadIdx.x; i < CELLS; i += split * FEW_WARPS * 32) {
-    const int r = i / (LANES * 4), col = i % (LANES * 4);
-    float top = NEG_INF, lsum = 0.f, sum = 0.f;
-    for (int b = 0; b < split; ++b) top = fmaxf(top, *cluster.map_shared_rank(&s.m[0][r], b));
-    const float ref = top == NEG_INF ? 0.f : top;
+#pragma unroll 4
     for (int b = 0; b < split; ++b) {
-      const float f = exp2_fast(*cluster.map_shared_rank(&s.m[0][r], b) - ref);
-      lsum += *cluster.map_shared_rank(&s.l[0][r], b) * f;
-      sum += *cluster.map_shared_rank(&s.o[0][r][col], b) * f;
+      const float* const at = from + b * ROWS * (D + 2);
+      const float f = exp2_fast(load(at + CELLS + 2 * r) - ref);
+      total += load(at + CELLS + 2 * r + 1) * f;
+      sum += load(at + i) * f;
     }
-    if (r < rows && col < p.d)
-      p.y[((long long)n * p.tq + r / per) * q_row + (long long)(shared * per + r % per) * p.d + col] = lsum > 0.f ? sum / lsum : 0.f;
-    if (r < rows && col == 0)
-      p.lse[((long long)n * p.heads + shared * per + r % per) * p.tq + r / per] = lsum > 0.f ? top + log2f(lsum) : -NEG_INF;
+    store_cell<D>(p, blockIdx.x / p.shared, blockIdx.x % p.shared, i, top, total, sum);
   }
-  cluster.sync();                                                    // nobody leaves while others read its shared memory
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -1046,7 +1177,7 @@ int run(K kernel, const Problem& p, long long blocks, int threads, int smem, cud
 
 // Where the pieces of q, k, v and g lie in one buffer, behind them the units and the dots.
 struct Layout {
-  size_t tiles[4], units[4], dots, bytes;
+  size_t tiles[4], units[4], dots, bytes;      // (units and dots on 16-byte boundaries: they are copied in bulk)
   Layout(int n, int tq, int tk, int heads, int shared, int d, bool with_g) {
     const size_t tile = d <= 64 ? Tile<64, 128>::BYTES : Tile<128, 128>::BYTES;
     const size_t q = (size_t)n * heads * ((tq + 127) / 128), k = (size_t)n * shared * ((tk + 127) / 128);
@@ -1058,11 +1189,10 @@ struct Layout {
     }
     for (int i = 0; i < 4; ++i) {
       units[i] = bytes;
-      bytes += count[i] * 4;
+      bytes += (count[i] * 4 + 15) / 16 * 16;
     }
     dots = bytes;
-    if (with_g) bytes += (size_t)n * heads * tq * 4;
-    bytes = (bytes + 15) / 16 * 16;
+    bytes += count[3] * 128 * 4;
   }
   Pieces of(const char* base, int i) const { return {base + tiles[i], reinterpret_cast<const float*>(base + units[i])}; }
 };
@@ -1112,28 +1242,40 @@ int split(const Problem& p, const float* g, const float* y, const Layout& at, ch
                             : tsb_launch::launch(split_tiles<128>, dim3((unsigned)blocks), dim3(256), 0, st, all));
 }
 
-template <int LANES, int ROWS> int run_few(const Problem& p, cudaStream_t st) {
-  constexpr int BATCH = 4, MAX_SPLIT = 8;
-  // a cluster of blocks for a head's keys while SMs are idle and a block keeps four rounds of them
-  const long long pairs = (long long)p.n * p.shared;
-  int split = 1;
-  while (split < MAX_SPLIT && pairs * split * 2 <= 148 * 4 && p.tk >= split * 2 * FEW_WARPS * (32 / LANES) * BATCH) split *= 2;
+template <int D, int ROWS> int run_few(const Problem& p, cudaStream_t st) {
+  using S = FewShape<D, ROWS>;
+  constexpr int SMEM = S::FLOATS * 4;
+  // two blocks to an SM, of eight steps each at least (a block's beginning and end, and the join, cost about as much)
+  const long long pairs = (long long)p.n * p.shared, room = 148 * 2 / pairs, steps = (p.tk + S::KEYS - 1) / S::KEYS;
+  int split = (int)(room < steps / 8 ? room : steps / 8);
+  if (split < 1) split = 1;
   if (pairs * split > INT32_MAX) return TSB_ERR_ARG;
-  return launched(tsb_launch::launch_cluster(split > 1 ? split : 0, attend_few<LANES, ROWS, BATCH>, dim3((unsigned)(pairs * split)),
-                                             dim3(FEW_WARPS * 32), 0, st, p, split));
+  float* parts = nullptr;
+  if (split > 1) {
+    parts = static_cast<float*>(tsb_scratch::get(st, tsb_scratch::ATTENTION_PARTS, (size_t)(pairs * split) * ROWS * (D + 2) * 4));
+    if (!parts) return TSB_ERR_OOM;
+  }
+  static tsb_launch::SmemLimit limit;
+  cudaError_t e = limit.raise(attend_few<D, ROWS>, SMEM);
+  if (e == cudaSuccess)
+    e = tsb_launch::launch(attend_few<D, ROWS>, dim3((unsigned)(pairs * split)), dim3(FEW_WARPS * 32), SMEM, st, p, split, parts);
+  if (e == cudaSuccess && split > 1)
+    e = tsb_launch::launch(join_parts<D, ROWS>, dim3((unsigned)pairs), dim3(256), 0, st, p, split, parts);
+  return launched(e);
 }
-template <int LANES> int few(const Problem& p, int rows, cudaStream_t st) {
-  if (rows <= 1) return run_few<LANES, 1>(p, st);
-  if (rows <= 2) return run_few<LANES, 2>(p, st);
-  if (rows <= 4) return run_few<LANES, 4>(p, st);
-  return run_few<LANES, 8>(p, st);
+template <int D> int few(const Problem& p, int rows, cudaStream_t st) {
+  if (rows <= 1) return run_few<D, 1>(p, st);
+  if (rows <= 2) return run_few<D, 2>(p, st);
+  if (rows <= 4) return run_few<D, 4>(p, st);
+  return run_few<D, 8>(p, st);
 }
 
 }  // namespace
 
 extern "C" {
 
-// y [N, Tq, H, d] and lse [N, H, Tq]: log2 of the sum of the keys' 2^S, +inf for a query without keys.  key may be null.
+// y [N, Tq, H, d], and lse [N, H, Tq up to a multiple of 128]: log2 of the sum of the keys' 2^S, +inf for a query without keys
+// and behind the last one.  key may be null.
 int tsb_cross_attention(const float* q, const float* kv, const float* key, float* y, float* lse, int n, int tq, int tk, int heads,
                         int shared, int d, float scale, void* stream) {
   Problem p;
@@ -1144,7 +1286,7 @@ int tsb_cross_attention(const float* q, const float* kv, const float* key, float
   p.y = y;
   p.lse = lse;
   const long long rows = (long long)(heads / shared) * tq;
-  if (rows <= FEW_ROWS) return d <= 32 ? few<8>(p, (int)rows, st) : d <= 64 ? few<16>(p, (int)rows, st) : few<32>(p, (int)rows, st);
+  if (rows <= FEW_ROWS) return d <= 32 ? few<32>(p, (int)rows, st) : d <= 64 ? few<64>(p, (int)rows, st) : few<128>(p, (int)rows, st);
   const Layout at(n, tq, tk, heads, shared, d, false);
   char* pieces = static_cast<char*>(tsb_scratch::get(st, tsb_scratch::ATTENTION_PIECES, at.bytes));
   if (!pieces) return TSB_ERR_OOM;
@@ -1153,8 +1295,8 @@ int tsb_cross_attention(const float* q, const float* kv, const float* key, float
   if (rc) return rc;
   const long long blocks = (long long)n * heads * p.qtiles;
   static tsb_launch::SmemLimit limit64, limit128;
-  if (d <= 64) return run(attend<64>, p, blocks, 192, ForwardShape<64>::SMEM, st, limit64);
-  return run(attend<128>, p, blocks, 192, ForwardShape<128>::SMEM, st, limit128);
+  if (d <= 64) return run(attend<64>, p, blocks, ForwardShape<64>::BLOCK, ForwardShape<64>::SMEM, st, limit64);
+  return run(attend<128>, p, blocks, ForwardShape<128>::BLOCK, ForwardShape<128>::SMEM, st, limit128);
 }
 
 // The pieces of q, kv and g, and the sums of g y over a head's row, for both gradients.  prepared: `have` bytes on a
@@ -1175,15 +1317,15 @@ int tsb_cross_attention_grad_q(const void* prepared, long long have, const float
   if (!describe(p, n, tq, tk, heads, shared, d, scale, nullptr, nullptr, key, dq)) return TSB_ERR_ARG;
   if (n == 0 || tq == 0) return TSB_OK;
   const Layout at(n, tq, tk, heads, shared, d, true);
-  if (!lse || !dq || !fits(prepared, have, at)) return TSB_ERR_ARG;
+  if (!lse || (reinterpret_cast<uintptr_t>(lse) & 15) || !dq || !fits(prepared, have, at)) return TSB_ERR_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   use(p, at, static_cast<const char*>(prepared));
   p.lse = const_cast<float*>(lse);
   p.dq = dq;
   const long long blocks = (long long)n * heads * p.qtiles;
   static tsb_launch::SmemLimit limit64, limit128;
-  if (d <= 64) return run(grad_of_queries<64>, p, blocks, 192, QueryShape<64>::SMEM, st, limit64);
-  return run(grad_of_queries<128>, p, blocks, 192, QueryShape<128>::SMEM, st, limit128);
+  if (d <= 64) return run(grad_of_queries<64>, p, blocks, QueryShape<64>::BLOCK, QueryShape<64>::SMEM, st, limit64);
+  return run(grad_of_queries<128>, p, blocks, QueryShape<128>::BLOCK, QueryShape<128>::SMEM, st, limit128);
 }
 
 int tsb_cross_attention_grad_kv(const void* prepared, long long have, const float* key, const float* lse, float* dkv, int n, int tq, int tk, int heads,
@@ -1192,7 +1334,7 @@ int tsb_cross_attention_grad_kv(const void* prepared, long long have, const floa
   if (!describe(p, n, tq, tk, heads, shared, d, scale, nullptr, nullptr, key, dkv)) return TSB_ERR_ARG;
   if (n == 0 || tk == 0) return TSB_OK;
   const Layout at(n, tq, tk, heads, shared, d, true);
-  if (!dkv || (tq && !lse) || !fits(prepared, have, at)) return TSB_ERR_ARG;
+  if (!dkv || (tq && !lse) || (reinterpret_cast<uintptr_t>(lse) & 15) || !fits(prepared, have, at)) return TSB_ERR_ARG;
   if ((long long)((tq + 63) / 64) * (heads / shared) > INT32_MAX / 2) return TSB_ERR_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   use(p, at, static_cast<const char*>(prepared));
@@ -1200,8 +1342,8 @@ int tsb_cross_attention_grad_kv(const void* prepared, long long have, const floa
   p.dkv = dkv;
   const long long blocks = (long long)n * shared * p.ktiles;
   static tsb_launch::SmemLimit limit64, limit128;
-  if (d <= 64) return run(grad_of_states<64>, p, blocks, 320, StateShape<64>::SMEM, st, limit64);
-  return run(grad_of_states<128>, p, blocks, 320, StateShape<128>::SMEM, st, limit128);
+  if (d <= 64) return run(grad_of_states<64>, p, blocks, StateShape<64>::BLOCK, StateShape<64>::SMEM, st, limit64);
+  return run(grad_of_states<128>, p, blocks, StateShape<128>::BLOCK, StateShape<128>::SMEM, st, limit128);
 }
 
 }  // extern "C"

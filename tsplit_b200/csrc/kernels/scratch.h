@@ -18,7 +18,7 @@ enum Tag {
   CONV_SPLITK = 0, CONV_FILTER_T = 1, CONV_UPSAMPLE = 2,
   GEMM_SPLITK = 10, GEMM_PAD_A = 11, GEMM_PAD_B = 12,
   NORM_PARTIALS = 20, POOL_ARGMAX = 30, LOSS_ROWS = 31, COLSUM_PARTIALS = 40, EMBED_SORT = 50,
-  ATTENTION_PIECES = 51,
+  ATTENTION_PIECES = 51, ATTENTION_PARTS = 52,
 };
 
 // At least `bytes` (and at least `floor_bytes` when a new buffer has to be obtained); nullptr when the

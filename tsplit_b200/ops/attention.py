@@ -76,8 +76,8 @@ class CrossAttentionOp(Op):
         sizes = _sizes(iv[0].shape, iv[1].shape, iv[2].shape if len(iv) > 2 else None)
         n, tq, _, h, _, d = sizes
         st = node.state
-        if "lse" not in st or st["lse"].shape != (n, h, tq) or st["lse"].ctx != iv[0].ctx:
-            st["lse"] = _rows((n, h, tq), iv[0].ctx)
+        if "lse" not in st or st["lse"].shape != (n, h, _whole_tiles(tq)) or st["lse"].ctx != iv[0].ctx:
+            st["lse"] = _rows((n, h, _whole_tiles(tq)), iv[0].ctx)
         G.cross_attention(iv[0], iv[1], iv[2] if len(iv) > 2 else None, out, st["lse"], sizes, self.scale_of(node, d), stream)
 
     def gradient(self, node, g):
@@ -96,11 +96,15 @@ def _rows(shape, ctx):
     return ndarray.empty(shape, ctx, use_pool=False)
 
 
+def _whole_tiles(t):
+    return -(-t // 128) * 128
+
+
 def _prepared_floats(n, tq, tk, h, shared, d):
     """Length of what the gradients read: tiles of 128 rows and 64 or 128 columns of q, k, v and g, one number for each, and
     one for every row of g."""
-    q, k, columns = n * h * (-(-tq // 128)), n * shared * (-(-tk // 128)), 64 if d <= 64 else 128
-    return -(-((2 * q + 2 * k) * (128 * columns + 1) + n * h * tq) // 4) * 4
+    q, k, columns = n * h * _whole_tiles(tq) // 128, n * shared * _whole_tiles(tk) // 128, 64 if d <= 64 else 128
+    return 128 * columns * 2 * (q + k) + 2 * (-(-q // 4) * 4 + -(-k // 4) * 4) + 128 * q
 
 
 class CrossAttentionPrepareOp(Op):
@@ -147,7 +151,7 @@ class _CrossAttentionGradient(Op):
         key = iv[4] if len(iv) > 4 else None
         sizes = _sizes(iv[2].shape, iv[3].shape, key.shape if key is not None else None)
         lse = node.attrs["fwd"].state.get("lse")
-        assert lse is not None and lse.shape == (sizes[0], sizes[3], sizes[1]) and lse.ctx == out.ctx, \
+        assert lse is not None and lse.shape == (sizes[0], sizes[3], _whole_tiles(sizes[1])) and lse.ctx == out.ctx, \
             "the gradient of a cross attention needs its forward pass on the same device first"
         self._launch(iv[0], key, lse, out, sizes, CrossAttentionOp.scale_of(node, sizes[5]), stream)
 
