@@ -7,9 +7,15 @@
 // makes the row's results NaN and is no alternative itself (id -1 where fewer than `top` others are left).  Equal logits are
 // taken by their column, the lowest first.
 //
-// One pass over the logits: every thread keeps a running (max, Z, sum e^u u).  The top tokens: every warp keeps the best 32
-// it has seen, one per lane, as 64-bit numbers that order by logit and then by column, and collects what is above its
-// bound (the top-th best of any warp of the block) in shared memory until there are 32 of them, which are sorted and merged.
+// One pass over the logits: every thread keeps a running (max, Z, sum e^u u).  The top tokens come from the maxima of units of
+// the row (1 KB or more each that a warp reads in one go; in short rows the 8 columns that a thread reads in one go).  With W
+// warps, a bound that the ceil(top / W)-th best unit of every warp reaches is reached by `top` columns, so by every top token;
+// of the units that reach it the top-th best one is the bound.  Their columns are read again (about `top` KB a row); what reaches the bound, some dozens, is collected in shared memory as
+// 64-bit numbers that order by logit and then by column, and each one's place is how many are larger.  Where more are found
+// than there is room for (ties, many equal units), every warp merges what it finds into a sorted list of the best 32, one
+// per lane, against a rising bound.  (4096 x 128001, 20 alternatives, without any 310 us: such lists in the first pass 572 us,
+// in the second 497, sorting networks in place of counting 415; now 373.)
+// What a row's end takes is latency that other rows on the SM have to cover, so it is kept short.
 // Few rows are split over a cluster of blocks that join through distributed shared memory.
 #include <cuda_runtime.h>
 #include <cooperative_groups.h>
@@ -27,7 +33,8 @@ namespace cg = cooperative_groups;
 using tsb_launch::load;
 typedef unsigned long long u64;
 
-constexpr int MAX_WARPS = 8, MAX_TOP = 32, PENDING = 64, MAX_SPLIT = 8;
+constexpr int MAX_WARPS = 8, MAX_TOP = 32, PENDING = 64, MAX_SPLIT = 8, MAX_UNITS = 1024, FOUND = 512, REACHED = 256;
+constexpr unsigned CHUNK = 64;             // 16-byte pieces that a warp reads in one go, two a lane
 constexpr float NEG_INF = -__builtin_huge_valf();
 constexpr unsigned ALL = 0xffffffffu;
 
@@ -51,19 +58,18 @@ __device__ __forceinline__ float logit_of(u64 key) {
 __device__ __forceinline__ unsigned col_of(u64 key) { return ALL - (unsigned)key; }
 
 __device__ __forceinline__ u64 larger(u64 a, u64 b) { return a > b ? a : b; }
-__device__ __forceinline__ u64 smaller(u64 a, u64 b) { return a < b ? a : b; }
 
 // One compare-exchange of a bitonic network between lanes `d` apart; `falling`: the larger one to the lower lane.
-__device__ __forceinline__ u64 exchange(u64 v, int d, bool falling) {
-  const u64 o = __shfl_xor_sync(ALL, v, d);
-  return (((threadIdx.x & d) == 0) == falling) ? larger(v, o) : smaller(v, o);
+template <class T> __device__ __forceinline__ T exchange(T v, int d, bool falling) {
+  const T o = __shfl_xor_sync(ALL, v, d);
+  return (((threadIdx.x & d) == 0) == falling) == (v > o) ? v : o;
 }
-__device__ __forceinline__ u64 merge_falling(u64 v) {      // a bitonic sequence of 32 into falling order
+template <class T> __device__ __forceinline__ T merge_falling(T v) {      // a bitonic sequence of 32 into falling order
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v = exchange(v, d, true);
   return v;
 }
-__device__ __forceinline__ u64 sort_falling(u64 v) {
+template <class T> __device__ __forceinline__ T sort_falling(T v) {
 #pragma unroll
   for (int size = 2; size < 32; size <<= 1)
 #pragma unroll
@@ -71,7 +77,10 @@ __device__ __forceinline__ u64 sort_falling(u64 v) {
   return merge_falling(v);
 }
 // The best 32 of two falling lists.
-__device__ __forceinline__ u64 best_of(u64 a, u64 b) { return merge_falling(larger(a, __shfl_sync(ALL, b, 31 - (threadIdx.x & 31)))); }
+template <class T> __device__ __forceinline__ T best_of(T a, T b) {
+  const T o = __shfl_sync(ALL, b, 31 - (threadIdx.x & 31));
+  return merge_falling(a > o ? a : o);
+}
 
 struct Sums {
   float m, z, t;               // max, sum e^(x - m), sum e^(x - m) (x - m)
@@ -87,9 +96,10 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
   return r;
 }
 
-// Takes logits of up to N columns into the sums.  What is below every real logit by more than e^-10000 counts as nothing.
+// Takes logits of up to N columns into the sums; their maximum.  What is below every real logit by more than e^-10000 counts as
+// nothing.
 template <int N>
-__device__ __forceinline__ void take(Sums& s, const float (&x)[N]) {
+__device__ __forceinline__ float take(Sums& s, const float (&x)[N]) {
   float m = x[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
@@ -102,15 +112,30 @@ __device__ __forceinline__ void take(Sums& s, const float (&x)[N]) {
     s.z += e;
     s.t += e * fmaxf(u, -1e4f);
   }
+  return m;
+}
+
+__device__ __forceinline__ float warp_max(float v) {     // of numbers: a NaN counts as none
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
 
 struct Shared {
-  u64 pending[MAX_WARPS][PENDING];
-  u64 best[MAX_WARPS][32];
+  union {
+    u64 pending[MAX_WARPS][PENDING];         // of the lists
+    u64 found[FOUND];                        // columns that reach the bound
+  };
+  u64 lists[MAX_WARPS][32];
+  u64 best_of_block[32];
   u64 bound;                   // no key below it is among the top of the row
+  float maxima[MAX_UNITS];     // of the units, a share for every warp
+  float least[MAX_WARPS];      // what each warp has as many units above as it has to
+  float reached[REACHED], refined;           // maxima of the units that reach the first bound; the second bound
+  unsigned units, count;       // how many these are; columns found
+  float lse;                   // of the row; NaN-free rows of -inf: -inf
   Sums sums[MAX_WARPS];
   Sums of_block;
-  u64 best_of_block[32];
 };
 
 // A warp's list of the best, and what waits to be merged into it.
@@ -130,20 +155,15 @@ __device__ __forceinline__ void merge_waiting(Chosen& c, Shared& s, int top, int
   if ((int)lane < c.waiting) s.pending[warp][lane] = s.pending[warp][count + lane];
   __syncwarp();
 }
-// `any`: whether a lane holds something that may be above the bound.  All lanes of the warp call it.
+// Columns col to col + N - 1 of a lane, those below `limit`.  All lanes of the warp call it.
 template <int N>
 __device__ __forceinline__ void choose(Chosen& c, Shared& s, int top, const float (&x)[N], unsigned col, unsigned limit) {
   const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   u64 bound = *(volatile u64*)&s.bound;
-  const float least = bound ? logit_of(bound) : NEG_INF;
-  bool may = false;
-#pragma unroll
-  for (int i = 0; i < N; ++i) may |= x[i] >= least;
-  if (!__any_sync(ALL, may)) return;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const u64 key = order_of(x[i], col + i);
-    const bool in = x[i] >= least && key > bound && col + i < limit;          // (a NaN is not)
+    const bool in = x[i] == x[i] && key > bound && col + i < limit;             // (a NaN is not)
     const unsigned mask = __ballot_sync(ALL, in);
     if (!mask) continue;
     if (in) s.pending[warp][c.waiting + __popc(mask & ((1u << lane) - 1))] = key;
@@ -155,94 +175,251 @@ __device__ __forceinline__ void choose(Chosen& c, Shared& s, int top, const floa
   }
 }
 
+// Of n keys (0: none) the larger ones each at the place that the number of still larger ones tells: put(place, key).
+// Returns how many there are.
+template <class Put> __device__ __forceinline__ unsigned place(const u64* keys, unsigned n, Put put) {
+  unsigned there = 0;
+  for (unsigned t = threadIdx.x; t < n || t == threadIdx.x; t += blockDim.x) {
+    const u64 key = t < n ? keys[t] : 0;
+    unsigned larger = 0;
+    there = 0;
+#pragma unroll 4
+    for (unsigned j = 0; j < n; ++j) {
+      larger += keys[j] > key;
+      there += keys[j] != 0;
+    }
+    if (key) put(larger, key);
+  }
+  return there;
+}
+
 // Grid: (rows * split) blocks in clusters of `split`; a block takes a contiguous part of its row.
 template <bool TOP>
-__global__ void __launch_bounds__(MAX_WARPS * 32) score_rows(const float* x, const float* ids, float* __restrict__ out,
-                                                             long long cols, int top, int split) {
+__global__ void __launch_bounds__(MAX_WARPS * 32, 6) score_rows(const float* x, const float* ids, float* __restrict__ out,
+                                                                long long cols, int top, int split) {
   tsb_launch::enter();
   __shared__ Shared s;
   const long long row = blockIdx.x / split;
   const int part = blockIdx.x % split;
   const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const float* xr = x + row * cols;
+  float* const to = out + row * (3 + 2 * top);
   // whole parts of 4 columns; a part's first columns up to a 16-byte boundary are taken one by one
   const unsigned per = (unsigned)((cols + split - 1) / split + 3) / 4 * 4;
   const unsigned begin = min((long long)part * per, cols), end = min((long long)begin + per, cols);
   const unsigned odd = (unsigned)((-(long long)(reinterpret_cast<uintptr_t>(xr + begin) >> 2)) & 3);
   const unsigned body = min(begin + odd, end), pieces = (end - body) / 4, tail = body + pieces * 4;
-  if (TOP && threadIdx.x == 0) s.bound = 0;
-  if (TOP) __syncthreads();
+  // (the last warp writes the row's numbers: its loads are under way from the start)
+  const long long id = (long long)load(ids + row);
+  const bool given = id >= 0 && id < cols;
+  const float own_x = given && warp == warps - 1 ? load(xr + id) : 0.f;
 
   Sums a{NEG_INF, 0.f, 0.f};
-  Chosen c{0, 0};
   const float4* xv = reinterpret_cast<const float4*>(xr + body);
-  for (unsigned first = 0; first < pieces; first += 2 * blockDim.x) {          // (the same trips for all threads)
-    const unsigned i = first + threadIdx.x, j = i + blockDim.x;
-    const float4 none = make_float4(NEG_INF, NEG_INF, NEG_INF, NEG_INF);
-    const float4 v = i < pieces ? load(xv + i) : none, w = j < pieces ? load(xv + j) : none;
-    const float f[8] = {v.x, v.y, v.z, v.w, w.x, w.y, w.z, w.w};
-    take(a, f);
-    if (TOP) {
-      const float g[4] = {v.x, v.y, v.z, v.w}, h[4] = {w.x, w.y, w.z, w.w};
-      choose(c, s, top, g, body + i * 4, i < pieces ? end : 0);
-      choose(c, s, top, h, body + j * 4, j < pieces ? end : 0);
+  const float4 none = make_float4(NEG_INF, NEG_INF, NEG_INF, NEG_INF);
+  // chunk by chunk, `length` of them a run; a unit is a run, or, in short rows, a lane's part of a chunk
+  const unsigned chunks = (pieces + CHUNK - 1) / CHUNK, share = MAX_UNITS / warps;
+  const unsigned per_warp = (chunks + warps - 1) / warps;
+  const bool lanes_apart = per_warp * 32 <= share;
+  const unsigned length = lanes_apart ? 1 : (per_warp + share - 1) / share;
+  float* const maxima = s.maxima + warp * share;
+  auto get = [&](unsigned chunk, float4& v, float4& w) {
+    const unsigned i = chunk * CHUNK + lane;
+    v = i < pieces ? load(xv + i) : none;
+    w = i + 32 < pieces ? load(xv + i + 32) : none;
+  };
+  if (TOP && threadIdx.x < 32) {
+    s.best_of_block[lane] = 0;
+    if (lane == 0) s.count = s.units = 0, s.refined = NEG_INF;
+  }
+  // this warp's chunks in their order; two are read at a time (it takes some 60 KB under way to an SM to keep memory busy)
+  auto chunk_of = [&](unsigned i) { return length == 1 ? warp + i * warps : (i / length * warps + warp) * length + i % length; };
+  float most = NEG_INF;
+  unsigned units = 0;                        // of this warp
+  auto keep = [&](float m, unsigned i) {     // (a NaN is never a maximum here)
+    if (lanes_apart) {
+      maxima[units + lane] = m;
+      units += 32;
+      return;
+    }
+    most = fmaxf(most, m);
+    if (length > 1 && (i + 1) % length && chunk_of(i + 1) < chunks) return;
+    const float all = warp_max(most);
+    if (lane == 0) maxima[units] = all;
+    ++units;
+    most = NEG_INF;
+  };
+  for (unsigned i = 0; chunk_of(i) < chunks; i += 2) {
+    const bool more = chunk_of(i + 1) < chunks;
+    float4 v[4];
+    get(chunk_of(i), v[0], v[1]);
+    if (more) get(chunk_of(i + 1), v[2], v[3]);
+    const float f[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+    const float m = take(a, f);
+    if (TOP) keep(m, i);
+    if (more) {
+      const float h[8] = {v[2].x, v[2].y, v[2].z, v[2].w, v[3].x, v[3].y, v[3].z, v[3].w};
+      const float n = take(a, h);
+      if (TOP) keep(n, i + 1);
     }
   }
-  {                                                                             // up to three columns at either end
-    const unsigned heads = body - begin, rest = end - tail;
-    const unsigned col = threadIdx.x < heads ? begin + threadIdx.x : tail + (threadIdx.x - heads);
-    const bool in = threadIdx.x < heads + rest;
-    const float f[1] = {in ? load(xr + col) : NEG_INF};
-    if (warp == 0) {
-      take(a, f);
-      if (TOP) choose(c, s, top, f, col, in ? end : 0);
-    }
-  }
+  // up to three columns at either end, a thread of warp 0 each
+  const unsigned heads = body - begin, rest = end - tail;
+  const unsigned odd_col = threadIdx.x < heads ? begin + threadIdx.x : tail + (threadIdx.x - heads);
+  const bool has_odd = threadIdx.x < heads + rest;
+  const float odd_x[1] = {has_odd ? load(xr + odd_col) : NEG_INF};
+  if (warp == 0) take(a, odd_x);
+  {
+    const float m = warp_max(a.m);           // one rescaling, then plain sums
+    a = join(a, Sums{m, 0.f, 0.f});
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1)
-    a = join(a, Sums{__shfl_xor_sync(ALL, a.m, d), __shfl_xor_sync(ALL, a.z, d), __shfl_xor_sync(ALL, a.t, d)});
+    for (int d = 16; d > 0; d >>= 1) {
+      a.z += __shfl_xor_sync(ALL, a.z, d);
+      a.t += __shfl_xor_sync(ALL, a.t, d);
+    }
+  }
   if (lane == 0) s.sums[warp] = a;
+  float least = NEG_INF;
   if (TOP) {
-    merge_waiting(c, s, top, c.waiting);
-    s.best[warp][lane] = c.best;
+    __syncwarp();
+    // the need-th best unit: the best one is taken out that many times less one
+    unsigned gone = 0;                       // of the lane's units (bit k: unit 32 k + lane)
+    for (int need = (top + warps - 1) / warps; need > 0; --need) {
+      float own = NEG_INF;
+      unsigned at = 32;
+      for (unsigned k = 0; k * 32 + lane < units; ++k)
+        if (!(gone >> k & 1) && (at == 32 || maxima[k * 32 + lane] > own)) own = maxima[k * 32 + lane], at = k;
+      least = warp_max(own);
+      const unsigned holders = __ballot_sync(ALL, own == least && at < 32);
+      if (!holders) {                        // fewer units than needed
+        least = NEG_INF;
+        break;
+      }
+      if (lane == __ffs(holders) - 1) gone |= 1u << at;
+    }
+    if (lane == 0) s.least[warp] = least;
   }
   __syncthreads();
-  if (warp == 0) {
-    for (unsigned k = 1; k < warps; ++k) a = join(a, s.sums[k]);
-    if (TOP)
-      for (unsigned k = 1; k < warps; ++k) c.best = best_of(c.best, s.best[k][lane]);
-  }
-  if (split > 1) {
-    cg::cluster_group cluster = cg::this_cluster();
-    if (warp == 0) {
-      if (lane == 0) s.of_block = a;
-      if (TOP) s.best_of_block[lane] = c.best;
-    }
-    cluster.sync();
-    if (part == 0 && warp == 0) {
-      for (int k = 1; k < split; ++k) {
-        a = join(a, *cluster.map_shared_rank(&s.of_block, k));
-        if (TOP) c.best = best_of(c.best, *cluster.map_shared_rank(&s.best_of_block[lane], k));
-      }
-    }
-    cluster.sync();
-    if (part) return;
-  }
-  if (warp) return;
-  float* to = out + row * (3 + 2 * top);
-  const bool empty = a.m == NEG_INF && a.z == 0.f;                              // (NaN leaves z a NaN)
-  const float lse = empty ? NEG_INF : a.m + (float)log((double)a.z);
-  if (lane == 0) {
-    const long long id = (long long)load(ids + row);
-    to[0] = id >= 0 && id < cols ? (empty ? NEG_INF : load(xr + id) - lse) : 0.f;
-    to[1] = empty ? 0.f : (float)(log((double)a.z) - (double)a.t / (double)a.z);
+  auto finish = [&](Sums r) {                // the row's numbers
+    const bool empty = r.m == NEG_INF && r.z == 0.f;                            // (NaN leaves z a NaN)
+    const double z = (double)r.z, log_z = log(z);
+    const float lse = empty ? NEG_INF : r.m + (float)log_z;
+    s.lse = lse;
+    to[0] = given ? (empty ? NEG_INF : own_x - lse) : 0.f;
+    to[1] = empty ? 0.f : (float)(log_z - (double)r.t / z);
     to[2] = lse;
+  };
+  if (warp == warps - 1) {                   // the sums of the block, while the others look for columns
+    a = lane < warps ? s.sums[lane] : Sums{NEG_INF, 0.f, 0.f};
+#pragma unroll
+    for (int d = MAX_WARPS / 2; d > 0; d >>= 1)
+      a = join(a, Sums{__shfl_xor_sync(ALL, a.m, d), __shfl_xor_sync(ALL, a.z, d), __shfl_xor_sync(ALL, a.t, d)});
+    if (lane == 0) {
+      if (split > 1) s.of_block = a;
+      else finish(a);
+    }
   }
-  if (TOP && (int)lane < top) {
-    const float v = c.best ? logit_of(c.best) : __int_as_float(0x7fc00000);
-    to[3 + lane] = empty ? NEG_INF : v - lse;
-    to[3 + top + lane] = c.best ? (float)col_of(c.best) : -1.f;
+  if (!TOP && split == 1) return;
+  auto write = [&](unsigned at, u64 key) {   // an alternative of the row
+    if ((int)at >= top) return;
+    to[3 + at] = s.lse == NEG_INF ? NEG_INF : logit_of(key) - s.lse;
+    to[3 + top + at] = (float)col_of(key);
+  };
+  auto fill = [&](unsigned there) {          // fewer numbers than alternatives
+    if (threadIdx.x >= there && (int)threadIdx.x < top) {
+      to[3 + threadIdx.x] = __int_as_float(0x7fc00000);
+      to[3 + top + threadIdx.x] = -1.f;
+    }
+  };
+  if (TOP) {
+    for (unsigned k = 0; k < warps; ++k) least = fminf(least, s.least[k]);
+    for (unsigned first = 0; first < units; first += 32) {
+      const bool in = first + lane < units && maxima[first + lane] >= least;
+      const unsigned mask = __ballot_sync(ALL, in);
+      unsigned at = 0;
+      if (lane == 0 && mask) at = atomicAdd(&s.units, __popc(mask));            // (their order does not matter)
+      at = __shfl_sync(ALL, at, 0) + __popc(mask & ((1u << lane) - 1));
+      if (in && at < REACHED) s.reached[at] = maxima[first + lane];
+    }
+    __syncthreads();
+    if (s.units <= REACHED) {
+      for (unsigned t = threadIdx.x; t < s.units; t += blockDim.x) {
+        const float v = s.reached[t];
+        int better = 0;
+        for (unsigned j = 0; j < s.units; ++j) better += s.reached[j] > v || (s.reached[j] == v && j < t);
+        if (better == top - 1) s.refined = v;
+      }
+      __syncthreads();
+      least = fmaxf(least, s.refined);
+    }
+    const u64 bound = order_of(least, ALL);  // below every column of that value
+    // every warp its own units again, by chunks: f(columns of a lane, first column, limit)
+    auto again = [&](auto f) {
+      auto both = [&](unsigned chunk, bool mine) {
+        float4 v = none, w = none;
+        if (mine) get(chunk, v, w);
+        const unsigned i = chunk * CHUNK + lane, col = body + i * 4;
+        const float p[4] = {v.x, v.y, v.z, v.w}, q[4] = {w.x, w.y, w.z, w.w};
+        f(p, col, mine && i < pieces ? end : 0);
+        f(q, col + 128, mine && i + 32 < pieces ? end : 0);
+      };
+      if (lanes_apart) {
+        for (unsigned k = 0; k < units; k += 32) {
+          const bool mine = maxima[k + lane] >= least;
+          if (__any_sync(ALL, mine)) both(chunk_of(k / 32), mine);
+        }
+      } else {
+        for (unsigned first = 0; first < units; first += 32)
+          for (unsigned left = __ballot_sync(ALL, first + lane < units && maxima[first + lane] >= least); left; left &= left - 1) {
+            const unsigned at = (first + __ffs(left) - 1) * length;
+            for (unsigned k = at; k < at + length && chunk_of(k) < chunks; ++k) both(chunk_of(k), true);
+          }
+      }
+      if (warp == 0) f(odd_x, odd_col, has_odd ? end : 0);
+    };
+    again([&](const auto& x, unsigned col, unsigned limit) {
+#pragma unroll
+      for (int i = 0; i < (int)(sizeof(x) / sizeof(x[0])); ++i)
+        if (x[i] >= least && col + i < limit) {                                    // (a NaN is not)
+          const unsigned at = atomicAdd(&s.count, 1u);                          // (their order does not matter)
+          if (at < FOUND) s.found[at] = order_of(x[i], col + i);
+        }
+    });
+    __syncthreads();
+    unsigned count = s.count;
+    const u64* keys = s.found;
+    if (count > FOUND) {                     // (the same for all threads)
+      __syncthreads();
+      if (threadIdx.x == 0) s.bound = bound;
+      __syncthreads();
+      Chosen c{0, 0};
+      again([&](const auto& x, unsigned col, unsigned limit) { choose(c, s, top, x, col, limit); });
+      merge_waiting(c, s, top, c.waiting);
+      s.lists[warp][lane] = c.best;
+      __syncthreads();
+      keys = s.lists[0];
+      count = warps * 32;
+    }
+    if (split == 1) {
+      fill(place(keys, count, write));
+      return;
+    }
+    place(keys, count, [&](unsigned at, u64 key) {
+      if (at < 32) s.best_of_block[at] = key;
+    });
   }
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  if (part == 0) {
+    if (TOP)
+      for (int t = threadIdx.x; t < split * top; t += blockDim.x) s.lists[0][t] = *cluster.map_shared_rank(&s.best_of_block[t % top], t / top);
+    if (warp == warps - 1 && lane == 0) {
+      for (int k = 1; k < split; ++k) a = join(a, *cluster.map_shared_rank(&s.of_block, k));
+      finish(a);
+    }
+  }
+  cluster.sync();
+  if (TOP && part == 0) fill(place(s.lists[0], split * top, write));
 }
 
 // dx_c = sum_i w_i (1[c = id_i] - p_c) + w_lse p_c - w_H p_c (log p_c + H), with w the gradient of `out` and the sum over
@@ -307,8 +484,11 @@ int tsb_token_score(const float* x, const float* ids, float* out, long long rows
   // a cluster of blocks for a row while the rows leave SMs idle and a block keeps 2048 columns
   int split = 1;
   while (split < MAX_SPLIT && rows * split * 2 <= 148 && cols >= 4096ll * split) split *= 2;
-  int warps = 1;                         // 16 columns a thread, where the row has as many
-  while (warps < MAX_WARPS && cols / split >= 512ll * warps * 2) warps *= 2;
+  // 16 columns a thread where the row has as many, but eight warps only for few rows or long ones: a row's end is latency,
+  // which more rows on an SM cover (8160 x 32000, 20 alternatives: four warps 234 us, eight 256; 4096 x 128001: 395, 373)
+  const int most = cols / split >= 65536 || rows * split <= 4 * 148 ? MAX_WARPS : MAX_WARPS / 2;
+  int warps = 1;
+  while (warps < most && cols / split >= 512ll * warps * 2) warps *= 2;
   const dim3 grid((unsigned)(rows * split)), block(warps * 32);
   const unsigned cluster = split > 1 ? split : 0;
   if (top)
