@@ -68,8 +68,9 @@ __global__ void __launch_bounds__(256) scaled_lookup(const T* table, const float
 
 // ------------------------------------------------------------------------------------------------ sort
 // Keys are token ids, `vocab` for positions that give no gradient (they end up last).  What fills the last tile behind
-// position n has all bits set, so it stays behind everything in every pass.  Digits of up to 8 bits, the lowest first.  A position's rank among equal digits is counted in the order of the positions: lanes by match.any, the
-// rounds of a warp by a running count, warps and blocks by prefix sums.
+// position n has all bits set, so it stays behind everything in every pass.  Digits of up to 8 bits, the lowest first.  A
+// position's rank among equal digits is counted in the order of the positions: lanes by a ballot for each bit, the rounds of
+// a warp by a running count, warps and blocks by prefix sums.
 constexpr int SORT_THREADS = 1024, SORT_ITEMS = 4, SORT_TILE = SORT_THREADS * SORT_ITEMS, SORT_WARPS = SORT_THREADS / 32;
 constexpr int DIGITS = 256, MAX_CLUSTER = 8;
 constexpr unsigned FILL = 0xffffffffu;
@@ -89,13 +90,18 @@ __device__ __forceinline__ unsigned key_of(const float* ids, long long r, long l
 }
 
 // rank[i]: positions of the same digit before item i in this warp (items of a warp lie 32 apart, lane by lane)
-__device__ __forceinline__ void rank_items(const unsigned (&key)[SORT_ITEMS], int shift, unsigned mask, unsigned* count,
-                                           unsigned (&rank)[SORT_ITEMS]) {
+template <int ITEMS>
+__device__ __forceinline__ void rank_items(const unsigned (&key)[ITEMS], int shift, unsigned mask, unsigned* count, unsigned (&rank)[ITEMS]) {
   const unsigned lane = threadIdx.x & 31;
 #pragma unroll
-  for (int i = 0; i < SORT_ITEMS; ++i) {
+  for (int i = 0; i < ITEMS; ++i) {
     const unsigned d = (key[i] >> shift) & mask;
-    const unsigned same = __match_any_sync(0xffffffffu, d);
+    unsigned same = 0xffffffffu;             // lanes with this digit
+#pragma unroll
+    for (int bit = 0; bit < 8; ++bit) {
+      const unsigned ones = __ballot_sync(0xffffffffu, d >> bit & 1);
+      same &= d >> bit & 1 ? ones : ~ones;
+    }
     const unsigned before = __popc(same & ((1u << lane) - 1));
     const unsigned old = count[d];
     __syncwarp();
@@ -112,12 +118,13 @@ __device__ __forceinline__ void clear_counts(SortShared& s) {
 // Per digit: what lies before each warp, and the block's total.
 __device__ __forceinline__ void scan_warps(SortShared& s) {
   if (threadIdx.x < DIGITS) {
-    unsigned sum = 0;
-#pragma unroll 8
+    unsigned c[SORT_WARPS], sum = 0;         // (all loads before the first store)
+#pragma unroll
+    for (int w = 0; w < SORT_WARPS; ++w) c[w] = s.counts[w][threadIdx.x];
+#pragma unroll
     for (int w = 0; w < SORT_WARPS; ++w) {
-      const unsigned c = s.counts[w][threadIdx.x];
       s.counts[w][threadIdx.x] = sum;
-      sum += c;
+      sum += c[w];
     }
     s.total[threadIdx.x] = sum;
   }
@@ -139,36 +146,48 @@ __device__ __forceinline__ unsigned scan_digits(SortShared& s, unsigned v) {
   return before + sum - v;
 }
 
-// Up to 32768 positions: one cluster of up to eight blocks holds them all in shared memory and trades them through
-// distributed shared memory, one launch for all digits.  The other clusters of the grid fill the table's gradient with
-// zeros meanwhile, which takes longer than the sort for a table of any size.
-__global__ void __launch_bounds__(SORT_THREADS) sort_cluster(const float* ids, long long n, unsigned vocab, long long padding,
-                                                             int bits, int passes, unsigned* __restrict__ out_key,
-                                                             unsigned* __restrict__ out_pos, float* __restrict__ dtable,
-                                                             long long cells, bool aligned) {
+// The table's gradient begins as zeros.  What the sort needs of the chip is little, so the blocks behind those of the sort, in
+// all of its launches, fill a share of it each: part `part` of `parts`, by `blocks` blocks of SORT_THREADS.
+struct Zeros {
+  float* at;
+  long long cells;
+  int part, parts, blocks;
+  bool aligned;
+};
+__device__ __forceinline__ void fill_share(const Zeros& z, unsigned block) {
+  const long long all = z.aligned ? z.cells / 4 : z.cells, begin = all / z.parts * z.part;
+  const long long end = z.part == z.parts - 1 ? all : all / z.parts * (z.part + 1), step = (long long)z.blocks * SORT_THREADS;
+  long long i = begin + (long long)block * SORT_THREADS + threadIdx.x;
+  if (z.aligned) {
+    for (; i < end; i += step) reinterpret_cast<float4*>(z.at)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (z.part == z.parts - 1 && block == 0 && threadIdx.x < z.cells % 4) z.at[z.cells / 4 * 4 + threadIdx.x] = 0.f;
+  } else {
+    for (; i < end; i += step) z.at[i] = 0.f;
+  }
+}
+
+// Up to 32768 positions: one cluster of up to eight blocks keeps them in registers, ITEMS a thread, and trades them through
+// distributed shared memory, one launch for all digits.  Counting the ranks is what takes its time, so as many blocks share it
+// as there are warps to fill (4099 positions, 10007 x 301: two blocks of four a thread 12.5 us, eight of one 8.9).  The other
+// clusters of the grid fill zeros.
+template <int ITEMS>
+__global__ void __launch_bounds__(SORT_THREADS) sort_cluster(const float* ids, long long n, unsigned vocab, long long padding, int bits,
+                                                             int passes, unsigned* __restrict__ out_key, unsigned* __restrict__ out_pos,
+                                                             const Zeros zeros) {
   tsb_launch::enter();
   extern __shared__ uint4 raw[];
+  constexpr unsigned TILE = SORT_THREADS * ITEMS;
   cg::cluster_group cluster = cg::this_cluster();
   const unsigned size = cluster.num_blocks(), me = cluster.block_rank();
-  if (blockIdx.x >= size) {
-    const long long step = (long long)(gridDim.x - size) * SORT_THREADS;
-    long long i = (long long)(blockIdx.x - size) * SORT_THREADS + threadIdx.x;
-    if (aligned) {
-      for (long long j = i; j < cells / 4; j += step) reinterpret_cast<float4*>(dtable)[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-      i += cells / 4 * 4;
-    }
-    for (; i < cells; i += step) dtable[i] = 0.f;
-    return;
-  }
+  if (blockIdx.x >= size) return fill_share(zeros, blockIdx.x - size);
   SortShared& s = *reinterpret_cast<SortShared*>(raw);
-  unsigned* keys = reinterpret_cast<unsigned*>(&s + 1);
-  unsigned* poss = keys + SORT_TILE;
-  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = warp * (32 * SORT_ITEMS) + lane;
+  uint2* const items = reinterpret_cast<uint2*>(&s + 1);
+  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = warp * (32 * ITEMS) + lane;
   const int step = (bits + passes - 1) / passes;
-  unsigned key[SORT_ITEMS], pos[SORT_ITEMS], rank[SORT_ITEMS];
+  unsigned key[ITEMS], pos[ITEMS], rank[ITEMS];
 #pragma unroll
-  for (int i = 0; i < SORT_ITEMS; ++i) {
-    pos[i] = me * SORT_TILE + at + i * 32;
+  for (int i = 0; i < ITEMS; ++i) {
+    pos[i] = me * TILE + at + i * 32;
     key[i] = key_of(ids, pos[i], n, vocab, padding);
   }
   for (int p = 0; p < passes; ++p) {
@@ -182,32 +201,35 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_cluster(const float* ids, l
     cluster.sync();                          // totals are there, and every item is in registers
     unsigned all = 0, mine = 0;
     if (threadIdx.x < DIGITS) {
-      for (unsigned b = 0; b < size; ++b) {
-        const unsigned c = *cluster.map_shared_rank(&s.total[threadIdx.x], b);
-        if (b < me) mine += c;
-        all += c;
+      unsigned c[MAX_CLUSTER];
+#pragma unroll
+      for (unsigned b = 0; b < MAX_CLUSTER; ++b) c[b] = b < size ? *cluster.map_shared_rank(&s.total[threadIdx.x], b) : 0;
+#pragma unroll
+      for (unsigned b = 0; b < MAX_CLUSTER; ++b) {
+        if (b < me) mine += c[b];
+        all += c[b];
       }
     }
     const unsigned before = scan_digits(s, all);
     if (threadIdx.x < DIGITS) s.base[threadIdx.x] = before + mine;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < SORT_ITEMS; ++i) {
+    for (int i = 0; i < ITEMS; ++i) {
       const unsigned d = (key[i] >> shift) & mask;
       const unsigned to = s.base[d] + s.counts[warp][d] + rank[i];
-      *cluster.map_shared_rank(&keys[to % SORT_TILE], to / SORT_TILE) = key[i];
-      *cluster.map_shared_rank(&poss[to % SORT_TILE], to / SORT_TILE) = pos[i];
+      *cluster.map_shared_rank(&items[to % TILE], to / TILE) = make_uint2(key[i], pos[i]);
     }
     cluster.sync();
 #pragma unroll
-    for (int i = 0; i < SORT_ITEMS; ++i) {
-      key[i] = keys[at + i * 32];
-      pos[i] = poss[at + i * 32];
+    for (int i = 0; i < ITEMS; ++i) {
+      const uint2 v = items[at + i * 32];
+      key[i] = v.x;
+      pos[i] = v.y;
     }
   }
 #pragma unroll
-  for (int i = 0; i < SORT_ITEMS; ++i) {
-    const unsigned to = me * SORT_TILE + at + i * 32;
+  for (int i = 0; i < ITEMS; ++i) {
+    const unsigned to = me * TILE + at + i * 32;
     if (to < n) {
       out_key[to] = key[i];
       out_pos[to] = pos[i];
@@ -232,8 +254,9 @@ __device__ __forceinline__ void load_items(const float* ids, const unsigned* in_
 
 __global__ void __launch_bounds__(SORT_THREADS) tile_histogram(const float* ids, const unsigned* in_key, long long n,
                                                                unsigned vocab, long long padding, int shift, unsigned mask,
-                                                               unsigned* __restrict__ hist, unsigned tiles) {
+                                                               unsigned* __restrict__ hist, unsigned tiles, const Zeros zeros) {
   tsb_launch::enter();
+  if (blockIdx.x >= tiles) return fill_share(zeros, blockIdx.x - tiles);
   __shared__ unsigned count[DIGITS];
   if (threadIdx.x < DIGITS) count[threadIdx.x] = 0;
   __syncthreads();
@@ -248,8 +271,9 @@ __global__ void __launch_bounds__(SORT_THREADS) tile_histogram(const float* ids,
   if (threadIdx.x < DIGITS) hist[(size_t)threadIdx.x * tiles + blockIdx.x] = count[threadIdx.x];
 }
 
-__global__ void __launch_bounds__(1024) scan_histogram(unsigned* hist, unsigned entries) {
+__global__ void __launch_bounds__(1024) scan_histogram(unsigned* hist, unsigned entries, const Zeros zeros) {
   tsb_launch::enter();
+  if (blockIdx.x) return fill_share(zeros, blockIdx.x - 1);
   __shared__ unsigned sums[32];
   __shared__ unsigned carry;
   if (threadIdx.x == 0) carry = 0;
@@ -285,8 +309,10 @@ __global__ void __launch_bounds__(1024) scan_histogram(unsigned* hist, unsigned 
 __global__ void __launch_bounds__(SORT_THREADS) scatter_tiles(const float* ids, const unsigned* in_key, const unsigned* in_pos,
                                                               long long n, unsigned vocab, long long padding, int shift,
                                                               unsigned mask, const unsigned* hist, unsigned tiles,
-                                                              unsigned* __restrict__ out_key, unsigned* __restrict__ out_pos) {
+                                                              unsigned* __restrict__ out_key, unsigned* __restrict__ out_pos,
+                                                              const Zeros zeros) {
   tsb_launch::enter();
+  if (blockIdx.x >= tiles) return fill_share(zeros, blockIdx.x - tiles);
   extern __shared__ uint4 raw[];
   SortShared& s = *reinterpret_cast<SortShared*>(raw);
   unsigned key[SORT_ITEMS], pos[SORT_ITEMS], rank[SORT_ITEMS];
@@ -310,10 +336,9 @@ __global__ void __launch_bounds__(SORT_THREADS) scatter_tiles(const float* ids, 
   }
 }
 
-template <class T>
-__global__ void __launch_bounds__(256) fill_zero(T* __restrict__ y, long long n) {
+__global__ void __launch_bounds__(SORT_THREADS) fill_zero(const Zeros zeros) {
   tsb_launch::enter();
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) y[i] = zero<T>();
+  fill_share(zeros, blockIdx.x);
 }
 
 // ------------------------------------------------------------------------------------------------ sums
@@ -373,15 +398,17 @@ __global__ void __launch_bounds__(256) join_tokens(const T* part, const unsigned
   const unsigned tile = blockIdx.x;
   const long long begin = tile * (long long)size, end = begin + size;
   if (end >= n) return;
-  const unsigned token = load(key + end - 1);
-  if (token == vocab || load(key + end) != token) return;
-  if (begin > 0 && load(key + begin - 1) == token) return;             // it began earlier
-  // the last tile that holds the token
+  const unsigned token = load(key + end - 1), after = load(key + end), before = begin > 0 ? load(key + begin - 1) : vocab;
+  if (token == vocab || after != token || before == token) return;     // it does not go on, or began earlier
+  // the last tile that holds the token: 32 places at a time
   unsigned lo = tile + 1, hi = tiles - 1;
   while (lo < hi) {
-    const unsigned mid = lo + (hi - lo + 1) / 2;
-    if (load(key + (long long)mid * size) == token) lo = mid;
-    else hi = mid - 1;
+    const unsigned step = (hi - lo + 31) / 32, at = min(lo + (threadIdx.x + 1) * step, hi);
+    const unsigned more = __popc(__ballot_sync(0xffffffffu, load(key + (long long)at * size) == token));
+    // (a place that is hi again counts as often as it is looked at)
+    const unsigned next = min(lo + more * step, hi);
+    hi = min(next + step - 1, hi);
+    lo = next;
   }
   const unsigned rows = lo - tile + 1;                                 // partial rows: its tail, then the heads
   const unsigned c = blockIdx.y * 32 + threadIdx.x, group = threadIdx.y;
@@ -412,6 +439,17 @@ int bits_of(long long v) {
   int b = 1;
   while (b < 32 && (v >> b)) ++b;
   return b;
+}
+
+template <int ITEMS>
+cudaError_t sort_in_cluster(const float* ids, long long n, long long vocab, long long padding, int bits, int passes, unsigned* key,
+                            unsigned* pos, const Zeros& zeros, unsigned blocks, cudaStream_t st) {
+  constexpr int smem = (int)sizeof(SortShared) + SORT_THREADS * ITEMS * 8;
+  static tsb_launch::SmemLimit limit;
+  const cudaError_t e = limit.raise(sort_cluster<ITEMS>, smem);
+  if (e != cudaSuccess) return e;
+  return tsb_launch::launch_cluster(blocks, sort_cluster<ITEMS>, dim3(blocks + zeros.blocks), dim3(SORT_THREADS), smem, st, ids, n,
+                                    (unsigned)vocab, padding, bits, passes, key, pos, zeros);
 }
 
 template <class T>
@@ -458,40 +496,33 @@ int tsb_embedding_sorted_grad(const float* g, const float* ids, float* dtable, l
   const long long cells = vocab * dim;
   const bool out16 = (reinterpret_cast<uintptr_t>(dtable) & 15) == 0;
   const bool v4 = dim % 4 == 0 && out16 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
-  const bool cluster_sort = n <= (long long)MAX_CLUSTER * SORT_TILE;
-  if (n == 0 || !cluster_sort) {
-    const cudaError_t e =
-        out16 && cells % 4 == 0
-            ? tsb_launch::launch(fill_zero<float4>, dim3(148 * 8), dim3(256), 0, st, reinterpret_cast<float4*>(dtable), cells / 4)
-            : tsb_launch::launch(fill_zero<float>, dim3(148 * 8), dim3(256), 0, st, dtable, cells);
-    if (e != cudaSuccess || n == 0) return launch_status(e);
-  }
+  const bool one_cluster = n <= (long long)MAX_CLUSTER * SORT_TILE;
+  Zeros zeros{dtable, cells, 0, 1, 2 * 148, out16};
+  if (n == 0) return launch_status(tsb_launch::launch(fill_zero, dim3(zeros.blocks), dim3(SORT_THREADS), 0, st, zeros));
   const int size = n <= 16384 ? 16 : MAX_TILE;
   const unsigned tiles = (unsigned)((n + size - 1) / size);
   const unsigned sort_tiles = (unsigned)((n + SORT_TILE - 1) / SORT_TILE);
   const size_t list = ((size_t)n * 4 + 255) / 256 * 256;
-  const size_t hist_bytes = cluster_sort ? 0 : (size_t)DIGITS * sort_tiles * 4;
+  const size_t hist_bytes = one_cluster ? 0 : (size_t)DIGITS * sort_tiles * 4;
   const size_t part_bytes = (size_t)2 * tiles * dim * 4;
-  char* base = static_cast<char*>(tsb_scratch::get(st, tsb_scratch::EMBED_SORT, list * (cluster_sort ? 2 : 4) + hist_bytes + part_bytes));
+  char* base = static_cast<char*>(tsb_scratch::get(st, tsb_scratch::EMBED_SORT, list * (one_cluster ? 2 : 4) + hist_bytes + part_bytes));
   if (!base) return TSB_ERR_OOM;
   unsigned* key[2] = {reinterpret_cast<unsigned*>(base), nullptr};
   unsigned* pos[2] = {reinterpret_cast<unsigned*>(base + list), nullptr};
   char* rest = base + 2 * list;
   const int bits = bits_of(vocab), passes = (bits + 7) / 8, step = (bits + passes - 1) / passes;
   int last = 0;
-  if (cluster_sort) {
+  if (one_cluster) {
     unsigned blocks = 1;
-    while (blocks < sort_tiles) blocks *= 2;
-    // zeros: 64 KB a block, in whole clusters, as many as the chip takes beside the sort
-    long long fillers = (cells * 4 + 65535) / 65536;
-    if (fillers > 148) fillers = 148;
-    fillers = (fillers + blocks - 1) / blocks * blocks;
-    const int smem = (int)sizeof(SortShared) + SORT_TILE * 8;
-    static tsb_launch::SmemLimit limit;
-    cudaError_t e = limit.raise(sort_cluster, smem);
-    if (e == cudaSuccess)
-      e = tsb_launch::launch_cluster(blocks, sort_cluster, dim3(blocks + (unsigned)fillers), dim3(SORT_THREADS), smem, st, ids, n,
-                                     (unsigned)vocab, padding, bits, passes, key[0], pos[0], dtable, cells, out16);
+    while (blocks < MAX_CLUSTER && (long long)blocks * SORT_THREADS < n) blocks *= 2;
+    // zeros: 64 KB a block, in whole clusters, as many as run at once beside the sort (two to an SM: 8192 x 32000 x 512 takes
+    // 16 us so, 20 us with 128)
+    const long long fillers = (cells * 4 + 65535) / 65536;
+    zeros.blocks = (int)((fillers < 2 * 148 ? fillers : 2 * 148) + blocks - 1) / blocks * blocks;
+    const cudaError_t e =
+        n <= blocks * SORT_THREADS * 1ll   ? sort_in_cluster<1>(ids, n, vocab, padding, bits, passes, key[0], pos[0], zeros, blocks, st)
+        : n <= blocks * SORT_THREADS * 2ll ? sort_in_cluster<2>(ids, n, vocab, padding, bits, passes, key[0], pos[0], zeros, blocks, st)
+                                           : sort_in_cluster<4>(ids, n, vocab, padding, bits, passes, key[0], pos[0], zeros, blocks, st);
     if (e != cudaSuccess) return launch_status(e);
   } else {
     key[1] = reinterpret_cast<unsigned*>(rest);
@@ -499,17 +530,21 @@ int tsb_embedding_sorted_grad(const float* g, const float* ids, float* dtable, l
     unsigned* hist = reinterpret_cast<unsigned*>(rest + 2 * list);
     rest += 2 * list + hist_bytes;
     const unsigned mask = (1u << step) - 1;
+    zeros.parts = 3 * passes;
     for (int p = 0; p < passes; ++p) {
       const unsigned* in_key = p ? key[(p + 1) & 1] : nullptr;
       const unsigned* in_pos = p ? pos[(p + 1) & 1] : nullptr;
       last = p & 1;
-      cudaError_t e = tsb_launch::launch(tile_histogram, dim3(sort_tiles), dim3(SORT_THREADS), 0, st, ids, in_key, n,
-                                         (unsigned)vocab, padding, p * step, mask, hist, sort_tiles);
+      cudaError_t e = tsb_launch::launch(tile_histogram, dim3(sort_tiles + zeros.blocks), dim3(SORT_THREADS), 0, st, ids, in_key, n,
+                                         (unsigned)vocab, padding, p * step, mask, hist, sort_tiles, zeros);
+      ++zeros.part;
       if (e == cudaSuccess)
-        e = tsb_launch::launch(scan_histogram, dim3(1), dim3(1024), 0, st, hist, DIGITS * sort_tiles);
+        e = tsb_launch::launch(scan_histogram, dim3(1 + zeros.blocks), dim3(SORT_THREADS), 0, st, hist, DIGITS * sort_tiles, zeros);
+      ++zeros.part;
       if (e == cudaSuccess)
-        e = tsb_launch::launch(scatter_tiles, dim3(sort_tiles), dim3(SORT_THREADS), sizeof(SortShared), st, ids, in_key, in_pos, n,
-                               (unsigned)vocab, padding, p * step, mask, hist, sort_tiles, key[last], pos[last]);
+        e = tsb_launch::launch(scatter_tiles, dim3(sort_tiles + zeros.blocks), dim3(SORT_THREADS), sizeof(SortShared), st, ids, in_key, in_pos,
+                               n, (unsigned)vocab, padding, p * step, mask, hist, sort_tiles, key[last], pos[last], zeros);
+      ++zeros.part;
       if (e != cudaSuccess) return launch_status(e);
     }
   }
