@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(ForwardShape<D>::BLOCK, ForwardShape<D>::TWO ?
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bar->tmem;
+  const uint32_t tmem = __shfl_sync(ALL, bar->tmem, 0);
   tsb_launch::enter();
 
   const int qt = blockIdx.x % p.qtiles, h = blockIdx.x / p.qtiles % p.heads, n = blockIdx.x / p.qtiles / p.heads;
@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(QueryShape<D>::BLOCK, QueryShape<D>::TWO ? 2 :
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bar->tmem;
+  const uint32_t tmem = __shfl_sync(ALL, bar->tmem, 0);
   tsb_launch::enter();
 
   const int qt = blockIdx.x % p.qtiles, h = blockIdx.x / p.qtiles % p.heads, n = blockIdx.x / p.qtiles / p.heads;
@@ -770,7 +770,7 @@ __global__ void __launch_bounds__(StateShape<D>::BLOCK, 1) grad_of_states(const 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bar->tmem;
+  const uint32_t tmem = __shfl_sync(ALL, bar->tmem, 0);
   tsb_launch::enter();
 
   const int kt = blockIdx.x % p.ktiles, shared = blockIdx.x / p.ktiles % p.shared, n = blockIdx.x / p.ktiles / p.shared;
