@@ -19,12 +19,15 @@ def extra(p):
     p.add_argument("--maxlen2", type=int, default=256)
     p.add_argument("--dropout_rate", type=float, default=0.0)
     p.add_argument("--lr", type=float, default=0.0003)
+    p.add_argument("--scaled_embedding", type=int, default=0, help="1: lookup and scale of the tokens in one operator")
+    p.add_argument("--cross_attention", type=int, default=0, help="1: the decoder's attention over the encoder in one operator")
 
 
 def run(batch_size, args, ctx):
     t = transformer(vocab_size=args.vocab_size, d_model=args.d_model, d_ff=args.d_ff, num_blocks=args.num_blocks,
                     num_heads=args.num_heads, maxlen1=args.maxlen1, maxlen2=args.maxlen2,
-                    dropout_rate=args.dropout_rate, batch_size=batch_size)
+                    dropout_rate=args.dropout_rate, batch_size=batch_size, scaled_embedding=args.scaled_embedding,
+                    cross_attention=args.cross_attention)
     opt = optimizer.AdamOptimizer(args.lr, ctx=ctx)
     train = opt.minimize(t.loss)
     attach(opt, args.comm)

@@ -16,7 +16,7 @@ from .common import Params
 class TransformerConfig(object):
     def __init__(self, vocab_size=32000, d_model=512, num_heads=8, d_ff=2048, num_blocks=6, maxlen1=256,
                  maxlen2=256, dropout_rate=0.0, layer_norm=True, batch_size=8, head_layout=True,
-                 fused_softmax=True):
+                 fused_softmax=True, scaled_embedding=False, cross_attention=False):
         self.vocab_size, self.d_model, self.num_heads, self.d_ff = vocab_size, d_model, num_heads, d_ff
         self.num_blocks, self.maxlen1, self.maxlen2 = num_blocks, maxlen1, maxlen2
         self.dropout_rate, self.layer_norm, self.batch_size = dropout_rate, layer_norm, batch_size
@@ -24,6 +24,12 @@ class TransformerConfig(object):
         self.head_layout = bool(head_layout) and os.environ.get("TSPLIT_HEAD_LAYOUT", "1") != "0"
         #: scale + padding mask + causal mask + soft-max as one operator (``ad.masked_softmax_op``)
         self.fused_softmax = bool(fused_softmax) and os.environ.get("TSPLIT_FUSED_SOFTMAX", "1") != "0"
+        #: lookup and scale of the tokens in one operator whose gradient is summed in one fixed order, padding (token 0)
+        #: without any (``ad.scaled_embedding_op``)
+        self.scaled_embedding = bool(scaled_embedding)
+        #: the decoder's attention over the encoder's states as one operator that keeps no scores and fp32 accuracy; keys and
+        #: values come from one projection ``<name>_kv`` (``ad.cross_attention_op``; not with dropout of the probabilities)
+        self.cross_attention = bool(cross_attention) and not dropout_rate
 
 
 class TransformerModel(object):
@@ -110,6 +116,16 @@ class TransformerModel(object):
         out = ad.array_reshape_op(self.dense(ad.array_reshape_op(out, (-1, d)), d, d, name + "_o"), (N, Tq, d))
         return self.norm(out + q_in, name)
 
+    def attention_across(self, q_in, states, Tq, Tk, name, key_tokens):
+        """What :meth:`attention` computes without a causal mask, from queries over the states of another sequence."""
+        hp = self.hp
+        N, H, d = hp.batch_size, hp.num_heads, hp.d_model
+        q = ad.array_reshape_op(self.dense(ad.array_reshape_op(q_in, (-1, d)), d, d, name + "_q"), (N, Tq, H, d // H))
+        kv = ad.array_reshape_op(self.dense(ad.array_reshape_op(states, (-1, d)), d, 2 * d, name + "_kv"), (N, Tk, 2, H, d // H))
+        ctx = ad.cross_attention_op(q, kv, key_tokens)
+        out = ad.array_reshape_op(self.dense(ad.array_reshape_op(ctx, (-1, d)), d, d, name + "_o"), (N, Tq, d))
+        return self.norm(out + q_in, name)
+
     def ff(self, x, T, name):
         hp = self.hp
         h = ad.array_reshape_op(x, (-1, hp.d_model))
@@ -118,7 +134,9 @@ class TransformerModel(object):
         return self.norm(ad.array_reshape_op(h, (hp.batch_size, T, hp.d_model)) + x, name + "_ff")
 
     def embed(self, tokens, T, maxlen, name):
-        e = ad.embedding_lookup_op(self.embeddings, tokens) * (self.hp.d_model ** 0.5)
+        scale = self.hp.d_model ** 0.5
+        e = (ad.scaled_embedding_op(self.embeddings, tokens, scale=scale, padding_id=0) if self.hp.scaled_embedding
+             else ad.embedding_lookup_op(self.embeddings, tokens) * scale)
         return e + self.positional(tokens, T, maxlen, name)
 
     # -- model -----------------------------------------------------------------------
@@ -132,7 +150,8 @@ class TransformerModel(object):
         dec = self.embed(self.ys_in, T2, hp.maxlen2, "dec")
         for i in range(hp.num_blocks):
             dec = self.attention(dec, dec, T2, T2, "dec%d_self" % i, key_tokens=self.ys_in, causal=True)
-            dec = self.attention(dec, enc, T2, T1, "dec%d_cross" % i, key_tokens=self.xs)
+            across = self.attention_across if hp.cross_attention else self.attention
+            dec = across(dec, enc, T2, T1, "dec%d_cross" % i, key_tokens=self.xs)
             dec = self.ff(dec, T2, "dec%d" % i)
         logits = ad.matmul_op(ad.array_reshape_op(dec, (-1, hp.d_model)), self.embeddings, trans_B=True)
         self.logits = logits
@@ -140,6 +159,12 @@ class TransformerModel(object):
         eps = 0.1
         smooth = ad.addbyconst_op(ad.mul_byconst_op(onehot, 1 - eps), eps / hp.vocab_size)
         return ad.softmaxcrossentropy_op(logits, smooth)
+
+    def token_scores(self, top_k=0):
+        """What the model says about the target tokens ``ys_out``: [positions, 3 + 2 * top_k] with each one's log probability,
+        the entropy, the log-sum-exp, and the ``top_k`` likeliest tokens' log probabilities and ids
+        (``ad.token_log_prob_op``)."""
+        return ad.token_log_prob_op(self.logits, self.ys_out, top_k)
 
     def synthetic_batch(self, seed=0):
         hp = self.hp

@@ -75,10 +75,8 @@ class CrossAttentionOp(Op):
     def gpu_compute(self, node, iv, out, stream):
         sizes = _sizes(iv[0].shape, iv[1].shape, iv[2].shape if len(iv) > 2 else None)
         n, tq, _, h, _, d = sizes
-        st = node.state
-        if "lse" not in st or st["lse"].shape != (n, h, _whole_tiles(tq)) or st["lse"].ctx != iv[0].ctx:
-            st["lse"] = _rows((n, h, _whole_tiles(tq)), iv[0].ctx)
-        G.cross_attention(iv[0], iv[1], iv[2] if len(iv) > 2 else None, out, st["lse"], sizes, self.scale_of(node, d), stream)
+        G.cross_attention(iv[0], iv[1], iv[2] if len(iv) > 2 else None, out, _row_sums(node, sizes, iv[0].ctx), sizes,
+                          self.scale_of(node, d), stream)
 
     def gradient(self, node, g):
         return cross_attention_gradient_op(node, g) + [None] * (len(node.inputs) - 2)
@@ -91,9 +89,14 @@ class CrossAttentionOp(Op):
         return 4.0 * np.prod(s[0]) * s[1][1]
 
 
-def _rows(shape, ctx):
-    from .. import ndarray
-    return ndarray.empty(shape, ctx, use_pool=False)
+def _row_sums(node, sizes, ctx, make=True):
+    """The rows' log-sum-exps, which the forward kernel leaves for the gradients: an array for every size that the node has run
+    at, since a step that was captured at one goes on using its own."""
+    key = ("lse", sizes, ctx)
+    if key not in node.state and make:
+        from .. import ndarray
+        node.state[key] = ndarray.empty((sizes[0], sizes[3], _whole_tiles(sizes[1])), ctx, use_pool=False)
+    return node.state.get(key)
 
 
 def _whole_tiles(t):
@@ -150,9 +153,8 @@ class _CrossAttentionGradient(Op):
     def gpu_compute(self, node, iv, out, stream):
         key = iv[4] if len(iv) > 4 else None
         sizes = _sizes(iv[2].shape, iv[3].shape, key.shape if key is not None else None)
-        lse = node.attrs["fwd"].state.get("lse")
-        assert lse is not None and lse.shape == (sizes[0], sizes[3], _whole_tiles(sizes[1])) and lse.ctx == out.ctx, \
-            "the gradient of a cross attention needs its forward pass on the same device first"
+        lse = _row_sums(node.attrs["fwd"], sizes, out.ctx, make=False)
+        assert lse is not None, "the gradient of a cross attention needs its forward pass on the same device first"
         self._launch(iv[0], key, lse, out, sizes, CrossAttentionOp.scale_of(node, sizes[5]), stream)
 
     def gradient(self, node, g):
