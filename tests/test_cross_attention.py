@@ -8,7 +8,7 @@ from tsplit_b200 import ndarray, gpu_ops as ad
 #: a pair of fp16 pieces keeps a number to 2^-22, the product of the low pieces that is left out is another 2^-22
 PIECE = 2.0 ** -22
 #: fp16 ends at 2^-25 (half of its last step): of a tile whose largest number is at least 2^13, of dS whose bound
-#: d (2 max|g|) (2 max|v|) + max|dot| is at least 2^14, of P whose 1 is 2^14
+#: |g| |v| + max|dot| (of the longest rows) is at least 2^14, of P whose 1 is 2^14
 TILE, LAST = 2.0 ** -38, 2.0 ** -39
 
 
@@ -51,7 +51,7 @@ def definition(q, kv, key, scale, g):
             tol[0][b, :, j] = dy
             ddp = np.abs(gg) @ np.abs(v).T * step + TILE * (ag * np.abs(v).sum(1)[None, :] + av * np.abs(gg).sum(1)[:, None])
             ddot = (np.abs(gg) * dy).sum(1, keepdims=True) + d * 2.0 ** -23 * (np.abs(gg) * np.abs(y)).sum(1, keepdims=True)
-            dds = abs(scale) * p * (ddp + ddot) + rel * np.abs(ds) + abs(scale) * LAST * (4 * d * ag * av + np.abs(dot).max(initial=0))
+            dds = abs(scale) * p * (ddp + ddot) + rel * np.abs(ds) + abs(scale) * LAST * (1.1 * np.sqrt((gg ** 2).sum(1).max(initial=0) * (v ** 2).sum(1).max()) + np.abs(dot).max(initial=0))
             tol[1][b, :, j] = dds @ np.abs(k) + long * (np.abs(ds) @ np.abs(k)) + TILE * ak * np.abs(ds).sum(1, keepdims=True)
             tol[2][b, kept, 0, t] += dds.T @ np.abs(qq) + long * (np.abs(ds).T @ np.abs(qq)) + TILE * aq * np.abs(ds).sum(0)[:, None]
             tol[2][b, kept, 1, t] += (rel * p + LAST).T @ np.abs(gg) + long * (p.T @ np.abs(gg)) + TILE * ag * p.sum(0)[:, None]

@@ -35,10 +35,10 @@ using tsb_launch::load;
 constexpr float NEG_INF = -__builtin_huge_valf(), LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr unsigned ALL = 0xffffffffu;
 
-// Tiles of pieces, [n][head][tile], and what a number of each tile stands for.
+// Tiles of pieces, [n][head][tile], and of each tile what a number of it stands for (x) and the length of its longest row (y).
 struct Pieces {
   const char* tiles;
-  const float* units;
+  const float2* units;
 };
 
 struct Problem {
@@ -86,7 +86,7 @@ struct Source {
   const float* tokens;                       // [n][t], a row whose token is 0 counts as zeros and is not read; or null
   float* dots;
   char* tiles;
-  float* units;
+  float2* units;
   long long batch, row, head;                // strides
   int rows, heads, count;                    // rows of a batch; tiles of a head
   float mult;
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(256) split_tiles(const Sources all) {
   tsb_launch::enter();
   using L = Tile<D, 128>;
   constexpr int UNITS = D / 8, TRIPS = 128 * UNITS / 256;
-  __shared__ uint32_t largest[8];
+  __shared__ uint32_t largest[8], longest[8];
   int which = 0;
   while ((int)blockIdx.x >= all.first[which + 1]) ++which;
   const Source& s = all.s[which];
@@ -144,22 +144,33 @@ __global__ void __launch_bounds__(256) split_tiles(const Sources all) {
       if (i % UNITS == 0) s.dots[(size_t)b * 128 + row] = sum;
     }
   }
-  uint32_t most = 0;
+  uint32_t most = 0, most_squares = 0;
 #pragma unroll
-  for (int u = 0; u < TRIPS; ++u)
+  for (int u = 0; u < TRIPS; ++u) {
+    float squares = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       v[u][k] *= s.mult;
       most = max(most, __float_as_uint(v[u][k]) & 0x7fffffffu);
+      squares += v[u][k] * v[u][k];
     }
+#pragma unroll
+    for (int o = UNITS / 2; o > 0; o >>= 1) squares += __shfl_xor_sync(ALL, squares, o);
+    most_squares = max(most_squares, __float_as_uint(squares));
+  }
   most = __reduce_max_sync(ALL, most);
-  if ((threadIdx.x & 31) == 0) largest[threadIdx.x >> 5] = most;
+  most_squares = __reduce_max_sync(ALL, most_squares);
+  if ((threadIdx.x & 31) == 0) largest[threadIdx.x >> 5] = most, longest[threadIdx.x >> 5] = most_squares;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 8; ++w) most = max(most, largest[w]);
+  for (int w = 0; w < 8; ++w) most = max(most, largest[w]), most_squares = max(most_squares, longest[w]);
   const int e = exponent_to(most, TOP);
   const float scale = power_of_two(e);
-  if (threadIdx.x == 0) s.units[b] = power_of_two(-e);
+  // (a row whose squares overflow, or vanish, has its largest number instead)
+  if (threadIdx.x == 0) {
+    const float length = sqrtf(__uint_as_float(most_squares)), least = __uint_as_float(most);
+    s.units[b] = make_float2(power_of_two(-e), length < 1e15f && length > 1e-15f ? length : least * (float)D);
+  }
   char* out = s.tiles + (size_t)b * L::BYTES;
 #pragma unroll
   for (int u = 0; u < TRIPS; ++u) {
@@ -226,34 +237,36 @@ __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uin
 }
 constexpr uint32_t DESC_HI = smem_desc_hi(1024);       // 128-byte swizzle, groups of eight rows 1024 bytes apart
 
-// D [128 x ROWS_B] = A B^T over the D columns of both tiles.
+// D [128 x ROWS_B] = A B^T over the D columns of both tiles.  The small products come first: a step of tcgen05 drops what is below
+// the last bit of the sum so far, and the sum is at its full size for a third of the steps only (700 x 900, 128 columns: y off by
+// 4.9e-7 in place of 1.2e-6, plain fp32 operators 6.7e-7).
 template <int D, int ROWS_A, int ROWS_B>
 __device__ __forceinline__ void product_of_rows(uint32_t to, uint32_t a, uint32_t b) {
   using LA = Tile<D, ROWS_A>;
   using LB = Tile<D, ROWS_B>;
   const uint32_t al = smem_desc_lo(a, 16), bl = smem_desc_lo(b, 16);
+  auto at = [&](int k, uint32_t lo, int chunk) { return smem_desc_join(DESC_HI, lo + ((k / 4 * chunk + k % 4 * 32) >> 4)); };
 #pragma unroll
   for (int k = 0; k < D / 16; ++k) {
-    const uint32_t ao = (k / 4 * LA::CHUNK + k % 4 * 32) >> 4, bo = (k / 4 * LB::CHUNK + k % 4 * 32) >> 4;
-    const uint64_t ah = smem_desc_join(DESC_HI, al + ao), bh = smem_desc_join(DESC_HI, bl + bo);
-    const uint64_t a2 = smem_desc_join(DESC_HI, al + ao + (LA::PLANE >> 4)), b2 = smem_desc_join(DESC_HI, bl + bo + (LB::PLANE >> 4));
-    mma_smem(to, ah, bh, idesc_f16(ROWS_B, 0), k > 0);
-    mma_smem(to, ah, b2, idesc_f16(ROWS_B, 0), 1);
-    mma_smem(to, a2, bh, idesc_f16(ROWS_B, 0), 1);
+    mma_smem(to, at(k, al, LA::CHUNK), at(k, bl + (LB::PLANE >> 4), LB::CHUNK), idesc_f16(ROWS_B, 0), k > 0);
+    mma_smem(to, at(k, al + (LA::PLANE >> 4), LA::CHUNK), at(k, bl, LB::CHUNK), idesc_f16(ROWS_B, 0), 1);
   }
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) mma_smem(to, at(k, al, LA::CHUNK), at(k, bl, LB::CHUNK), idesc_f16(ROWS_B, 0), 1);
 }
 // D [128 x D] = A B, A [128 x ROWS] in tensor memory: 16 columns for every 16 of its, hi pieces in the first eight.
 template <int D, int ROWS>
 __device__ __forceinline__ void product_with_columns(uint32_t to, uint32_t a, uint32_t b) {
   using L = Tile<D, ROWS>;
   const uint32_t bl = smem_desc_lo(b, L::CHUNK);
+  auto at = [&](int k, int plane) { return smem_desc_join(DESC_HI, bl + ((k * 2048 + plane) >> 4)); };
 #pragma unroll
   for (int k = 0; k < ROWS / 16; ++k) {
-    const uint64_t bh = smem_desc_join(DESC_HI, bl + (k * 2048 >> 4)), b2 = smem_desc_join(DESC_HI, bl + ((k * 2048 + L::PLANE) >> 4));
-    mma_tmem(to, a + 16 * k, bh, idesc_f16(D, 1), k > 0);
-    mma_tmem(to, a + 16 * k, b2, idesc_f16(D, 1), 1);
-    mma_tmem(to, a + 16 * k + 8, bh, idesc_f16(D, 1), 1);
+    mma_tmem(to, a + 16 * k, at(k, L::PLANE), idesc_f16(D, 1), k > 0);
+    mma_tmem(to, a + 16 * k + 8, at(k, 0), idesc_f16(D, 1), 1);
   }
+#pragma unroll
+  for (int k = 0; k < ROWS / 16; ++k) mma_tmem(to, a + 16 * k, at(k, 0), idesc_f16(D, 1), 1);
 }
 
 // Loads from tensor memory run behind what the thread does until tmem_ld_wait; tmem_arrived then names the registers, so
@@ -428,7 +441,7 @@ __global__ void __launch_bounds__(ForwardShape<D>::BLOCK, ForwardShape<D>::TWO ?
   if (warp < 4) {
     if (Shape::TWO) more_registers<200>();
     float acc[D], m = NEG_INF, l = 0.f, before = 1.f, v_unit = 0.f;
-    const float q_unit = load(p.qp.units + q_at);
+    const float q_unit = load(p.qp.units + q_at).x;
 #pragma unroll
     for (int c = 0; c < D; ++c) acc[c] = 0.f;
     const uint32_t mine = tmem + ((uint32_t)warp << 21);         // this warp's 32 lanes
@@ -445,7 +458,7 @@ __global__ void __launch_bounds__(ForwardShape<D>::BLOCK, ForwardShape<D>::TWO ?
       unsigned in[4];
 #pragma unroll
       for (int w = 0; w < 4; ++w) in[w] = keys_mask(tokens, j * 128 + w * 32, p.tk);
-      const float unit = q_unit * load(p.kp.units + k_at + j), next_unit = load(p.vp.units + k_at + j);
+      const float unit = q_unit * load(p.kp.units + k_at + j).x, next_unit = load(p.vp.units + k_at + j).x;
       if (!mbar_wait(&bar->s_full[b], j / BUFFERS & 1, p.status, 0x302)) { ok = false; break; }
       tc_fence_after();
       if (BUFFERS == 1 && j > 0 && !(ok = add_tile(j - 1))) break;             // (its product ran before S)
@@ -550,9 +563,9 @@ __global__ void __launch_bounds__(ForwardShape<D>::BLOCK, ForwardShape<D>::TWO ?
 }
 
 // ------------------------------------------------------------------------------------------------ gradients
-// A bound of |dP - dot| over a tile: e with (d |g| |v| + |dot|) 2^e below 2^15 (units: what 2^14 of a tile stands for).
-__device__ __forceinline__ int exponent_of_ds(int d, float g_unit, float v_unit, float dot) {
-  const float most = (float)d * (LARGEST * g_unit) * (LARGEST * v_unit) + fabsf(dot);
+// A bound of |dP - dot| over a tile: e with (|g| |v| + |dot|) 2^e below 2^15, |g| and |v| the lengths of the longest rows.
+__device__ __forceinline__ int exponent_of_ds(float g_length, float v_length, float dot) {
+  const float most = 1.001f * (g_length * v_length) + fabsf(dot);
   return exponent_to(__float_as_uint(most), TOP + 1);
 }
 
@@ -619,7 +632,8 @@ __global__ void __launch_bounds__(QueryShape<D>::BLOCK, QueryShape<D>::TWO ? 2 :
     for (int c = 0; c < D; ++c) acc[c] = 0.f;
     const uint32_t mine = tmem + ((uint32_t)warp << 21);
     const float lse = load(p.lse + q_at * 128 + threadIdx.x), dot = load(p.dot + q_at * 128 + threadIdx.x);
-    const float q_unit = load(p.qp.units + q_at), g_unit = load(p.gp.units + q_at);
+    const float q_unit = load(p.qp.units + q_at).x;
+    const float2 g_unit = load(p.gp.units + q_at);
     bool ok = true;
     auto add_tile = [&](int j) {
       const int b = j % BUFFERS;
@@ -631,9 +645,11 @@ __global__ void __launch_bounds__(QueryShape<D>::BLOCK, QueryShape<D>::TWO ? 2 :
     for (int j = 0; j < tiles; ++j) {
       const int b = j % BUFFERS;
       const unsigned in[2] = {keys_mask(tokens, j * 64, p.tk), keys_mask(tokens, j * 64 + 32, p.tk)};
-      const float k_unit = load(p.kp.units + k_at + j / 2), v_unit = load(p.vp.units + k_at + j / 2);
-      const int e = exponent_of_ds(p.d, g_unit, v_unit, dot);
-      const float s_unit = q_unit * k_unit, dp_unit = g_unit * v_unit, shift = (float)e - lse;
+      const float k_unit = load(p.kp.units + k_at + j / 2).x;
+      const float2 v_unit = load(p.vp.units + k_at + j / 2);
+      const int e = exponent_of_ds(g_unit.y, v_unit.y, dot);
+      // (2^e is not in the exponent, whose rounding it would make coarser)
+      const float f = power_of_two(e), s_unit = q_unit * k_unit, dp_unit = g_unit.x * v_unit.x * f, dot_unit = dot * f;
       if (!mbar_wait(&bar->s_full[b], j / BUFFERS & 1, p.status, 0x312)) { ok = false; break; }
       tc_fence_after();
       if (BUFFERS == 1 && j > 0 && !(ok = add_tile(j - 1))) break;
@@ -653,7 +669,7 @@ __global__ void __launch_bounds__(QueryShape<D>::BLOCK, QueryShape<D>::TWO ? 2 :
           tmem_begin(at + DP_AT + 16 * w + 16, dp[(w + 1) & 1]);
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = exp2_fast(v[i] * s_unit + shift) * (x[i] * dp_unit - dot);
+        for (int i = 0; i < 16; ++i) v[i] = exp2_fast(v[i] * s_unit - lse) * (x[i] * dp_unit - dot_unit);
         if (in[w / 2] != ALL) {
           const unsigned mask = in[w / 2] >> (w % 2 * 16);
 #pragma unroll
@@ -789,7 +805,8 @@ __global__ void __launch_bounds__(StateShape<D>::BLOCK, 1) grad_of_states(const 
     for (int c = 0; c < D; ++c) acc[c] = 0.f;
     const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);
     const int half = warp >> 2, row = threadIdx.x & 127;
-    const float k_unit = load(p.kp.units + k_at), v_unit = load(p.vp.units + k_at);
+    const float k_unit = load(p.kp.units + k_at).x;
+    const float2 v_unit = load(p.vp.units + k_at);
     bool ok = true;
     auto add_tile = [&](int j) {
       if (!mbar_wait(&bar->sum_full, j & 1, p.status, 0x322)) return false;
@@ -800,14 +817,15 @@ __global__ void __launch_bounds__(StateShape<D>::BLOCK, 1) grad_of_states(const 
     for (int j = 0; j < tiles; ++j) {
       const int b = j & 1, qs = 2 * j % SLOTS, gs = (2 * j + 1) % SLOTS;
       const long long t = tile_of(j);
-      const float q_unit = load(p.qp.units + t), g_unit = load(p.gp.units + t);
+      const float q_unit = load(p.qp.units + t).x;
+      const float2 g_unit = load(p.gp.units + t);
       if (!mbar_wait(&bar->full[gs], (2 * j + 1) / SLOTS & 1, p.status, 0x321)) { ok = false; break; }
       if (!mbar_wait(&bar->full[qs], 2 * j / SLOTS & 1, p.status, 0x321)) { ok = false; break; }
       const float *const lse = rows + qs * 64, *const dots = rows + gs * 64;
       const uint32_t largest = max(__float_as_uint(fabsf(dots[lane])), __float_as_uint(fabsf(dots[lane + 32])));
-      const int e = exponent_of_ds(p.d, g_unit, v_unit, __uint_as_float(__reduce_max_sync(ALL, largest)));
+      const int e = exponent_of_ds(g_unit.y, v_unit.y, __uint_as_float(__reduce_max_sync(ALL, largest)));
       // p = 2^14 P, then dS = p (dP - dot) 2^(e - 14)
-      const float s_unit = q_unit * k_unit, f = power_of_two(max(e - TOP - 1, -126)), dp_unit = g_unit * v_unit * f;
+      const float s_unit = q_unit * k_unit, f = power_of_two(max(e - TOP - 1, -126)), dp_unit = g_unit.x * v_unit.x * f;
       if (!mbar_wait(&bar->s_full[b], j >> 1 & 1, p.status, 0x321)) { ok = false; break; }
       tc_fence_after();
       const uint32_t at = mine + b * 64 + half * 32;
@@ -843,7 +861,7 @@ __global__ void __launch_bounds__(StateShape<D>::BLOCK, 1) grad_of_states(const 
       if (j > 0 && !(ok = add_tile(j - 1))) break;
       tc_fence_before();
       mbar_arrive(&bar->ds_full[b]);                              // (the sums of the tile before are in registers by now)
-      before = half ? q_unit * power_of_two(-e) : g_unit * (1.f / LARGEST);
+      before = half ? q_unit * power_of_two(-e) : g_unit.x * (1.f / LARGEST);
     }
     if (ok && tiles > 0) ok = add_tile(tiles - 1);
     if (ok && k0 + row < p.tk) {
@@ -1189,12 +1207,12 @@ struct Layout {
     }
     for (int i = 0; i < 4; ++i) {
       units[i] = bytes;
-      bytes += (count[i] * 4 + 15) / 16 * 16;
+      bytes += (count[i] * 8 + 15) / 16 * 16;
     }
     dots = bytes;
     bytes += count[3] * 128 * 4;
   }
-  Pieces of(const char* base, int i) const { return {base + tiles[i], reinterpret_cast<const float*>(base + units[i])}; }
+  Pieces of(const char* base, int i) const { return {base + tiles[i], reinterpret_cast<const float2*>(base + units[i])}; }
 };
 bool fits(const void* prepared, long long have, const Layout& at) {
   return prepared && (reinterpret_cast<uintptr_t>(prepared) & 15) == 0 && have >= (long long)at.bytes;
@@ -1227,7 +1245,7 @@ int split(const Problem& p, const float* g, const float* y, const Layout& at, ch
     s.mult = i == 0 ? p.scale * LOG2E : 1.f;
     s.tokens = state ? p.key : nullptr;
     s.tiles = base + at.tiles[i];
-    s.units = reinterpret_cast<float*>(base + at.units[i]);
+    s.units = reinterpret_cast<float2*>(base + at.units[i]);
     if (i == 3) {
       s.with = y;
       s.dots = reinterpret_cast<float*>(base + at.dots);

@@ -104,10 +104,10 @@ def _whole_tiles(t):
 
 
 def _prepared_floats(n, tq, tk, h, shared, d):
-    """Length of what the gradients read: tiles of 128 rows and 64 or 128 columns of q, k, v and g, one number for each, and
+    """Length of what the gradients read: tiles of 128 rows and 64 or 128 columns of q, k, v and g, two numbers for each, and
     one for every row of g."""
     q, k, columns = n * h * _whole_tiles(tq) // 128, n * shared * _whole_tiles(tk) // 128, 64 if d <= 64 else 128
-    return 128 * columns * 2 * (q + k) + 2 * (-(-q // 4) * 4 + -(-k // 4) * 4) + 128 * q
+    return 128 * columns * 2 * (q + k) + 2 * (-(-q // 2) * 4 + -(-k // 2) * 4) + 128 * q
 
 
 class CrossAttentionPrepareOp(Op):
