@@ -157,6 +157,37 @@ def test_what_masked_states_hold_does_not_matter(tq, what, ctx):
         assert np.array_equal(a, b)
 
 
+@pytest.mark.parametrize("tq", [1, 4, 33, 200])
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
+def test_a_query_that_is_no_number_stays_alone(tq, what, ctx):
+    """Its own row is NaN, and through it its head's states; other rows, heads and sentences keep their results to the bit."""
+    f = case(2, tq, 150, 4, 2, 64, "holes")
+    clean = check(f, ctx)
+    f["q"][1, tq // 2, 2, 5] = what
+    y, dq, dkv = evaluate(graph(True, None), f, ctx)
+    rows = np.zeros(y.shape, bool)
+    rows[1, tq // 2, 2] = True
+    states = np.zeros(dkv.shape, bool)
+    states[1, f["key"][1] != 0, :, 1] = True
+    for got, was, bad in ((y, clean[0], rows), (dq, clean[1], rows), (dkv, clean[2], states)):
+        assert np.isnan(got[bad]).all() and np.array_equal(got[~bad], was[~bad])
+
+
+@pytest.mark.parametrize("tq", [1, 4, 33, 200])
+@pytest.mark.parametrize("which", [0, 1])
+def test_a_state_that_is_no_number_shows(tq, which, ctx):
+    """Every query that reads it is NaN (with a NaN value: in its column at least); no other head's or sentence's is."""
+    f = case(2, tq, 150, 4, 2, 64, "holes")
+    clean = check(f, ctx)
+    f["key"][1, 70] = 1
+    f["kv"][1, 70, which, 1, 9] = np.nan
+    y = evaluate(graph(True, None), f, ctx)[0]
+    assert np.isnan(y[1, :, 2:, 9]).all() and (which or np.isnan(y[1, :, 2:]).all())
+    assert np.array_equal(y[0], clean[0][0])
+    f["key"][1, 70] = 0
+    assert np.isfinite(evaluate(graph(True, None), f, ctx)[0]).all()
+
+
 @pytest.mark.parametrize("n,tq,tk", [(0, 4, 5), (2, 0, 5), (2, 4, 0), (2, 20, 0)])
 def test_empty_attention(n, tq, tk, ctx):
     y, dq, dkv = evaluate(graph(True, None), case(n, tq, tk, 2, 2, 16, None) | {"key": np.ones((n, tk), np.float32)}, ctx)

@@ -98,7 +98,8 @@ struct Sources {
   bool vec;
 };
 
-// A block splits a tile of 128 rows.
+// A block splits a tile of 128 rows.  Infinities and NaN have no part in the tile's unit, so they stay within their row: its pieces
+// are NaN (inf - inf), and so is what is computed with them.
 template <int D>
 __global__ void __launch_bounds__(256) split_tiles(const Sources all) {
   tsb_launch::enter();
@@ -151,7 +152,8 @@ __global__ void __launch_bounds__(256) split_tiles(const Sources all) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       v[u][k] *= s.mult;
-      most = max(most, __float_as_uint(v[u][k]) & 0x7fffffffu);
+      const uint32_t size = __float_as_uint(v[u][k]) & 0x7fffffffu;
+      if (size < 0x7f800000u) most = max(most, size);
       squares += v[u][k] * v[u][k];
     }
 #pragma unroll
@@ -166,7 +168,7 @@ __global__ void __launch_bounds__(256) split_tiles(const Sources all) {
   for (int w = 0; w < 8; ++w) most = max(most, largest[w]), most_squares = max(most_squares, longest[w]);
   const int e = exponent_to(most, TOP);
   const float scale = power_of_two(e);
-  // (a row whose squares overflow, or vanish, has its largest number instead)
+  // (a row whose squares overflow, or vanish, or are NaN, has its largest number instead)
   if (threadIdx.x == 0) {
     const float length = sqrtf(__uint_as_float(most_squares)), least = __uint_as_float(most);
     s.units[b] = make_float2(power_of_two(-e), length < 1e15f && length > 1e-15f ? length : least * (float)D);
@@ -254,15 +256,29 @@ __device__ __forceinline__ void product_of_rows(uint32_t to, uint32_t a, uint32_
 #pragma unroll
   for (int k = 0; k < D / 16; ++k) mma_smem(to, at(k, al, LA::CHUNK), at(k, bl, LB::CHUNK), idesc_f16(ROWS_B, 0), 1);
 }
-// D [128 x D] = A B, A [128 x ROWS] in tensor memory: 16 columns for every 16 of its, hi pieces in the first eight.
+// The same with A in tensor memory: its hi pieces in D / 2 columns, two to each, then the lo pieces.
+template <int D, int ROWS_B>
+__device__ __forceinline__ void product_of_kept_rows(uint32_t to, uint32_t a, uint32_t b) {
+  using L = Tile<D, ROWS_B>;
+  const uint32_t bl = smem_desc_lo(b, 16);
+  auto at = [&](int k, int plane) { return smem_desc_join(DESC_HI, bl + ((k / 4 * L::CHUNK + k % 4 * 32 + plane) >> 4)); };
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) {
+    mma_tmem(to, a + 8 * k, at(k, L::PLANE), idesc_f16(ROWS_B, 0), k > 0);
+    mma_tmem(to, a + D / 2 + 8 * k, at(k, 0), idesc_f16(ROWS_B, 0), 1);
+  }
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) mma_tmem(to, a + 8 * k, at(k, 0), idesc_f16(ROWS_B, 0), 1);
+}
+// D [128 x D] (+)= A B, A [128 x ROWS] in tensor memory: 16 columns for every 16 of its, hi pieces in the first eight.
 template <int D, int ROWS>
-__device__ __forceinline__ void product_with_columns(uint32_t to, uint32_t a, uint32_t b) {
+__device__ __forceinline__ void product_with_columns(uint32_t to, uint32_t a, uint32_t b, bool accumulate = false) {
   using L = Tile<D, ROWS>;
   const uint32_t bl = smem_desc_lo(b, L::CHUNK);
   auto at = [&](int k, int plane) { return smem_desc_join(DESC_HI, bl + ((k * 2048 + plane) >> 4)); };
 #pragma unroll
   for (int k = 0; k < ROWS / 16; ++k) {
-    mma_tmem(to, a + 16 * k, at(k, L::PLANE), idesc_f16(D, 1), k > 0);
+    mma_tmem(to, a + 16 * k, at(k, L::PLANE), idesc_f16(D, 1), accumulate || k > 0);
     mma_tmem(to, a + 16 * k + 8, at(k, 0), idesc_f16(D, 1), 1);
   }
 #pragma unroll
@@ -310,42 +326,41 @@ template <int COUNT> __device__ __forceinline__ void tmem_st_pieces(uint32_t add
         : "memory");
   }
 }
-// acc = acc times + what the tensor memory holds from addr on, times unit
+// acc = acc times + what the tensor memory holds from addr on, times unit; two loads under way
 template <bool TIMES, int COUNT>
-__device__ __forceinline__ void add_columns(uint32_t addr, float (&acc)[COUNT], int first, int count, float times, float unit) {
+__device__ __forceinline__ void add_columns(uint32_t addr, float (&acc)[COUNT], float times, float unit) {
+  float v[2][16];
+  tmem_begin(addr, v[0]);
 #pragma unroll
-  for (int c = 0; c < COUNT; c += 64) {
-    if (c < first || c >= first + count) continue;
-    float v[32], w[32];
-    tmem_begin(addr + c, v);
-    tmem_begin(addr + c + 32, w);
+  for (int c = 0; c < COUNT; c += 16) {
+    float(&x)[16] = v[c / 16 & 1];
     tmem_ld_wait();
-    tmem_arrived(v);
-    tmem_arrived(w);
+    tmem_arrived(x);
+    if (c + 16 < COUNT) tmem_begin(addr + c + 16, v[(c / 16 + 1) & 1]);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      acc[c + i] = (TIMES ? acc[c + i] * times : acc[c + i]) + v[i] * unit;
-      acc[c + 32 + i] = (TIMES ? acc[c + 32 + i] * times : acc[c + 32 + i]) + w[i] * unit;
-    }
+    for (int i = 0; i < 16; ++i) acc[c + i] = (TIMES ? acc[c + i] * times : acc[c + i]) + x[i] * unit;
   }
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Keys up to the last one that is in, rounded up to what the block looks at in one go.  All threads call it.
+// Keys up to the last one that is in, rounded up to the 256 that a warp looks at in one go.  Every warp finds out for itself.
 __device__ __forceinline__ int keys_in(const float* tokens, int tk) {
   if (!tokens) return tk;
-  int end = tk;
-  while (end > 0) {
-    const int i = end - 1 - (int)threadIdx.x;
-    if (__syncthreads_or(i >= 0 && load(tokens + i) != 0.f)) break;
-    end -= (int)blockDim.x;
+  for (int end = tk; end > 0; end -= 256) {
+    bool in = false;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = end - 1 - u * 32 - (int)(threadIdx.x & 31);
+      in |= i >= 0 && load(tokens + max(i, 0)) != 0.f;
+    }
+    if (__any_sync(ALL, in)) return end;
   }
-  return end < 0 ? 0 : end;
+  return 0;
 }
-// Bit i: whether key `first + i` is in.
-__device__ __forceinline__ unsigned keys_mask(const float* tokens, int first, int tk) {
+// The token of key `first` + lane; 0 for a key that is out or that there is not.
+__device__ __forceinline__ float token_of(const float* tokens, int first, int tk) {
   const int k = first + (int)(threadIdx.x & 31);
-  return __ballot_sync(ALL, k < tk && (!tokens || load(tokens + k) != 0.f));
+  return k < tk ? (tokens ? load(tokens + k) : 1.f) : 0.f;
 }
 
 // After a wait that ran out: the products that were issued still use shared and tensor memory.
@@ -364,10 +379,41 @@ template <class Control> __device__ __forceinline__ Control* control_at(int byte
   return reinterpret_cast<Control*>(tiles_of_block + bytes_of_tiles);
 }
 
-// Blocks of up to 64 columns: two to an SM, so that one's products run while the other computes its soft-max or begins or
-// ends.  They have 256 threads; of the 128 registers a thread, the four warps that compute take 200 and the rest 56.
+// A block has 384 threads: eight warps that compute, and four others of which one copies and one issues the products; the
+// registers go to the former.  A row belongs to two threads, in warps w and w + 4.
 template <int R> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
 template <int R> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
+
+// Half of a row's pieces (columns D / 2 * half on) of a tile: read from memory, and put into tensor memory as
+// product_of_kept_rows takes them.
+template <int D> struct KeptRow {
+  uint4 v[2][D / 16];
+  __device__ __forceinline__ void read(const Pieces& p, long long tile, int row, int half) {
+    using L = Tile<D, 128>;
+    const char* const from = p.tiles + tile * L::BYTES + row * 128;
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane)
+#pragma unroll
+      for (int u = 0; u < D / 16; ++u) {
+        const int at = half * (D / 16) + u;
+        v[plane][u] = load(reinterpret_cast<const uint4*>(from + plane * L::PLANE + at / 8 * L::CHUNK + (((at & 7) ^ (row & 7)) << 4)));
+      }
+  }
+  __device__ __forceinline__ void keep(uint32_t to, int half) const {
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane)
+#pragma unroll
+      for (int u = 0; u < D / 16; u += 4)                            // four pieces of 16 bytes: 16 columns
+        asm volatile(
+            "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+            "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+            ::"r"(v[plane][u].x), "r"(v[plane][u].y), "r"(v[plane][u].z), "r"(v[plane][u].w), "r"(v[plane][u + 1].x),
+              "r"(v[plane][u + 1].y), "r"(v[plane][u + 1].z), "r"(v[plane][u + 1].w), "r"(v[plane][u + 2].x), "r"(v[plane][u + 2].y),
+              "r"(v[plane][u + 2].z), "r"(v[plane][u + 2].w), "r"(v[plane][u + 3].x), "r"(v[plane][u + 3].y), "r"(v[plane][u + 3].z),
+              "r"(v[plane][u + 3].w), "r"(to + plane * (D / 2) + half * (D / 4) + u * 4)
+            : "memory");
+  }
+};
 
 // Writes the d first numbers of a row.
 template <int COUNT>
@@ -384,173 +430,213 @@ __device__ __forceinline__ void store_row(float* to, const float (&v)[COUNT], fl
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// A block takes 128 queries of a head and tiles of 128 keys.  Warps 0 to 3: soft-max, a row per thread; 4: copies; 5 issues
-// the products.  P takes the place of its S.  With 128 columns a block has an SM to itself and two tiles of scores in tensor
-// memory: S of the next tile runs while a thread works on this one, and y of a tile is added to the registers while the next
-// tile's product runs.
+// A block takes 128 queries of a head, kept in tensor memory, and tiles of 128 keys; keys and values share a ring of slots of
+// 32 KB.  Warps 0 to 7: soft-max, w and w + 4 half of the keys of 32 rows each; 8: copies; 9 issues the products.  Two tiles of
+// scores are in tensor memory, so S of the next tile runs while the threads work on this one.  P takes the place of its S, and y
+// of a tile is added to the registers before the next one's product.
+//
+// Bound by the tensor cores and by the threads between two products.  With the splitting: 2 x 2000 x 4111, 16 heads of 128 on 4:
+// 356 us, 379 TFLOP/s, so 1.14 PFLOP/s of fp16 products; 4 x 2048 x 2048, 16 heads of 64: 227 us; 32 x 255 x 256, 8 heads of 64:
+// 50 us.  (A row to a thread and two blocks to an SM, operands in shared memory: 444, 278 and 47 us.  A block's beginning and
+// end are not hidden now, which a few key tiles show, but a product with A in tensor memory takes 32 cycles for 16 x 64 numbers
+// of B, with A in shared memory 48, and two threads do a row's soft-max in half the time.)
 template <int D> struct ForwardShape {
-  static constexpr bool TWO = D == 64;       // blocks to an SM
-  static constexpr int BUFFERS = TWO ? 1 : 2, BLOCK = TWO ? 256 : 192, COLUMNS = TWO ? 256 : 512, Y_AT = 128 * BUFFERS;
-  using L = Tile<D, 128>;
-  static constexpr int TILES = 3 * L::BYTES, SMEM = TILES + CONTROL;
+  static constexpr int PARTS = D / 64, ROWS = 128 / PARTS, SLOTS = 6;              // of a tile in a slot each
+  static constexpr int S_AT = D, Y_AT = S_AT + 2 * 128;                            // behind the queries
+  using L = Tile<D, ROWS>;
+  static constexpr int TILES = SLOTS * L::BYTES, SMEM = TILES + CONTROL + 2 * 1024;
 };
 struct ForwardControl {
-  uint64_t q_full, k_full, k_empty, v_full, v_empty, s_full[2], p_full[2], y_full[2], drained;
+  uint64_t q_full, full[6], empty[6], s_full[2], p_full[2], y_full, pair[4], drained;
   uint32_t tmem;
 };
+constexpr int BLOCK = 384, TMEM_COLUMNS = 512;
 
 template <int D>
-__global__ void __launch_bounds__(ForwardShape<D>::BLOCK, ForwardShape<D>::TWO ? 2 : 1) attend(const Problem p) {
+__global__ void __launch_bounds__(BLOCK, 1) attend(const Problem p) {
   using Shape = ForwardShape<D>;
   using L = typename Shape::L;
-  constexpr int BUFFERS = Shape::BUFFERS, Y_AT = Shape::Y_AT;
-  char *const q_tile = tiles_of_block, *const k_tile = q_tile + L::BYTES, *const v_tile = k_tile + L::BYTES;
+  constexpr int SLOTS = Shape::SLOTS, PARTS = Shape::PARTS;
   ForwardControl* bar = control_at<ForwardControl>(Shape::TILES);
+  float(*const shared_max)[2][128] = reinterpret_cast<float(*)[2][128]>(tiles_of_block + Shape::TILES + CONTROL);      // [tile & 1][half]
   const int warp = __shfl_sync(ALL, threadIdx.x >> 5, 0);
   if (threadIdx.x == 0) {
-    mbar_init(&bar->q_full, 1);
-    mbar_init(&bar->k_full, 1);
-    mbar_init(&bar->k_empty, 1);
-    mbar_init(&bar->v_full, 1);
-    mbar_init(&bar->v_empty, 1);
+    mbar_init(&bar->q_full, 256);
+    for (int i = 0; i < SLOTS; ++i) {
+      mbar_init(&bar->full[i], 1);
+      mbar_init(&bar->empty[i], 1);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar->s_full[i], 1);
-      mbar_init(&bar->p_full[i], 128);
-      mbar_init(&bar->y_full[i], 1);
+      mbar_init(&bar->p_full[i], 256);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(&bar->pair[i], 64);
+    mbar_init(&bar->y_full, 1);
     mbar_init(&bar->drained, 1);
     fence_barrier_init();
   }
-  if (warp == 5) {
-    tmem_alloc(&bar->tmem, Shape::COLUMNS);
+  if (warp == 9) {
+    tmem_alloc(&bar->tmem, TMEM_COLUMNS);
     tmem_relinquish();
   }
+  tsb_launch::enter();
+  const int qt = blockIdx.x % p.qtiles, h = blockIdx.x / p.qtiles % p.heads, n = blockIdx.x / p.qtiles / p.heads;
+  const int shared = h / (p.heads / p.shared), q0 = qt * 128, half = warp >> 2, row = threadIdx.x & 127;
+  const float* tokens = p.key ? p.key + (long long)n * p.tk : nullptr;
+  const long long q_row = (long long)p.heads * p.d;
+  const long long q_at = ((long long)n * p.heads + h) * p.qtiles + qt, k_at = ((long long)n * p.shared + shared) * p.ktiles;
+  KeptRow<D> kept;                             // (under way while the block sets itself up)
+  if (warp < 8) kept.read(p.qp, q_at, row, half);
+  const int tiles = (keys_in(tokens, p.tk) + 127) / 128;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(ALL, bar->tmem, 0);
-  tsb_launch::enter();
 
-  const int qt = blockIdx.x % p.qtiles, h = blockIdx.x / p.qtiles % p.heads, n = blockIdx.x / p.qtiles / p.heads;
-  const int shared = h / (p.heads / p.shared), q0 = qt * 128;
-  const float* tokens = p.key ? p.key + (long long)n * p.tk : nullptr;
-  const int tiles = (keys_in(tokens, p.tk) + 127) / 128;
-  const long long q_row = (long long)p.heads * p.d;
-  const long long q_at = ((long long)n * p.heads + h) * p.qtiles + qt, k_at = ((long long)n * p.shared + shared) * p.ktiles;
-
-  if (warp < 4) {
-    if (Shape::TWO) more_registers<200>();
-    float acc[D], m = NEG_INF, l = 0.f, before = 1.f, v_unit = 0.f;
+  if (warp < 8) {
+    more_registers<208>();
+    constexpr int OWN = D / 2;                                   // columns of y of a thread
+    const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);   // this warp's 32 lanes
+    kept.keep(mine, half);
+    tmem_st_wait();
+    tc_fence_before();
+    mbar_arrive(&bar->q_full);
+    float acc[OWN], m = NEG_INF, l = 0.f, before = 1.f, v_unit = 0.f;
     const float q_unit = load(p.qp.units + q_at).x;
 #pragma unroll
-    for (int c = 0; c < D; ++c) acc[c] = 0.f;
-    const uint32_t mine = tmem + ((uint32_t)warp << 21);         // this warp's 32 lanes
+    for (int c = 0; c < OWN; ++c) acc[c] = 0.f;
     bool ok = true;
     auto add_tile = [&](int j) {                                 // before: from the maximum then to the one that tile j has
-      const int b = j % BUFFERS;
-      if (!mbar_wait(&bar->y_full[b], j / BUFFERS & 1, p.status, 0x301)) return false;
+      if (!mbar_wait(&bar->y_full, j & 1, p.status, 0x301)) return false;
       tc_fence_after();
-      add_columns<true>(mine + Y_AT + b * 128, acc, 0, D, before, v_unit);
+      add_columns<true>(mine + Shape::Y_AT + half * OWN, acc, before, v_unit);
       return true;
     };
+    // (what a tile needs from memory besides its scores is read a tile ahead)
+    float token[2], k_next = 0.f, v_next = 0.f;
+    auto look_at = [&](int j) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) token[w] = token_of(tokens, j * 128 + half * 64 + w * 32, p.tk);
+      k_next = j < tiles ? load(p.kp.units + k_at + j).x : 0.f;
+      v_next = j < tiles ? load(p.vp.units + k_at + j).x : 0.f;
+    };
+    look_at(0);
     for (int j = 0; j < tiles; ++j) {
-      const int b = j % BUFFERS;
-      unsigned in[4];
+      const int b = j & 1;
+      unsigned in[2];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) in[w] = keys_mask(tokens, j * 128 + w * 32, p.tk);
-      const float unit = q_unit * load(p.kp.units + k_at + j).x, next_unit = load(p.vp.units + k_at + j).x;
-      if (!mbar_wait(&bar->s_full[b], j / BUFFERS & 1, p.status, 0x302)) { ok = false; break; }
+      for (int w = 0; w < 2; ++w) in[w] = __ballot_sync(ALL, token[w] != 0.f);
+      const float unit = q_unit * k_next, next_unit = v_next;
+      look_at(j + 1);
+      if (!mbar_wait(&bar->s_full[b], j >> 1 & 1, p.status, 0x302)) { ok = false; break; }
       tc_fence_after();
-      if (BUFFERS == 1 && j > 0 && !(ok = add_tile(j - 1))) break;             // (its product ran before S)
-      const uint32_t at = mine + b * 128;
-      float part[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};     // (four chains: a thread has few others to wait behind)
+      const uint32_t at = mine + Shape::S_AT + b * 128 + half * 64;
+      float part[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};     // (chains that do not wait for one another)
 #pragma unroll
-      for (int w = 0; w < 4; w += 2) {
-        float s[2][32];
-        tmem_begin(at + 32 * w, s[0]);
-        tmem_begin(at + 32 * w + 32, s[1]);
+      for (int w = 0; w < 2; ++w) {
+        float s[32];
+        tmem_begin(at + 32 * w, s);
         tmem_ld_wait();
+        tmem_arrived(s);
+        if (in[w] == ALL) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          tmem_arrived(s[k]);
-          if (in[w + k] == ALL) {
+          for (int i = 0; i < 32; ++i) part[i & 3] = fmaxf(part[i & 3], s[i]);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) part[i & 3] = fmaxf(part[i & 3], s[k][i]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) part[i & 3] = fmaxf(part[i & 3], (in[w + k] >> i) & 1 ? s[k][i] : NEG_INF);
-          }
+          for (int i = 0; i < 32; ++i) part[i & 3] = fmaxf(part[i & 3], (in[w] >> i) & 1 ? s[i] : NEG_INF);
         }
       }
-      const float most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+      const float own = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+      shared_max[j & 1][half][row] = own;
+      mbar_arrive(&bar->pair[warp & 3]);
+      if (!mbar_wait(&bar->pair[warp & 3], j & 1, p.status, 0x309)) { ok = false; break; }
+      const float most = fmaxf(own, shared_max[j & 1][half ^ 1][row]);
       const float top = fmaxf(m, most == NEG_INF ? NEG_INF : most * unit), ref = top == NEG_INF ? 0.f : top;
       const float factor = exp2_fast(m - ref), shift = TOP + 1 - ref;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f}, s[2][32];
+      float sum[4] = {0.f, 0.f, 0.f, 0.f}, s[2][16];
       tmem_begin(at, s[0]);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        float(&v)[32] = s[w & 1];
+        float(&v)[16] = s[w & 1];
         tmem_ld_wait();
         tmem_arrived(v);
-        if (w < 3) tmem_begin(at + 32 * w + 32, s[(w + 1) & 1]);
+        if (w < 3) tmem_begin(at + 16 * w + 16, s[(w + 1) & 1]);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = exp2_fast(v[i] * unit + shift);
-        if (in[w] != ALL) {
+        for (int i = 0; i < 16; ++i) v[i] = exp2_fast(v[i] * unit + shift);
+        if (in[w / 2] != ALL) {
+          const unsigned mask = in[w / 2] >> (w % 2 * 16);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = (in[w] >> i) & 1 ? v[i] : 0.f;
+          for (int i = 0; i < 16; ++i) v[i] = (mask >> i) & 1 ? v[i] : 0.f;
         }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) sum[i & 3] += v[i];
-        tmem_st_pieces(at + 32 * w, v);
+        for (int i = 0; i < 16; ++i) sum[i & 3] += v[i];
+        tmem_st_pieces(at + 16 * w, v);
       }
       tmem_st_wait();
+      if (j > 0 && !(ok = add_tile(j - 1))) break;
       tc_fence_before();
       mbar_arrive(&bar->p_full[b]);
       l = l * factor + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
       m = top;
-      if (BUFFERS == 2 && j > 0 && !(ok = add_tile(j - 1))) break;
       before = factor;
       v_unit = next_unit;
     }
     if (ok && tiles > 0) ok = add_tile(tiles - 1);
-    const int t = q0 + threadIdx.x;
-    if (ok) {
-      if (t < p.tq) store_row(p.y + ((long long)n * p.tq + t) * q_row + (long long)h * p.d, acc, l > 0.f ? 1.f / l : 0.f, p.d, p.vec);
-      // (a row without keys, or behind the last one: exp2(S - inf) = 0 in the backward pass)
-      p.lse[q_at * 128 + threadIdx.x] = l > 0.f && t < p.tq ? m - (TOP + 1) + log2f(l) : -NEG_INF;
+    // the halves' sums
+    shared_max[tiles & 1][half][row] = l;
+    mbar_arrive(&bar->pair[warp & 3]);
+    if (ok && mbar_wait(&bar->pair[warp & 3], tiles & 1, p.status, 0x309)) {
+      l += shared_max[tiles & 1][half ^ 1][row];
+      const int t = q0 + row;
+      if (t < p.tq)
+        store_row(p.y + ((long long)n * p.tq + t) * q_row + (long long)h * p.d + half * OWN, acc, l != 0.f ? 1.f / l : 0.f, p.d - half * OWN,
+                  p.vec);
+      // (a row without keys, or behind the last one: exp2(S - inf) = 0 in the backward pass; l may be NaN)
+      if (half == 0) p.lse[q_at * 128 + row] = l != 0.f && t < p.tq ? m - (TOP + 1) + log2f(l) : -NEG_INF;
     }
   } else {
-    if (Shape::TWO) fewer_registers<56>();
-    if (warp == 4 && elect_one() && tiles > 0) {
-      copy_tile<D>(q_tile, p.qp, q_at, &bar->q_full);
-      for (int j = 0; j < tiles; ++j) {
-        if (!mbar_wait(&bar->k_empty, (j & 1) ^ 1, p.status, 0x303)) break;
-        copy_tile<D>(k_tile, p.kp, k_at + j, &bar->k_full);
-        if (!mbar_wait(&bar->v_empty, (j & 1) ^ 1, p.status, 0x304)) break;
-        copy_tile<D>(v_tile, p.vp, k_at + j, &bar->v_full);
+    fewer_registers<88>();
+    if (warp == 8 && elect_one()) {
+      for (int i = 0; i < 2 * PARTS * tiles; ++i) {
+        const int s = i % SLOTS, j = i / (2 * PARTS);
+        const Pieces& from = i / PARTS & 1 ? p.vp : p.kp;
+        if (!mbar_wait(&bar->empty[s], (i / SLOTS & 1) ^ 1, p.status, 0x303)) break;
+        if (PARTS == 1) copy_tile<D>(tiles_of_block + s * L::BYTES, from, k_at + j, &bar->full[s]);
+        else copy_half<D>(tiles_of_block + s * L::BYTES, from, k_at + j, i % PARTS, &bar->full[s]);
       }
     }
-    if (warp == 5 && elect_one() && tiles > 0) {
-      const uint32_t qa = smem_u32(q_tile), ka = smem_u32(k_tile), va = smem_u32(v_tile);
+    if (warp == 9 && elect_one() && tiles > 0) {
+      const uint32_t ring = smem_u32(tiles_of_block);
       bool ok = mbar_wait(&bar->q_full, 0, p.status, 0x305);
+      tc_fence_after();
       auto scores = [&](int j) {
-        if (!mbar_wait(&bar->k_full, j & 1, p.status, 0x306)) return false;
-        tc_fence_after();
-        product_of_rows<D, 128, 128>(tmem + j % BUFFERS * 128, qa, ka);
-        umma_commit(&bar->s_full[j % BUFFERS]);
-        umma_commit(&bar->k_empty);
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+          const int i = 2 * PARTS * j + part, s = i % SLOTS;
+          if (!mbar_wait(&bar->full[s], i / SLOTS & 1, p.status, 0x306)) return false;
+          tc_fence_after();
+          product_of_kept_rows<D, Shape::ROWS>(tmem + Shape::S_AT + (j & 1) * 128 + part * Shape::ROWS, tmem, ring + s * L::BYTES);
+          umma_commit(&bar->empty[s]);
+        }
+        umma_commit(&bar->s_full[j & 1]);
         return true;
       };
-      for (int j = 0; j < BUFFERS && j < tiles && ok; ++j) ok = scores(j);
+      for (int j = 0; j < 2 && j < tiles && ok; ++j) ok = scores(j);
       for (int j = 0; j < tiles && ok; ++j) {
-        const int b = j % BUFFERS;
-        if (!(ok = mbar_wait(&bar->v_full, j & 1, p.status, 0x307))) break;
-        if (!(ok = mbar_wait(&bar->p_full[b], j / BUFFERS & 1, p.status, 0x308))) break;
-        tc_fence_after();
-        product_with_columns<D, 128>(tmem + Y_AT + b * 128, tmem + b * 128, va);
-        umma_commit(&bar->y_full[b]);
-        umma_commit(&bar->v_empty);
-        if (j + BUFFERS < tiles) ok = scores(j + BUFFERS);
+        const int b = j & 1;
+        if (!(ok = mbar_wait(&bar->p_full[b], j >> 1 & 1, p.status, 0x308))) break;
+#pragma unroll
+        for (int part = 0; part < PARTS && ok; ++part) {
+          const int i = 2 * PARTS * j + PARTS + part, s = i % SLOTS;
+          if (!(ok = mbar_wait(&bar->full[s], i / SLOTS & 1, p.status, 0x307))) break;
+          tc_fence_after();
+          product_with_columns<D, Shape::ROWS>(tmem + Shape::Y_AT, tmem + Shape::S_AT + b * 128 + part * Shape::ROWS, ring + s * L::BYTES,
+                                               part > 0);
+          umma_commit(&bar->empty[s]);
+        }
+        if (!ok) break;
+        umma_commit(&bar->y_full);
+        if (j + 2 < tiles) ok = scores(j + 2);
       }
       if (!ok) drain(&bar->drained);
     }
@@ -559,7 +645,7 @@ __global__ void __launch_bounds__(ForwardShape<D>::BLOCK, ForwardShape<D>::TWO ?
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) tmem_dealloc(tmem, Shape::COLUMNS);
+  if (warp == 9) tmem_dealloc(tmem, TMEM_COLUMNS);
 }
 
 // ------------------------------------------------------------------------------------------------ gradients
@@ -569,161 +655,180 @@ __device__ __forceinline__ int exponent_of_ds(float g_length, float v_length, fl
   return exponent_to(__float_as_uint(most), TOP + 1);
 }
 
-// dq: a block takes 128 queries of a head and tiles of 64 keys; the same roles.  dS takes the place of its S.
+// dq: a block takes 128 queries of a head and tiles of 64 keys; the same roles.  The queries, and with 64 columns their gradients
+// too, are kept in tensor memory, else these lie before the ring.  dS takes the place of its S.  The cases of attend: 534, 235 and 35
+// us (a row to a thread, two blocks to an SM, operands in shared memory: 672, 301 and 32).
 template <int D> struct QueryShape {
-  static constexpr bool TWO = D == 64;
-  static constexpr int BUFFERS = TWO ? 1 : 2, BLOCK = TWO ? 256 : 192, COLUMNS = TWO ? 256 : 512;
-  static constexpr int DP_AT = 64 * BUFFERS, DQ_AT = 128 * BUFFERS;
+  static constexpr bool BOTH = D == 64;
+  static constexpr int SLOTS = BOTH ? 8 : 5;
+  static constexpr int G_AT = D, S_AT = BOTH ? 2 * D : D, DP_AT = S_AT + 2 * 64, DQ_AT = DP_AT + 2 * 64;
   using LQ = Tile<D, 128>;
   using LK = Tile<D, 64>;
-  static constexpr int TILES = 2 * LQ::BYTES + 3 * LK::BYTES, SMEM = TILES + CONTROL;       // two of keys, one of values
+  static constexpr int RING_AT = BOTH ? 0 : LQ::BYTES, TILES = RING_AT + SLOTS * LK::BYTES, SMEM = TILES + CONTROL;
 };
 struct QueryControl {
-  uint64_t q_full, g_full, k_full[2], k_empty[2], v_full, v_empty, s_full[2], ds_full[2], dq_full[2], drained;
+  uint64_t q_full, g_full, full[8], empty[8], s_full[2], ds_full[2], dq_full, drained;
   uint32_t tmem;
 };
 
 template <int D>
-__global__ void __launch_bounds__(QueryShape<D>::BLOCK, QueryShape<D>::TWO ? 2 : 1) grad_of_queries(const Problem p) {
+__global__ void __launch_bounds__(BLOCK, 1) grad_of_queries(const Problem p) {
   using Shape = QueryShape<D>;
   using LQ = typename Shape::LQ;
   using LK = typename Shape::LK;
-  constexpr int BUFFERS = Shape::BUFFERS, DP_AT = Shape::DP_AT, DQ_AT = Shape::DQ_AT;
-  char *const q_tile = tiles_of_block, *const g_tile = q_tile + LQ::BYTES, *const k_tile = g_tile + LQ::BYTES;
-  char* const v_tile = k_tile + 2 * LK::BYTES;
+  constexpr int SLOTS = Shape::SLOTS;
+  char *const g_tile = tiles_of_block, *const ring = tiles_of_block + Shape::RING_AT;
   QueryControl* bar = control_at<QueryControl>(Shape::TILES);
   const int warp = __shfl_sync(ALL, threadIdx.x >> 5, 0);
   if (threadIdx.x == 0) {
-    mbar_init(&bar->q_full, 1);
+    mbar_init(&bar->q_full, 256);
     mbar_init(&bar->g_full, 1);
-    mbar_init(&bar->v_full, 1);
-    mbar_init(&bar->v_empty, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar->k_full[i], 1);
-      mbar_init(&bar->k_empty[i], 1);
-      mbar_init(&bar->s_full[i], 1);
-      mbar_init(&bar->ds_full[i], 128);
-      mbar_init(&bar->dq_full[i], 1);
+    for (int i = 0; i < SLOTS; ++i) {
+      mbar_init(&bar->full[i], 1);
+      mbar_init(&bar->empty[i], 1);
     }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar->s_full[i], 1);
+      mbar_init(&bar->ds_full[i], 256);
+    }
+    mbar_init(&bar->dq_full, 1);
     mbar_init(&bar->drained, 1);
     fence_barrier_init();
   }
-  if (warp == 5) {
-    tmem_alloc(&bar->tmem, Shape::COLUMNS);
+  if (warp == 9) {
+    tmem_alloc(&bar->tmem, TMEM_COLUMNS);
     tmem_relinquish();
   }
+  tsb_launch::enter();
+  const int qt = blockIdx.x % p.qtiles, h = blockIdx.x / p.qtiles % p.heads, n = blockIdx.x / p.qtiles / p.heads;
+  const int shared = h / (p.heads / p.shared), q0 = qt * 128, half = warp >> 2, row = threadIdx.x & 127;
+  const float* tokens = p.key ? p.key + (long long)n * p.tk : nullptr;
+  const long long q_row = (long long)p.heads * p.d;
+  const long long q_at = ((long long)n * p.heads + h) * p.qtiles + qt, k_at = ((long long)n * p.shared + shared) * p.ktiles;
+  KeptRow<D> kept;                             // (under way while the block sets itself up)
+  KeptRow<Shape::BOTH ? D : 64> kept_g;
+  if (warp < 8) {
+    kept.read(p.qp, q_at, row, half);
+    if (Shape::BOTH) kept_g.read(p.gp, q_at, row, half);
+  }
+  const int tiles = (keys_in(tokens, p.tk) + 63) / 64;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(ALL, bar->tmem, 0);
-  tsb_launch::enter();
 
-  const int qt = blockIdx.x % p.qtiles, h = blockIdx.x / p.qtiles % p.heads, n = blockIdx.x / p.qtiles / p.heads;
-  const int shared = h / (p.heads / p.shared), q0 = qt * 128;
-  const float* tokens = p.key ? p.key + (long long)n * p.tk : nullptr;
-  const int tiles = (keys_in(tokens, p.tk) + 63) / 64;
-  const long long q_row = (long long)p.heads * p.d;
-  const long long q_at = ((long long)n * p.heads + h) * p.qtiles + qt, k_at = ((long long)n * p.shared + shared) * p.ktiles;
-
-  if (warp < 4) {
-    if (Shape::TWO) more_registers<200>();
-    float acc[D], before = 0.f;
+  if (warp < 8) {
+    more_registers<208>();
+    constexpr int OWN = D / 2;
+    const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);
+    kept.keep(mine, half);
+    if (Shape::BOTH) kept_g.keep(mine + Shape::G_AT, half);
+    tmem_st_wait();
+    tc_fence_before();
+    mbar_arrive(&bar->q_full);
+    float acc[OWN], before = 0.f;
 #pragma unroll
-    for (int c = 0; c < D; ++c) acc[c] = 0.f;
-    const uint32_t mine = tmem + ((uint32_t)warp << 21);
-    const float lse = load(p.lse + q_at * 128 + threadIdx.x), dot = load(p.dot + q_at * 128 + threadIdx.x);
+    for (int c = 0; c < OWN; ++c) acc[c] = 0.f;
+    const float lse = load(p.lse + q_at * 128 + row), dot = load(p.dot + q_at * 128 + row);
     const float q_unit = load(p.qp.units + q_at).x;
     const float2 g_unit = load(p.gp.units + q_at);
     bool ok = true;
     auto add_tile = [&](int j) {
-      const int b = j % BUFFERS;
-      if (!mbar_wait(&bar->dq_full[b], j / BUFFERS & 1, p.status, 0x311)) return false;
+      if (!mbar_wait(&bar->dq_full, j & 1, p.status, 0x311)) return false;
       tc_fence_after();
-      add_columns<false>(mine + DQ_AT + b * 128, acc, 0, D, 1.f, before);
+      add_columns<false>(mine + Shape::DQ_AT + half * OWN, acc, 1.f, before);
       return true;
     };
+    float token = 0.f, k_next = 0.f;
+    float2 v_next = make_float2(0.f, 0.f);
+    auto look_at = [&](int j) {
+      token = token_of(tokens, j * 64 + half * 32, p.tk);
+      if (j < tiles) k_next = load(p.kp.units + k_at + j / 2).x, v_next = load(p.vp.units + k_at + j / 2);
+    };
+    look_at(0);
     for (int j = 0; j < tiles; ++j) {
-      const int b = j % BUFFERS;
-      const unsigned in[2] = {keys_mask(tokens, j * 64, p.tk), keys_mask(tokens, j * 64 + 32, p.tk)};
-      const float k_unit = load(p.kp.units + k_at + j / 2).x;
-      const float2 v_unit = load(p.vp.units + k_at + j / 2);
+      const int b = j & 1;
+      const unsigned in = __ballot_sync(ALL, token != 0.f);
+      const float k_unit = k_next;
+      const float2 v_unit = v_next;
+      look_at(j + 1);
       const int e = exponent_of_ds(g_unit.y, v_unit.y, dot);
       // (2^e is not in the exponent, whose rounding it would make coarser)
       const float f = power_of_two(e), s_unit = q_unit * k_unit, dp_unit = g_unit.x * v_unit.x * f, dot_unit = dot * f;
-      if (!mbar_wait(&bar->s_full[b], j / BUFFERS & 1, p.status, 0x312)) { ok = false; break; }
+      if (!mbar_wait(&bar->s_full[b], j >> 1 & 1, p.status, 0x312)) { ok = false; break; }
       tc_fence_after();
-      if (BUFFERS == 1 && j > 0 && !(ok = add_tile(j - 1))) break;
-      const uint32_t at = mine + b * 64;
+      const uint32_t at = mine + Shape::S_AT + b * 64 + half * 32, dp_at = mine + Shape::DP_AT + b * 64 + half * 32;
       float s[2][16], dp[2][16];
       tmem_begin(at, s[0]);
-      tmem_begin(at + DP_AT, dp[0]);
+      tmem_begin(dp_at, dp[0]);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        float(&v)[16] = s[w & 1];
-        float(&x)[16] = dp[w & 1];
+      for (int w = 0; w < 2; ++w) {
+        float(&v)[16] = s[w];
+        float(&x)[16] = dp[w];
         tmem_ld_wait();
         tmem_arrived(v);
         tmem_arrived(x);
-        if (w < 3) {
-          tmem_begin(at + 16 * w + 16, s[(w + 1) & 1]);
-          tmem_begin(at + DP_AT + 16 * w + 16, dp[(w + 1) & 1]);
+        if (w < 1) {
+          tmem_begin(at + 16, s[1]);
+          tmem_begin(dp_at + 16, dp[1]);
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = exp2_fast(v[i] * s_unit - lse) * (x[i] * dp_unit - dot_unit);
-        if (in[w / 2] != ALL) {
-          const unsigned mask = in[w / 2] >> (w % 2 * 16);
+        if (in != ALL) {
+          const unsigned mask = in >> (w * 16);
 #pragma unroll
           for (int i = 0; i < 16; ++i) v[i] = (mask >> i) & 1 ? v[i] : 0.f;
         }
         tmem_st_pieces(at + 16 * w, v);
       }
       tmem_st_wait();
+      if (j > 0 && !(ok = add_tile(j - 1))) break;
       tc_fence_before();
       mbar_arrive(&bar->ds_full[b]);
-      if (BUFFERS == 2 && j > 0 && !(ok = add_tile(j - 1))) break;
       before = k_unit * power_of_two(-e);
     }
     if (ok && tiles > 0) ok = add_tile(tiles - 1);
-    const int t = q0 + threadIdx.x;
-    if (ok && t < p.tq) store_row(p.dq + ((long long)n * p.tq + t) * q_row + (long long)h * p.d, acc, p.scale, p.d, p.vec);
+    const int t = q0 + row;
+    if (ok && t < p.tq)
+      store_row(p.dq + ((long long)n * p.tq + t) * q_row + (long long)h * p.d + half * OWN, acc, p.scale, p.d - half * OWN, p.vec);
   } else {
-    if (Shape::TWO) fewer_registers<56>();
-    if (warp == 4 && elect_one() && tiles > 0) {
-      copy_tile<D>(q_tile, p.qp, q_at, &bar->q_full);
-      for (int j = 0; j < tiles; ++j) {
-        const int s = j & 1;
-        if (!mbar_wait(&bar->k_empty[s], (j >> 1 & 1) ^ 1, p.status, 0x313)) break;
-        copy_half<D>(k_tile + s * LK::BYTES, p.kp, k_at + j / 2, j & 1, &bar->k_full[s]);
-        if (j == 0) copy_tile<D>(g_tile, p.gp, q_at, &bar->g_full);
-        if (!mbar_wait(&bar->v_empty, (j & 1) ^ 1, p.status, 0x314)) break;
-        copy_half<D>(v_tile, p.vp, k_at + j / 2, j & 1, &bar->v_full);
+    fewer_registers<88>();
+    if (warp == 8 && elect_one()) {
+      for (int i = 0; i < 2 * tiles; ++i) {
+        const int s = i % SLOTS, j = i / 2;
+        if (i == 1 && !Shape::BOTH) copy_tile<D>(g_tile, p.gp, q_at, &bar->g_full);
+        if (!mbar_wait(&bar->empty[s], (i / SLOTS & 1) ^ 1, p.status, 0x313)) break;
+        copy_half<D>(ring + s * LK::BYTES, i & 1 ? p.vp : p.kp, k_at + j / 2, j & 1, &bar->full[s]);
       }
     }
-    if (warp == 5 && elect_one() && tiles > 0) {
-      const uint32_t qa = smem_u32(q_tile), ga = smem_u32(g_tile), ka = smem_u32(k_tile), va = smem_u32(v_tile);
+    if (warp == 9 && elect_one() && tiles > 0) {
+      const uint32_t ga = smem_u32(g_tile), ra = smem_u32(ring);
       bool ok = mbar_wait(&bar->q_full, 0, p.status, 0x315);
+      tc_fence_after();
       auto scores = [&](int j) {
-        const int s = j & 1, b = j % BUFFERS;
-        if (!mbar_wait(&bar->k_full[s], j >> 1 & 1, p.status, 0x316)) return false;
+        const int b = j & 1, ks = 2 * j % SLOTS, vs = (2 * j + 1) % SLOTS;
+        if (!mbar_wait(&bar->full[ks], 2 * j / SLOTS & 1, p.status, 0x316)) return false;
         tc_fence_after();
-        product_of_rows<D, 128, 64>(tmem + b * 64, qa, ka + s * LK::BYTES);
-        if (j == 0 && !mbar_wait(&bar->g_full, 0, p.status, 0x315)) return false;
-        if (!mbar_wait(&bar->v_full, j & 1, p.status, 0x317)) return false;
+        product_of_kept_rows<D, 64>(tmem + Shape::S_AT + b * 64, tmem, ra + ks * LK::BYTES);
+        if (!Shape::BOTH && j == 0 && !mbar_wait(&bar->g_full, 0, p.status, 0x315)) return false;
+        if (!mbar_wait(&bar->full[vs], (2 * j + 1) / SLOTS & 1, p.status, 0x317)) return false;
         tc_fence_after();
-        product_of_rows<D, 128, 64>(tmem + DP_AT + b * 64, ga, va);
+        if (Shape::BOTH) product_of_kept_rows<D, 64>(tmem + Shape::DP_AT + b * 64, tmem + Shape::G_AT, ra + vs * LK::BYTES);
+        else product_of_rows<D, 128, 64>(tmem + Shape::DP_AT + b * 64, ga, ra + vs * LK::BYTES);
         umma_commit(&bar->s_full[b]);
-        umma_commit(&bar->v_empty);
+        umma_commit(&bar->empty[vs]);
         return true;
       };
-      for (int j = 0; j < BUFFERS && j < tiles && ok; ++j) ok = scores(j);
+      // (keys stay in their slot until dq is computed)
+      for (int j = 0; j < 2 && j < tiles && ok; ++j) ok = scores(j);
       for (int j = 0; j < tiles && ok; ++j) {
-        const int b = j % BUFFERS;
-        if (!(ok = mbar_wait(&bar->ds_full[b], j / BUFFERS & 1, p.status, 0x318))) break;
+        const int b = j & 1, ks = 2 * j % SLOTS;
+        if (!(ok = mbar_wait(&bar->ds_full[b], j >> 1 & 1, p.status, 0x318))) break;
         tc_fence_after();
-        product_with_columns<D, 64>(tmem + DQ_AT + b * 128, tmem + b * 64, ka + (j & 1) * LK::BYTES);
-        umma_commit(&bar->k_empty[j & 1]);
-        umma_commit(&bar->dq_full[b]);
-        if (j + BUFFERS < tiles) ok = scores(j + BUFFERS);
+        product_with_columns<D, 64>(tmem + Shape::DQ_AT, tmem + Shape::S_AT + b * 64, ra + ks * LK::BYTES);
+        umma_commit(&bar->empty[ks]);
+        umma_commit(&bar->dq_full);
+        if (j + 2 < tiles) ok = scores(j + 2);
       }
       if (!ok) drain(&bar->drained);
     }
@@ -732,17 +837,17 @@ __global__ void __launch_bounds__(QueryShape<D>::BLOCK, QueryShape<D>::TWO ? 2 :
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) tmem_dealloc(tmem, Shape::COLUMNS);
+  if (warp == 9) tmem_dealloc(tmem, TMEM_COLUMNS);
 }
 
 // dk and dv: a block takes 128 keys of a shared head and tiles of 64 queries of every head that reads it.  S^T and dP^T have
 // the keys as rows, so P^T and dS^T are A operands as they lie.  Halves of the tiles of queries and of gradients share a ring
 // of slots (q, g, q, g, ...), each with its rows' log-sum-exps or dots.  Warps 0 to 3 take the first 32 queries of a tile and
-// add up dv, 4 to 7 the others and dk; 8: copies; 9 issues.  Two tiles of S^T and dP^T are in tensor memory.  (Two blocks of
-// four such warps to an SM, as above, took 516 us in place of 397 for 4 x 2048 x 2048, 16 heads of 64: the two sums leave a
-// thread no registers.)
+// add up dv, 4 to 7 the others and dk; 8: copies; 9 issues.  Two tiles of S^T and dP^T are in tensor memory.  4 x 2048 x 2048, 16
+// heads of 64: 358 us; 2 x 2000 x 4111, 16 heads of 128 on 4: 860 us, 313 TFLOP/s, so 940 of fp16 products.  (Two blocks of four
+// such warps to an SM were a third slower, 516 us in place of 397 for the former: the two sums leave a thread no registers.)
 template <int D> struct StateShape {
-  static constexpr int BLOCK = 384, DP_AT = 128, DV_AT = 256, DK_AT = 384, SLOTS = D == 64 ? 6 : 3;
+  static constexpr int DP_AT = 128, DV_AT = 256, DK_AT = 384, SLOTS = D == 64 ? 6 : 3;
   using LK = Tile<D, 128>;
   using LQ = Tile<D, 64>;
   static constexpr int TILES = 2 * LK::BYTES + SLOTS * LQ::BYTES, SMEM = TILES + CONTROL + (SLOTS - 3) * 256;
@@ -755,7 +860,7 @@ constexpr int ROWS_AT = 256;                   // of the slots' log-sum-exps and
 static_assert(sizeof(StateControl) <= ROWS_AT && ROWS_AT + 3 * 256 <= CONTROL, "");
 
 template <int D>
-__global__ void __launch_bounds__(StateShape<D>::BLOCK, 1) grad_of_states(const Problem p) {
+__global__ void __launch_bounds__(BLOCK, 1) grad_of_states(const Problem p) {
   using Shape = StateShape<D>;
   using LQ = typename Shape::LQ;
   using LK = typename Shape::LK;
@@ -811,7 +916,7 @@ __global__ void __launch_bounds__(StateShape<D>::BLOCK, 1) grad_of_states(const 
     auto add_tile = [&](int j) {
       if (!mbar_wait(&bar->sum_full, j & 1, p.status, 0x322)) return false;
       tc_fence_after();
-      add_columns<false>(mine + (half ? Shape::DK_AT : Shape::DV_AT), acc, 0, D, 1.f, before);
+      add_columns<false>(mine + (half ? Shape::DK_AT : Shape::DV_AT), acc, 1.f, before);
       return true;
     };
     for (int j = 0; j < tiles; ++j) {
@@ -968,8 +1073,8 @@ __device__ __forceinline__ void copy_piece(float* to, const float* from, int cou
 template <int D> __device__ __forceinline__ void store_cell(const Problem& p, int n, int shared, int i, float top, float total, float sum) {
   const int r = i / D, c = i % D, per = p.heads / p.shared, t = r / per, h = shared * per + r % per;
   if (t >= p.tq) return;
-  if (c < p.d) p.y[(((long long)n * p.tq + t) * p.heads + h) * p.d + c] = total > 0.f ? sum / total : 0.f;
-  if (c == 0) p.lse[((long long)n * p.heads + h) * 128 + t] = total > 0.f ? top + log2f(total) : -NEG_INF;
+  if (c < p.d) p.y[(((long long)n * p.tq + t) * p.heads + h) * p.d + c] = total != 0.f ? sum / total : 0.f;
+  if (c == 0) p.lse[((long long)n * p.heads + h) * 128 + t] = total != 0.f ? top + log2f(total) : -NEG_INF;
 }
 
 template <int D, int ROWS>
@@ -1162,13 +1267,14 @@ int launched(cudaError_t e) {
   return late ? TSB_ERR_TIMEOUT | (late << 8) : TSB_OK;
 }
 
-constexpr int MAX_DIM = 128, FEW_ROWS = 8;
+constexpr int MAX_DIM = 128, FEW_ROWS = 8, MAX_ROWS = INT32_MAX - 65536;      // (room to round up and look ahead in 32 bits)
 
 // False: not a problem that the kernels take.  `vec` holds for all arrays given.
 template <class... A>
 bool describe(Problem& p, int n, int tq, int tk, int heads, int shared, int d, float scale, const float* q, const float* kv,
               const float* key, A... others) {
   if (n < 0 || tq < 0 || tk < 0 || heads <= 0 || shared <= 0 || heads % shared || d <= 0 || d > MAX_DIM) return false;
+  if (tq > MAX_ROWS || tk > MAX_ROWS) return false;
   const float* all[] = {q, kv, static_cast<const float*>(others)...};
   uintptr_t bits = 0;
   for (const float* a : all) bits |= reinterpret_cast<uintptr_t>(a);
@@ -1183,13 +1289,13 @@ bool describe(Problem& p, int n, int tq, int tk, int heads, int shared, int d, f
 }
 
 template <class K>
-int run(K kernel, const Problem& p, long long blocks, int threads, int smem, cudaStream_t st, tsb_launch::SmemLimit& limit) {
+int run(K kernel, const Problem& p, long long blocks, int smem, cudaStream_t st, tsb_launch::SmemLimit& limit) {
   if (blocks > INT32_MAX) return TSB_ERR_ARG;
   Problem q = p;
   q.status = tsb_host::status_word(st);
   if (!q.status) return TSB_ERR_LAUNCH;
   cudaError_t e = limit.raise(kernel, smem);
-  if (e == cudaSuccess) e = tsb_launch::launch(kernel, dim3((unsigned)blocks), dim3(threads), smem, st, q);
+  if (e == cudaSuccess) e = tsb_launch::launch(kernel, dim3((unsigned)blocks), dim3(BLOCK), smem, st, q);
   return launched(e);
 }
 
@@ -1313,8 +1419,8 @@ int tsb_cross_attention(const float* q, const float* kv, const float* key, float
   if (rc) return rc;
   const long long blocks = (long long)n * heads * p.qtiles;
   static tsb_launch::SmemLimit limit64, limit128;
-  if (d <= 64) return run(attend<64>, p, blocks, ForwardShape<64>::BLOCK, ForwardShape<64>::SMEM, st, limit64);
-  return run(attend<128>, p, blocks, ForwardShape<128>::BLOCK, ForwardShape<128>::SMEM, st, limit128);
+  if (d <= 64) return run(attend<64>, p, blocks, ForwardShape<64>::SMEM, st, limit64);
+  return run(attend<128>, p, blocks, ForwardShape<128>::SMEM, st, limit128);
 }
 
 // The pieces of q, kv and g, and the sums of g y over a head's row, for both gradients.  prepared: `have` bytes on a
@@ -1342,8 +1448,8 @@ int tsb_cross_attention_grad_q(const void* prepared, long long have, const float
   p.dq = dq;
   const long long blocks = (long long)n * heads * p.qtiles;
   static tsb_launch::SmemLimit limit64, limit128;
-  if (d <= 64) return run(grad_of_queries<64>, p, blocks, QueryShape<64>::BLOCK, QueryShape<64>::SMEM, st, limit64);
-  return run(grad_of_queries<128>, p, blocks, QueryShape<128>::BLOCK, QueryShape<128>::SMEM, st, limit128);
+  if (d <= 64) return run(grad_of_queries<64>, p, blocks, QueryShape<64>::SMEM, st, limit64);
+  return run(grad_of_queries<128>, p, blocks, QueryShape<128>::SMEM, st, limit128);
 }
 
 int tsb_cross_attention_grad_kv(const void* prepared, long long have, const float* key, const float* lse, float* dkv, int n, int tq, int tk, int heads,
@@ -1360,8 +1466,8 @@ int tsb_cross_attention_grad_kv(const void* prepared, long long have, const floa
   p.dkv = dkv;
   const long long blocks = (long long)n * shared * p.ktiles;
   static tsb_launch::SmemLimit limit64, limit128;
-  if (d <= 64) return run(grad_of_states<64>, p, blocks, StateShape<64>::BLOCK, StateShape<64>::SMEM, st, limit64);
-  return run(grad_of_states<128>, p, blocks, StateShape<128>::BLOCK, StateShape<128>::SMEM, st, limit128);
+  if (d <= 64) return run(grad_of_states<64>, p, blocks, StateShape<64>::SMEM, st, limit64);
+  return run(grad_of_states<128>, p, blocks, StateShape<128>::SMEM, st, limit128);
 }
 
 }  // extern "C"

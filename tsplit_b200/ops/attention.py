@@ -189,7 +189,10 @@ class CrossAttentionGradStatesOp(_CrossAttentionGradient):
     def np_compute(self, node, iv):
         ds, p, g, q, _ = self._ds(node, iv)
         dk, dv = ((np.swapaxes(a, 3, 4) @ b).sum(2, keepdims=True) for a, b in ((ds, q), (p, g)))
-        return np.stack([_back(dk), _back(dv)], 2).astype(np.float32)
+        both = np.stack([_back(dk), _back(dv)], 2).astype(np.float32)
+        if len(iv) > 4:                                        # (also where a query that is no number meets them)
+            both[iv[4] == 0] = 0
+        return both
 
     def infer_shape(self, node, s):
         self._check(s)
