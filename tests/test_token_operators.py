@@ -79,6 +79,17 @@ def test_embedding_of_unusual_ids(what, n, ctx):
     check_embed(r.standard_normal((v, d), np.float32), ids.astype(np.float32), r.standard_normal((n, d), np.float32), 1.0, 7, ctx)
 
 
+@pytest.mark.parametrize("n,v,d", [(1, 64000, 8), (2, 3, 130), (511, 100, 5), (512, 1, 33), (512, 2000, 132), (513, 2000, 132),
+                                   (300, 70001, 12), (400, 40, 260), (500, 1100000, 4)])
+@pytest.mark.parametrize("what", ["spread", "skewed", "two"])
+def test_embedding_gradient_of_a_few_tokens(n, v, d, what, ctx):
+    """Around the length up to which tokens are not sorted; rows that few, more than 32 or all positions have."""
+    r = rng(n, v, d)
+    ids = {"spread": r.integers(0, v, n), "skewed": np.exp(r.random(n) * np.log(v)).astype(np.int64),
+           "two": np.where(r.random(n) < 0.9, v - 1, 0)}[what]
+    check_embed(r.standard_normal((v, d), np.float32), ids.astype(np.float32), r.standard_normal((n, d), np.float32), -1.5, None, ctx)
+
+
 def test_embedding_of_no_number_is_outside(ctx):
     ids = np.array([np.nan, np.inf, -np.inf, 1e30, 2], np.float32)
     if ctx is None:
