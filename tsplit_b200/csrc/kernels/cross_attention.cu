@@ -1236,26 +1236,26 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) attend_few(const Problem p,
   }
 }
 
-// A block per sentence and shared head: the parts of its keys, in their order.
+// 64 cells of the rows that read a shared head: the parts of its keys, in their order.
 template <int D, int ROWS>
-__global__ void __launch_bounds__(256) join_parts(const Problem p, int split, const float* parts) {
+__global__ void __launch_bounds__(64) join_parts(const Problem p, int split, const float* parts) {
   tsb_launch::enter();
-  constexpr int CELLS = ROWS * D;
-  const float* const from = parts + (long long)blockIdx.x * split * ROWS * (D + 2);
-  for (int i = threadIdx.x; i < CELLS; i += 256) {
-    const int r = i / D;
-    float top = NEG_INF, total = 0.f, sum = 0.f;
-    for (int b = 0; b < split; ++b) top = fmaxf(top, load(from + b * ROWS * (D + 2) + CELLS + 2 * r));
-    const float ref = top == NEG_INF ? 0.f : top;
-#pragma unroll 4
-    for (int b = 0; b < split; ++b) {
-      const float* const at = from + b * ROWS * (D + 2);
-      const float f = exp2_fast(load(at + CELLS + 2 * r) - ref);
-      total += load(at + CELLS + 2 * r + 1) * f;
-      sum += load(at + i) * f;
-    }
-    store_cell<D>(p, blockIdx.x / p.shared, blockIdx.x % p.shared, i, top, total, sum);
+  constexpr int CELLS = ROWS * D, BLOCKS = (CELLS + 63) / 64;
+  const int pair = blockIdx.x / BLOCKS, i = blockIdx.x % BLOCKS * 64 + threadIdx.x, r = i / D;
+  if (i >= CELLS) return;
+  const float* const from = parts + (long long)pair * split * ROWS * (D + 2);
+  float top = NEG_INF, total = 0.f, sum = 0.f;
+#pragma unroll 8
+  for (int b = 0; b < split; ++b) top = fmaxf(top, load(from + b * ROWS * (D + 2) + CELLS + 2 * r));
+  const float ref = top == NEG_INF ? 0.f : top;
+#pragma unroll 8
+  for (int b = 0; b < split; ++b) {
+    const float* const at = from + b * ROWS * (D + 2);
+    const float f = exp2_fast(load(at + CELLS + 2 * r) - ref);
+    total += load(at + CELLS + 2 * r + 1) * f;
+    sum += load(at + i) * f;
   }
+  store_cell<D>(p, pair / p.shared, pair % p.shared, i, top, total, sum);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -1384,7 +1384,7 @@ template <int D, int ROWS> int run_few(const Problem& p, cudaStream_t st) {
   if (e == cudaSuccess)
     e = tsb_launch::launch(attend_few<D, ROWS>, dim3((unsigned)(pairs * split)), dim3(FEW_WARPS * 32), SMEM, st, p, split, parts);
   if (e == cudaSuccess && split > 1)
-    e = tsb_launch::launch(join_parts<D, ROWS>, dim3((unsigned)pairs), dim3(256), 0, st, p, split, parts);
+    e = tsb_launch::launch(join_parts<D, ROWS>, dim3((unsigned)pairs * ((ROWS * D + 63) / 64)), dim3(64), 0, st, p, split, parts);
   return launched(e);
 }
 template <int D> int few(const Problem& p, int rows, cudaStream_t st) {
