@@ -74,9 +74,9 @@ class CrossAttentionOp(Op):
 
     def gpu_compute(self, node, iv, out, stream):
         sizes = _sizes(iv[0].shape, iv[1].shape, iv[2].shape if len(iv) > 2 else None)
-        n, tq, _, h, _, d = sizes
+        node.state["runs"] = node.state.get("runs", 0) + 1
         G.cross_attention(iv[0], iv[1], iv[2] if len(iv) > 2 else None, out, _row_sums(node, sizes, iv[0].ctx), sizes,
-                          self.scale_of(node, d), stream)
+                          self.scale_of(node, sizes[5]), stream)
 
     def gradient(self, node, g):
         return cross_attention_gradient_op(node, g) + [None] * (len(node.inputs) - 2)
@@ -112,11 +112,14 @@ def _prepared_floats(n, tq, tk, h, shared, d):
 
 class CrossAttentionPrepareOp(Op):
     """Operands of both gradients as the tensor cores take them, and ``sum(g * y)`` over every row: a flat array that only the
-    kernels read."""
+    kernels read.  The gradients also read what the forward kernel has left, so it has to run before each of them: a result that
+    is fed in its place is refused."""
     name = "CrossAttentionPrepare"
 
     def __call__(self, g, forward):
-        return Op.__call__(self, g, forward, *forward.inputs, scale=forward.attrs["scale"])
+        node = Op.__call__(self, g, forward, *forward.inputs, scale=forward.attrs["scale"], fwd=forward)
+        node.state = {}
+        return node
 
     def np_compute(self, node, iv):
         return np.zeros(self.infer_shape(node, [v.shape for v in iv]), np.float32)
@@ -125,6 +128,10 @@ class CrossAttentionPrepareOp(Op):
         g, y, q, kv = iv[:4]
         key = iv[4] if len(iv) > 4 else None
         sizes = _sizes(q.shape, kv.shape, key.shape if key is not None else None)
+        runs = node.attrs["fwd"].state.get("runs", 0)
+        if runs == node.state.get("of", 0):
+            raise ValueError("the gradient of a cross attention takes the forward pass of the same step, not a result that was fed")
+        node.state["of"] = runs
         G.cross_attention_prepare(q, kv, key, g, y, out, sizes, CrossAttentionOp.scale_of(node, sizes[5]), stream)
 
     def gradient(self, node, g):
