@@ -44,9 +44,10 @@ def _probabilities(q, kv, key, scale):
     keep = np.ones((kv.shape[0], kv.shape[1]), bool) if key is None else key != 0
     at = keep[:, None, None, :, None]
     k, v = np.where(at, k, 0), np.where(at, v, 0)
-    x = np.where(keep[:, None, None, None, :], q @ np.swapaxes(k, 3, 4) * scale, -np.inf)
-    m = x.max(axis=4, keepdims=True, initial=-np.inf)
-    p = np.exp(x - np.where(np.isneginf(m), 0, m))
+    with np.errstate(invalid="ignore"):                     # (a query that is no number)
+        x = np.where(keep[:, None, None, None, :], q @ np.swapaxes(k, 3, 4) * scale, -np.inf)
+        m = x.max(axis=4, keepdims=True, initial=-np.inf)
+        p = np.exp(x - np.where(np.isneginf(m), 0, m))
     z = p.sum(axis=4, keepdims=True)
     return p / np.where(z == 0, 1, z), q, k, v
 
