@@ -132,6 +132,54 @@ def single(op, batch, channel, hw, iters):
             fn = lambda: G.gemm(sc, v, ctxv, False, False, st, batch=n * heads, m=t, n=d, k=t, sa=t * t, sb=d, sc=d,
                                 lda=t, ldb=heads * d, ldc=heads * d, heads=heads, head_mask=6)
             work, unit = (sc.nbytes + v.nbytes + ctxv.nbytes) / 1e6, "GB/s"
+    elif op in ("cross_attention", "cross_attention_grad"):
+        # batch = N, channel = heads, hw = length of queries and states; head size 64
+        from .ops.attention import _prepared_floats
+        heads, t, d = c, hw, 64
+        q, g, y, dq = (ndarray.empty((n, t, heads, d), ctx, channels_last=False) for _ in range(4))
+        kv, dkv = (ndarray.empty((n, t, 2, heads, d), ctx) for _ in range(2))
+        tok, lse = ndarray.empty((n, t), ctx), ndarray.empty((n, heads, -(-t // 128) * 128), ctx)
+        sizes = (n, t, t, heads, heads, d)
+        prepared = ndarray.empty((_prepared_floats(*sizes),), ctx)
+        for a in (q, g, kv):
+            a.t.normal_()
+        tok.t.fill_(1.0)
+        G.cross_attention(q, kv, tok, y, lse, sizes, 0.125, st)
+        if op == "cross_attention":
+            fn = lambda: G.cross_attention(q, kv, tok, y, lse, sizes, 0.125, st)
+        else:
+            def fn():
+                G.cross_attention_prepare(q, kv, tok, g, y, prepared, sizes, 0.125, st)
+                G.cross_attention_grad_q(prepared, tok, lse, dq, sizes, 0.125, st)
+                G.cross_attention_grad_kv(prepared, tok, lse, dkv, sizes, 0.125, st)
+        work, unit = (4.0 if op == "cross_attention" else 14.0) * n * heads * t * t * d / 1e9, "TFLOP/s"
+    elif op in ("token_log_prob", "token_log_prob_grad"):
+        # rows = batch * channel, vocabulary = hw; five alternatives
+        rows, cols = n * c, hw
+        x, dx = (ndarray.empty((rows, cols), ctx) for _ in range(2))
+        out, g = (ndarray.empty((rows, 13), ctx) for _ in range(2))
+        ids = ndarray.empty((rows,), ctx)
+        x.t.normal_(), g.t.normal_(), ids.t.random_(0, cols)
+        G.token_score(x, ids, out, 5, st)
+        if op == "token_log_prob":
+            fn = lambda: G.token_score(x, ids, out, 5, st)
+            work, unit = x.nbytes / 1e6, "GB/s"
+        else:
+            fn = lambda: G.token_score_grad(x, ids, out, g, dx, st)
+            work, unit = 2.0 * x.nbytes / 1e6, "GB/s"
+    elif op in ("scaled_embedding", "scaled_embedding_grad"):
+        # tokens = batch * channel, a vocabulary of 32000 with Zipf's frequencies, hw columns
+        tokens, vocab = n * c, 32000
+        table, dtable = (ndarray.empty((vocab, hw), ctx) for _ in range(2))
+        y, ids = ndarray.empty((tokens, hw), ctx), ndarray.empty((tokens,), ctx)
+        table.t.normal_(), y.t.normal_()
+        ids.t.copy_(torch.exp(torch.rand(tokens, device="cuda", dtype=torch.float64) * float(np.log(vocab))).floor())
+        if op == "scaled_embedding":
+            fn = lambda: G.scaled_embedding(table, ids, y, 2.0, st)
+            work, unit = (y.nbytes + min(y.nbytes, table.nbytes)) / 1e6, "GB/s"
+        else:
+            fn = lambda: G.scaled_embedding_grad(y, ids, dtable, 2.0, None, st)
+            work, unit = (y.nbytes + dtable.nbytes) / 1e6, "GB/s"
     elif op in ("allreduce_emulate", "optimizer"):
         # elements = batch * channel * hw * hw
         elems = n * c * hw * hw // 4 * 4
@@ -214,7 +262,8 @@ def main():
                                   "conv_wgrad", "bnrelu_bwd", "softmax", "softmax_grad", "ce_grad",
                                   "allreduce_emulate", "optimizer", "maxpool_fwd", "maxpool_bwd",
                                   "conv_dgrad_s2", "conv_dgrad_s2_1x1", "masked_softmax", "attention_scores",
-                                  "attention_context"])
+                                  "attention_context", "cross_attention", "cross_attention_grad", "token_log_prob",
+                                  "token_log_prob_grad", "scaled_embedding", "scaled_embedding_grad"])
     p.add_argument("--sweep", default="batch", choices=["batch", "channel", "hw"])
     p.add_argument("--single", action="store_true", help="one configuration (for profiler captures)")
     p.add_argument("--batch", type=int, default=32)
