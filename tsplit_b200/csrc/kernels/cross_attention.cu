@@ -436,10 +436,11 @@ __device__ __forceinline__ void store_row(float* to, const float (&v)[COUNT], fl
 // of a tile is added to the registers before the next one's product.
 //
 // Bound by the tensor cores and by the threads between two products.  With the splitting: 2 x 2000 x 4111, 16 heads of 128 on 4:
-// 356 us, 379 TFLOP/s, so 1.14 PFLOP/s of fp16 products; 4 x 2048 x 2048, 16 heads of 64: 227 us; 32 x 255 x 256, 8 heads of 64:
-// 50 us.  (A row to a thread and two blocks to an SM, operands in shared memory: 444, 278 and 47 us.  A block's beginning and
+// 356 us, 379 TFLOP/s, so 1.14 PFLOP/s of fp16 products; 4 x 2048 x 2048, 16 heads of 64: 222 us; 32 x 255 x 256, 8 heads of 64:
+// 49 us.  (A row to a thread and two blocks to an SM, operands in shared memory: 444, 278 and 47 us.  A block's beginning and
 // end are not hidden now, which a few key tiles show, but a product with A in tensor memory takes 32 cycles for 16 x 64 numbers
-// of B, with A in shared memory 48, and two threads do a row's soft-max in half the time.)
+// of B, with A in shared memory 48, and two threads do a row's soft-max in half the time.  Two tiles of queries to a block, sixteen
+// soft-max warps: 51 and 258 us for 64 columns, fewer blocks that share the SMs less evenly.)
 template <int D> struct ForwardShape {
   static constexpr int PARTS = D / 64, ROWS = 128 / PARTS, SLOTS = 6;              // of a tile in a slot each
   static constexpr int S_AT = D, Y_AT = S_AT + 2 * 128;                            // behind the queries
@@ -526,25 +527,25 @@ __global__ void __launch_bounds__(BLOCK, 1) attend(const Problem p) {
       unsigned in[2];
 #pragma unroll
       for (int w = 0; w < 2; ++w) in[w] = __ballot_sync(ALL, token[w] != 0.f);
-      const float unit = q_unit * k_next, next_unit = v_next;
+      // (above 0, so that -inf stays so: tiles of nothing but zeros have the least unit, and scores of 2^-90 are as good as none)
+      const float unit = fmaxf(q_unit * k_next, 1.2e-38f), next_unit = v_next;
       look_at(j + 1);
       if (!mbar_wait(&bar->s_full[b], j >> 1 & 1, p.status, 0x302)) { ok = false; break; }
       tc_fence_after();
       const uint32_t at = mine + Shape::S_AT + b * 128 + half * 64;
-      float part[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};     // (chains that do not wait for one another)
+      float s[2][32], part[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};                // (chains that do not wait for one another)
+      tmem_begin(at, s[0]);
+      tmem_begin(at + 32, s[1]);
+      tmem_ld_wait();
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        float s[32];
-        tmem_begin(at + 32 * w, s);
-        tmem_ld_wait();
-        tmem_arrived(s);
-        if (in[w] == ALL) {
+        tmem_arrived(s[w]);
+        if (in[w] != ALL) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) part[i & 3] = fmaxf(part[i & 3], s[i]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) part[i & 3] = fmaxf(part[i & 3], (in[w] >> i) & 1 ? s[i] : NEG_INF);
+          for (int i = 0; i < 32; ++i) s[w][i] = (in[w] >> i) & 1 ? s[w][i] : NEG_INF;
         }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) part[i & 3] = fmaxf(part[i & 3], s[w][i]);
       }
       const float own = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
       shared_max[j & 1][half][row] = own;
@@ -553,24 +554,15 @@ __global__ void __launch_bounds__(BLOCK, 1) attend(const Problem p) {
       const float most = fmaxf(own, shared_max[j & 1][half ^ 1][row]);
       const float top = fmaxf(m, most == NEG_INF ? NEG_INF : most * unit), ref = top == NEG_INF ? 0.f : top;
       const float factor = exp2_fast(m - ref), shift = TOP + 1 - ref;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f}, s[2][16];
-      tmem_begin(at, s[0]);
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        float(&v)[16] = s[w & 1];
-        tmem_ld_wait();
-        tmem_arrived(v);
-        if (w < 3) tmem_begin(at + 16 * w + 16, s[(w + 1) & 1]);
+      for (int w = 0; w < 2; ++w) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = exp2_fast(v[i] * unit + shift);
-        if (in[w / 2] != ALL) {
-          const unsigned mask = in[w / 2] >> (w % 2 * 16);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = (mask >> i) & 1 ? v[i] : 0.f;
+        for (int i = 0; i < 32; ++i) {
+          s[w][i] = exp2_fast(s[w][i] * unit + shift);           // (a masked one: 2^-inf)
+          sum[i & 3] += s[w][i];
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sum[i & 3] += v[i];
-        tmem_st_pieces(at + 16 * w, v);
+        tmem_st_pieces(at + 32 * w, s[w]);
       }
       tmem_st_wait();
       if (j > 0 && !(ok = add_tile(j - 1))) break;
