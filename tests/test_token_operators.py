@@ -272,6 +272,44 @@ def test_alternatives_of_unusual_rows(kind, v, ctx):
     check_score(x, ids, 11, g, ctx)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [31, 32, 33, 128, 129, 512, 513, 1024, 1025, 2048, 2049, 4096, 4097, 6144, 6145, 8192, 8193, 12288, 12289, 16384,
+                               16385, 32768, 32769])
+@pytest.mark.parametrize("rows,top", [(3, 0), (5, 17), (150, 1), (150, 32)])
+def test_scores_at_the_borders_between_layouts(rows, v, top):
+    """Rows of one warp, of several, of a block, of a cluster, and the number of rows from which another is taken."""
+    top = min(top, v)
+    x, ids, g = score_case(rows, v, top)
+    check_score(x, ids, top, g, ndarray.gpu(0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,v,top", [(1183, 40, 5), (1184, 40, 5), (1185, 2047, 3), (1184, 2048, 32), (1190, 2049, 1), (3001, 700, 0)])
+def test_gradients_of_many_short_rows(rows, v, top):
+    x, ids, g = score_case(rows, v, top)
+    check_score(x, ids, top, g, ndarray.gpu(0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [30, 1000, 2000, 5000, 20000])
+@pytest.mark.parametrize("top", [1, 32])
+def test_alternatives_of_many_equal_and_missing_logits(v, top):
+    """More columns that reach the bound than there is room for, and rows with fewer numbers than alternatives."""
+    top = min(top, v)
+    x = np.full((6, v), 2.5, np.float32)
+    x[1, : v // 2] = -np.inf
+    x[2] = -np.inf
+    x[3] = np.nan
+    x[4, 1:] = np.nan
+    x[5, ::3] = 9.0
+    ids = np.array([0, v - 1, 3, 4, 0, v + 5], np.float32)
+    feeds = {"x": x, "i": ids, "g": np.ones((6, 3 + 2 * top), np.float32)}
+    want = evaluate(score_graph(top), feeds, None)[0]
+    got = evaluate(score_graph(top), feeds, ndarray.gpu(0))[0]
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[:, 3 + top:], want[:, 3 + top:])
+    assert np.allclose(got, want, rtol=0, atol=1e-5, equal_nan=True)          # (numbers of size 10: 10 steps of 2^-20 each)
+
+
 def test_rows_of_masked_logits(ctx):
     """Rows with fewer tokens that can be said than alternatives are asked for, and none at all."""
     x = np.full((4, 300), -np.inf, np.float32)

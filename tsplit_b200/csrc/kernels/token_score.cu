@@ -7,16 +7,18 @@
 // makes the row's results NaN and is no alternative itself (id -1 where fewer than `top` others are left).  Equal logits are
 // taken by their column, the lowest first.
 //
-// One pass over the logits: every thread keeps a running (max, Z, sum e^u u).  The top tokens come from the maxima of units of
-// the row (1 KB or more each that a warp reads in one go; in short rows the 8 columns that a thread reads in one go).  With W
-// warps, a bound that the ceil(top / W)-th best unit of every warp reaches is reached by `top` columns, so by every top token;
-// of the units that reach it the top-th best one is the bound.  Their columns are read again (about `top` KB a row); what reaches the bound, some dozens, is collected in shared memory as
-// 64-bit numbers that order by logit and then by column, and each one's place is how many are larger.  Where more are found
-// than there is room for (ties, many equal units), every warp merges what it finds into a sorted list of the best 32, one
-// per lane, against a rising bound.  (4096 x 128001, 20 alternatives, without any 310 us: such lists in the first pass 572 us,
-// in the second 497, sorting networks in place of counting 415; now 373.)
+// One pass over the logits: every thread keeps a running (max, Z, sum e^u u).  Rows of up to 16384 columns, and of up to 32768 where
+// there are no more rows than SMs, stay in registers (score_short_rows).  In longer ones (score_rows) the top tokens come from the
+// maxima of units of the row (1 KB or more each that a warp reads in one go; in the shares of a cluster that splits a row the 8
+// columns that a thread reads in one go).  With W warps, a bound that the ceil(top / W)-th best unit of every warp reaches is
+// reached by `top` columns, so by every top token; of the units that reach it the top-th best one is the bound.  Their columns are
+// read again (about `top` KB a row); what reaches the bound, some dozens, is collected in shared memory as 64-bit numbers that order
+// by logit and then by column, and each one's place is how many are larger.  Where more are found than there is room for (ties,
+// many equal units), every warp merges what it finds into a sorted list of the best 32, one per lane, against a rising bound.
+// (4096 x 128001, 20 alternatives, without any 310 us: such lists in the first pass 572 us, in the second 497, sorting networks in
+// place of counting 415; now 373.)
 // What a row's end takes is latency that other rows on the SM have to cover, so it is kept short.
-// Few rows are split over a cluster of blocks that join through distributed shared memory.
+// Few long rows are split over a cluster of blocks that join through distributed shared memory.
 #include <cuda_runtime.h>
 #include <cooperative_groups.h>
 #include <stdint.h>
@@ -422,24 +424,163 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 6) score_rows(const float* x, 
   if (TOP && part == 0) fill(place(s.lists[0], split * top, write));
 }
 
-// dx_c = sum_i w_i (1[c = id_i] - p_c) + w_lse p_c - w_H p_c (log p_c + H), with w the gradient of `out` and the sum over
-// the given token and the top ones.  Columns that are an id are computed apart, with 1 - p as -expm1(log p), after the
-// rest; a block takes a chunk of a row.
-__global__ void __launch_bounds__(256) score_grad(const float* x, const float* ids, const float* out, const float* g,
-                                                  float* __restrict__ dx, long long cols, int top, unsigned chunk, int chunks) {
+// Short rows stay in registers: WARPS warps take a row of up to 32 N WARPS columns, a warp every WARPS-th 32 of them; with one warp to
+// a row a block takes eight rows.  The need-th best of a warp's lane maxima, need = top / WARPS rounded up, is reached by as many
+// columns, so the least of these bounds the top columns from below; what reaches it goes to shared memory, where each one's place is
+// how many are larger.  Where that is more than there is room for (ties), the best one below the last is looked for `top` times.
+// What does not fit one SM's registers with rows to spare goes to score_rows.  (Without alternatives, with five, with twenty: 8192 x
+// 1000 5.8, 9.7 and 14 us, by units that are read again 13, 45 and 97; 8192 x 5000 28, 46 and 49, 35, 80 and 114; one row of 32000 3.7,
+// 5.8 and 6.2, of which a cluster makes 4, 9 and 14.)
+constexpr int SHORT_WARPS = 8, SHORT_FOUND = 128;
+template <int N, int WARPS, bool TOP>
+__global__ void __launch_bounds__(WARPS > SHORT_WARPS ? WARPS * 32 : SHORT_WARPS * 32) score_short_rows(const float* x, const float* ids, float* __restrict__ out, long long rows,
+                                                                     int cols, int top) {
   tsb_launch::enter();
-  const long long row = blockIdx.x / chunks;
-  const unsigned begin = (unsigned)(blockIdx.x % chunks) * chunk, end = (unsigned)min((long long)begin + chunk, cols);
-  const float* xr = x + row * cols;
-  float* dr = dx + row * cols;
-  const float* o = out + row * (3 + 2 * top);
-  const float* w = g + row * (3 + 2 * top);
+  constexpr int ROWS = WARPS == 1 ? SHORT_WARPS : 1, ROOM = WARPS == 1 ? SHORT_FOUND : FOUND;
+  __shared__ u64 found[TOP ? ROWS : 1][ROOM], best_of[WARPS];
+  __shared__ Sums sums[WARPS];
+  __shared__ float leasts[WARPS], lse_of_row;
+  __shared__ int all;
+  const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5, own_row = WARPS == 1 ? threadIdx.x >> 5 : 0;
+  const long long row = blockIdx.x * (long long)ROWS + own_row;
+  if (row >= rows) return;                   // (whole warps, and no block that has barriers)
+  auto sync = [] {
+    if (WARPS == 1) __syncwarp();
+    else __syncthreads();
+  };
+  const int first = warp * 32 + lane;        // the lane's columns: first + i * 32 WARPS
+  const float* const xr = x + row * cols + first;
+  float* const to = out + row * (3 + 2 * top);
+  float v[N], own = NEG_INF;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = first + i * (32 * WARPS) < cols ? load(xr + i * (32 * WARPS)) : NEG_INF;
   const long long id = (long long)load(ids + row);
   const bool given = id >= 0 && id < cols;
-  const float entropy = load(o + 1), lse = load(o + 2), wh = load(w + 1);
-  float weights = given ? load(w) : 0.f;
-  for (int k = 0; k < top; ++k)
-    if (load(o + 3 + top + k) >= 0.f) weights += load(w + 3 + k);
+  const float own_x = given ? load(x + row * cols + id) : 0.f;
+  if (WARPS > 1 && threadIdx.x == 0) all = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) own = fmaxf(own, v[i]);
+  const float most = warp_max(own), ref = most == NEG_INF ? 0.f : most;
+  float z[2] = {0.f, 0.f}, t[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float u = v[i] - ref, e = __expf(u);
+    z[i & 1] += e;
+    t[i & 1] += e * fmaxf(u, -1e4f);
+  }
+  Sums a{most, z[0] + z[1], t[0] + t[1]};
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    a.z += __shfl_xor_sync(ALL, a.z, d);
+    a.t += __shfl_xor_sync(ALL, a.t, d);
+  }
+  float least = TOP ? __shfl_sync(ALL, sort_falling(own), (top + WARPS - 1) / WARPS - 1) : NEG_INF;
+  if (WARPS > 1) {
+    if (lane == 0) sums[warp] = a, leasts[warp] = least;
+    __syncthreads();
+    for (int w = 0; w < WARPS; ++w) least = fminf(least, leasts[w]);
+    if (warp == WARPS - 1) {
+      a = lane < WARPS ? sums[lane] : Sums{NEG_INF, 0.f, 0.f};
+#pragma unroll
+      for (int d = WARPS / 2; d > 0; d >>= 1)
+        a = join(a, Sums{__shfl_xor_sync(ALL, a.m, d), __shfl_xor_sync(ALL, a.z, d), __shfl_xor_sync(ALL, a.t, d)});
+    }
+  }
+  float lse = 0.f;
+  if (warp == WARPS - 1) {
+    const bool empty = a.m == NEG_INF && a.z == 0.f;
+    const double log_z = log((double)a.z);
+    lse = empty ? NEG_INF : a.m + (float)log_z;
+    if (lane == 0) {
+      to[0] = given ? (empty ? NEG_INF : own_x - lse) : 0.f;
+      to[1] = empty ? 0.f : (float)(log_z - (double)a.t / (double)a.z);
+      to[2] = lse;
+      if (WARPS > 1) lse_of_row = lse;
+    }
+  }
+  if (!TOP) return;
+  // which of the lane's columns reach the bound (a NaN does not), and where they go
+  u64 bits = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) bits |= (u64)(v[i] >= least) << i;
+  const int there = first < cols ? (cols - first + 32 * WARPS - 1) / (32 * WARPS) : 0;
+  if (there < 64) bits &= (1ull << there) - 1;
+  int count = __popcll(bits), at = count;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(ALL, at, d);
+    if (lane >= d) at += o;
+  }
+  at -= count;
+  count = __shfl_sync(ALL, at + count, 31);
+  if (WARPS > 1) {
+    if (lane == 0 && count) count = atomicAdd(&all, count);                       // (their order does not matter)
+    at += __shfl_sync(ALL, count, 0);
+  }
+  u64* const keys = found[own_row];
+  for (; bits && at < ROOM; bits &= bits - 1, ++at) {
+    const int i = (__ffsll((long long)bits) - 1) * (32 * WARPS);
+    keys[at] = order_of(load(xr + i), first + i);
+  }
+  sync();
+  if (WARPS > 1) count = all, lse = lse_of_row;
+  auto write = [&](int place, u64 key) {
+    to[3 + place] = !key ? __int_as_float(0x7fc00000) : lse == NEG_INF ? NEG_INF : logit_of(key) - lse;
+    to[3 + top + place] = key ? (float)col_of(key) : -1.f;
+  };
+  if (count <= ROOM) {
+    for (int c = first; c < max(count, top); c += 32 * WARPS) {
+      const u64 key = c < count ? keys[c] : 0;
+      int place = c < count ? 0 : c;
+#pragma unroll 4
+      for (int j = 0; j < count; ++j) place += c < count && keys[j] > key;
+      if (place < top) write(place, key);    // (fewer numbers than alternatives: the places behind them have none)
+    }
+    return;
+  }
+  u64 last = ~0ull;
+  for (int k = 0; k < top; ++k) {
+    u64 best = 0;
+#pragma unroll 1
+    for (int col = first; col < cols; col += 32 * WARPS) {       // (from memory: the columns' registers are free by now)
+      const float y = load(x + row * cols + col);
+      const u64 key = y == y ? order_of(y, col) : 0;
+      if (key < last) best = larger(best, key);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) best = larger(best, __shfl_xor_sync(ALL, best, d));
+    if (WARPS > 1) {
+      if (lane == 0) best_of[warp] = best;
+      __syncthreads();
+      for (int w = 0; w < WARPS; ++w) best = larger(best, best_of[w]);
+      __syncthreads();
+    }
+    if (first == 0) write(k, best);
+    last = best;
+  }
+}
+template <int N, int WARPS>
+int short_rows(const float* x, const float* ids, float* out, long long rows, int cols, int top, cudaStream_t st) {
+  const dim3 grid((unsigned)(WARPS == 1 ? (rows + SHORT_WARPS - 1) / SHORT_WARPS : rows)), block(WARPS == 1 ? SHORT_WARPS * 32 : WARPS * 32);
+  if (top) return launch_status(tsb_launch::launch(score_short_rows<N, WARPS, true>, grid, block, 0, st, x, ids, out, rows, cols, top));
+  return launch_status(tsb_launch::launch(score_short_rows<N, WARPS, false>, grid, block, 0, st, x, ids, out, rows, cols, top));
+}
+
+// dx_c = sum_i w_i (1[c = id_i] - p_c) + w_lse p_c - w_H p_c (log p_c + H), with w the gradient of `out` and the sum over
+// the given token and the top ones, of which each lane of a warp has one.  Columns that are an id are computed apart, with 1 - p as
+// -expm1(log p), after the rest.  Columns [begin, end) of a row, by `threads` threads that `sync` is for.
+template <class Sync>
+__device__ __forceinline__ void grad_of_columns(const float* xr, const float* o, const float* w, float* dr, long long id, long long cols, int top,
+                                                unsigned begin, unsigned end, unsigned thread, unsigned threads, Sync sync) {
+  const int lane = threadIdx.x & 31;
+  const bool given = id >= 0 && id < cols;
+  const float entropy = load(o + 1), lse = load(o + 2), wh = load(w + 1), w_given = given ? load(w) : 0.f;
+  const long long alternative = lane < top ? (long long)load(o + 3 + top + lane) : -1;
+  const float w_alternative = alternative >= 0 ? load(w + 3 + lane) : 0.f;
+  float weights = w_alternative;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) weights += __shfl_xor_sync(ALL, weights, d);
+  weights += w_given;
   const bool empty = lse == NEG_INF;
   const float plain = load(w + 2) - weights;
   auto rest = [&](float v) {                                                    // of a column that is no id
@@ -447,29 +588,44 @@ __global__ void __launch_bounds__(256) score_grad(const float* x, const float* i
     return empty || v == NEG_INF ? 0.f : p * (plain - wh * (lp + entropy));
   };
   const unsigned odd = (unsigned)((-(long long)(reinterpret_cast<uintptr_t>(xr + begin) >> 2)) & 3);
-  const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
+  const bool same = ((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(dr)) & 15) == 0;
   const unsigned body = same ? min(begin + odd, end) : end, pieces = (end - body) / 4, tail = body + pieces * 4;
   const float4* xv = reinterpret_cast<const float4*>(xr + body);
   float4* dv = reinterpret_cast<float4*>(dr + body);
-  tsb_launch::read_then_write<4>(threadIdx.x, pieces, 256u, [&](unsigned i) { return load(xv + i); },
+  tsb_launch::read_then_write<4>(thread, pieces, threads, [&](unsigned i) { return load(xv + i); },
                                  [&](unsigned i, float4 v) { dv[i] = make_float4(rest(v.x), rest(v.y), rest(v.z), rest(v.w)); });
-  for (unsigned i = begin + threadIdx.x; i < body; i += 256) dr[i] = rest(load(xr + i));
-  for (unsigned i = tail + threadIdx.x; i < end; i += 256) dr[i] = rest(load(xr + i));
-  __syncthreads();                       // the columns below are written a second time
-  const int k = (int)threadIdx.x - 1;    // thread 0: the given token, the others: the top ones
-  if (k >= top || empty) return;
-  const long long col = k < 0 ? (given ? id : -1) : (long long)load(o + 3 + top + k);
-  if (col < (long long)begin || col >= (long long)end) return;
-  float own = k < 0 ? load(w) : load(w + 3 + k);
-  if (k < 0) {
-    for (int j = 0; j < top; ++j)
-      if ((long long)load(o + 3 + top + j) == col) return;                      // the thread of that one does it
-  } else if (given && id == col) {
-    own += load(w);
-  }
-  const float v = load(xr + col), lp = v - lse, p = expf(lp);
-  const float other = v == NEG_INF ? 0.f : p * (load(w + 2) - (weights - own) - wh * (lp + entropy));
-  dr[col] = own * -expm1f(lp) + other;
+  for (unsigned i = begin + thread; i < body; i += threads) dr[i] = rest(load(xr + i));
+  for (unsigned i = tail + thread; i < end; i += threads) dr[i] = rest(load(xr + i));
+  sync();                                // the columns below are written a second time
+  if (thread >= 32 || empty) return;
+  auto of_id = [&](long long col, float own) {
+    if (col < (long long)begin || col >= (long long)end) return;
+    const float v = load(xr + col), lp = v - lse, p = expf(lp);
+    const float other = v == NEG_INF ? 0.f : p * (load(w + 2) - (weights - own) - wh * (lp + entropy));
+    dr[col] = own * -expm1f(lp) + other;
+  };
+  of_id(alternative, w_alternative + (given && alternative == id ? w_given : 0.f));
+  const bool both = __any_sync(ALL, alternative == id);                         // the lane of that one has done it
+  if (lane == 0 && given && !both) of_id(id, w_given);
+}
+
+// A block takes a chunk of a row.
+__global__ void __launch_bounds__(256) score_grad(const float* x, const float* ids, const float* out, const float* g,
+                                                  float* __restrict__ dx, long long cols, int top, unsigned chunk, int chunks) {
+  tsb_launch::enter();
+  const long long row = blockIdx.x / chunks;
+  const unsigned begin = (unsigned)(blockIdx.x % chunks) * chunk, end = (unsigned)min((long long)begin + chunk, cols);
+  grad_of_columns(x + row * cols, out + row * (3 + 2 * top), g + row * (3 + 2 * top), dx + row * cols, (long long)load(ids + row), cols, top, begin,
+                  end, threadIdx.x, 256u, [] { __syncthreads(); });
+}
+// A warp takes a row.
+__global__ void __launch_bounds__(SHORT_WARPS * 32) score_grad_short(const float* x, const float* ids, const float* out, const float* g,
+                                                                     float* __restrict__ dx, long long rows, long long cols, int top) {
+  tsb_launch::enter();
+  const long long row = blockIdx.x * (long long)SHORT_WARPS + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  grad_of_columns(x + row * cols, out + row * (3 + 2 * top), g + row * (3 + 2 * top), dx + row * cols, (long long)load(ids + row), cols, top, 0,
+                  (unsigned)cols, threadIdx.x & 31, 32u, [] { __syncwarp(); });
 }
 
 }  // namespace
@@ -481,14 +637,26 @@ int tsb_token_score(const float* x, const float* ids, float* out, long long rows
   if (rows == 0) return TSB_OK;
   if (!x || !ids || !out) return TSB_ERR_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // short rows: as few warps as hold them (8192 x 5000, five alternatives: four warps of 48 columns a lane 46 us, eight of 32 65); a row
+  // of more than 16384 columns takes an SM, so there may be no more of them than SMs (445 x 17000: 13 us by score_rows, 17 so)
+  const int c = (int)cols;
+  if (cols <= 32) return short_rows<1, 1>(x, ids, out, rows, c, top, st);
+  if (cols <= 128) return short_rows<4, 1>(x, ids, out, rows, c, top, st);
+  if (cols <= 512) return short_rows<16, 1>(x, ids, out, rows, c, top, st);
+  if (cols <= 1024) return short_rows<32, 1>(x, ids, out, rows, c, top, st);
+  if (cols <= 2048) return short_rows<32, 2>(x, ids, out, rows, c, top, st);
+  if (cols <= 4096) return short_rows<32, 4>(x, ids, out, rows, c, top, st);
+  if (cols <= 6144) return short_rows<48, 4>(x, ids, out, rows, c, top, st);
+  if (cols <= 8192) return short_rows<64, 4>(x, ids, out, rows, c, top, st);
+  if (cols <= 12288) return short_rows<48, 8>(x, ids, out, rows, c, top, st);
+  if (cols <= 16384) return short_rows<64, 8>(x, ids, out, rows, c, top, st);
+  if (cols <= 32768 && rows <= 148) return short_rows<64, 16>(x, ids, out, rows, c, top, st);
   // a cluster of blocks for a row while the rows leave SMs idle and a block keeps 2048 columns
   int split = 1;
   while (split < MAX_SPLIT && rows * split * 2 <= 148 && cols >= 4096ll * split) split *= 2;
-  // 16 columns a thread where the row has as many, but eight warps only for few rows or long ones: a row's end is latency,
-  // which more rows on an SM cover (8160 x 32000, 20 alternatives: four warps 234 us, eight 256; 4096 x 128001: 395, 373)
-  const int most = cols / split >= 65536 || rows * split <= 4 * 148 ? MAX_WARPS : MAX_WARPS / 2;
-  int warps = 1;
-  while (warps < most && cols / split >= 512ll * warps * 2) warps *= 2;
+  // eight warps for few rows or long ones only: a row's end is latency, which more rows on an SM cover (8160 x 32000, 20
+  // alternatives: four warps 234 us, eight 256; 4096 x 128001: 395, 373)
+  const int warps = cols / split >= 65536 || rows * split <= 4 * 148 ? MAX_WARPS : MAX_WARPS / 2;
   const dim3 grid((unsigned)(rows * split)), block(warps * 32);
   const unsigned cluster = split > 1 ? split : 0;
   if (top)
@@ -502,6 +670,11 @@ int tsb_token_score_grad(const float* x, const float* ids, const float* out, con
   if (rows == 0) return TSB_OK;
   if (!x || !ids || !out || !g || !dx) return TSB_ERR_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // (a block's barrier and the row's numbers are most of a short row: 8192 x 1000, five alternatives, 10 us by warps, 23 by blocks; 300 x
+  // 1000 3.3 and 2.2)
+  if (cols <= 2048 && rows >= 148 * SHORT_WARPS)
+    return launch_status(tsb_launch::launch(score_grad_short, dim3((unsigned)((rows + SHORT_WARPS - 1) / SHORT_WARPS)), dim3(SHORT_WARPS * 32), 0, st,
+                                            x, ids, out, g, dx, rows, cols, top));
   // chunks of a row that keep 4 x 4 columns a thread, until there are four blocks for every SM
   long long chunks = 1;
   while (rows * chunks < 148 * 4 && cols >= 8192 * chunks) chunks *= 2;
