@@ -341,3 +341,18 @@ def test_a_result_that_was_fed_has_no_gradient():
         ad.Executor(nodes[1:], ctx=ctx).run(feeds)
     again = ad.Executor(nodes, ctx=ctx).run({names[k]: v for k, v in f.items()}, convert_to_numpy_ret_vals=True)
     assert all(np.array_equal(a, np.asarray(b)) for a, b in zip(first, again))
+
+
+@pytest.mark.gpu
+def test_states_that_grow_take_no_more_room():
+    """A decoder's states grow by one a step: the node keeps one array of log-sum-exps for all of them."""
+    ctx = ndarray.gpu(0)
+    q, kv, g = (ad.Variable(v) for v in ("q", "kv", "g"))
+    y = ad.cross_attention_op(q, kv)
+    ex = ad.Executor([y] + ad.cross_attention_gradient_op(y, g), ctx=ctx)
+    for tk in (5, 6, 7, 130):
+        f = case(2, 1, tk, 4, 2, 32, None)
+        got = [np.asarray(o, np.float64) for o in ex.run({q: f["q"], kv: f["kv"], g: f["g"]}, convert_to_numpy_ret_vals=True)]
+        want, tol = definition(f["q"], f["kv"], None, 32 ** -0.5, f["g"])
+        assert all(np.all(np.abs(a - b) <= t) for a, b, t in zip(got, want, tol))
+    assert sum(isinstance(v, ndarray.NDArray) for v in y.state.values()) == 1

@@ -91,12 +91,13 @@ class CrossAttentionOp(Op):
 
 
 def _row_sums(node, sizes, ctx, make=True):
-    """The rows' log-sum-exps, which the forward kernel leaves for the gradients: an array for every size that the node has run
-    at, since a step that was captured at one goes on using its own."""
-    key = ("lse", sizes, ctx)
+    """The rows' log-sum-exps, which the forward kernel leaves for the gradients: an array for every number of rows that the
+    node has run at, since a step that was captured at one goes on using its own (a sentence of states that grows needs no more)."""
+    shape = (sizes[0], sizes[3], _whole_tiles(sizes[1]))
+    key = ("lse", shape, ctx)
     if key not in node.state and make:
         from .. import ndarray
-        node.state[key] = ndarray.empty((sizes[0], sizes[3], _whole_tiles(sizes[1])), ctx, use_pool=False)
+        node.state[key] = ndarray.empty(shape, ctx, use_pool=False)
     return node.state.get(key)
 
 
