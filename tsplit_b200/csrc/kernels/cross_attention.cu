@@ -270,6 +270,21 @@ __device__ __forceinline__ void product_of_kept_rows(uint32_t to, uint32_t a, ui
 #pragma unroll
   for (int k = 0; k < D / 16; ++k) mma_tmem(to, a + 8 * k, at(k, 0), idesc_f16(ROWS_B, 0), 1);
 }
+// The same with A's hi pieces in tensor memory and the lo ones, a plane, in shared memory.
+template <int D, int ROWS_A, int ROWS_B>
+__device__ __forceinline__ void product_of_half_kept_rows(uint32_t to, uint32_t a_hi, uint32_t a_lo, uint32_t b) {
+  using LA = Tile<D, ROWS_A>;
+  using LB = Tile<D, ROWS_B>;
+  const uint32_t al = smem_desc_lo(a_lo, 16), bl = smem_desc_lo(b, 16);
+  auto at = [&](int k, uint32_t lo, int chunk) { return smem_desc_join(DESC_HI, lo + ((k / 4 * chunk + k % 4 * 32) >> 4)); };
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) {
+    mma_tmem(to, a_hi + 8 * k, at(k, bl + (LB::PLANE >> 4), LB::CHUNK), idesc_f16(ROWS_B, 0), k > 0);
+    mma_smem(to, at(k, al, LA::CHUNK), at(k, bl, LB::CHUNK), idesc_f16(ROWS_B, 0), 1);
+  }
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) mma_tmem(to, a_hi + 8 * k, at(k, bl, LB::CHUNK), idesc_f16(ROWS_B, 0), 1);
+}
 // D [128 x D] (+)= A B, A [128 x ROWS] in tensor memory: 16 columns for every 16 of its, hi pieces in the first eight.
 template <int D, int ROWS>
 __device__ __forceinline__ void product_with_columns(uint32_t to, uint32_t a, uint32_t b, bool accumulate = false) {
@@ -384,15 +399,15 @@ template <class Control> __device__ __forceinline__ Control* control_at(int byte
 template <int R> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
 template <int R> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 
-// Half of a row's pieces (columns D / 2 * half on) of a tile: read from memory, and put into tensor memory as
+// Half of a row's pieces (columns D / 2 * half on; the hi ones alone with PLANES = 1) of a tile: read from memory, and put into tensor memory as
 // product_of_kept_rows takes them.
-template <int D> struct KeptRow {
-  uint4 v[2][D / 16];
+template <int D, int PLANES = 2> struct KeptRow {
+  uint4 v[PLANES][D / 16];
   __device__ __forceinline__ void read(const Pieces& p, long long tile, int row, int half) {
     using L = Tile<D, 128>;
     const char* const from = p.tiles + tile * L::BYTES + row * 128;
 #pragma unroll
-    for (int plane = 0; plane < 2; ++plane)
+    for (int plane = 0; plane < PLANES; ++plane)
 #pragma unroll
       for (int u = 0; u < D / 16; ++u) {
         const int at = half * (D / 16) + u;
@@ -401,7 +416,7 @@ template <int D> struct KeptRow {
   }
   __device__ __forceinline__ void keep(uint32_t to, int half) const {
 #pragma unroll
-    for (int plane = 0; plane < 2; ++plane)
+    for (int plane = 0; plane < PLANES; ++plane)
 #pragma unroll
       for (int u = 0; u < D / 16; u += 4)                            // four pieces of 16 bytes: 16 columns
         asm volatile(
@@ -835,34 +850,42 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_queries(const Problem p) {
 // dk and dv: a block takes 128 keys of a shared head and tiles of 64 queries of every head that reads it.  S^T and dP^T have
 // the keys as rows, so P^T and dS^T are A operands as they lie.  Halves of the tiles of queries and of gradients share a ring
 // of slots (q, g, q, g, ...), each with its rows' log-sum-exps or dots.  Warps 0 to 3 take the first 32 queries of a tile and
-// add up dv, 4 to 7 the others and dk; 8: copies; 9 issues.  Two tiles of S^T and dP^T are in tensor memory.  4 x 2048 x 2048, 16
-// heads of 64: 358 us; 2 x 2000 x 4111, 16 heads of 128 on 4: 860 us, 313 TFLOP/s, so 940 of fp16 products.  (Two blocks of four
-// such warps to an SM were a third slower, 516 us in place of 397 for the former: the two sums leave a thread no registers.)
+// add up dv, 4 to 7 the others and dk; 8: copies; 9 issues.  Two tiles of S^T and dP^T are in tensor memory; with 128 columns one
+// of dP^T, and the keys' hi pieces in its place, so that shared memory has room for two tiles of queries and gradients (three
+// halves and all pieces of the keys: 855 us in place of 665, a product and a copy more on the way from dS to the next dP).
+// 4 x 2048 x 2048, 16 heads of 64: 360 us; 2 x 2000 x 4111, 16 heads of 128 on 4: 665 us, 405 TFLOP/s, so 1.21 PFLOP/s of fp16
+// products.  (Two blocks of four such warps to an SM were a third slower, 516 us in place of 397 for the former: the two sums
+// leave a thread no registers.  Keys and values of 64 columns in tensor memory: no quicker.)
 template <int D> struct StateShape {
-  static constexpr int DP_AT = 128, DV_AT = 256, DK_AT = 384, SLOTS = D == 64 ? 6 : 3;
+  static constexpr bool WIDE = D == 64;
+  static constexpr int S_AT = WIDE ? 0 : 64, DP_AT = S_AT + 128, DP_BUFFERS = WIDE ? 2 : 1, DV_AT = 256, DK_AT = 384;
+  static constexpr int SLOTS = WIDE ? 6 : 4;
   using LK = Tile<D, 128>;
   using LQ = Tile<D, 64>;
-  static constexpr int TILES = 2 * LK::BYTES + SLOTS * LQ::BYTES, SMEM = TILES + CONTROL + (SLOTS - 3) * 256;
+  static constexpr int K_BYTES = WIDE ? LK::BYTES : LK::PLANE, TILES = K_BYTES + LK::BYTES + SLOTS * LQ::BYTES;
+  static constexpr int ROWS_AT = 256;            // of the slots' log-sum-exps and dots, behind the barriers
+  static constexpr int SMEM = TILES + ROWS_AT + SLOTS * 256;
 };
 struct StateControl {
-  uint64_t k_full, v_full, full[6], empty[6], s_full[2], ds_full[2], sum_full, drained;
+  uint64_t k_full, kept, v_full, full[6], empty[6], s_full[2], ds_full[2], sum_full, drained;
   uint32_t tmem;
 };
-constexpr int ROWS_AT = 256;                   // of the slots' log-sum-exps and dots, behind the barriers
-static_assert(sizeof(StateControl) <= ROWS_AT && ROWS_AT + 3 * 256 <= CONTROL, "");
+static_assert(sizeof(StateControl) <= StateShape<64>::ROWS_AT, "");
 
 template <int D>
 __global__ void __launch_bounds__(BLOCK, 1) grad_of_states(const Problem p) {
   using Shape = StateShape<D>;
   using LQ = typename Shape::LQ;
   using LK = typename Shape::LK;
-  constexpr int SLOTS = Shape::SLOTS, DP_AT = Shape::DP_AT;
-  char *const k_tile = tiles_of_block, *const v_tile = k_tile + LK::BYTES, *const ring = v_tile + LK::BYTES;
+  constexpr bool WIDE = Shape::WIDE;
+  constexpr int SLOTS = Shape::SLOTS;
+  char *const k_tile = tiles_of_block, *const v_tile = k_tile + Shape::K_BYTES, *const ring = v_tile + LK::BYTES;
   StateControl* bar = control_at<StateControl>(Shape::TILES);
-  float* const rows = reinterpret_cast<float*>(reinterpret_cast<char*>(bar) + ROWS_AT);        // [SLOTS][64]
+  float* const rows = reinterpret_cast<float*>(reinterpret_cast<char*>(bar) + Shape::ROWS_AT);        // [SLOTS][64]
   const int warp = __shfl_sync(ALL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(&bar->k_full, 1);
+    mbar_init(&bar->kept, 256);
     mbar_init(&bar->v_full, 1);
     for (int i = 0; i < SLOTS; ++i) {
       mbar_init(&bar->full[i], 1);
@@ -880,19 +903,20 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_states(const Problem p) {
     tmem_alloc(&bar->tmem, 512);
     tmem_relinquish();
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = __shfl_sync(ALL, bar->tmem, 0);
   tsb_launch::enter();
-
   const int kt = blockIdx.x % p.ktiles, shared = blockIdx.x / p.ktiles % p.shared, n = blockIdx.x / p.ktiles / p.shared;
   const int k0 = kt * 128, per = p.heads / p.shared, halves = (p.tq + 63) / 64;
   const float* tokens = p.key ? p.key + (long long)n * p.tk : nullptr;
   const long long kv_row = 2ll * p.shared * p.d, k_at = ((long long)n * p.shared + shared) * p.ktiles + kt;
   const long long q_at = ((long long)n * p.heads + shared * per) * p.qtiles;                // of the first head that reads it
   const bool mine_in = threadIdx.x < 128 && k0 + (int)threadIdx.x < p.tk && (!tokens || load(tokens + k0 + threadIdx.x) != 0.f);
+  const int half = warp >> 2, row = threadIdx.x & 127;
+  KeptRow<D, 1> kept;                          // (under way while the block sets itself up)
+  if (!WIDE && warp < 8) kept.read(p.kp, k_at, row, half);
+  tc_fence_before();
   const int tiles = __syncthreads_or(mine_in) ? halves * per : 0;
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(ALL, bar->tmem, 0);
   auto tile_of = [&](int j) { return q_at + (long long)(j / halves) * p.qtiles + j % halves / 2; };
 
   if (warp < 8) {
@@ -901,7 +925,12 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_states(const Problem p) {
 #pragma unroll
     for (int c = 0; c < D; ++c) acc[c] = 0.f;
     const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);
-    const int half = warp >> 2, row = threadIdx.x & 127;
+    if (!WIDE) {
+      kept.keep(mine, half);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&bar->kept);
+    }
     const float k_unit = load(p.kp.units + k_at).x;
     const float2 v_unit = load(p.vp.units + k_at);
     bool ok = true;
@@ -925,10 +954,10 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_states(const Problem p) {
       const float s_unit = q_unit * k_unit, f = power_of_two(max(e - TOP - 1, -126)), dp_unit = g_unit.x * v_unit.x * f;
       if (!mbar_wait(&bar->s_full[b], j >> 1 & 1, p.status, 0x321)) { ok = false; break; }
       tc_fence_after();
-      const uint32_t at = mine + b * 64 + half * 32;
+      const uint32_t at = mine + Shape::S_AT + b * 64 + half * 32, dp_at = mine + Shape::DP_AT + b % Shape::DP_BUFFERS * 64 + half * 32;
       float s[2][16], dp[2][16];
       tmem_begin(at, s[0]);
-      tmem_begin(at + DP_AT, dp[0]);
+      tmem_begin(dp_at, dp[0]);
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         float(&v)[16] = s[w & 1];
@@ -938,7 +967,7 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_states(const Problem p) {
         tmem_arrived(x);
         if (w + 1 < 2) {
           tmem_begin(at + 16 * w + 16, s[(w + 1) & 1]);
-          tmem_begin(at + DP_AT + 16 * w + 16, dp[(w + 1) & 1]);
+          tmem_begin(dp_at + 16 * w + 16, dp[(w + 1) & 1]);
         }
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
@@ -952,7 +981,7 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_states(const Problem p) {
           }
         }
         tmem_st_pieces(at + 16 * w, v);
-        tmem_st_pieces(at + DP_AT + 16 * w, x);
+        tmem_st_pieces(dp_at + 16 * w, x);
       }
       tmem_st_wait();
       if (j > 0 && !(ok = add_tile(j - 1))) break;
@@ -973,7 +1002,8 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_states(const Problem p) {
   } else {
     fewer_registers<88>();
     if (warp == 8 && elect_one() && tiles > 0) {
-      copy_tile<D>(k_tile, p.kp, k_at, &bar->k_full);
+      mbar_expect_tx(&bar->k_full, Shape::K_BYTES);                // (the lo pieces are behind the hi ones)
+      bulk_copy(k_tile, p.kp.tiles + (k_at + 1) * LK::BYTES - Shape::K_BYTES, Shape::K_BYTES, &bar->k_full);
       for (int i = 0; i < 2 * tiles; ++i) {
         const int s = i % SLOTS, j = i / 2;
         const long long t = tile_of(j);
@@ -987,35 +1017,32 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_states(const Problem p) {
     }
     if (warp == 9 && elect_one() && tiles > 0) {
       const uint32_t ra = smem_u32(ring), ka = smem_u32(k_tile), va = smem_u32(v_tile);
-      bool ok = mbar_wait(&bar->k_full, 0, p.status, 0x324);
+      bool ok = mbar_wait(&bar->k_full, 0, p.status, 0x324) && (WIDE || mbar_wait(&bar->kept, 0, p.status, 0x324));
       // S^T or dP^T of tile j; the latter commits both
       auto half_of_scores = [&](int j, int half) {
         const int i = 2 * j + half, s = i % SLOTS, b = j & 1;
         if (i == 1 && !mbar_wait(&bar->v_full, 0, p.status, 0x324)) return false;
         if (!mbar_wait(&bar->full[s], i / SLOTS & 1, p.status, 0x325)) return false;
         tc_fence_after();
-        product_of_rows<D, 128, 64>(tmem + half * DP_AT + b * 64, half ? va : ka, ra + s * LQ::BYTES);
+        const uint32_t to = tmem + (half ? Shape::DP_AT + b % Shape::DP_BUFFERS * 64 : Shape::S_AT + b * 64), from = ra + s * LQ::BYTES;
+        if (!WIDE && !half) product_of_half_kept_rows<D, 128, 64>(to, tmem, ka, from);
+        else product_of_rows<D, 128, 64>(to, half ? va : ka, from);
         if (half) umma_commit(&bar->s_full[b]);
         return true;
       };
-      // With six slots the scores of two tiles are under way; with three there is room for the next tile's queries only
-      constexpr bool WIDE = SLOTS == 6;
-      for (int i = 0; i < (WIDE ? 4 : 2) && i < 2 * tiles && ok; ++i) ok = half_of_scores(i / 2, i & 1);
+      // (with one buffer of dP^T that of tile 1 waits for dk of tile 0)
+      for (int i = 0; i < (WIDE ? 4 : 3) && i < 2 * tiles && ok; ++i) ok = half_of_scores(i / 2, i & 1);
       for (int j = 0; j < tiles && ok; ++j) {
         const int b = j & 1, qs = 2 * j % SLOTS, gs = (2 * j + 1) % SLOTS;
-        if (!WIDE && j + 1 < tiles && !(ok = half_of_scores(j + 1, 0))) break;
         if (!(ok = mbar_wait(&bar->ds_full[b], j >> 1 & 1, p.status, 0x326))) break;
         tc_fence_after();
-        product_with_columns<D, 64>(tmem + Shape::DK_AT, tmem + DP_AT + b * 64, ra + qs * LQ::BYTES);
+        product_with_columns<D, 64>(tmem + Shape::DK_AT, tmem + Shape::DP_AT + b % Shape::DP_BUFFERS * 64, ra + qs * LQ::BYTES);
         umma_commit(&bar->empty[qs]);
-        product_with_columns<D, 64>(tmem + Shape::DV_AT, tmem + b * 64, ra + gs * LQ::BYTES);
+        if (!WIDE && j + 1 < tiles && !(ok = half_of_scores(j + 1, 1))) break;
+        product_with_columns<D, 64>(tmem + Shape::DV_AT, tmem + Shape::S_AT + b * 64, ra + gs * LQ::BYTES);
         umma_commit(&bar->empty[gs]);
         umma_commit(&bar->sum_full);
-        if (WIDE) {
-          if (j + 2 < tiles) ok = half_of_scores(j + 2, 0) && half_of_scores(j + 2, 1);
-        } else if (j + 1 < tiles) {
-          ok = half_of_scores(j + 1, 1);
-        }
+        if (j + 2 < tiles) ok = half_of_scores(j + 2, 0) && (!WIDE || half_of_scores(j + 2, 1));
       }
       if (!ok) drain(&bar->drained);
     }
