@@ -458,6 +458,7 @@ __device__ __forceinline__ void store_row(float* to, const float (&v)[COUNT], fl
 // soft-max warps: 51 and 258 us for 64 columns, fewer blocks that share the SMs less evenly.)
 template <int D> struct ForwardShape {
   static constexpr int PARTS = D / 64, ROWS = 128 / PARTS, SLOTS = 6;              // of a tile in a slot each
+  static constexpr int K_SLOTS = PARTS == 1 ? 3 : 2, V_SLOTS = SLOTS - K_SLOTS;
   static constexpr int S_AT = D, Y_AT = S_AT + 2 * 128;                            // behind the queries
   using L = Tile<D, ROWS>;
   static constexpr int TILES = SLOTS * L::BYTES, SMEM = TILES + CONTROL + 2 * 1024;
@@ -605,9 +606,10 @@ __global__ void __launch_bounds__(BLOCK, 1) attend(const Problem p) {
     fewer_registers<88>();
     if (warp == 8 && elect_one()) {
       for (int i = 0; i < 2 * PARTS * tiles; ++i) {
-        const int s = i % SLOTS, j = i / (2 * PARTS);
-        const Pieces& from = i / PARTS & 1 ? p.vp : p.kp;
-        if (!mbar_wait(&bar->empty[s], (i / SLOTS & 1) ^ 1, p.status, 0x303)) break;
+        const int j = i / (2 * PARTS), v = i / PARTS & 1, at = j * PARTS + i % PARTS;
+        const int s = v ? Shape::K_SLOTS + at % Shape::V_SLOTS : at % Shape::K_SLOTS;
+        const Pieces& from = v ? p.vp : p.kp;
+        if (!mbar_wait(&bar->empty[s], (at / (v ? Shape::V_SLOTS : Shape::K_SLOTS) & 1) ^ 1, p.status, 0x303)) break;
         if (PARTS == 1) copy_tile<D>(tiles_of_block + s * L::BYTES, from, k_at + j, &bar->full[s]);
         else copy_half<D>(tiles_of_block + s * L::BYTES, from, k_at + j, i % PARTS, &bar->full[s]);
       }
@@ -619,8 +621,8 @@ __global__ void __launch_bounds__(BLOCK, 1) attend(const Problem p) {
       auto scores = [&](int j) {
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
-          const int i = 2 * PARTS * j + part, s = i % SLOTS;
-          if (!mbar_wait(&bar->full[s], i / SLOTS & 1, p.status, 0x306)) return false;
+          const int at = j * PARTS + part, s = at % Shape::K_SLOTS;
+          if (!mbar_wait(&bar->full[s], at / Shape::K_SLOTS & 1, p.status, 0x306)) return false;
           tc_fence_after();
           product_of_kept_rows<D, Shape::ROWS>(tmem + Shape::S_AT + (j & 1) * 128 + part * Shape::ROWS, tmem, ring + s * L::BYTES);
           umma_commit(&bar->empty[s]);
@@ -634,8 +636,8 @@ __global__ void __launch_bounds__(BLOCK, 1) attend(const Problem p) {
         if (!(ok = mbar_wait(&bar->p_full[b], j >> 1 & 1, p.status, 0x308))) break;
 #pragma unroll
         for (int part = 0; part < PARTS && ok; ++part) {
-          const int i = 2 * PARTS * j + PARTS + part, s = i % SLOTS;
-          if (!(ok = mbar_wait(&bar->full[s], i / SLOTS & 1, p.status, 0x307))) break;
+          const int at = j * PARTS + part, s = Shape::K_SLOTS + at % Shape::V_SLOTS;
+          if (!(ok = mbar_wait(&bar->full[s], at / Shape::V_SLOTS & 1, p.status, 0x307))) break;
           tc_fence_after();
           product_with_columns<D, Shape::ROWS>(tmem + Shape::Y_AT, tmem + Shape::S_AT + b * 128 + part * Shape::ROWS, ring + s * L::BYTES,
                                                part > 0);
@@ -667,7 +669,7 @@ __device__ __forceinline__ int exponent_of_ds(float g_length, float v_length, fl
 // us (a row to a thread, two blocks to an SM, operands in shared memory: 672, 301 and 32).
 template <int D> struct QueryShape {
   static constexpr bool BOTH = D == 64;
-  static constexpr int SLOTS = BOTH ? 8 : 5;
+  static constexpr int K_SLOTS = BOTH ? 4 : 3, V_SLOTS = BOTH ? 4 : 2, SLOTS = K_SLOTS + V_SLOTS;
   static constexpr int G_AT = D, S_AT = BOTH ? 2 * D : D, DP_AT = S_AT + 2 * 64, DQ_AT = DP_AT + 2 * 64;
   using LQ = Tile<D, 128>;
   using LK = Tile<D, 64>;
@@ -802,9 +804,9 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_queries(const Problem p) {
     fewer_registers<88>();
     if (warp == 8 && elect_one()) {
       for (int i = 0; i < 2 * tiles; ++i) {
-        const int s = i % SLOTS, j = i / 2;
+        const int j = i / 2, of_kind = i & 1 ? Shape::V_SLOTS : Shape::K_SLOTS, s = i & 1 ? Shape::K_SLOTS + j % Shape::V_SLOTS : j % Shape::K_SLOTS;
         if (i == 1 && !Shape::BOTH) copy_tile<D>(g_tile, p.gp, q_at, &bar->g_full);
-        if (!mbar_wait(&bar->empty[s], (i / SLOTS & 1) ^ 1, p.status, 0x313)) break;
+        if (!mbar_wait(&bar->empty[s], (j / of_kind & 1) ^ 1, p.status, 0x313)) break;
         copy_half<D>(ring + s * LK::BYTES, i & 1 ? p.vp : p.kp, k_at + j / 2, j & 1, &bar->full[s]);
       }
     }
@@ -813,12 +815,12 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_queries(const Problem p) {
       bool ok = mbar_wait(&bar->q_full, 0, p.status, 0x315);
       tc_fence_after();
       auto scores = [&](int j) {
-        const int b = j & 1, ks = 2 * j % SLOTS, vs = (2 * j + 1) % SLOTS;
-        if (!mbar_wait(&bar->full[ks], 2 * j / SLOTS & 1, p.status, 0x316)) return false;
+        const int b = j & 1, ks = j % Shape::K_SLOTS, vs = Shape::K_SLOTS + j % Shape::V_SLOTS;
+        if (!mbar_wait(&bar->full[ks], j / Shape::K_SLOTS & 1, p.status, 0x316)) return false;
         tc_fence_after();
         product_of_kept_rows<D, 64>(tmem + Shape::S_AT + b * 64, tmem, ra + ks * LK::BYTES);
         if (!Shape::BOTH && j == 0 && !mbar_wait(&bar->g_full, 0, p.status, 0x315)) return false;
-        if (!mbar_wait(&bar->full[vs], (2 * j + 1) / SLOTS & 1, p.status, 0x317)) return false;
+        if (!mbar_wait(&bar->full[vs], j / Shape::V_SLOTS & 1, p.status, 0x317)) return false;
         tc_fence_after();
         if (Shape::BOTH) product_of_kept_rows<D, 64>(tmem + Shape::DP_AT + b * 64, tmem + Shape::G_AT, ra + vs * LK::BYTES);
         else product_of_rows<D, 128, 64>(tmem + Shape::DP_AT + b * 64, ga, ra + vs * LK::BYTES);
@@ -829,7 +831,7 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_queries(const Problem p) {
       // (keys stay in their slot until dq is computed)
       for (int j = 0; j < 2 && j < tiles && ok; ++j) ok = scores(j);
       for (int j = 0; j < tiles && ok; ++j) {
-        const int b = j & 1, ks = 2 * j % SLOTS;
+        const int b = j & 1, ks = j % Shape::K_SLOTS;
         if (!(ok = mbar_wait(&bar->ds_full[b], j >> 1 & 1, p.status, 0x318))) break;
         tc_fence_after();
         product_with_columns<D, 64>(tmem + Shape::DQ_AT, tmem + Shape::S_AT + b * 64, ra + ks * LK::BYTES);
