@@ -217,25 +217,31 @@ __device__ __forceinline__ void copy_half(char* to, const Pieces& p, long long t
 __host__ __device__ constexpr uint32_t idesc_f16(int n, int b_mn_major) {      // M = 128, D fp32, A and B fp16, A K-major
   return (1u << 4) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
-__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// One of the lanes that get here issues: the `leader`.
+__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t leader) {
   asm volatile(
       "{\n"
-      ".reg .pred p;\n"
+      ".reg .pred p, q;\n"
       "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      "setp.ne.b32 q, %5, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
       "}\n"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t leader) {
   asm volatile(
       "{\n"
-      ".reg .pred p;\n"
+      ".reg .pred p, q;\n"
       "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "setp.ne.b32 q, %5, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
       "}\n"
-      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
+}
+__device__ __forceinline__ void commit_if(uint32_t leader, uint64_t* bar) {
+  if (leader) umma_commit(bar);
 }
 constexpr uint32_t DESC_HI = smem_desc_hi(1024);       // 128-byte swizzle, groups of eight rows 1024 bytes apart
 
@@ -243,61 +249,61 @@ constexpr uint32_t DESC_HI = smem_desc_hi(1024);       // 128-byte swizzle, grou
 // the last bit of the sum so far, and the sum is at its full size for a third of the steps only (700 x 900, 128 columns: y off by
 // 4.9e-7 in place of 1.2e-6, plain fp32 operators 6.7e-7).
 template <int D, int ROWS_A, int ROWS_B>
-__device__ __forceinline__ void product_of_rows(uint32_t to, uint32_t a, uint32_t b) {
+__device__ __forceinline__ void product_of_rows(uint32_t to, uint32_t a, uint32_t b, uint32_t leader) {
   using LA = Tile<D, ROWS_A>;
   using LB = Tile<D, ROWS_B>;
   const uint32_t al = smem_desc_lo(a, 16), bl = smem_desc_lo(b, 16);
   auto at = [&](int k, uint32_t lo, int chunk) { return smem_desc_join(DESC_HI, lo + ((k / 4 * chunk + k % 4 * 32) >> 4)); };
 #pragma unroll
   for (int k = 0; k < D / 16; ++k) {
-    mma_smem(to, at(k, al, LA::CHUNK), at(k, bl + (LB::PLANE >> 4), LB::CHUNK), idesc_f16(ROWS_B, 0), k > 0);
-    mma_smem(to, at(k, al + (LA::PLANE >> 4), LA::CHUNK), at(k, bl, LB::CHUNK), idesc_f16(ROWS_B, 0), 1);
+    mma_smem(to, at(k, al, LA::CHUNK), at(k, bl + (LB::PLANE >> 4), LB::CHUNK), idesc_f16(ROWS_B, 0), k > 0, leader);
+    mma_smem(to, at(k, al + (LA::PLANE >> 4), LA::CHUNK), at(k, bl, LB::CHUNK), idesc_f16(ROWS_B, 0), 1, leader);
   }
 #pragma unroll
-  for (int k = 0; k < D / 16; ++k) mma_smem(to, at(k, al, LA::CHUNK), at(k, bl, LB::CHUNK), idesc_f16(ROWS_B, 0), 1);
+  for (int k = 0; k < D / 16; ++k) mma_smem(to, at(k, al, LA::CHUNK), at(k, bl, LB::CHUNK), idesc_f16(ROWS_B, 0), 1, leader);
 }
 // The same with A in tensor memory: its hi pieces in D / 2 columns, two to each, then the lo pieces.
 template <int D, int ROWS_B>
-__device__ __forceinline__ void product_of_kept_rows(uint32_t to, uint32_t a, uint32_t b) {
+__device__ __forceinline__ void product_of_kept_rows(uint32_t to, uint32_t a, uint32_t b, uint32_t leader) {
   using L = Tile<D, ROWS_B>;
   const uint32_t bl = smem_desc_lo(b, 16);
   auto at = [&](int k, int plane) { return smem_desc_join(DESC_HI, bl + ((k / 4 * L::CHUNK + k % 4 * 32 + plane) >> 4)); };
 #pragma unroll
   for (int k = 0; k < D / 16; ++k) {
-    mma_tmem(to, a + 8 * k, at(k, L::PLANE), idesc_f16(ROWS_B, 0), k > 0);
-    mma_tmem(to, a + D / 2 + 8 * k, at(k, 0), idesc_f16(ROWS_B, 0), 1);
+    mma_tmem(to, a + 8 * k, at(k, L::PLANE), idesc_f16(ROWS_B, 0), k > 0, leader);
+    mma_tmem(to, a + D / 2 + 8 * k, at(k, 0), idesc_f16(ROWS_B, 0), 1, leader);
   }
 #pragma unroll
-  for (int k = 0; k < D / 16; ++k) mma_tmem(to, a + 8 * k, at(k, 0), idesc_f16(ROWS_B, 0), 1);
+  for (int k = 0; k < D / 16; ++k) mma_tmem(to, a + 8 * k, at(k, 0), idesc_f16(ROWS_B, 0), 1, leader);
 }
 // The same with A's hi pieces in tensor memory and the lo ones, a plane, in shared memory.
 template <int D, int ROWS_A, int ROWS_B>
-__device__ __forceinline__ void product_of_half_kept_rows(uint32_t to, uint32_t a_hi, uint32_t a_lo, uint32_t b) {
+__device__ __forceinline__ void product_of_half_kept_rows(uint32_t to, uint32_t a_hi, uint32_t a_lo, uint32_t b, uint32_t leader) {
   using LA = Tile<D, ROWS_A>;
   using LB = Tile<D, ROWS_B>;
   const uint32_t al = smem_desc_lo(a_lo, 16), bl = smem_desc_lo(b, 16);
   auto at = [&](int k, uint32_t lo, int chunk) { return smem_desc_join(DESC_HI, lo + ((k / 4 * chunk + k % 4 * 32) >> 4)); };
 #pragma unroll
   for (int k = 0; k < D / 16; ++k) {
-    mma_tmem(to, a_hi + 8 * k, at(k, bl + (LB::PLANE >> 4), LB::CHUNK), idesc_f16(ROWS_B, 0), k > 0);
-    mma_smem(to, at(k, al, LA::CHUNK), at(k, bl, LB::CHUNK), idesc_f16(ROWS_B, 0), 1);
+    mma_tmem(to, a_hi + 8 * k, at(k, bl + (LB::PLANE >> 4), LB::CHUNK), idesc_f16(ROWS_B, 0), k > 0, leader);
+    mma_smem(to, at(k, al, LA::CHUNK), at(k, bl, LB::CHUNK), idesc_f16(ROWS_B, 0), 1, leader);
   }
 #pragma unroll
-  for (int k = 0; k < D / 16; ++k) mma_tmem(to, a_hi + 8 * k, at(k, bl, LB::CHUNK), idesc_f16(ROWS_B, 0), 1);
+  for (int k = 0; k < D / 16; ++k) mma_tmem(to, a_hi + 8 * k, at(k, bl, LB::CHUNK), idesc_f16(ROWS_B, 0), 1, leader);
 }
 // D [128 x D] (+)= A B, A [128 x ROWS] in tensor memory: 16 columns for every 16 of its, hi pieces in the first eight.
 template <int D, int ROWS>
-__device__ __forceinline__ void product_with_columns(uint32_t to, uint32_t a, uint32_t b, bool accumulate = false) {
+__device__ __forceinline__ void product_with_columns(uint32_t to, uint32_t a, uint32_t b, uint32_t leader, bool accumulate = false) {
   using L = Tile<D, ROWS>;
   const uint32_t bl = smem_desc_lo(b, L::CHUNK);
   auto at = [&](int k, int plane) { return smem_desc_join(DESC_HI, bl + ((k * 2048 + plane) >> 4)); };
 #pragma unroll
   for (int k = 0; k < ROWS / 16; ++k) {
-    mma_tmem(to, a + 16 * k, at(k, L::PLANE), idesc_f16(D, 1), accumulate || k > 0);
-    mma_tmem(to, a + 16 * k + 8, at(k, 0), idesc_f16(D, 1), 1);
+    mma_tmem(to, a + 16 * k, at(k, L::PLANE), idesc_f16(D, 1), accumulate || k > 0, leader);
+    mma_tmem(to, a + 16 * k + 8, at(k, 0), idesc_f16(D, 1), 1, leader);
   }
 #pragma unroll
-  for (int k = 0; k < ROWS / 16; ++k) mma_tmem(to, a + 16 * k, at(k, 0), idesc_f16(D, 1), 1);
+  for (int k = 0; k < ROWS / 16; ++k) mma_tmem(to, a + 16 * k, at(k, 0), idesc_f16(D, 1), 1, leader);
 }
 
 // Loads from tensor memory run behind what the thread does until tmem_ld_wait; tmem_arrived then names the registers, so
@@ -451,7 +457,7 @@ __device__ __forceinline__ void store_row(float* to, const float (&v)[COUNT], fl
 // of a tile is added to the registers before the next one's product.
 //
 // Bound by the tensor cores and by the threads between two products.  With the splitting: 2 x 2000 x 4111, 16 heads of 128 on 4:
-// 356 us, 379 TFLOP/s, so 1.14 PFLOP/s of fp16 products; 4 x 2048 x 2048, 16 heads of 64: 222 us; 32 x 255 x 256, 8 heads of 64:
+// 323 us, 417 TFLOP/s, so 1.25 PFLOP/s of fp16 products; 4 x 2048 x 2048, 16 heads of 64: 222 us; 32 x 255 x 256, 8 heads of 64:
 // 49 us.  (A row to a thread and two blocks to an SM, operands in shared memory: 444, 278 and 47 us.  A block's beginning and
 // end are not hidden now, which a few key tiles show, but a product with A in tensor memory takes 32 cycles for 16 x 64 numbers
 // of B, with A in shared memory 48, and two threads do a row's soft-max in half the time.  Two tiles of queries to a block, sixteen
@@ -614,7 +620,8 @@ __global__ void __launch_bounds__(BLOCK, 1) attend(const Problem p) {
         else copy_half<D>(tiles_of_block + s * L::BYTES, from, k_at + j, i % PARTS, &bar->full[s]);
       }
     }
-    if (warp == 9 && elect_one() && tiles > 0) {
+    if (warp == 9 && tiles > 0) {
+      const uint32_t leader = elect_one();      // (all lanes wait and loop, so that descriptors are the warp's: 343 -> 323 us)
       const uint32_t ring = smem_u32(tiles_of_block);
       bool ok = mbar_wait(&bar->q_full, 0, p.status, 0x305);
       tc_fence_after();
@@ -624,10 +631,10 @@ __global__ void __launch_bounds__(BLOCK, 1) attend(const Problem p) {
           const int at = j * PARTS + part, s = at % Shape::K_SLOTS;
           if (!mbar_wait(&bar->full[s], at / Shape::K_SLOTS & 1, p.status, 0x306)) return false;
           tc_fence_after();
-          product_of_kept_rows<D, Shape::ROWS>(tmem + Shape::S_AT + (j & 1) * 128 + part * Shape::ROWS, tmem, ring + s * L::BYTES);
-          umma_commit(&bar->empty[s]);
+          product_of_kept_rows<D, Shape::ROWS>(tmem + Shape::S_AT + (j & 1) * 128 + part * Shape::ROWS, tmem, ring + s * L::BYTES, leader);
+          commit_if(leader, &bar->empty[s]);
         }
-        umma_commit(&bar->s_full[j & 1]);
+        commit_if(leader, &bar->s_full[j & 1]);
         return true;
       };
       for (int j = 0; j < 2 && j < tiles && ok; ++j) ok = scores(j);
@@ -639,15 +646,15 @@ __global__ void __launch_bounds__(BLOCK, 1) attend(const Problem p) {
           const int at = j * PARTS + part, s = Shape::K_SLOTS + at % Shape::V_SLOTS;
           if (!(ok = mbar_wait(&bar->full[s], at / Shape::V_SLOTS & 1, p.status, 0x307))) break;
           tc_fence_after();
-          product_with_columns<D, Shape::ROWS>(tmem + Shape::Y_AT, tmem + Shape::S_AT + b * 128 + part * Shape::ROWS, ring + s * L::BYTES,
+          product_with_columns<D, Shape::ROWS>(tmem + Shape::Y_AT, tmem + Shape::S_AT + b * 128 + part * Shape::ROWS, ring + s * L::BYTES, leader,
                                                part > 0);
-          umma_commit(&bar->empty[s]);
+          commit_if(leader, &bar->empty[s]);
         }
         if (!ok) break;
-        umma_commit(&bar->y_full);
+        commit_if(leader, &bar->y_full);
         if (j + 2 < tiles) ok = scores(j + 2);
       }
-      if (!ok) drain(&bar->drained);
+      if (!ok && leader) drain(&bar->drained);
     }
   }
   __syncwarp();
@@ -665,7 +672,7 @@ __device__ __forceinline__ int exponent_of_ds(float g_length, float v_length, fl
 }
 
 // dq: a block takes 128 queries of a head and tiles of 64 keys; the same roles.  The queries, and with 64 columns their gradients
-// too, are kept in tensor memory, else these lie before the ring.  dS takes the place of its S.  The cases of attend: 534, 235 and 35
+// too, are kept in tensor memory, else these lie before the ring.  dS takes the place of its S.  The cases of attend: 459, 235 and 34
 // us (a row to a thread, two blocks to an SM, operands in shared memory: 672, 301 and 32).
 template <int D> struct QueryShape {
   static constexpr bool BOTH = D == 64;
@@ -810,7 +817,8 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_queries(const Problem p) {
         copy_half<D>(ring + s * LK::BYTES, i & 1 ? p.vp : p.kp, k_at + j / 2, j & 1, &bar->full[s]);
       }
     }
-    if (warp == 9 && elect_one() && tiles > 0) {
+    if (warp == 9 && tiles > 0) {
+      const uint32_t leader = elect_one();      // (as in attend: 472 -> 459 us with 128 columns)
       const uint32_t ga = smem_u32(g_tile), ra = smem_u32(ring);
       bool ok = mbar_wait(&bar->q_full, 0, p.status, 0x315);
       tc_fence_after();
@@ -818,14 +826,14 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_queries(const Problem p) {
         const int b = j & 1, ks = j % Shape::K_SLOTS, vs = Shape::K_SLOTS + j % Shape::V_SLOTS;
         if (!mbar_wait(&bar->full[ks], j / Shape::K_SLOTS & 1, p.status, 0x316)) return false;
         tc_fence_after();
-        product_of_kept_rows<D, 64>(tmem + Shape::S_AT + b * 64, tmem, ra + ks * LK::BYTES);
+        product_of_kept_rows<D, 64>(tmem + Shape::S_AT + b * 64, tmem, ra + ks * LK::BYTES, leader);
         if (!Shape::BOTH && j == 0 && !mbar_wait(&bar->g_full, 0, p.status, 0x315)) return false;
         if (!mbar_wait(&bar->full[vs], j / Shape::V_SLOTS & 1, p.status, 0x317)) return false;
         tc_fence_after();
-        if (Shape::BOTH) product_of_kept_rows<D, 64>(tmem + Shape::DP_AT + b * 64, tmem + Shape::G_AT, ra + vs * LK::BYTES);
-        else product_of_rows<D, 128, 64>(tmem + Shape::DP_AT + b * 64, ga, ra + vs * LK::BYTES);
-        umma_commit(&bar->s_full[b]);
-        umma_commit(&bar->empty[vs]);
+        if (Shape::BOTH) product_of_kept_rows<D, 64>(tmem + Shape::DP_AT + b * 64, tmem + Shape::G_AT, ra + vs * LK::BYTES, leader);
+        else product_of_rows<D, 128, 64>(tmem + Shape::DP_AT + b * 64, ga, ra + vs * LK::BYTES, leader);
+        commit_if(leader, &bar->s_full[b]);
+        commit_if(leader, &bar->empty[vs]);
         return true;
       };
       // (keys stay in their slot until dq is computed)
@@ -834,12 +842,12 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_queries(const Problem p) {
         const int b = j & 1, ks = j % Shape::K_SLOTS;
         if (!(ok = mbar_wait(&bar->ds_full[b], j >> 1 & 1, p.status, 0x318))) break;
         tc_fence_after();
-        product_with_columns<D, 64>(tmem + Shape::DQ_AT, tmem + Shape::S_AT + b * 64, ra + ks * LK::BYTES);
-        umma_commit(&bar->empty[ks]);
-        umma_commit(&bar->dq_full);
+        product_with_columns<D, 64>(tmem + Shape::DQ_AT, tmem + Shape::S_AT + b * 64, ra + ks * LK::BYTES, leader);
+        commit_if(leader, &bar->empty[ks]);
+        commit_if(leader, &bar->dq_full);
         if (j + 2 < tiles) ok = scores(j + 2);
       }
-      if (!ok) drain(&bar->drained);
+      if (!ok && leader) drain(&bar->drained);
     }
   }
   __syncwarp();
@@ -1018,6 +1026,7 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_states(const Problem p) {
       }
     }
     if (warp == 9 && elect_one() && tiles > 0) {
+      constexpr uint32_t leader = 1;             // (64 columns: 354 us so, 394 if all lanes take part)
       const uint32_t ra = smem_u32(ring), ka = smem_u32(k_tile), va = smem_u32(v_tile);
       bool ok = mbar_wait(&bar->k_full, 0, p.status, 0x324) && (WIDE || mbar_wait(&bar->kept, 0, p.status, 0x324));
       // S^T or dP^T of tile j; the latter commits both
@@ -1027,9 +1036,9 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_states(const Problem p) {
         if (!mbar_wait(&bar->full[s], i / SLOTS & 1, p.status, 0x325)) return false;
         tc_fence_after();
         const uint32_t to = tmem + (half ? Shape::DP_AT + b % Shape::DP_BUFFERS * 64 : Shape::S_AT + b * 64), from = ra + s * LQ::BYTES;
-        if (!WIDE && !half) product_of_half_kept_rows<D, 128, 64>(to, tmem, ka, from);
-        else product_of_rows<D, 128, 64>(to, half ? va : ka, from);
-        if (half) umma_commit(&bar->s_full[b]);
+        if (!WIDE && !half) product_of_half_kept_rows<D, 128, 64>(to, tmem, ka, from, leader);
+        else product_of_rows<D, 128, 64>(to, half ? va : ka, from, leader);
+        if (half) commit_if(leader, &bar->s_full[b]);
         return true;
       };
       // (with one buffer of dP^T that of tile 1 waits for dk of tile 0)
@@ -1038,12 +1047,12 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_states(const Problem p) {
         const int b = j & 1, qs = 2 * j % SLOTS, gs = (2 * j + 1) % SLOTS;
         if (!(ok = mbar_wait(&bar->ds_full[b], j >> 1 & 1, p.status, 0x326))) break;
         tc_fence_after();
-        product_with_columns<D, 64>(tmem + Shape::DK_AT, tmem + Shape::DP_AT + b % Shape::DP_BUFFERS * 64, ra + qs * LQ::BYTES);
-        umma_commit(&bar->empty[qs]);
+        product_with_columns<D, 64>(tmem + Shape::DK_AT, tmem + Shape::DP_AT + b % Shape::DP_BUFFERS * 64, ra + qs * LQ::BYTES, leader);
+        commit_if(leader, &bar->empty[qs]);
         if (!WIDE && j + 1 < tiles && !(ok = half_of_scores(j + 1, 1))) break;
-        product_with_columns<D, 64>(tmem + Shape::DV_AT, tmem + Shape::S_AT + b * 64, ra + gs * LQ::BYTES);
-        umma_commit(&bar->empty[gs]);
-        umma_commit(&bar->sum_full);
+        product_with_columns<D, 64>(tmem + Shape::DV_AT, tmem + Shape::S_AT + b * 64, ra + gs * LQ::BYTES, leader);
+        commit_if(leader, &bar->empty[gs]);
+        commit_if(leader, &bar->sum_full);
         if (j + 2 < tiles) ok = half_of_scores(j + 2, 0) && (!WIDE || half_of_scores(j + 2, 1));
       }
       if (!ok) drain(&bar->drained);
