@@ -69,6 +69,16 @@ def test_embedding_of_many_tokens(n, v, d):
     check_embed(r.standard_normal((v, d), np.float32), ids, r.standard_normal((n, d), np.float32), 0.5, None, ndarray.gpu(0))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,v,d", [(37887, 90, 33), (37889, 90, 33), (37888, 90, 128), (37890, 50, 127), (37891, 50, 132), (70, 90, 31), (70, 90, 1023),
+                                   (9, 70, 4100)])
+def test_lookups_of_whole_rows(n, v, d):
+    """Rows of fewer and of more than 32 pieces, one and several to a warp, ids outside among them."""
+    r = rng(n, v, d)
+    ids = r.integers(-2, v + 2, n).astype(np.float32)
+    check_embed(r.standard_normal((v, d), np.float32), ids, r.standard_normal((n, d), np.float32), 3.0, 1, ndarray.gpu(0))
+
+
 @pytest.mark.parametrize("what", ["same", "none", "padding", "outside", "falling", "runs"])
 @pytest.mark.parametrize("n", [33, 1500, pytest.param(40000, marks=pytest.mark.gpu)])
 def test_embedding_of_unusual_ids(what, n, ctx):

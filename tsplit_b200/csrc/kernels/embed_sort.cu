@@ -67,6 +67,38 @@ __global__ void __launch_bounds__(256) scaled_lookup(const T* table, const float
     if (i + u * 256 < pieces) y[i + u * 256] = v[u];
 }
 
+// Rows of 32 pieces or more, a warp to each ROWS of them: no piece's place has to be divided by the row's length.  With one row U
+// pieces are in flight per thread, with several one of each.
+template <class T, int U, int ROWS>
+__global__ void __launch_bounds__(256) scaled_lookup_rows(const T* table, const float* ids, T* __restrict__ y, long long n, long long vocab,
+                                                          unsigned dim, float scale) {
+  tsb_launch::enter();
+  const long long r = (blockIdx.x * 8ll + (threadIdx.x >> 5)) * ROWS;
+  bool known[ROWS];
+  const T* from[ROWS];
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    const long long id = r + k < n ? (long long)load(ids + r + k) : -1;
+    known[k] = id >= 0 && id < vocab;
+    from[k] = table + (known[k] ? id * dim : 0);
+  }
+  T* const to = y + r * dim;
+  if (ROWS == 1) {
+    if (r < n)
+      tsb_launch::read_then_write<U>(threadIdx.x & 31, dim, 32u, [&](unsigned c) { return known[0] ? times(load(from[0] + c), scale) : zero<T>(); },
+                                     [&](unsigned c, T v) { to[c] = v; });
+    return;
+  }
+  for (unsigned c = threadIdx.x & 31; c < dim; c += 32) {
+    T v[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) v[k] = known[k] ? times(load(from[k] + c), scale) : zero<T>();
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k)
+      if (r + k < n) to[k * dim + c] = v[k];
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ sort
 // Keys are token ids, `vocab` for positions that give no gradient (they end up last).  What fills the last tile behind
 // position n has all bits set, so it stays behind everything in every pass.  Digits of up to 8 bits, the lowest first.  A
@@ -456,40 +488,46 @@ struct FewShared {
   unsigned found[8];
 };
 
-// The positions of row r among places [from, to) of the list, added in their order; BATCH rows in flight.
-template <class T>
-__device__ __forceinline__ T sum_of_row(const FewShared& s, unsigned r, unsigned from, unsigned to, const T* column, unsigned dim, bool in) {
+// The positions of row r among places [from, to) of the list, added in their order; BATCH rows in flight.  A lane has U columns, 32
+// apart, the first `there` of them inside.
+template <class T, int U>
+__device__ __forceinline__ void sum_of_row(const FewShared& s, unsigned r, unsigned from, unsigned to, const T* column, unsigned dim, int there,
+                                           T (&sum)[U]) {
   const unsigned lane = threadIdx.x & 31;
-  T sum = zero<T>();
+#pragma unroll
+  for (int k = 0; k < U; ++k) sum[k] = zero<T>();
   for (unsigned i = from; i < to; i += 32) {
     const unsigned item = i + lane < to ? s.list[i + lane] : 0xffffffffu;
     for (unsigned mask = __ballot_sync(0xffffffffu, item >> 16 == r); mask;) {
-      T v[BATCH];
+      T v[BATCH / U][U];
       int count = 0;
 #pragma unroll
-      for (int u = 0; u < BATCH; ++u)
+      for (int u = 0; u < BATCH / U; ++u)
         if (mask) {
           const unsigned at = __shfl_sync(0xffffffffu, item, __ffs(mask) - 1) & 0xffff;
           mask &= mask - 1;
-          v[u] = in ? load(column + (size_t)at * dim) : zero<T>();
+#pragma unroll
+          for (int k = 0; k < U; ++k) v[u][k] = k < there ? load(column + (size_t)at * dim + k * 32) : zero<T>();
           count = u + 1;
         }
 #pragma unroll
-      for (int u = 0; u < BATCH; ++u)
-        if (u < count) sum = plus(sum, v[u]);
+      for (int u = 0; u < BATCH / U; ++u)
+        if (u < count)
+#pragma unroll
+          for (int k = 0; k < U; ++k) sum[k] = plus(sum[k], v[u][k]);
     }
   }
-  return sum;
 }
 
-template <class T>
+template <class T, int U>
 __global__ void __launch_bounds__(256) grad_by_rows(const T* g, const float* ids, int n, unsigned vocab, long long padding, unsigned dim,
                                                     int apart, unsigned chunks, float scale, T* __restrict__ dtable) {
   tsb_launch::enter();
   __shared__ FewShared s;
-  __shared__ T parts[8][32];
+  __shared__ T parts[8][U][32];
   const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const unsigned row0 = blockIdx.x / chunks, count = (vocab - row0 + (1u << apart) - 1) >> apart, c = blockIdx.x % chunks * 32 + lane;
+  const unsigned row0 = blockIdx.x / chunks, count = (vocab - row0 + (1u << apart) - 1) >> apart, c = blockIdx.x % chunks * (32 * U) + lane;
+  const int there = c < dim ? min((int)((dim - c + 31) / 32), U) : 0;      // columns of the lane, 32 apart
   constexpr int ITEMS = FEW_TOKENS / 256;
   const int items = (n + 255) / 256;         // 32 positions each that a warp looks at
   unsigned key[ITEMS], mask[ITEMS], own = 0;
@@ -531,20 +569,34 @@ __global__ void __launch_bounds__(256) grad_by_rows(const T* g, const float* ids
     const unsigned r = s.list[i] >> 16;
     if (s.times[r] <= LONG || s.first[r] != i) continue;
     __syncthreads();                         // (the row before has been joined)
-    parts[warp][lane] = sum_of_row(s, r, min(warp * run, all), min(warp * run + run, all), column, dim, c < dim);
-    __syncthreads();
-    if (warp == 0 && c < dim) {
-      T sum = parts[0][lane];
+    T sum[U];
+    sum_of_row(s, r, min(warp * run, all), min(warp * run + run, all), column, dim, there, sum);
 #pragma unroll
-      for (int w = 1; w < 8; ++w) sum = plus(sum, parts[w][lane]);
-      out[r * step] = times(sum, scale);
-    }
+    for (int k = 0; k < U; ++k) parts[warp][k][lane] = sum[k];
+    __syncthreads();
+    if (warp == 0)
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+#pragma unroll
+        for (int w = 1; w < 8; ++w) sum[k] = plus(sum[k], parts[w][k][lane]);
+        if (k < there) out[r * step + k * 32] = times(sum[k], scale);
+      }
   }
   for (unsigned r = warp; r < count; r += 8) {
     const unsigned times_of = s.times[r];
     if (times_of > LONG) continue;
-    const T sum = times_of ? times(sum_of_row(s, r, s.first[r], all, column, dim, c < dim), scale) : zero<T>();
-    if (c < dim) out[r * step] = sum;
+    T sum[U];
+    if (times_of) {
+      sum_of_row(s, r, s.first[r], all, column, dim, there, sum);
+#pragma unroll
+      for (int k = 0; k < U; ++k) sum[k] = times(sum[k], scale);
+    } else {
+#pragma unroll
+      for (int k = 0; k < U; ++k) sum[k] = zero<T>();
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (k < there) out[r * step + k * 32] = sum[k];
   }
 }
 
@@ -552,12 +604,13 @@ template <class T>
 int sums_of_few(const T* g, const float* ids, long long n, long long vocab, long long padding, long long dim, float scale, T* dtable,
                 cudaStream_t st) {
   // as many blocks as run at once, eight to an SM, of at most FEW_ROWS rows
-  const long long chunks = (dim + 31) / 32;
+  constexpr int U = sizeof(T) == 4 ? 4 : 1;
+  const long long chunks = (dim + 32 * U - 1) / (32 * U);
   int apart = 0;
   while ((1ll << apart) * FEW_ROWS < vocab || ((2ll << apart) <= vocab && (2ll << apart) * chunks <= 148 * 8)) ++apart;
   const long long blocks = chunks << apart;
   if (blocks > INT32_MAX) return TSB_ERR_ARG;
-  return launch_status(tsb_launch::launch(grad_by_rows<T>, dim3((unsigned)blocks), dim3(256), 0, st, g, ids, (int)n, (unsigned)vocab, padding,
+  return launch_status(tsb_launch::launch(grad_by_rows<T, U>, dim3((unsigned)blocks), dim3(256), 0, st, g, ids, (int)n, (unsigned)vocab, padding,
                                           (unsigned)dim, apart, (unsigned)chunks, scale, dtable));
 }
 
@@ -592,6 +645,21 @@ int sums(const T* g, const unsigned* key, const unsigned* pos, long long n, unsi
   return launch_status(e);
 }
 
+template <class T>
+int lookup(const T* table, const float* ids, T* y, long long n, long long vocab, long long dim, float scale, cudaStream_t st) {
+  // (8000 x 1023: 7.8 us, piece by piece 18.  Short rows need others beside them, where there are enough: 131072 x 128 16 us by
+  // pieces, 25 by single rows)
+  const bool rows = dim >= 32;
+  const int each = dim < 128 && n >= 148 * 8 * 8 * 4 ? 4 : 1;
+  const long long blocks = rows ? (n + 8 * each - 1) / (8 * each) : (n * dim + 1023) / 1024;
+  if (blocks > INT32_MAX) return TSB_ERR_ARG;
+  const dim3 grid((unsigned)blocks), block(256);
+  if (rows && each == 4)
+    return launch_status(tsb_launch::launch(scaled_lookup_rows<T, 1, 4>, grid, block, 0, st, table, ids, y, n, vocab, (unsigned)dim, scale));
+  if (rows) return launch_status(tsb_launch::launch(scaled_lookup_rows<T, 8, 1>, grid, block, 0, st, table, ids, y, n, vocab, (unsigned)dim, scale));
+  return launch_status(tsb_launch::launch(scaled_lookup<T, 4>, grid, block, 0, st, table, ids, y, n * dim, vocab, (unsigned)dim, scale));
+}
+
 constexpr long long MAX_TOKENS = 1ll << 30, MAX_VOCAB = 1ll << 24, MAX_DIM = 1ll << 20;     // (ids are whole numbers in fp32)
 
 }  // namespace
@@ -605,15 +673,8 @@ int tsb_embedding_scaled(const float* table, const float* ids, float* y, long lo
   if (!table || !ids || !y) return TSB_ERR_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool v4 = dim % 4 == 0 && ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(y)) & 15) == 0;
-  const long long pieces = v4 ? n * (dim / 4) : n * dim;
-  const long long blocks = (pieces + 1023) / 1024;
-  if (blocks > INT32_MAX) return TSB_ERR_ARG;
-  if (v4)
-    return launch_status(tsb_launch::launch(scaled_lookup<float4, 4>, dim3((unsigned)blocks), dim3(256), 0, st,
-                                            reinterpret_cast<const float4*>(table), ids, reinterpret_cast<float4*>(y), pieces,
-                                            vocab, (unsigned)(dim / 4), scale));
-  return launch_status(tsb_launch::launch(scaled_lookup<float, 4>, dim3((unsigned)blocks), dim3(256), 0, st, table, ids, y,
-                                          pieces, vocab, (unsigned)dim, scale));
+  return v4 ? lookup(reinterpret_cast<const float4*>(table), ids, reinterpret_cast<float4*>(y), n, vocab, dim / 4, scale, st)
+            : lookup(table, ids, y, n, vocab, dim, scale, st);
 }
 
 // Scratch of a gradient: sorted keys and positions (twice, and the histograms, above one cluster's share), partial rows.
