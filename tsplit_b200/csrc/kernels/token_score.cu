@@ -433,8 +433,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 6) score_rows(const float* x, 
 // 5.8 and 6.2, of which a cluster makes 4, 9 and 14.)
 constexpr int SHORT_WARPS = 8, SHORT_FOUND = 128;
 template <int N, int WARPS, bool TOP>
-__global__ void __launch_bounds__(WARPS > SHORT_WARPS ? WARPS * 32 : SHORT_WARPS * 32) score_short_rows(const float* x, const float* ids, float* __restrict__ out, long long rows,
-                                                                     int cols, int top) {
+__global__ void __launch_bounds__(WARPS > SHORT_WARPS ? WARPS * 32 : SHORT_WARPS * 32)
+    score_short_rows(const float* x, const float* ids, float* __restrict__ out, long long rows, int cols, int top) {
   tsb_launch::enter();
   constexpr int ROWS = WARPS == 1 ? SHORT_WARPS : 1, ROOM = WARPS == 1 ? SHORT_FOUND : FOUND;
   __shared__ u64 found[TOP ? ROWS : 1][ROOM], best_of[WARPS];
