@@ -356,3 +356,47 @@ def test_states_that_grow_take_no_more_room():
         want, tol = definition(f["q"], f["kv"], None, 32 ** -0.5, f["g"])
         assert all(np.all(np.abs(a - b) <= t) for a, b, t in zip(got, want, tol))
     assert sum(isinstance(v, ndarray.NDArray) for v in y.state.values()) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,tq,tk,h,s,d", [(2, 300, 700, 4, 2, 64), (1, 200, 400, 2, 2, 128), (8, 2000, 20, 8, 8, 64), (2, 10, 5000, 2, 2, 64), (1, 5, 6, 1, 1, 3),
+                                           (4, 900, 1000, 16, 16, 32)])
+def test_both_gradients_in_one_call_in_a_captured_chain(n, tq, tk, h, s, d):
+    """Many blocks and few ones of either kernel, beside one another: the bits of two calls, and whoever reads the first
+    gradient right behind the second finds it done."""
+    import torch
+    from tsplit_b200.ops import _gpu as G
+    from tsplit_b200.ops.attention import _prepared_floats
+    from tsplit_b200.runtime import cudagraph
+    from tsplit_b200.stream import create_stream_handle
+    ctx = ndarray.gpu(0)
+    st, sizes = create_stream_handle(ctx), (n, tq, tk, h, s, d)
+    f = {k: torch.from_numpy(v).cuda() for k, v in case(n, tq, tk, h, s, d, "holes").items()}
+    y, dq, dq2, seen = (torch.zeros_like(f["q"]) for _ in range(4))
+    dkv, dkv2, seen2 = (torch.zeros_like(f["kv"]) for _ in range(3))
+    lse = torch.zeros(n, h, -(-tq // 128) * 128, device="cuda")
+    prepared = torch.zeros(_prepared_floats(*sizes), device="cuda")
+    q, kv, key, g, Y, DQ, DQ2, S, DKV, DKV2, S2, L, P = (ndarray.from_tensor(t, ctx) for t in (
+        f["q"], f["kv"], f["key"], f["g"], y, dq, dq2, seen, dkv, dkv2, seen2, lse, prepared))
+    torch.cuda.synchronize()
+    G.cross_attention(q, kv, key, Y, L, sizes, 0.3, st)
+    G.cross_attention_prepare(q, kv, key, g, Y, P, sizes, 0.3, st)
+    G.cross_attention_grad_q(P, key, L, DQ, sizes, 0.3, st)
+    G.cross_attention_grad_kv(P, key, L, DKV, sizes, 0.3, st)
+
+    def step():
+        for _ in range(3):
+            for a in (P, L, DQ2, DKV2):
+                G.fill(a, 0.0, st)
+            G.cross_attention(q, kv, key, Y, L, sizes, 0.3, st)
+            G.cross_attention_prepare(q, kv, key, g, Y, P, sizes, 0.3, st)
+            G.cross_attention_grads(P, key, L, DQ2, DKV2, sizes, 0.3, st)
+            G.unary(G.UN_MULC, DQ2, S, st, alpha=1.0)
+            G.unary(G.UN_MULC, DKV2, S2, st, alpha=1.0)
+    step()
+    st.sync()
+    captured = cudagraph.capture(st, step)
+    for _ in range(20):
+        captured.launch(st)
+        st.sync()
+        assert torch.equal(seen, dq) and torch.equal(seen2, dkv)

@@ -49,6 +49,7 @@ struct Problem {
   float scale;
   int qtiles, ktiles;
   bool vec;                                  // rows are whole 16-byte pieces on 16-byte boundaries
+  bool together;                             // both gradients in one call, see tsb_cross_attention_grads
   int* status;
 };
 
@@ -716,6 +717,7 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_queries(const Problem p) {
     tmem_relinquish();
   }
   tsb_launch::enter();
+  if (p.together) tsb_launch::allow_next();
   const int qt = blockIdx.x % p.qtiles, h = blockIdx.x / p.qtiles % p.heads, n = blockIdx.x / p.qtiles / p.heads;
   const int shared = h / (p.heads / p.shared), q0 = qt * 128, half = warp >> 2, row = threadIdx.x & 127;
   const float* tokens = p.key ? p.key + (long long)n * p.tk : nullptr;
@@ -913,7 +915,7 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_states(const Problem p) {
     tmem_alloc(&bar->tmem, 512);
     tmem_relinquish();
   }
-  tsb_launch::enter();
+  if (!p.together) tsb_launch::enter();
   const int kt = blockIdx.x % p.ktiles, shared = blockIdx.x / p.ktiles % p.shared, n = blockIdx.x / p.ktiles / p.shared;
   const int k0 = kt * 128, per = p.heads / p.shared, halves = (p.tq + 63) / 64;
   const float* tokens = p.key ? p.key + (long long)n * p.tk : nullptr;
@@ -1062,6 +1064,7 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_states(const Problem p) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (p.together) tsb_launch::wait_previous();
   if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
@@ -1424,6 +1427,43 @@ template <int D> int few(const Problem& p, int rows, cudaStream_t st) {
   return run_few<D, 8>(p, st);
 }
 
+int grad_q(const void* prepared, long long have, const float* key, const float* lse, float* dq, int n, int tq, int tk, int heads, int shared, int d,
+           float scale, void* stream, bool together) {
+  Problem p;
+  if (!describe(p, n, tq, tk, heads, shared, d, scale, nullptr, nullptr, key, dq)) return TSB_ERR_ARG;
+  if (n == 0 || tq == 0) return TSB_OK;
+  const Layout at(n, tq, tk, heads, shared, d, true);
+  if (!lse || (reinterpret_cast<uintptr_t>(lse) & 15) || !dq || !fits(prepared, have, at)) return TSB_ERR_ARG;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  use(p, at, static_cast<const char*>(prepared));
+  p.lse = const_cast<float*>(lse);
+  p.dq = dq;
+  p.together = together;
+  const long long blocks = (long long)n * heads * p.qtiles;
+  static tsb_launch::SmemLimit limit64, limit128;
+  if (d <= 64) return run(grad_of_queries<64>, p, blocks, QueryShape<64>::SMEM, st, limit64);
+  return run(grad_of_queries<128>, p, blocks, QueryShape<128>::SMEM, st, limit128);
+}
+
+int grad_kv(const void* prepared, long long have, const float* key, const float* lse, float* dkv, int n, int tq, int tk, int heads, int shared, int d,
+            float scale, void* stream, bool together) {
+  Problem p;
+  if (!describe(p, n, tq, tk, heads, shared, d, scale, nullptr, nullptr, key, dkv)) return TSB_ERR_ARG;
+  if (n == 0 || tk == 0) return TSB_OK;
+  const Layout at(n, tq, tk, heads, shared, d, true);
+  if (!dkv || (tq && !lse) || (reinterpret_cast<uintptr_t>(lse) & 15) || !fits(prepared, have, at)) return TSB_ERR_ARG;
+  if ((long long)((tq + 63) / 64) * (heads / shared) > INT32_MAX / 2) return TSB_ERR_ARG;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  use(p, at, static_cast<const char*>(prepared));
+  p.lse = const_cast<float*>(lse);
+  p.dkv = dkv;
+  p.together = together;
+  const long long blocks = (long long)n * shared * p.ktiles;
+  static tsb_launch::SmemLimit limit64, limit128;
+  if (d <= 64) return run(grad_of_states<64>, p, blocks, StateShape<64>::SMEM, st, limit64);
+  return run(grad_of_states<128>, p, blocks, StateShape<128>::SMEM, st, limit128);
+}
+
 }  // namespace
 
 extern "C" {
@@ -1467,37 +1507,23 @@ int tsb_cross_attention_prepare(const float* q, const float* kv, const float* ke
 
 int tsb_cross_attention_grad_q(const void* prepared, long long have, const float* key, const float* lse, float* dq, int n, int tq, int tk, int heads,
                                int shared, int d, float scale, void* stream) {
-  Problem p;
-  if (!describe(p, n, tq, tk, heads, shared, d, scale, nullptr, nullptr, key, dq)) return TSB_ERR_ARG;
-  if (n == 0 || tq == 0) return TSB_OK;
-  const Layout at(n, tq, tk, heads, shared, d, true);
-  if (!lse || (reinterpret_cast<uintptr_t>(lse) & 15) || !dq || !fits(prepared, have, at)) return TSB_ERR_ARG;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  use(p, at, static_cast<const char*>(prepared));
-  p.lse = const_cast<float*>(lse);
-  p.dq = dq;
-  const long long blocks = (long long)n * heads * p.qtiles;
-  static tsb_launch::SmemLimit limit64, limit128;
-  if (d <= 64) return run(grad_of_queries<64>, p, blocks, QueryShape<64>::SMEM, st, limit64);
-  return run(grad_of_queries<128>, p, blocks, QueryShape<128>::SMEM, st, limit128);
+  return grad_q(prepared, have, key, lse, dq, n, tq, tk, heads, shared, d, scale, stream, false);
 }
 
 int tsb_cross_attention_grad_kv(const void* prepared, long long have, const float* key, const float* lse, float* dkv, int n, int tq, int tk, int heads,
                                 int shared, int d, float scale, void* stream) {
-  Problem p;
-  if (!describe(p, n, tq, tk, heads, shared, d, scale, nullptr, nullptr, key, dkv)) return TSB_ERR_ARG;
-  if (n == 0 || tk == 0) return TSB_OK;
-  const Layout at(n, tq, tk, heads, shared, d, true);
-  if (!dkv || (tq && !lse) || (reinterpret_cast<uintptr_t>(lse) & 15) || !fits(prepared, have, at)) return TSB_ERR_ARG;
-  if ((long long)((tq + 63) / 64) * (heads / shared) > INT32_MAX / 2) return TSB_ERR_ARG;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  use(p, at, static_cast<const char*>(prepared));
-  p.lse = const_cast<float*>(lse);
-  p.dkv = dkv;
-  const long long blocks = (long long)n * shared * p.ktiles;
-  static tsb_launch::SmemLimit limit64, limit128;
-  if (d <= 64) return run(grad_of_states<64>, p, blocks, StateShape<64>::SMEM, st, limit64);
-  return run(grad_of_states<128>, p, blocks, StateShape<128>::SMEM, st, limit128);
+  return grad_kv(prepared, have, key, lse, dkv, n, tq, tk, heads, shared, d, scale, stream, false);
+}
+
+// Both.  The second kernel reads nothing of the first, so its blocks take the SMs that the first one's last blocks leave idle: the
+// first lets it be placed once all its own blocks run, which is behind their wait for what both of them read; the second waits
+// for the first at its end, so that what comes next finds both done.  (32 x 255 x 256, 8 heads of 64: 76 us, one
+// after the other 84; 1 x 512 x 512, 4 heads: 17 and 27.)
+int tsb_cross_attention_grads(const void* prepared, long long have, const float* key, const float* lse, float* dq, float* dkv, int n, int tq, int tk,
+                              int heads, int shared, int d, float scale, void* stream) {
+  const bool together = n > 0 && tq > 0 && tk > 0;
+  const int rc = grad_q(prepared, have, key, lse, dq, n, tq, tk, heads, shared, d, scale, stream, together);
+  return rc ? rc : grad_kv(prepared, have, key, lse, dkv, n, tq, tk, heads, shared, d, scale, stream, together);
 }
 
 }  // extern "C"

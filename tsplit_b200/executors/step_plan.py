@@ -1,6 +1,6 @@
 """The order in which the keep-all executors issue a step on the GPU, worked out once per feed shape.
 
-Nine things are taken out of the node-by-node loop.  They change no value, but for the rounding of a loss whose labels
+Ten things are taken out of the node-by-node loop.  They change no value, but for the rounding of a loss whose labels
 come from class ids (the same sum, added up in another order):
 
 * element-wise operators over the same elements are collected and run as one ``tsb_pointwise`` program, at the first
@@ -14,7 +14,8 @@ come from class ids (the same sum, added up in another order):
 * a loss and its gradient come from one pass over the logits, when the gradient is due;
 * a residual addition and its ReLU are taken by the batch norm before them, where nothing else reads that;
 * of two convolutions' gradients that only their sum reads, the first is written where the sum goes, and the other, if its
-  stride is 2, adds itself to it.
+  stride is 2, adds itself to it;
+* the gradients of a cross attention's queries and states go in one call, so that one's blocks run beside the other's last.
 
 Element-wise nodes are taken as soon as their inputs are there, the others in creation order, and nothing moves past a
 node with effects of its own (an optimizer update, a collective, a swap).  The memory-planning executors have
@@ -28,6 +29,7 @@ import numpy as np
 
 from .. import ndarray
 from ..ops import _gpu as G
+from ..ops.attention import CrossAttentionGradQueryOp, CrossAttentionGradStatesOp, both_gradients
 from ..ops.conv import Conv2dGradDataOp
 from ..ops.elementwise import AddConstOp, AddOp, AddReluOp, MulConstOp, ReluOp, _Binary, _Unary, _is_scalar_shape
 from ..ops.linalg import MatMulOp, _mm_shape
@@ -463,6 +465,8 @@ class StepPlan(object):
             shape, axes = self.shapes[n.inputs[0]], n.attrs["axes"]
             if len(shape) == 2 and list(axes) == [0] and 1 < shape[0] <= GROUP_ROWS and shape[1] <= 1024:
                 return ("sums",), 1
+        if isinstance(n.op, (CrossAttentionGradQueryOp, CrossAttentionGradStatesOp)):
+            return ("attention", n.inputs[0]), 1           # (whoever has the same operands: one of each)
         return None
 
     def _mates(self, n):
@@ -598,6 +602,8 @@ class StepPlan(object):
                 self._products(x, vals, stream)
             elif what == "sums":
                 self._sums(x, vals, stream)
+            elif what == "attention":
+                self._attention(x, vals, stream)
             elif what == "join":
                 self._joined(x, vals, stream)
             elif what == "program":
@@ -697,6 +703,17 @@ class StepPlan(object):
         else:
             for n in nodes:
                 self._node(n, vals, stream)
+
+    def _attention(self, nodes, vals, stream):
+        """Gradients of one cross attention."""
+        pair = sorted(nodes, key=lambda n: isinstance(n.op, CrossAttentionGradStatesOp))
+        if [type(n.op) for n in pair] != [CrossAttentionGradQueryOp, CrossAttentionGradStatesOp] or pair[0].inputs != pair[1].inputs:
+            for n in nodes:
+                self._node(n, vals, stream)
+            return
+        both_gradients(pair, [vals[i] for i in pair[0].inputs], [self.arrays[n] for n in pair], stream)
+        for n in pair:
+            vals[n] = self.arrays[n]
 
     def _joined(self, n, vals, stream):
         """(The inner node's own array is not written: nobody else reads it.)"""

@@ -392,6 +392,15 @@ def cross_attention_grad_kv(prepared, key, lse, dkv, sizes, scale, stream):
                "cross_attention_gradient")
 
 
+def cross_attention_grads(prepared, key, lse, dq, dkv, sizes, scale, stream):
+    """Both gradients, the second one's blocks beside the last ones of the first."""
+    _dense_rows("cross_attention_gradient", prepared, lse, dq, dkv, *([key] if key is not None else []))
+    with _on_device(dq):
+        _check(lib().tsb_cross_attention_grads(_p(prepared), c_int64(prepared.nbytes), c_void_p(key.ptr if key is not None else 0),
+                                               _p(lse), _p(dq), _p(dkv), *[c_int(s) for s in sizes], c_float(scale), _s(stream)),
+               "cross_attention_gradient")
+
+
 def dropout(x, y, keep_prob, seed, stream, step_dev=0, offset=0):
     """``step_dev``: device address of the executor's step counter (0 = ``seed`` is already step-mixed);
     ``offset``: index of ``x``'s first element in the whole tensor when ``x`` is a batch piece of it."""

@@ -159,12 +159,18 @@ class _CrossAttentionGradient(Op):
         ds = p * (dp - (dp * p).sum(4, keepdims=True)) * CrossAttentionOp.scale_of(node, kv.shape[4])
         return ds, p, g, q, k
 
-    def gpu_compute(self, node, iv, out, stream):
+    @staticmethod
+    def _arguments(node, iv, ctx):
+        """(prepared, key tokens, log-sum-exps), sizes, scale."""
         key = iv[4] if len(iv) > 4 else None
         sizes = _sizes(iv[2].shape, iv[3].shape, key.shape if key is not None else None)
-        lse = _row_sums(node.attrs["fwd"], sizes, out.ctx, make=False)
+        lse = _row_sums(node.attrs["fwd"], sizes, ctx, make=False)
         assert lse is not None, "the gradient of a cross attention needs its forward pass on the same device first"
-        self._launch(iv[0], key, lse, out, sizes, CrossAttentionOp.scale_of(node, sizes[5]), stream)
+        return (iv[0], key, lse), sizes, CrossAttentionOp.scale_of(node, sizes[5])
+
+    def gpu_compute(self, node, iv, out, stream):
+        inputs, sizes, scale = self._arguments(node, iv, out.ctx)
+        self._launch(*inputs, out, sizes, scale, stream)
 
     def gradient(self, node, g):
         raise NotImplementedError
@@ -209,6 +215,13 @@ class CrossAttentionGradStatesOp(_CrossAttentionGradient):
 
     def flops(self, node, s, out):
         return 8.0 * np.prod(s[2]) * s[3][1]
+
+
+def both_gradients(nodes, iv, out, stream):
+    """The gradients of the queries and of the states (``nodes``, of one forward pass and one set of operands ``iv``) into the
+    arrays ``out``, in one call."""
+    inputs, sizes, scale = nodes[0].op._arguments(nodes[0], iv, out[0].ctx)
+    G.cross_attention_grads(*inputs, *out, sizes, scale, stream)
 
 
 _ca, _cap, _cagq, _cagkv = CrossAttentionOp(), CrossAttentionPrepareOp(), CrossAttentionGradQueryOp(), CrossAttentionGradStatesOp()
