@@ -400,3 +400,27 @@ def test_both_gradients_in_one_call_in_a_captured_chain(n, tq, tk, h, s, d):
         captured.launch(st)
         st.sync()
         assert torch.equal(seen, dq) and torch.equal(seen2, dkv)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tq,heads,kept", [(9, 2, True), (8, 2, False), (3, 8, True), (40, 2, True)])
+def test_a_step_splits_its_operands_once(tq, heads, kept):
+    """The pieces of q, k and v that the forward pass makes are those of the gradients, but for single tokens, which make none;
+    both gradients go in one call; a second gradient of the same node takes operands of its own."""
+    ctx, f = ndarray.gpu(0), case(2, tq, 70, heads, 2, 16, "holes")
+    v = {k: ad.Variable(k) for k in f}
+    y = ad.cross_attention_op(v["q"], v["kv"], v["key"])
+    nodes = [y] + ad.cross_attention_gradient_op(y, v["g"])
+    want, tol = definition(f["q"], f["kv"], f["key"], 0.25, f["g"])
+    for more in (False, True):
+        if more:
+            nodes = nodes + ad.cross_attention_gradient_op(y, ad.mul_byconst_op(v["g"], 2.0))
+        ex = ad.Executor(nodes, ctx=ctx)
+        for _ in range(2):
+            got = [np.asarray(o, np.float64) for o in ex.run({v[k]: a for k, a in f.items()}, convert_to_numpy_ret_vals=True)]
+        for a, b, t in zip(got, want, tol):
+            assert np.all(np.abs(a - b) <= t + 1e-37)
+        for a, b, t in zip(got[3:], want[1:], tol[1:]):
+            assert np.all(np.abs(a - 2 * b) <= 2 * t + 1e-37)
+        kinds = [what for what, _ in ex._step_plan.actions]
+        assert kinds.count("keep") == (2 if kept and not more else 0) and kinds.count("attention") == (2 if more else 1)

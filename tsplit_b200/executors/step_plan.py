@@ -1,6 +1,6 @@
 """The order in which the keep-all executors issue a step on the GPU, worked out once per feed shape.
 
-Ten things are taken out of the node-by-node loop.  They change no value, but for the rounding of a loss whose labels
+Eleven things are taken out of the node-by-node loop.  They change no value, but for the rounding of a loss whose labels
 come from class ids (the same sum, added up in another order):
 
 * element-wise operators over the same elements are collected and run as one ``tsb_pointwise`` program, at the first
@@ -15,6 +15,7 @@ come from class ids (the same sum, added up in another order):
 * a residual addition and its ReLU are taken by the batch norm before them, where nothing else reads that;
 * of two convolutions' gradients that only their sum reads, the first is written where the sum goes, and the other, if its
   stride is 2, adds itself to it;
+* a cross attention's forward pass leaves the pieces of its operands where its gradients look for them;
 * the gradients of a cross attention's queries and states go in one call, so that one's blocks run beside the other's last.
 
 Element-wise nodes are taken as soon as their inputs are there, the others in creation order, and nothing moves past a
@@ -29,7 +30,8 @@ import numpy as np
 
 from .. import ndarray
 from ..ops import _gpu as G
-from ..ops.attention import CrossAttentionGradQueryOp, CrossAttentionGradStatesOp, both_gradients
+from ..ops.attention import (CrossAttentionOp, CrossAttentionPrepareOp, CrossAttentionGradQueryOp, CrossAttentionGradStatesOp,
+                             both_gradients, keeps_operands)
 from ..ops.conv import Conv2dGradDataOp
 from ..ops.elementwise import AddConstOp, AddOp, AddReluOp, MulConstOp, ReluOp, _Binary, _Unary, _is_scalar_shape
 from ..ops.linalg import MatMulOp, _mm_shape
@@ -191,6 +193,9 @@ class StepPlan(object):
             self._join(n)
         for n in own.get(AddOp, ()):
             self._add_gradients(n)
+        self.kept = {}                           # cross attention -> the operands of its gradients, and these -> None
+        for n in of(CrossAttentionOp):
+            self._keep_operands(n)
         self.root = {}                    # view -> the node whose array it looks at
         self.actions = []
         self.open = {}                    # key -> Program that still collects
@@ -320,6 +325,14 @@ class StepPlan(object):
                 and self.arrays.get(grads[0]) is not None):
             self.both[grads[0]] = loss
 
+    def _keep_operands(self, n):
+        """Into the array of the one node that would split them again, while nothing stands between that changes them."""
+        takers = [u for u in self.users.get(n, ()) if isinstance(u.op, CrossAttentionPrepareOp) and u.inputs[1:] == [n] + n.inputs]
+        if (len(takers) == 1 and self.place[takers[0]] == self.place[n] and not self._has_effects(n) and not self._has_effects(takers[0])
+                and self.arrays.get(n) is not None and self.arrays.get(takers[0]) is not None
+                and keeps_operands(self.shapes[n.inputs[0]], self.shapes[n.inputs[1]])):
+            self.kept[n], self.kept[takers[0]] = takers[0], None
+
     def _dense(self, product):
         """``product + row`` that nothing else reads the product of, and the one ReLU of the result (or of the product
         itself): the product's launch can store them.  The row is there from the start, a parameter: an addition behind its
@@ -446,6 +459,7 @@ class StepPlan(object):
                                     ("smooth", n) if n in self.smooth else
                                     ("loss", n) if n in self.both or n in self.late else
                                     ("join", n) if n in self.joined else
+                                    ("keep", n) if n in self.kept else
                                     ("products", taken) if n in self.dense or not self.sliced.isdisjoint(n.inputs) else
                                     ("node", n))
                 for m in taken[1:]:
@@ -602,6 +616,8 @@ class StepPlan(object):
                 self._products(x, vals, stream)
             elif what == "sums":
                 self._sums(x, vals, stream)
+            elif what == "keep":
+                self._keep(x, vals, stream)
             elif what == "attention":
                 self._attention(x, vals, stream)
             elif what == "join":
@@ -703,6 +719,15 @@ class StepPlan(object):
         else:
             for n in nodes:
                 self._node(n, vals, stream)
+
+    def _keep(self, n, vals, stream):
+        """A cross attention or the operands of its gradients."""
+        out, ins = self.arrays[n], [vals[i] for i in n.inputs]
+        if self.kept[n] is None:
+            n.op.gpu_compute(n, ins, out, stream, kept=True)
+        else:
+            n.op.gpu_compute(n, ins, out, stream, prepared=self.arrays[self.kept[n]])
+        vals[n] = out
 
     def _attention(self, nodes, vals, stream):
         """Gradients of one cross attention."""

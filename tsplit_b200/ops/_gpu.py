@@ -359,10 +359,16 @@ def token_score_grad(logits, ids, out, g, dx, stream):
                                           c_int((out.shape[1] - 3) // 2), _s(stream)), "token_log_prob_gradient")
 
 
-def cross_attention(q, kv, key, y, lse, sizes, scale, stream):
-    """``sizes``: (N, Tq, Tk, heads, heads of the states, d).  ``lse`` [N, heads, Tq] is written for the gradients."""
-    _dense_rows("cross_attention", q, kv, y, lse, *([key] if key is not None else []))
+def cross_attention(q, kv, key, y, lse, sizes, scale, stream, prepared=None):
+    """``sizes``: (N, Tq, Tk, heads, heads of the states, d).  ``lse`` [N, heads, Tq] is written for the gradients.  ``prepared``:
+    where the operands' pieces stay for :func:`cross_attention_prepare_g`."""
+    _dense_rows("cross_attention", q, kv, y, lse, *[a for a in (key, prepared) if a is not None])
     with _on_device(q):
+        if prepared is not None:
+            _check(lib().tsb_cross_attention_keep(_p(q), _p(kv), c_void_p(key.ptr if key is not None else 0), _p(y), _p(lse), _p(prepared),
+                                                  c_int64(prepared.nbytes), *[c_int(s) for s in sizes], c_float(scale), _s(stream)),
+                   "cross_attention")
+            return
         _check(lib().tsb_cross_attention(_p(q), _p(kv), c_void_p(key.ptr if key is not None else 0), _p(y), _p(lse),
                                          *[c_int(s) for s in sizes], c_float(scale), _s(stream)), "cross_attention")
 
@@ -373,6 +379,14 @@ def cross_attention_prepare(q, kv, key, g, y, prepared, sizes, scale, stream):
     with _on_device(q):
         _check(lib().tsb_cross_attention_prepare(_p(q), _p(kv), c_void_p(key.ptr if key is not None else 0), _p(g), _p(y), _p(prepared),
                                                  c_int64(prepared.nbytes), *[c_int(s) for s in sizes], c_float(scale), _s(stream)),
+               "cross_attention_gradient")
+
+
+def cross_attention_prepare_g(g, y, prepared, sizes, stream):
+    """What is left of :func:`cross_attention_prepare` when the forward pass has kept the pieces of its operands."""
+    _dense_rows("cross_attention_gradient", g, y, prepared)
+    with _on_device(g):
+        _check(lib().tsb_cross_attention_prepare_g(_p(g), _p(y), _p(prepared), c_int64(prepared.nbytes), *[c_int(s) for s in sizes], _s(stream)),
                "cross_attention_gradient")
 
 

@@ -73,11 +73,11 @@ class CrossAttentionOp(Op):
         p, _, _, v = _probabilities(iv[0], iv[1], iv[2] if len(iv) > 2 else None, self.scale_of(node, iv[0].shape[3]))
         return _back(p @ v).astype(np.float32)
 
-    def gpu_compute(self, node, iv, out, stream):
+    def gpu_compute(self, node, iv, out, stream, prepared=None):
         sizes = _sizes(iv[0].shape, iv[1].shape, iv[2].shape if len(iv) > 2 else None)
         node.state["runs"] = node.state.get("runs", 0) + 1
         G.cross_attention(iv[0], iv[1], iv[2] if len(iv) > 2 else None, out, _row_sums(node, sizes, iv[0].ctx), sizes,
-                          self.scale_of(node, sizes[5]), stream)
+                          self.scale_of(node, sizes[5]), stream, prepared)
 
     def gradient(self, node, g):
         return cross_attention_gradient_op(node, g) + [None] * (len(node.inputs) - 2)
@@ -126,7 +126,8 @@ class CrossAttentionPrepareOp(Op):
     def np_compute(self, node, iv):
         return np.zeros(self.infer_shape(node, [v.shape for v in iv]), np.float32)
 
-    def gpu_compute(self, node, iv, out, stream):
+    def gpu_compute(self, node, iv, out, stream, kept=False):
+        """``kept``: the forward pass of this step has left the pieces of its operands in ``out``."""
         g, y, q, kv = iv[:4]
         key = iv[4] if len(iv) > 4 else None
         sizes = _sizes(q.shape, kv.shape, key.shape if key is not None else None)
@@ -134,6 +135,9 @@ class CrossAttentionPrepareOp(Op):
         if runs == node.state.get("of", 0):
             raise ValueError("the gradient of a cross attention takes the forward pass of the same step, not a result that was fed")
         node.state["of"] = runs
+        if kept:
+            G.cross_attention_prepare_g(g, y, out, sizes, stream)
+            return
         G.cross_attention_prepare(q, kv, key, g, y, out, sizes, CrossAttentionOp.scale_of(node, sizes[5]), stream)
 
     def gradient(self, node, g):
@@ -215,6 +219,11 @@ class CrossAttentionGradStatesOp(_CrossAttentionGradient):
 
     def flops(self, node, s, out):
         return 8.0 * np.prod(s[2]) * s[3][1]
+
+
+def keeps_operands(q, kv):
+    """Whether the forward pass over these shapes splits its operands: all but single tokens do."""
+    return q[2] // kv[3] * q[1] > 8
 
 
 def both_gradients(nodes, iv, out, stream):
