@@ -583,9 +583,10 @@ __device__ __forceinline__ void grad_of_columns(const float* xr, const float* o,
   weights += w_given;
   const bool empty = lse == NEG_INF;
   const float plain = load(w + 2) - weights;
-  auto rest = [&](float v) {                                                    // of a column that is no id
+  // of a column that is no id (w_H log p alone may be beyond fp32 where p is 0: a logit masked by the type's lowest number)
+  auto rest = [&](float v) {
     const float lp = v - lse, p = __expf(lp);
-    return empty || v == NEG_INF ? 0.f : p * (plain - wh * (lp + entropy));
+    return empty || v == NEG_INF || p == 0.f ? 0.f : p * (plain - wh * (lp + entropy));
   };
   const unsigned odd = (unsigned)((-(long long)(reinterpret_cast<uintptr_t>(xr + begin) >> 2)) & 3);
   const bool same = ((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(dr)) & 15) == 0;
@@ -601,7 +602,7 @@ __device__ __forceinline__ void grad_of_columns(const float* xr, const float* o,
   auto of_id = [&](long long col, float own) {
     if (col < (long long)begin || col >= (long long)end) return;
     const float v = load(xr + col), lp = v - lse, p = expf(lp);
-    const float other = v == NEG_INF ? 0.f : p * (load(w + 2) - (weights - own) - wh * (lp + entropy));
+    const float other = v == NEG_INF || p == 0.f ? 0.f : p * (load(w + 2) - (weights - own) - wh * (lp + entropy));
     dr[col] = own * -expm1f(lp) + other;
   };
   of_id(alternative, w_alternative + (given && alternative == id ? w_given : 0.f));
