@@ -156,6 +156,8 @@ class Executor(object):
                 shp = node.op.infer_shape(node, [])
             else:
                 shp = node.op.infer_shape(node, [self.node_to_shape_map[i] for i in node.inputs])
+                if self.on_device:
+                    node.op.check_feeds(node, feed_shapes)
             if shp is not None:
                 shp = tuple(int(s) for s in shp)
             self.node_to_shape_map[node] = shp
@@ -269,6 +271,7 @@ class Executor(object):
         node_to_val = self._ingest(feed_dict)
         feed_shapes = {n: _shape_of(v) for n, v in node_to_val.items()}
         if feed_shapes != self.feed_shapes:
+            self.feed_shapes = None                  # (feeds that are refused are looked at again the next time)
             self.infer_shape(feed_shapes)
             self.feed_shapes = feed_shapes
             if not self.use_numpy:

@@ -542,8 +542,9 @@ class MemoryExecutor(Executor):
         node_to_val = self._ingest(feed_dict)
         feed_shapes = {n: tuple(v.shape) for n, v in node_to_val.items()}
         if feed_shapes != self.feed_shapes:
-            self.feed_shapes = feed_shapes
+            self.feed_shapes = None                  # (feeds that are refused are looked at again the next time)
             self.infer_shape(feed_shapes)
+            self.feed_shapes = feed_shapes
             self.memory_plan(feed_shapes)
         if self.use_graph and self._graph_eligible():
             return self._run_graphed(node_to_val, convert_to_numpy_ret_vals)

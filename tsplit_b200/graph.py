@@ -134,6 +134,9 @@ class Op(object):
     def infer_shape(self, node, input_shapes):
         raise NotImplementedError(self.name)
 
+    def check_feeds(self, node, fed):
+        """Raises where the kernels cannot compute ``node`` in a step in which the nodes of ``fed`` are given."""
+
     # -- cost model hooks (see profiler.py) -----------------------------------
     def flops(self, node, input_shapes, output_shape):
         """Floating point operations of one execution (default: 1 per output)."""

@@ -114,8 +114,8 @@ def _prepared_floats(n, tq, tk, h, shared, d):
 
 class CrossAttentionPrepareOp(Op):
     """Operands of both gradients as the tensor cores take them, and ``sum(g * y)`` over every row: a flat array that only the
-    kernels read.  The gradients also read what the forward kernel has left, so it has to run before each of them: a result that
-    is fed in its place is refused."""
+    kernels read.  The gradients also read what the forward kernel has left, so it has to run in the same step: where its result
+    is fed, the step is refused as it is planned (the NumPy path computes everything from its inputs)."""
     name = "CrossAttentionPrepare"
 
     def __call__(self, g, forward):
@@ -142,6 +142,10 @@ class CrossAttentionPrepareOp(Op):
 
     def gradient(self, node, g):
         raise NotImplementedError
+
+    def check_feeds(self, node, fed):
+        if node.attrs["fwd"] in fed:
+            raise ValueError("the gradient of a cross attention takes the forward pass of the same step, not a result that was fed")
 
     def infer_shape(self, node, s):
         assert tuple(s[0]) == tuple(s[1]) == tuple(s[2]), "gradient %s of a result %s" % (tuple(s[0]), tuple(s[1]))
