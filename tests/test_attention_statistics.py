@@ -52,3 +52,16 @@ def test_a_fed_result_is_refused_whatever_ran_before(cls):
                 e.run({**feeds(v, 1), y: first})
     got = ex.run(feeds(v, 2), convert_to_numpy_ret_vals=True)
     assert all(np.array_equal(a, b) for a, b in zip(got, want[1]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", [ad.recomputeExecutor, ad.microopExecutor])
+def test_operators_are_timed_one_by_one(cls):
+    """Each node several times on its own, as a measured plan wants it; the same results afterwards."""
+    ctx = ndarray.gpu(0)
+    v, y, grads = graph()
+    ex = cls([y] + grads, ctx=ctx)
+    times = ex.measure_ops(feeds(v, 1))                # (before a plan that cuts operators in pieces)
+    want = ad.Executor([y] + grads, ctx=ctx).run(feeds(v, 1), convert_to_numpy_ret_vals=True)
+    assert {y, grads[0], grads[1], grads[0].inputs[0]} <= set(times) and all(t > 0 for t in times.values())
+    assert all(np.array_equal(a, b) for a, b in zip(want, ex.run(feeds(v, 1), convert_to_numpy_ret_vals=True)))

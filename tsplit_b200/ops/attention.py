@@ -75,7 +75,6 @@ class CrossAttentionOp(Op):
 
     def gpu_compute(self, node, iv, out, stream, prepared=None):
         sizes = _sizes(iv[0].shape, iv[1].shape, iv[2].shape if len(iv) > 2 else None)
-        node.state["runs"] = node.state.get("runs", 0) + 1
         G.cross_attention(iv[0], iv[1], iv[2] if len(iv) > 2 else None, out, _row_sums(node, sizes, iv[0].ctx), sizes,
                           self.scale_of(node, sizes[5]), stream, prepared)
 
@@ -119,9 +118,7 @@ class CrossAttentionPrepareOp(Op):
     name = "CrossAttentionPrepare"
 
     def __call__(self, g, forward):
-        node = Op.__call__(self, g, forward, *forward.inputs, scale=forward.attrs["scale"], fwd=forward)
-        node.state = {}
-        return node
+        return Op.__call__(self, g, forward, *forward.inputs, scale=forward.attrs["scale"], fwd=forward)
 
     def np_compute(self, node, iv):
         return np.zeros(self.infer_shape(node, [v.shape for v in iv]), np.float32)
@@ -131,10 +128,6 @@ class CrossAttentionPrepareOp(Op):
         g, y, q, kv = iv[:4]
         key = iv[4] if len(iv) > 4 else None
         sizes = _sizes(q.shape, kv.shape, key.shape if key is not None else None)
-        runs = node.attrs["fwd"].state.get("runs", 0)
-        if runs == node.state.get("of", 0):
-            raise ValueError("the gradient of a cross attention takes the forward pass of the same step, not a result that was fed")
-        node.state["of"] = runs
         if kept:
             G.cross_attention_prepare_g(g, y, out, sizes, stream)
             return
