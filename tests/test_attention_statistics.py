@@ -1,9 +1,13 @@
 """The rows' log-sum-exps, which a cross attention's forward pass leaves for its gradients: whose they are, and that nobody takes
 another pass's."""
+import gc
+
 import numpy as np
 import pytest
 
 from tsplit_b200 import ndarray, gpu_ops as ad
+from tsplit_b200.ops import attention as A
+from tsplit_b200.stream import Stream, create_stream_handle
 
 
 def graph():
@@ -65,3 +69,53 @@ def test_operators_are_timed_one_by_one(cls):
     want = ad.Executor([y] + grads, ctx=ctx).run(feeds(v, 1), convert_to_numpy_ret_vals=True)
     assert {y, grads[0], grads[1], grads[0].inputs[0]} <= set(times) and all(t > 0 for t in times.values())
     assert all(np.array_equal(a, b) for a, b in zip(want, ex.run(feeds(v, 1), convert_to_numpy_ret_vals=True)))
+
+
+# ------------------------------------------------------------------------------------------------ two streams
+def test_every_stream_has_log_sum_exps_of_its_own():
+    """... which are given back once neither the stream nor what was captured on it is there."""
+    ctx, sizes = ndarray.cpu(0), (2, 20, 30, 2, 2, 16)
+    _, y, _ = graph()
+    a, b = Stream(ctx), Stream(ctx)
+    assert A._row_sums(y, sizes, ctx, a, make=False) is None
+    one, two = A._row_sums(y, sizes, ctx, a), A._row_sums(y, sizes, ctx, b)
+    assert one.ptr != two.ptr
+    assert A._row_sums(y, sizes, ctx, a) is one and A._row_sums(y, sizes, ctx, b, make=False) is two
+    assert A._row_sums(y, sizes[:1] + (200,) + sizes[2:], ctx, a) is not one and A._row_sums(y, sizes, ctx, a) is one
+    captured = a.buffers                                             # (as a captured graph holds it)
+    del a
+    gc.collect()
+    A._row_sums(y, sizes, ctx, Stream(ctx))
+    held = [x for x in y.state.values() if isinstance(x, ndarray.NDArray)]
+    assert any(x is one for x in held) and len(held) == 4
+    del captured, held
+    gc.collect()
+    three = Stream(ctx)
+    new = A._row_sums(y, sizes, ctx, three)
+    held = [x for x in y.state.values() if isinstance(x, ndarray.NDArray)]
+    assert len(held) == 2 and any(x is two for x in held) and any(x is new for x in held)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes", [dict(), dict(tq=1, h=4), dict(tq=150, tk=200, d=128)])
+def test_another_streams_forward_pass_in_between(sizes):
+    """Two executors of the same nodes: one's forward pass stands between the other's and its gradients."""
+    ctx = ndarray.gpu(0)
+    v, y, grads = graph()
+    f = [feeds(v, k, **sizes) for k in (1, 2)]
+    want = [ad.Executor([y] + grads, ctx=ctx).run(x, convert_to_numpy_ret_vals=True) for x in f]
+    st = [create_stream_handle(ctx) for _ in f]
+    arr = [{n: ndarray.array(a, ctx, channels_last=False) for n, a in x.items()} for x in f]
+    out = [{n: ndarray.empty(w.shape, ctx, channels_last=False) for n, w in zip([y] + grads, ws)} for ws in want]
+    pre = grads[0].inputs[0]
+    flat = ndarray.empty(pre.op.infer_shape(pre, [out[0][y].shape] * 2 + [arr[0][i].shape for i in y.inputs]), ctx)
+
+    def run(k, n):
+        vals = {**arr[k], **out[k], pre: flat}
+        n.op.gpu_compute(n, [vals[i] for i in n.inputs], vals[n], st[k])
+        st[k].sync()
+    for k, n in ((0, y), (1, y), (0, pre), (0, grads[0]), (0, grads[1]), (1, pre), (1, grads[0]), (1, grads[1])):
+        run(k, n)
+    for o, w in zip(out, want):
+        for n, a in zip([y] + grads, w):
+            assert np.array_equal(o[n].asnumpy(), a)

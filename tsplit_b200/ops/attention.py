@@ -6,9 +6,12 @@ The reference's example builds it from batched products, a scale, a padding mask
 """
 from __future__ import annotations
 
+import weakref
+
 import numpy as np
 
 from ..graph import Op
+from ..stream import Buffers
 from . import _gpu as G
 
 MAX_HEAD_DIM = 128
@@ -75,7 +78,7 @@ class CrossAttentionOp(Op):
 
     def gpu_compute(self, node, iv, out, stream, prepared=None):
         sizes = _sizes(iv[0].shape, iv[1].shape, iv[2].shape if len(iv) > 2 else None)
-        G.cross_attention(iv[0], iv[1], iv[2] if len(iv) > 2 else None, out, _row_sums(node, sizes, iv[0].ctx), sizes,
+        G.cross_attention(iv[0], iv[1], iv[2] if len(iv) > 2 else None, out, _row_sums(node, sizes, iv[0].ctx, stream), sizes,
                           self.scale_of(node, sizes[5]), stream, prepared)
 
     def gradient(self, node, g):
@@ -89,15 +92,29 @@ class CrossAttentionOp(Op):
         return 4.0 * np.prod(s[0]) * s[1][1]
 
 
-def _row_sums(node, sizes, ctx, make=True):
-    """The rows' log-sum-exps, which the forward kernel leaves for the gradients: an array for every number of rows that the
-    node has run at, since a step that was captured at one goes on using its own (a sentence of states that grows needs no more)."""
+_NO_STREAM = Buffers()
+
+
+def _row_sums(node, sizes, ctx, stream, make=True):
+    """The rows' log-sum-exps, which the forward kernel leaves for the gradients.  An array for every stream, since two executors of
+    one node may run at once or in turn, for as long as the stream or what was captured on it lives; and for every number of rows that
+    was run there, since a step that was captured at one goes on using its own (a sentence of states that grows needs no more)."""
     shape = (sizes[0], sizes[3], _whole_tiles(sizes[1]))
-    key = ("lse", shape, ctx)
-    if key not in node.state and make:
-        from .. import ndarray
-        node.state[key] = ndarray.empty(shape, ctx, use_pool=False)
-    return node.state.get(key)
+    held = stream.buffers if stream is not None else _NO_STREAM        # (one object for all that is launched on a stream)
+    key, owners = ("lse", shape, ctx, id(held)), node.state.setdefault("owners", {})
+    owner = owners.get(key)
+    if owner is not None and owner() is held:
+        return node.state[key]
+    if not make:
+        return None
+    for k, o in list(owners.items()):
+        if o() is None:
+            owners.pop(k, None)
+            node.state.pop(k, None)
+    from .. import ndarray
+    node.state[key] = ndarray.empty(shape, ctx, use_pool=False)
+    owners[key] = weakref.ref(held)
+    return node.state[key]
 
 
 def _whole_tiles(t):
@@ -161,16 +178,16 @@ class _CrossAttentionGradient(Op):
         return ds, p, g, q, k
 
     @staticmethod
-    def _arguments(node, iv, ctx):
+    def _arguments(node, iv, ctx, stream):
         """(prepared, key tokens, log-sum-exps), sizes, scale."""
         key = iv[4] if len(iv) > 4 else None
         sizes = _sizes(iv[2].shape, iv[3].shape, key.shape if key is not None else None)
-        lse = _row_sums(node.attrs["fwd"], sizes, ctx, make=False)
-        assert lse is not None, "the gradient of a cross attention needs its forward pass on the same device first"
+        lse = _row_sums(node.attrs["fwd"], sizes, ctx, stream, make=False)
+        assert lse is not None, "the gradient of a cross attention needs its forward pass on the same stream first"
         return (iv[0], key, lse), sizes, CrossAttentionOp.scale_of(node, sizes[5])
 
     def gpu_compute(self, node, iv, out, stream):
-        inputs, sizes, scale = self._arguments(node, iv, out.ctx)
+        inputs, sizes, scale = self._arguments(node, iv, out.ctx, stream)
         self._launch(*inputs, out, sizes, scale, stream)
 
     def gradient(self, node, g):
@@ -226,7 +243,7 @@ def keeps_operands(q, kv):
 def both_gradients(nodes, iv, out, stream):
     """The gradients of the queries and of the states (``nodes``, of one forward pass and one set of operands ``iv``) into the
     arrays ``out``, in one call."""
-    inputs, sizes, scale = nodes[0].op._arguments(nodes[0], iv, out[0].ctx)
+    inputs, sizes, scale = nodes[0].op._arguments(nodes[0], iv, out[0].ctx, stream)
     G.cross_attention_grads(*inputs, *out, sizes, scale, stream)
 
 
