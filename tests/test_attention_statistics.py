@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from tsplit_b200 import ndarray, gpu_ops as ad
-from tsplit_b200.ops import attention as A
+from tsplit_b200.ops import _gpu as G, attention as A
 from tsplit_b200.stream import Stream, create_stream_handle
 
 
@@ -119,3 +119,18 @@ def test_another_streams_forward_pass_in_between(sizes):
     for o, w in zip(out, want):
         for n, a in zip([y] + grads, w):
             assert np.array_equal(o[n].asnumpy(), a)
+
+
+# ------------------------------------------------------------------------------------------------ their room
+@pytest.mark.parametrize("tq,shape", [(3, (2, 4, 3)), (3, (2, 4, 127)), (129, (2, 4, 129)), (129, (2, 4, 255)), (1, (2, 3, 128))])
+def test_too_few_log_sum_exps_are_refused(tq, shape):
+    """The kernels write and read them for whole tiles of 128 queries, so an array of as many as there are queries is too short."""
+    e, sizes = ndarray.empty, (2, tq, 5, 4, 2, 8)
+    q, kv, lse, flat = e((2, tq, 4, 8)), e((2, 5, 2, 2, 8)), e(shape), e((A._prepared_floats(*sizes),))
+    for call in [lambda: G.cross_attention(q, kv, None, q, lse, sizes, 1.0, None),
+                 lambda: G.cross_attention(q, kv, None, q, lse, sizes, 1.0, None, flat),
+                 lambda: G.cross_attention_grad_q(flat, None, lse, q, sizes, 1.0, None),
+                 lambda: G.cross_attention_grad_kv(flat, None, lse, kv, sizes, 1.0, None),
+                 lambda: G.cross_attention_grads(flat, None, lse, q, kv, sizes, 1.0, None)]:
+        with pytest.raises(ValueError, match="log-sum-exps"):
+            call()

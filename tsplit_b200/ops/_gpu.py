@@ -359,10 +359,19 @@ def token_score_grad(logits, ids, out, g, dx, stream):
                                           c_int((out.shape[1] - 3) // 2), _s(stream)), "token_log_prob_gradient")
 
 
+def _room_for_rows(lse, sizes):
+    n, tq, _, heads = sizes[:4]
+    need = n * heads * (-(-tq // 128) * 128)
+    if _numel(lse.shape) < need:
+        raise ValueError("cross_attention: log-sum-exps of shape %s are fewer than the %d of %d queries in whole tiles of 128"
+                         % (tuple(lse.shape), need, tq))
+
+
 def cross_attention(q, kv, key, y, lse, sizes, scale, stream, prepared=None):
-    """``sizes``: (N, Tq, Tk, heads, heads of the states, d).  ``lse`` [N, heads, Tq] is written for the gradients.  ``prepared``:
-    where the operands' pieces stay for :func:`cross_attention_prepare_g`."""
+    """``sizes``: (N, Tq, Tk, heads, heads of the states, d).  ``lse`` [N, heads, Tq rounded up to a multiple of 128] is written for
+    the gradients, all of it.  ``prepared``: where the operands' pieces stay for :func:`cross_attention_prepare_g`."""
     _dense_rows("cross_attention", q, kv, y, lse, *[a for a in (key, prepared) if a is not None])
+    _room_for_rows(lse, sizes)
     with _on_device(q):
         if prepared is not None:
             _check(lib().tsb_cross_attention_keep(_p(q), _p(kv), c_void_p(key.ptr if key is not None else 0), _p(y), _p(lse), _p(prepared),
@@ -392,6 +401,7 @@ def cross_attention_prepare_g(g, y, prepared, sizes, stream):
 
 def cross_attention_grad_q(prepared, key, lse, dq, sizes, scale, stream):
     _dense_rows("cross_attention_gradient", prepared, lse, dq, *([key] if key is not None else []))
+    _room_for_rows(lse, sizes)
     with _on_device(dq):
         _check(lib().tsb_cross_attention_grad_q(_p(prepared), c_int64(prepared.nbytes), c_void_p(key.ptr if key is not None else 0),
                                                 _p(lse), _p(dq), *[c_int(s) for s in sizes], c_float(scale), _s(stream)),
@@ -400,6 +410,7 @@ def cross_attention_grad_q(prepared, key, lse, dq, sizes, scale, stream):
 
 def cross_attention_grad_kv(prepared, key, lse, dkv, sizes, scale, stream):
     _dense_rows("cross_attention_gradient", prepared, lse, dkv, *([key] if key is not None else []))
+    _room_for_rows(lse, sizes)
     with _on_device(dkv):
         _check(lib().tsb_cross_attention_grad_kv(_p(prepared), c_int64(prepared.nbytes), c_void_p(key.ptr if key is not None else 0),
                                                  _p(lse), _p(dkv), *[c_int(s) for s in sizes], c_float(scale), _s(stream)),
@@ -409,6 +420,7 @@ def cross_attention_grad_kv(prepared, key, lse, dkv, sizes, scale, stream):
 def cross_attention_grads(prepared, key, lse, dq, dkv, sizes, scale, stream):
     """Both gradients, the second one's blocks beside the last ones of the first."""
     _dense_rows("cross_attention_gradient", prepared, lse, dq, dkv, *([key] if key is not None else []))
+    _room_for_rows(lse, sizes)
     with _on_device(dq):
         _check(lib().tsb_cross_attention_grads(_p(prepared), c_int64(prepared.nbytes), c_void_p(key.ptr if key is not None else 0),
                                                _p(lse), _p(dq), _p(dkv), *[c_int(s) for s in sizes], c_float(scale), _s(stream)),
