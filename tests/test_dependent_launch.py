@@ -72,3 +72,14 @@ def test_small_writers_and_their_readers_in_a_captured_chain(blocks):
     assert want < 2 ** 24                                   # whole numbers below 2^24: every sum is exact
     assert torch.all(x == count) and torch.all(acc == want)
     assert torch.all(rows == 1) and torch.all(shifted == 7) and torch.all(sums == 7 * (n // 64))
+
+
+def test_no_kernel_goes_without_its_wait():
+    """A grid that is placed before the one in front of it has ended sees what that one saw only behind a wait of its own: every
+    kernel that is launched so waits, and on no condition."""
+    for path in glob.glob(os.path.join(KERNELS, "*.cu")) + glob.glob(os.path.join(KERNELS, "*.cuh")):
+        code = _code(path)
+        if os.path.basename(path) != "launch.cuh":
+            assert not re.search(r"griddepcontrol|\ballow_next\b", code), os.path.basename(path)
+        condition = r"(?:\bif\s*\((?:[^()]|\([^()]*\))*\)|\belse|\?|(?<!:):(?!:)|&&|\|\|)\s*(?:tsb_launch::)?(?:enter|wait_previous)\s*\(\)"
+        assert not re.search(condition, code), os.path.basename(path)

@@ -49,7 +49,7 @@ struct Problem {
   float scale;
   int qtiles, ktiles;
   bool vec;                                  // rows are whole 16-byte pieces on 16-byte boundaries
-  bool together;                             // both gradients in one call, see tsb_cross_attention_grads
+  int query_blocks;                          // of the gradients: blocks that compute those of queries
   int* status;
 };
 
@@ -689,7 +689,7 @@ struct QueryControl {
 };
 
 template <int D>
-__global__ void __launch_bounds__(BLOCK, 1) grad_of_queries(const Problem p) {
+__device__ __forceinline__ void grad_of_queries(const Problem& p, const int block) {
   using Shape = QueryShape<D>;
   using LQ = typename Shape::LQ;
   using LK = typename Shape::LK;
@@ -717,8 +717,7 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_queries(const Problem p) {
     tmem_relinquish();
   }
   tsb_launch::enter();
-  if (p.together) tsb_launch::allow_next();
-  const int qt = blockIdx.x % p.qtiles, h = blockIdx.x / p.qtiles % p.heads, n = blockIdx.x / p.qtiles / p.heads;
+  const int qt = block % p.qtiles, h = block / p.qtiles % p.heads, n = block / p.qtiles / p.heads;
   const int shared = h / (p.heads / p.shared), q0 = qt * 128, half = warp >> 2, row = threadIdx.x & 127;
   const float* tokens = p.key ? p.key + (long long)n * p.tk : nullptr;
   const long long q_row = (long long)p.heads * p.d;
@@ -885,7 +884,7 @@ struct StateControl {
 static_assert(sizeof(StateControl) <= StateShape<64>::ROWS_AT, "");
 
 template <int D>
-__global__ void __launch_bounds__(BLOCK, 1) grad_of_states(const Problem p) {
+__device__ __forceinline__ void grad_of_states(const Problem& p, const int block) {
   using Shape = StateShape<D>;
   using LQ = typename Shape::LQ;
   using LK = typename Shape::LK;
@@ -915,8 +914,8 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_states(const Problem p) {
     tmem_alloc(&bar->tmem, 512);
     tmem_relinquish();
   }
-  if (!p.together) tsb_launch::enter();
-  const int kt = blockIdx.x % p.ktiles, shared = blockIdx.x / p.ktiles % p.shared, n = blockIdx.x / p.ktiles / p.shared;
+  tsb_launch::enter();
+  const int kt = block % p.ktiles, shared = block / p.ktiles % p.shared, n = block / p.ktiles / p.shared;
   const int k0 = kt * 128, per = p.heads / p.shared, halves = (p.tq + 63) / 64;
   const float* tokens = p.key ? p.key + (long long)n * p.tk : nullptr;
   const long long kv_row = 2ll * p.shared * p.d, k_at = ((long long)n * p.shared + shared) * p.ktiles + kt;
@@ -1064,8 +1063,21 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_of_states(const Problem p) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (p.together) tsb_launch::wait_previous();
   if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+// The first `query_blocks` blocks compute gradients of queries, the others those of states.  Neither reads what the other writes, so
+// in one launch the latter take the SMs that the last of the former leave idle (32 x 255 x 256, 8 heads of 64: 75 us, two
+// launches 84; 1 x 512 x 512, 4 heads: 16.5 and 27.7).  Two kernels, the second of which does not wait for the
+// first, would need what stands before the first to be visible to a grid that has waited for nobody, which nothing promises.
+template <int D> constexpr int gradients_smem() {
+  return QueryShape<D>::SMEM > StateShape<D>::SMEM ? QueryShape<D>::SMEM : StateShape<D>::SMEM;
+}
+template <int D>
+__global__ void __launch_bounds__(BLOCK, 1) gradients(const Problem p) {
+  const int block = blockIdx.x;
+  if (block < p.query_blocks) grad_of_queries<D>(p, block);
+  else grad_of_states<D>(p, block - p.query_blocks);
 }
 
 // ------------------------------------------------------------------------------------------------ single tokens
@@ -1455,41 +1467,26 @@ int forward(const float* q, const float* kv, const float* key, float* y, float* 
   return run(attend<128>, p, blocks, ForwardShape<128>::SMEM, st, limit128);
 }
 
-int grad_q(const void* prepared, long long have, const float* key, const float* lse, float* dq, int n, int tq, int tk, int heads, int shared, int d,
-           float scale, void* stream, bool together) {
+// The gradients that are asked for: of the queries (dq), of the states (dkv), or both.
+int grads(const void* prepared, long long have, const float* key, const float* lse, float* dq, float* dkv, int n, int tq, int tk, int heads, int shared,
+          int d, float scale, void* stream) {
   Problem p;
-  if (!describe(p, n, tq, tk, heads, shared, d, scale, nullptr, nullptr, key, dq)) return TSB_ERR_ARG;
-  if (n == 0 || tq == 0) return TSB_OK;
+  if (!describe(p, n, tq, tk, heads, shared, d, scale, nullptr, nullptr, key, dq, dkv)) return TSB_ERR_ARG;
+  const long long queries = dq ? (long long)n * heads * p.qtiles : 0, states = dkv ? (long long)n * shared * p.ktiles : 0;
+  if (queries + states == 0) return TSB_OK;
   const Layout at(n, tq, tk, heads, shared, d, true);
-  if (!lse || (reinterpret_cast<uintptr_t>(lse) & 15) || !dq || !fits(prepared, have, at)) return TSB_ERR_ARG;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((tq && !lse) || (reinterpret_cast<uintptr_t>(lse) & 15) || !fits(prepared, have, at)) return TSB_ERR_ARG;
+  if ((long long)((tq + 63) / 64) * (heads / shared) > INT32_MAX / 2) return TSB_ERR_ARG;
+  if (queries > INT32_MAX || queries + states > INT32_MAX) return TSB_ERR_ARG;
   use(p, at, static_cast<const char*>(prepared));
   p.lse = const_cast<float*>(lse);
   p.dq = dq;
-  p.together = together;
-  const long long blocks = (long long)n * heads * p.qtiles;
-  static tsb_launch::SmemLimit limit64, limit128;
-  if (d <= 64) return run(grad_of_queries<64>, p, blocks, QueryShape<64>::SMEM, st, limit64);
-  return run(grad_of_queries<128>, p, blocks, QueryShape<128>::SMEM, st, limit128);
-}
-
-int grad_kv(const void* prepared, long long have, const float* key, const float* lse, float* dkv, int n, int tq, int tk, int heads, int shared, int d,
-            float scale, void* stream, bool together) {
-  Problem p;
-  if (!describe(p, n, tq, tk, heads, shared, d, scale, nullptr, nullptr, key, dkv)) return TSB_ERR_ARG;
-  if (n == 0 || tk == 0) return TSB_OK;
-  const Layout at(n, tq, tk, heads, shared, d, true);
-  if (!dkv || (tq && !lse) || (reinterpret_cast<uintptr_t>(lse) & 15) || !fits(prepared, have, at)) return TSB_ERR_ARG;
-  if ((long long)((tq + 63) / 64) * (heads / shared) > INT32_MAX / 2) return TSB_ERR_ARG;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  use(p, at, static_cast<const char*>(prepared));
-  p.lse = const_cast<float*>(lse);
   p.dkv = dkv;
-  p.together = together;
-  const long long blocks = (long long)n * shared * p.ktiles;
+  p.query_blocks = (int)queries;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
   static tsb_launch::SmemLimit limit64, limit128;
-  if (d <= 64) return run(grad_of_states<64>, p, blocks, StateShape<64>::SMEM, st, limit64);
-  return run(grad_of_states<128>, p, blocks, StateShape<128>::SMEM, st, limit128);
+  if (d <= 64) return run(gradients<64>, p, queries + states, gradients_smem<64>(), st, limit64);
+  return run(gradients<128>, p, queries + states, gradients_smem<128>(), st, limit128);
 }
 
 }  // namespace
@@ -1535,23 +1532,21 @@ int tsb_cross_attention_prepare(const float* q, const float* kv, const float* ke
 
 int tsb_cross_attention_grad_q(const void* prepared, long long have, const float* key, const float* lse, float* dq, int n, int tq, int tk, int heads,
                                int shared, int d, float scale, void* stream) {
-  return grad_q(prepared, have, key, lse, dq, n, tq, tk, heads, shared, d, scale, stream, false);
+  if (!dq && n > 0 && tq > 0) return TSB_ERR_ARG;
+  return grads(prepared, have, key, lse, dq, nullptr, n, tq, tk, heads, shared, d, scale, stream);
 }
 
 int tsb_cross_attention_grad_kv(const void* prepared, long long have, const float* key, const float* lse, float* dkv, int n, int tq, int tk, int heads,
                                 int shared, int d, float scale, void* stream) {
-  return grad_kv(prepared, have, key, lse, dkv, n, tq, tk, heads, shared, d, scale, stream, false);
+  if (!dkv && n > 0 && tk > 0) return TSB_ERR_ARG;
+  return grads(prepared, have, key, lse, nullptr, dkv, n, tq, tk, heads, shared, d, scale, stream);
 }
 
-// Both.  The second kernel reads nothing of the first, so its blocks take the SMs that the first one's last blocks leave idle: the
-// first lets it be placed once all its own blocks run, which is behind their wait for what both of them read; the second waits
-// for the first at its end, so that what comes next finds both done.  (32 x 255 x 256, 8 heads of 64: 76 us, one
-// after the other 84; 1 x 512 x 512, 4 heads: 17 and 27.)
+// Both, in one launch.
 int tsb_cross_attention_grads(const void* prepared, long long have, const float* key, const float* lse, float* dq, float* dkv, int n, int tq, int tk,
                               int heads, int shared, int d, float scale, void* stream) {
-  const bool together = n > 0 && tq > 0 && tk > 0;
-  const int rc = grad_q(prepared, have, key, lse, dq, n, tq, tk, heads, shared, d, scale, stream, together);
-  return rc ? rc : grad_kv(prepared, have, key, lse, dkv, n, tq, tk, heads, shared, d, scale, stream, together);
+  if ((!dq && n > 0 && tq > 0) || (!dkv && n > 0 && tk > 0)) return TSB_ERR_ARG;
+  return grads(prepared, have, key, lse, dq, dkv, n, tq, tk, heads, shared, d, scale, stream);
 }
 
 }  // extern "C"

@@ -16,7 +16,7 @@ come from class ids (the same sum, added up in another order):
 * of two convolutions' gradients that only their sum reads, the first is written where the sum goes, and the other, if its
   stride is 2, adds itself to it;
 * a cross attention's forward pass leaves the pieces of its operands where its gradients look for them;
-* the gradients of a cross attention's queries and states go in one call, so that one's blocks run beside the other's last.
+* the gradients of a cross attention's queries and states are one launch, so that one's blocks run beside the other's last.
 
 Element-wise nodes are taken as soon as their inputs are there, the others in creation order, and nothing moves past a
 node with effects of its own (an optimizer update, a collective, a swap).  The memory-planning executors have

@@ -418,7 +418,7 @@ def cross_attention_grad_kv(prepared, key, lse, dkv, sizes, scale, stream):
 
 
 def cross_attention_grads(prepared, key, lse, dq, dkv, sizes, scale, stream):
-    """Both gradients, the second one's blocks beside the last ones of the first."""
+    """Both gradients in one launch, the second one's blocks beside the last ones of the first."""
     _dense_rows("cross_attention_gradient", prepared, lse, dq, dkv, *([key] if key is not None else []))
     _room_for_rows(lse, sizes)
     with _on_device(dq):
