@@ -1,4 +1,5 @@
-"""Token scores and their gradient at the borders of fp32: logits masked by the type's lowest value under large weights."""
+"""Token scores and their gradient at the borders of fp32: logits masked by the type's lowest value under large weights, and
+tokens that are nearly certain."""
 import numpy as np
 import pytest
 
@@ -66,3 +67,34 @@ def test_gradients_of_logits_masked_by_the_lowest_number(rows, v, weight, ctx):
     # p is off by some 20 steps (sums of 20000 terms in fixed groups, a fast exponential), and the factors of p are at most
     # |g| + |weight| (|log p| + H) <= 4 + |weight| (20 + 10)
     assert np.abs(dx - want).max() <= 64 * HALF * (4 + abs(weight) * 30)
+
+
+@pytest.mark.parametrize("v", [30, 1000, 3000, 10000, 32000, 40000])
+@pytest.mark.parametrize("rows", [2, 160])
+@pytest.mark.parametrize("high", [12.0, 16.0, 20.0, 25.0, 90.0])
+@pytest.mark.parametrize("at", [0.0, 1000.0])
+def test_tokens_that_are_nearly_certain(v, rows, high, at, ctx):
+    """log p of a token with p near 1 is off by a few steps of 1, not by steps of its logit, and so is 1 - p in its gradient:
+    the row of the gradient adds up to nothing."""
+    x = np.full((rows, v), at, np.float32)
+    x[:, v // 3] = at + high
+    x[:, 5] = at + 1
+    ids = np.full(rows, v // 3, np.float32)
+    g = np.zeros((rows, 3 + 2 * 2), np.float32)
+    g[:, 0] = 1
+    g[1::2, 0], g[1::2, 3] = 0, 1                                      # as the given token, and as the likeliest one
+    out, dx = scores(x, ids, g, 2, ctx)
+    lp, best, cols, want = definition(x, ids, g, 2)
+    # Z in [1, 2): a sum of up to 32 terms of a thread (of long rows: v / 256), then some 24 joins, each off by 2^-24; fast
+    # exponentials are off by 2 + 1.2 |u| steps of what the others add; log p at the maximum is -log Z, rounded once
+    rest = np.expm1(-lp)[:, None]
+    step = HALF * (64 + v / 256 + (8 + 3 * high) * rest)
+    assert np.all(np.abs(out[:, 0] - lp) <= step[:, 0] + 2 * HALF * np.abs(lp))
+    assert np.all(np.abs(out[:, 3] - best[:, 0]) <= step[:, 0] + 2 * HALF * np.abs(best[:, 0]))
+    assert np.all(np.abs(out[:, 4] - best[:, 1]) <= step[:, 0] + 8 * HALF * np.abs(best[:, 1]))
+    own = dx[np.arange(rows), v // 3]
+    assert np.all(np.abs(own - want[np.arange(rows), v // 3]) <= step[:, 0] + 8 * HALF * np.abs(own))
+    # the others: p from logit - log-sum-exp, which is off by half a step of the largest
+    rel = HALF * (80 + 4 * (abs(at) + high) + v / 256)
+    others = np.delete(np.arange(v), v // 3)
+    assert np.all(np.abs(dx[:, others] - want[:, others]) <= rel * np.abs(want[:, others]) + 1e-37)

@@ -1,8 +1,10 @@
 // Log probabilities of given tokens, with the entropy of each row, its log-sum-exp and the `top` likeliest tokens.
 //
 //   out[r] = [ log p(id_r), H, lse, log p of the top tokens (falling), their ids ],   p = softmax(x[r, :])
-//   H = log Z - sum(e^u u) / Z   with u = x - max, Z = sum e^u
+//   H = log Z - sum(e^u u) / Z,  log p = u - log Z   with u = x - max, Z = sum e^u
 //
+// (log p = x - lse would lose what lies below half a step of the maximum, which is all there is of a token that is nearly
+// certain.)
 // An id outside [0, cols) means no token: 0.  A row of -inf alone has lse = log p = -inf and H = 0, and no gradient.  NaN
 // makes the row's results NaN and is no alternative itself (id -1 where fewer than `top` others are left).  Equal logits are
 // taken by their column, the lowest first.
@@ -117,6 +119,8 @@ __device__ __forceinline__ float take(Sums& s, const float (&x)[N]) {
   return m;
 }
 
+__device__ __forceinline__ float log_p(float x, float max, float log_z) { return (x - max) - log_z; }
+
 __device__ __forceinline__ float warp_max(float v) {     // of numbers: a NaN counts as none
   float r;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
@@ -135,7 +139,7 @@ struct Shared {
   float least[MAX_WARPS];      // what each warp has as many units above as it has to
   float reached[REACHED], refined;           // maxima of the units that reach the first bound; the second bound
   unsigned units, count;       // how many these are; columns found
-  float lse;                   // of the row; NaN-free rows of -inf: -inf
+  float lse, max, log_z;       // of the row; NaN-free rows of -inf: lse is -inf
   Sums sums[MAX_WARPS];
   Sums of_block;
 };
@@ -306,8 +310,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 6) score_rows(const float* x, 
     const bool empty = r.m == NEG_INF && r.z == 0.f;                            // (NaN leaves z a NaN)
     const double z = (double)r.z, log_z = log(z);
     const float lse = empty ? NEG_INF : r.m + (float)log_z;
-    s.lse = lse;
-    to[0] = given ? (empty ? NEG_INF : own_x - lse) : 0.f;
+    s.lse = lse, s.max = r.m, s.log_z = (float)log_z;
+    to[0] = given ? (empty ? NEG_INF : log_p(own_x, r.m, (float)log_z)) : 0.f;
     to[1] = empty ? 0.f : (float)(log_z - (double)r.t / z);
     to[2] = lse;
   };
@@ -324,7 +328,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 6) score_rows(const float* x, 
   if (!TOP && split == 1) return;
   auto write = [&](unsigned at, u64 key) {   // an alternative of the row
     if ((int)at >= top) return;
-    to[3 + at] = s.lse == NEG_INF ? NEG_INF : logit_of(key) - s.lse;
+    to[3 + at] = s.lse == NEG_INF ? NEG_INF : log_p(logit_of(key), s.max, s.log_z);
     to[3 + top + at] = (float)col_of(key);
   };
   auto fill = [&](unsigned there) {          // fewer numbers than alternatives
@@ -439,7 +443,7 @@ __global__ void __launch_bounds__(WARPS > SHORT_WARPS ? WARPS * 32 : SHORT_WARPS
   constexpr int ROWS = WARPS == 1 ? SHORT_WARPS : 1, ROOM = WARPS == 1 ? SHORT_FOUND : FOUND;
   __shared__ u64 found[TOP ? ROWS : 1][ROOM], best_of[WARPS];
   __shared__ Sums sums[WARPS];
-  __shared__ float leasts[WARPS], lse_of_row;
+  __shared__ float leasts[WARPS], lse_of_row, max_of_row, log_z_of_row;
   __shared__ int all;
   const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5, own_row = WARPS == 1 ? threadIdx.x >> 5 : 0;
   const long long row = blockIdx.x * (long long)ROWS + own_row;
@@ -486,16 +490,17 @@ __global__ void __launch_bounds__(WARPS > SHORT_WARPS ? WARPS * 32 : SHORT_WARPS
         a = join(a, Sums{__shfl_xor_sync(ALL, a.m, d), __shfl_xor_sync(ALL, a.z, d), __shfl_xor_sync(ALL, a.t, d)});
     }
   }
-  float lse = 0.f;
+  float lse = 0.f, log_z = 0.f;
   if (warp == WARPS - 1) {
     const bool empty = a.m == NEG_INF && a.z == 0.f;
-    const double log_z = log((double)a.z);
-    lse = empty ? NEG_INF : a.m + (float)log_z;
+    const double wide = log((double)a.z);
+    log_z = (float)wide;
+    lse = empty ? NEG_INF : a.m + log_z;
     if (lane == 0) {
-      to[0] = given ? (empty ? NEG_INF : own_x - lse) : 0.f;
-      to[1] = empty ? 0.f : (float)(log_z - (double)a.t / (double)a.z);
+      to[0] = given ? (empty ? NEG_INF : log_p(own_x, a.m, log_z)) : 0.f;
+      to[1] = empty ? 0.f : (float)(wide - (double)a.t / (double)a.z);
       to[2] = lse;
-      if (WARPS > 1) lse_of_row = lse;
+      if (WARPS > 1) lse_of_row = lse, max_of_row = a.m, log_z_of_row = log_z;
     }
   }
   if (!TOP) return;
@@ -523,9 +528,9 @@ __global__ void __launch_bounds__(WARPS > SHORT_WARPS ? WARPS * 32 : SHORT_WARPS
     keys[at] = order_of(load(xr + i), first + i);
   }
   sync();
-  if (WARPS > 1) count = all, lse = lse_of_row;
+  if (WARPS > 1) count = all, lse = lse_of_row, a.m = max_of_row, log_z = log_z_of_row;
   auto write = [&](int place, u64 key) {
-    to[3 + place] = !key ? __int_as_float(0x7fc00000) : lse == NEG_INF ? NEG_INF : logit_of(key) - lse;
+    to[3 + place] = !key ? __int_as_float(0x7fc00000) : lse == NEG_INF ? NEG_INF : log_p(logit_of(key), a.m, log_z);
     to[3 + top + place] = key ? (float)col_of(key) : -1.f;
   };
   if (count <= ROOM) {
@@ -567,8 +572,8 @@ int short_rows(const float* x, const float* ids, float* out, long long rows, int
 }
 
 // dx_c = sum_i w_i (1[c = id_i] - p_c) + w_lse p_c - w_H p_c (log p_c + H), with w the gradient of `out` and the sum over
-// the given token and the top ones, of which each lane of a warp has one.  Columns that are an id are computed apart, with 1 - p as
-// -expm1(log p), after the rest.  Columns [begin, end) of a row, by `threads` threads that `sync` is for.
+// the given token and the top ones, of which each lane of a warp has one.  Columns that are an id are computed apart, from the log p
+// of `out` and with 1 - p as -expm1(log p), after the rest.  Columns [begin, end) of a row, by `threads` threads that `sync` is for.
 template <class Sync>
 __device__ __forceinline__ void grad_of_columns(const float* xr, const float* o, const float* w, float* dr, long long id, long long cols, int top,
                                                 unsigned begin, unsigned end, unsigned thread, unsigned threads, Sync sync) {
@@ -599,15 +604,15 @@ __device__ __forceinline__ void grad_of_columns(const float* xr, const float* o,
   for (unsigned i = tail + thread; i < end; i += threads) dr[i] = rest(load(xr + i));
   sync();                                // the columns below are written a second time
   if (thread >= 32 || empty) return;
-  auto of_id = [&](long long col, float own) {
+  auto of_id = [&](long long col, float lp, float own) {
     if (col < (long long)begin || col >= (long long)end) return;
-    const float v = load(xr + col), lp = v - lse, p = expf(lp);
-    const float other = v == NEG_INF || p == 0.f ? 0.f : p * (load(w + 2) - (weights - own) - wh * (lp + entropy));
+    const float p = expf(lp);
+    const float other = p == 0.f ? 0.f : p * (load(w + 2) - (weights - own) - wh * (lp + entropy));
     dr[col] = own * -expm1f(lp) + other;
   };
-  of_id(alternative, w_alternative + (given && alternative == id ? w_given : 0.f));
+  of_id(alternative, lane < top ? load(o + 3 + lane) : 0.f, w_alternative + (given && alternative == id ? w_given : 0.f));
   const bool both = __any_sync(ALL, alternative == id);                         // the lane of that one has done it
-  if (lane == 0 && given && !both) of_id(id, w_given);
+  if (lane == 0 && given && !both) of_id(id, load(o), w_given);
 }
 
 // A block takes a chunk of a row.
