@@ -4,6 +4,7 @@ import gc
 
 import numpy as np
 import pytest
+import torch
 
 from tsplit_b200 import ndarray, gpu_ops as ad
 from tsplit_b200.ops import _gpu as G, attention as A
@@ -134,3 +135,50 @@ def test_too_few_log_sum_exps_are_refused(tq, shape):
                  lambda: G.cross_attention_grads(flat, None, lse, q, kv, sizes, 1.0, None)]:
         with pytest.raises(ValueError, match="log-sum-exps"):
             call()
+
+
+# ------------------------------------------------------------------------------------------------ launches
+@pytest.mark.gpu
+def test_launches_are_counted():
+    """Every entry's count against the kernels that a capture of it holds: never more, and the same where no size decides."""
+    from cuda.bindings import runtime as cudart
+    from tsplit_b200.utils import launch_counter
+    ctx = ndarray.gpu(0)
+    st, e = create_stream_handle(ctx), lambda *s: ndarray.empty(s, ctx, channels_last=False)
+    sizes = (2, 20, 30, 2, 2, 16)
+    q, kv, key, y, dq, dkv, lse, flat = (e(2, 20, 2, 16), e(2, 30, 2, 2, 16), e(2, 30), e(2, 20, 2, 16), e(2, 20, 2, 16), e(2, 30, 2, 2, 16),
+                                         e(2, 2, 128), e(A._prepared_floats(*sizes)))
+    table, ids, rows = e(50, 16), e(600), e(600, 16)
+    x, of_rows, out, g, dx = e(20, 100), e(20), e(20, 5), e(20, 5), e(20, 100)
+
+    def real(call):
+        def ok(r):
+            assert int(r[0]) == 0
+            return r[1] if len(r) > 1 else None
+        call()                                                     # (scratch is there)
+        st.sync()
+        ok(cudart.cudaStreamBeginCapture(st.handle, cudart.cudaStreamCaptureMode.cudaStreamCaptureModeThreadLocal))
+        before = launch_counter.count()
+        call()
+        counted = launch_counter.count() - before
+        captured = ok(cudart.cudaStreamEndCapture(st.handle))
+        r = cudart.cudaGraphGetNodes(captured)
+        r = cudart.cudaGraphGetNodes(captured, r[-1])
+        kernels = sum(ok(cudart.cudaGraphNodeGetType(n)) == cudart.cudaGraphNodeType.cudaGraphNodeTypeKernel for n in r[1])
+        ok(cudart.cudaGraphDestroy(captured))
+        return counted, kernels
+    for a in (q, kv, y, lse, flat, x, out, g, rows, table):
+        a.t.zero_()
+    for a in (key, ids, of_rows):
+        a.t.fill_(1.0)
+    torch.cuda.synchronize()
+    for call in [lambda: G.cross_attention(q, kv, key, y, lse, sizes, 1.0, st, flat), lambda: G.cross_attention_prepare_g(q, y, flat, sizes, st),
+                 lambda: G.cross_attention_prepare(q, kv, key, q, y, flat, sizes, 1.0, st), lambda: G.cross_attention_grad_q(flat, key, lse, dq, sizes, 1.0, st),
+                 lambda: G.cross_attention_grad_kv(flat, key, lse, dkv, sizes, 1.0, st),
+                 lambda: G.cross_attention_grads(flat, key, lse, dq, dkv, sizes, 1.0, st), lambda: G.scaled_embedding(table, ids, rows, 1.0, st),
+                 lambda: G.token_score(x, of_rows, out, 1, st), lambda: G.token_score_grad(x, of_rows, out, g, dx, st)]:
+        counted, kernels = real(call)
+        assert counted == kernels
+    for call in [lambda: G.cross_attention(q, kv, key, y, lse, sizes, 1.0, st), lambda: G.scaled_embedding_grad(rows, ids, table, 1.0, None, st)]:
+        counted, kernels = real(call)
+        assert 1 <= counted <= kernels
