@@ -20,7 +20,7 @@ def extra(p):
     p.add_argument("--dropout_rate", type=float, default=0.0)
     p.add_argument("--lr", type=float, default=0.0003)
     p.add_argument("--scaled_embedding", type=int, default=0, help="1: lookup and scale of the tokens in one operator")
-    p.add_argument("--cross_attention", type=int, default=0, help="1: the decoder's attention over the encoder in one operator")
+    p.add_argument("--cross_attention", type=int, default=0, help="1: the decoder's attention over the encoder in one operator (without dropout)")
 
 
 def run(batch_size, args, ctx):

@@ -28,8 +28,10 @@ class TransformerConfig(object):
         #: without any (``ad.scaled_embedding_op``)
         self.scaled_embedding = bool(scaled_embedding)
         #: the decoder's attention over the encoder's states as one operator that keeps no scores and fp32 accuracy; keys and
-        #: values come from one projection ``<name>_kv`` (``ad.cross_attention_op``; not with dropout of the probabilities)
-        self.cross_attention = bool(cross_attention) and not dropout_rate
+        #: values come from one projection ``<name>_kv`` (``ad.cross_attention_op``, which has no dropout of the probabilities)
+        self.cross_attention = bool(cross_attention)
+        if self.cross_attention and dropout_rate:
+            raise ValueError("cross_attention=True has no dropout of its probabilities: dropout_rate is to be 0, not %s" % dropout_rate)
 
 
 class TransformerModel(object):
