@@ -182,3 +182,25 @@ def test_launches_are_counted():
     for call in [lambda: G.cross_attention(q, kv, key, y, lse, sizes, 1.0, st), lambda: G.scaled_embedding_grad(rows, ids, table, 1.0, None, st)]:
         counted, kernels = real(call)
         assert 1 <= counted <= kernels
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,tq,tk,h,s,d", [(2, 200, 300, 4, 2, 64), (1, 129, 130, 3, 1, 80), (3, 9, 1, 1, 1, 8), (2, 1, 300, 4, 4, 64)])
+def test_what_a_forward_pass_takes_outside_of_the_step(n, tq, tk, h, s, d):
+    import ctypes
+    from tsplit_b200 import _base
+    ctx = ndarray.gpu(0)
+    v, y, _ = graph()
+    f = feeds(v, 1, n=n, tq=tq, tk=tk, h=h, d=d)
+    f[v["kv"]] = np.ascontiguousarray(f[v["kv"]][:, :, :, :s])
+    handle, held = ctypes.c_void_p(), _base.kernels().tsb_scratch_bytes
+    held.restype = ctypes.c_longlong
+    assert int(torch.cuda.cudart().cudaStreamCreate(ctypes.addressof(handle))) == 0        # (torch's streams come from a pool)
+    ex = ad.StreamExecutor([y], ctx=ctx, stream=Stream(ctx, torch_stream=torch.cuda.ExternalStream(handle.value)))
+    gc.collect()
+    torch.cuda.synchronize()
+    _base.kernels().tsb_scratch_trim()                               # (given-back buffers would be taken)
+    before = held()
+    ex.run(f)
+    rows = sum(a.nbytes for a in y.state.values() if isinstance(a, ndarray.NDArray))
+    assert rows + held() - before == y.op.workspace_bytes(y, [f[i].shape for i in y.inputs], f[v["q"]].shape)

@@ -91,6 +91,16 @@ class CrossAttentionOp(Op):
     def flops(self, node, s, out):
         return 4.0 * np.prod(s[0]) * s[1][1]
 
+    def workspace_bytes(self, node, s, out):
+        """The pieces of the operands, scratch of the stream outside any pool (where a step plan keeps them for the gradients, they lie
+        in an array of the step instead); and the log-sum-exps."""
+        n, tq, tk, h, shared, d = _sizes(s[0], s[1])
+        rows = 4 * n * h * _whole_tiles(tq)
+        if not keeps_operands(s[0], s[1]):
+            return rows
+        q, k = n * h * _whole_tiles(tq) // 128, n * shared * _whole_tiles(tk) // 128
+        return rows + 4 * _prepared_floats(n, tq, tk, h, shared, d) - q * (128 * (64 if d <= 64 else 128) * 4 + 128 * 4) - -(-q // 2) * 16
+
 
 _NO_STREAM = Buffers()
 
