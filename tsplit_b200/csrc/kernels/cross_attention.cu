@@ -42,7 +42,7 @@ struct Pieces {
 };
 
 struct Problem {
-  const float *q, *kv, *key, *dot;
+  const float *q, *kv, *key, *dot, *lengths;
   float *y, *lse, *dq, *dkv;
   Pieces qp, kp, vp, gp;
   int n, tq, tk, heads, shared, d;
@@ -85,7 +85,7 @@ struct Source {
   const float* x;
   const float* with;                         // an array like x: dots[n, head, tile, row] = sum of x with over a row; or null
   const float* tokens;                       // [n][t], a row whose token is 0 counts as zeros and is not read; or null
-  float* dots;
+  float *dots, *lengths;                     // with `with`: lengths[n, head, tile, row]
   char* tiles;
   float2* units;
   long long batch, row, head;                // strides
@@ -147,20 +147,24 @@ __global__ void __launch_bounds__(256) split_tiles(const Sources all) {
     }
   }
   uint32_t most = 0, most_squares = 0;
+  float squares[TRIPS];
 #pragma unroll
   for (int u = 0; u < TRIPS; ++u) {
-    float squares = 0.f;
+    squares[u] = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       v[u][k] *= s.mult;
       const uint32_t size = __float_as_uint(v[u][k]) & 0x7fffffffu;
       if (size < 0x7f800000u) most = max(most, size);
-      squares += v[u][k] * v[u][k];
+      squares[u] += v[u][k] * v[u][k];
     }
 #pragma unroll
-    for (int o = UNITS / 2; o > 0; o >>= 1) squares += __shfl_xor_sync(ALL, squares, o);
-    most_squares = max(most_squares, __float_as_uint(squares));
+    for (int o = UNITS / 2; o > 0; o >>= 1) squares[u] += __shfl_xor_sync(ALL, squares[u], o);
+    most_squares = max(most_squares, __float_as_uint(squares[u]));
   }
+  if (s.with && threadIdx.x % UNITS == 0)
+#pragma unroll
+    for (int u = 0; u < TRIPS; ++u) s.lengths[(size_t)b * 128 + (threadIdx.x + u * 256) / UNITS] = sqrtf(squares[u]);
   most = __reduce_max_sync(ALL, most);
   most_squares = __reduce_max_sync(ALL, most_squares);
   if ((threadIdx.x & 31) == 0) largest[threadIdx.x >> 5] = most, longest[threadIdx.x >> 5] = most_squares;
@@ -666,15 +670,19 @@ __global__ void __launch_bounds__(BLOCK, 1) attend(const Problem p) {
 }
 
 // ------------------------------------------------------------------------------------------------ gradients
-// A bound of |dP - dot| over a tile: e with (|g| |v| + |dot|) 2^e below 2^15, |g| and |v| the lengths of the longest rows.
+// A bound of |dP - dot| over rows: e with (|g| |v| + |dot|) 2^e below 2^15, |g| and |v| the lengths of the longest ones.
 __device__ __forceinline__ int exponent_of_ds(float g_length, float v_length, float dot) {
   const float most = 1.001f * (g_length * v_length) + fabsf(dot);
   return exponent_to(__float_as_uint(most), TOP + 1);
 }
 
 // dq: a block takes 128 queries of a head and tiles of 64 keys; the same roles.  The queries, and with 64 columns their gradients
-// too, are kept in tensor memory, else these lie before the ring.  dS takes the place of its S.  The cases of attend: 459, 235 and 34
-// us (a row to a thread, two blocks to an SM, operands in shared memory: 672, 301 and 32).
+// too, are kept in tensor memory, else these lie before the ring.  dS takes the place of its S.  A row's dS is bounded by the length
+// of its own g: gradients differ much from row to row (a token that is all but certain has next to none), and each has a row of dq to
+// itself.  (100 queries, 130 keys, one row of g 2^20 times its neighbours: bounded by the longest of all rows, dq of these was off by
+// 2e-3 of its largest number, and by more the more keys there are; now 1.2e-5, which is what pieces of g keep.  2^16 times: 1.4e-6, as
+// without it.)  The cases of attend: 459, 235 and 34 us (a row to a thread, two blocks to an SM, operands in shared memory: 672, 301
+// and 32).
 template <int D> struct QueryShape {
   static constexpr bool BOTH = D == 64;
   static constexpr int K_SLOTS = BOTH ? 4 : 3, V_SLOTS = BOTH ? 4 : 2, SLOTS = K_SLOTS + V_SLOTS;
@@ -749,6 +757,7 @@ __device__ __forceinline__ void grad_of_queries(const Problem& p, const int bloc
     const float lse = load(p.lse + q_at * 128 + row), dot = load(p.dot + q_at * 128 + row);
     const float q_unit = load(p.qp.units + q_at).x;
     const float2 g_unit = load(p.gp.units + q_at);
+    const float own = load(p.lengths + q_at * 128 + row), length = own < 1e15f && own > 1e-15f ? own : g_unit.y;
     bool ok = true;
     auto add_tile = [&](int j) {
       if (!mbar_wait(&bar->dq_full, j & 1, p.status, 0x311)) return false;
@@ -769,7 +778,7 @@ __device__ __forceinline__ void grad_of_queries(const Problem& p, const int bloc
       const float k_unit = k_next;
       const float2 v_unit = v_next;
       look_at(j + 1);
-      const int e = exponent_of_ds(g_unit.y, v_unit.y, dot);
+      const int e = exponent_of_ds(length, v_unit.y, dot);
       // (2^e is not in the exponent, whose rounding it would make coarser)
       const float f = power_of_two(e), s_unit = q_unit * k_unit, dp_unit = g_unit.x * v_unit.x * f, dot_unit = dot * f;
       if (!mbar_wait(&bar->s_full[b], j >> 1 & 1, p.status, 0x312)) { ok = false; break; }
@@ -1344,9 +1353,9 @@ int run(K kernel, const Problem& p, long long blocks, int smem, cudaStream_t st,
   return launched(e);
 }
 
-// Where the pieces of q, k, v and g lie in one buffer, behind them the units and the dots.
+// Where the pieces of q, k, v and g lie in one buffer, behind them the units, and the dots and the lengths of the rows of g.
 struct Layout {
-  size_t tiles[4], units[4], dots, bytes;      // (units and dots on 16-byte boundaries: they are copied in bulk)
+  size_t tiles[4], units[4], dots, lengths, bytes;             // (units and dots on 16-byte boundaries: they are copied in bulk)
   Layout(int n, int tq, int tk, int heads, int shared, int d, bool with_g) {
     const size_t tile = d <= 64 ? Tile<64, 128>::BYTES : Tile<128, 128>::BYTES;
     const size_t q = (size_t)n * heads * ((tq + 127) / 128), k = (size_t)n * shared * ((tk + 127) / 128);
@@ -1361,7 +1370,8 @@ struct Layout {
       bytes += (count[i] * 8 + 15) / 16 * 16;
     }
     dots = bytes;
-    bytes += count[3] * 128 * 4;
+    lengths = dots + count[3] * 128 * 4;
+    bytes = lengths + count[3] * 128 * 4;
   }
   Pieces of(const char* base, int i) const { return {base + tiles[i], reinterpret_cast<const float2*>(base + units[i])}; }
 };
@@ -1374,6 +1384,7 @@ void use(Problem& p, const Layout& at, const char* base) {
   p.vp = at.of(base, 2);
   p.gp = at.of(base, 3);
   p.dot = reinterpret_cast<const float*>(base + at.dots);
+  p.lengths = reinterpret_cast<const float*>(base + at.lengths);
 }
 
 // Splits q, k and v where they are given, and g (with the dots).
@@ -1400,6 +1411,7 @@ int split(const Problem& p, const float* g, const float* y, const Layout& at, ch
     if (i == 3) {
       s.with = y;
       s.dots = reinterpret_cast<float*>(base + at.dots);
+      s.lengths = reinterpret_cast<float*>(base + at.lengths);
     }
     all.first[i] = (int)blocks;
     if (i < 3 ? states : g != nullptr) blocks += (long long)p.n * s.heads * s.count;

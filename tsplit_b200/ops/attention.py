@@ -99,7 +99,7 @@ class CrossAttentionOp(Op):
         if not keeps_operands(s[0], s[1]):
             return rows
         q, k = n * h * _whole_tiles(tq) // 128, n * shared * _whole_tiles(tk) // 128
-        return rows + 4 * _prepared_floats(n, tq, tk, h, shared, d) - q * (128 * (64 if d <= 64 else 128) * 4 + 128 * 4) - -(-q // 2) * 16
+        return rows + 4 * _prepared_floats(n, tq, tk, h, shared, d) - q * (128 * (64 if d <= 64 else 128) * 4 + 2 * 128 * 4) - -(-q // 2) * 16
 
 
 _NO_STREAM = Buffers()
@@ -133,9 +133,9 @@ def _whole_tiles(t):
 
 def _prepared_floats(n, tq, tk, h, shared, d):
     """Length of what the gradients read: tiles of 128 rows and 64 or 128 columns of q, k, v and g, two numbers for each, and
-    one for every row of g."""
+    two for every row of g."""
     q, k, columns = n * h * _whole_tiles(tq) // 128, n * shared * _whole_tiles(tk) // 128, 64 if d <= 64 else 128
-    return 128 * columns * 2 * (q + k) + 2 * (-(-q // 2) * 4 + -(-k // 2) * 4) + 128 * q
+    return 128 * columns * 2 * (q + k) + 2 * (-(-q // 2) * 4 + -(-k // 2) * 4) + 2 * 128 * q
 
 
 class CrossAttentionPrepareOp(Op):
