@@ -33,3 +33,18 @@ def test_gradients_of_queries_beside_one_far_larger(power, most, tk, d):
     want = definition(f["q"], f["kv"], None, d ** -0.5, f["g"])[0][1]
     off = np.abs(dq - want).max(3) / np.abs(want).max(3)
     assert off[0, 7, 0] <= 4e-6 and np.delete(off[0, :, 0], 7).max() <= most
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e-28, 1e-32, 1e-35])
+@pytest.mark.parametrize("tq,d", [(100, 64), (100, 128), (1, 64)])
+def test_gradients_of_next_to_nothing(size, tq, d):
+    """Gradients near the end of fp32 do not vanish: their pieces and dS keep 2^-19 of the largest number of a row at the least,
+    and some hundred of such errors add up."""
+    f = case(2, tq, 130, 2, 1, d, None, seed=2)
+    f["g"] = f["g"] * np.float32(size)
+    _, dq, dkv = evaluate(graph(False, None), f, ndarray.gpu(0))
+    want = definition(f["q"], f["kv"], None, d ** -0.5, f["g"])[0]
+    for got, w in ((dq, want[1]), (dkv[:, :, 0], want[2][:, :, 0]), (dkv[:, :, 1], want[2][:, :, 1])):
+        # (what is below 2^-126, of g or of a result, counts as 0 in every kernel)
+        assert np.abs(got - w).max() <= 1e-4 * np.abs(w).max() + 4 * 2.0 ** -126

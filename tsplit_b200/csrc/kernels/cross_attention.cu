@@ -67,11 +67,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
-// e with |x| 2^e in [2^top, 2^(top+1)), kept where 2^e and 2^-e are normal numbers (0 and tiny x: the largest)
-__device__ __forceinline__ int exponent_to(uint32_t bits_of_abs, int top) {
-  return min(top + 127 - (int)(bits_of_abs >> 23), 126);
+// e with |x| 2^e in [2^top, 2^(top+1)), kept where 2^e and 2^-e are normal numbers (0 and tiny x: `most`)
+__device__ __forceinline__ int exponent_to(uint32_t bits_of_abs, int top, int most = 126) {
+  return min(top + 127 - (int)(bits_of_abs >> 23), most);
 }
 constexpr int TOP = 13;                      // of a tile's largest number
+constexpr int LEAST = 112;                   // a tile's unit is 2^-LEAST at the least, and normal when P's scale divides it
 constexpr float LARGEST = 16384.f;           // and what that is below, 2^(TOP+1); P is scaled by it too
 
 // A tile of ROWS x D numbers in shared memory: the plane of the hi pieces, then that of the lo pieces; a plane is D / 64
@@ -171,7 +172,7 @@ __global__ void __launch_bounds__(256) split_tiles(const Sources all) {
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < 8; ++w) most = max(most, largest[w]), most_squares = max(most_squares, longest[w]);
-  const int e = exponent_to(most, TOP);
+  const int e = exponent_to(most, TOP, LEAST);
   const float scale = power_of_two(e);
   // (a row whose squares overflow, or vanish, or are NaN, has its largest number instead)
   if (threadIdx.x == 0) {
@@ -670,10 +671,11 @@ __global__ void __launch_bounds__(BLOCK, 1) attend(const Problem p) {
 }
 
 // ------------------------------------------------------------------------------------------------ gradients
-// A bound of |dP - dot| over rows: e with (|g| |v| + |dot|) 2^e below 2^15, |g| and |v| the lengths of the longest ones.
-__device__ __forceinline__ int exponent_of_ds(float g_length, float v_length, float dot) {
+// A bound of |dP - dot| over rows: e with (|g| |v| + |dot|) 2^e below 2^15, |g| and |v| the lengths of the longest ones.  2^-e times
+// `unit`, which what is made of dS is multiplied by, stays a normal number.
+__device__ __forceinline__ int exponent_of_ds(float g_length, float v_length, float dot, float unit) {
   const float most = 1.001f * (g_length * v_length) + fabsf(dot);
-  return exponent_to(__float_as_uint(most), TOP + 1);
+  return min(exponent_to(__float_as_uint(most), TOP + 1), (int)(__float_as_uint(unit) >> 23) - 1);
 }
 
 // dq: a block takes 128 queries of a head and tiles of 64 keys; the same roles.  The queries, and with 64 columns their gradients
@@ -778,9 +780,9 @@ __device__ __forceinline__ void grad_of_queries(const Problem& p, const int bloc
       const float k_unit = k_next;
       const float2 v_unit = v_next;
       look_at(j + 1);
-      const int e = exponent_of_ds(length, v_unit.y, dot);
+      const int e = exponent_of_ds(length, v_unit.y, dot, k_unit);
       // (2^e is not in the exponent, whose rounding it would make coarser)
-      const float f = power_of_two(e), s_unit = q_unit * k_unit, dp_unit = g_unit.x * v_unit.x * f, dot_unit = dot * f;
+      const float f = power_of_two(e), s_unit = q_unit * k_unit, dp_unit = g_unit.x * f * v_unit.x, dot_unit = dot * f;
       if (!mbar_wait(&bar->s_full[b], j >> 1 & 1, p.status, 0x312)) { ok = false; break; }
       tc_fence_after();
       const uint32_t at = mine + Shape::S_AT + b * 64 + half * 32, dp_at = mine + Shape::DP_AT + b * 64 + half * 32;
@@ -969,9 +971,9 @@ __device__ __forceinline__ void grad_of_states(const Problem& p, const int block
       if (!mbar_wait(&bar->full[qs], 2 * j / SLOTS & 1, p.status, 0x321)) { ok = false; break; }
       const float *const lse = rows + qs * 64, *const dots = rows + gs * 64;
       const uint32_t largest = max(__float_as_uint(fabsf(dots[lane])), __float_as_uint(fabsf(dots[lane + 32])));
-      const int e = exponent_of_ds(g_unit.y, v_unit.y, __uint_as_float(__reduce_max_sync(ALL, largest)));
+      const int e = exponent_of_ds(g_unit.y, v_unit.y, __uint_as_float(__reduce_max_sync(ALL, largest)), q_unit);
       // p = 2^14 P, then dS = p (dP - dot) 2^(e - 14)
-      const float s_unit = q_unit * k_unit, f = power_of_two(max(e - TOP - 1, -126)), dp_unit = g_unit.x * v_unit.x * f;
+      const float s_unit = q_unit * k_unit, f = power_of_two(max(e - TOP - 1, -126)), dp_unit = g_unit.x * f * v_unit.x;
       if (!mbar_wait(&bar->s_full[b], j >> 1 & 1, p.status, 0x321)) { ok = false; break; }
       tc_fence_after();
       const uint32_t at = mine + Shape::S_AT + b * 64 + half * 32, dp_at = mine + Shape::DP_AT + b % Shape::DP_BUFFERS * 64 + half * 32;
