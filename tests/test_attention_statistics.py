@@ -204,3 +204,11 @@ def test_what_a_forward_pass_takes_outside_of_the_step(n, tq, tk, h, s, d):
     ex.run(f)
     rows = sum(a.nbytes for a in y.state.values() if isinstance(a, ndarray.NDArray))
     assert rows + held() - before == y.op.workspace_bytes(y, [f[i].shape for i in y.inputs], f[v["q"]].shape)
+
+
+def test_single_tokens_are_the_same_to_the_plan_and_to_the_kernels():
+    import os
+    import re
+    source = open(os.path.join(os.path.dirname(A.__file__), "..", "csrc", "kernels", "cross_attention.cu")).read()
+    assert int(re.search(r"\bFEW_ROWS = (\d+)", source).group(1)) == A.FEW_ROWS
+    assert [A.keeps_operands((1, t, 4, 8), (1, 9, 2, 2, 8)) for t in (3, 4, 5)] == [False, False, True]

@@ -21,7 +21,6 @@
 
 #define TSB_OK 0
 #define TSB_ERR_ARG 1
-#define TSB_ERR_UNSUPPORTED 2
 #define TSB_ERR_LAUNCH 3
 #define TSB_ERR_OOM 5
 

@@ -660,8 +660,8 @@ int tsb_token_score(const float* x, const float* ids, float* out, long long rows
   // a cluster of blocks for a row while the rows leave SMs idle and a block keeps 2048 columns
   int split = 1;
   while (split < MAX_SPLIT && rows * split * 2 <= 148 && cols >= 4096ll * split) split *= 2;
-  // eight warps for few rows or long ones only: a row's end is latency, which more rows on an SM cover (8160 x 32000, 20
-  // alternatives: four warps 234 us, eight 256; 4096 x 128001: 395, 373)
+  // eight warps for few rows or long ones only: a row's end is latency, which more rows on an SM cover (4096 rows, 20 alternatives,
+  // four warps and eight: 33000 columns 135 and 141 us, 48000 175 and 177, 64000 220 and 219, 96000 315 and 319, 128001 418 and 402)
   const int warps = cols / split >= 65536 || rows * split <= 4 * 148 ? MAX_WARPS : MAX_WARPS / 2;
   const dim3 grid((unsigned)(rows * split)), block(warps * 32);
   const unsigned cluster = split > 1 ? split : 0;

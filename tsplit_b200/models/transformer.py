@@ -27,7 +27,7 @@ class TransformerConfig(object):
         #: lookup and scale of the tokens in one operator whose gradient is summed in one fixed order, padding (token 0)
         #: without any (``ad.scaled_embedding_op``)
         self.scaled_embedding = bool(scaled_embedding)
-        #: the decoder's attention over the encoder's states as one operator that keeps no scores and fp32 accuracy; keys and
+        #: the decoder's attention over the encoder's states as one operator that keeps no scores; keys and
         #: values come from one projection ``<name>_kv`` (``ad.cross_attention_op``, which has no dropout of the probabilities)
         self.cross_attention = bool(cross_attention)
         if self.cross_attention and dropout_rate:

@@ -2,7 +2,13 @@
 
 The reference's example builds it from batched products, a scale, a padding mask and a soft-max
 (``examples/transformer.py:117-171``) and keeps the scores; here they never leave the chip
-(``csrc/kernels/cross_attention.cu``), forward or backward, and the products keep the accuracy of fp32.
+(``csrc/kernels/cross_attention.cu``), forward or backward.
+
+On the GPU a number takes part in the products to 2^-22 of itself or 2^-38 of the largest number in its tile, 128 rows of a head of
+the queries, keys, values or gradients, whichever is more, and a probability to 2^-39; sums are fp32.  So results have the accuracy of
+fp32 where the rows of a tile are within 2^16 of one another, and a row that is smaller loses some of its own (its gradient is off by
+1e-5 of itself where another row's is 2^20 times as large, by 1 % at 2^30).  The forward pass of up to eight rows of queries to a head
+of the states is plain fp32.
 """
 from __future__ import annotations
 
@@ -245,9 +251,14 @@ class CrossAttentionGradStatesOp(_CrossAttentionGradient):
         return 8.0 * np.prod(s[2]) * s[3][1]
 
 
+#: rows of queries to a head of the states up to which the forward pass takes the path for single tokens (the kernels' constant of
+#: that name; where they keep operands for such rows, they refuse)
+FEW_ROWS = 8
+
+
 def keeps_operands(q, kv):
     """Whether the forward pass over these shapes splits its operands: all but single tokens do."""
-    return q[2] // kv[3] * q[1] > 8
+    return q[2] // kv[3] * q[1] > FEW_ROWS
 
 
 def both_gradients(nodes, iv, out, stream):

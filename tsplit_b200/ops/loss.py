@@ -283,7 +283,7 @@ class TokenLogProbOp(Op):
 
 class TokenLogProbGradientOp(Op):
     """``sum_i w_i (1[c = id_i] - p_c) + w_lse p_c - w_H p_c (log p_c + H)``: w is the gradient ``g`` of a
-    :class:`TokenLogProbOp`'s result ``out``, i its given token and the likeliest ones."""
+    :class:`TokenLogProbOp`'s result ``out`` for these logits and ids, i its given token and the likeliest ones."""
     name = "TokenLogProbGradient"
 
     def __call__(self, logits, ids, out, g):
