@@ -48,3 +48,17 @@ def test_gradients_of_next_to_nothing(size, tq, d):
     for got, w in ((dq, want[1]), (dkv[:, :, 0], want[2][:, :, 0]), (dkv[:, :, 1], want[2][:, :, 1])):
         # (what is below 2^-126, of g or of a result, counts as 0 in every kernel)
         assert np.abs(got - w).max() <= 1e-4 * np.abs(w).max() + 4 * 2.0 ** -126
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tq,d", [(1, 64), (40, 64), (140, 128)])
+@pytest.mark.parametrize("size", [1e33, 1e36])
+def test_values_near_the_largest_number(tq, d, size):
+    """A result is a mean of values, so it is a number where they are; so are the gradients of small enough ones."""
+    f = case(2, tq, 150, 2, 1, d, "holes", seed=4)
+    f["kv"][:, :, 1] *= np.float32(size) / np.abs(f["kv"][:, :, 1]).max()
+    f["g"] = f["g"] * np.float32(1e-37)
+    got = evaluate(graph(True, None), f, ndarray.gpu(0))
+    g = np.where(np.abs(f["g"]) < 2.0 ** -126, 0, f["g"])             # (which count as 0 in every kernel)
+    for a, b, t in zip(got, *definition(f["q"], f["kv"], f["key"], d ** -0.5, g)):
+        assert np.isfinite(a).all() and np.all(np.abs(a - b) <= t + 4 * 2.0 ** -126)

@@ -74,7 +74,7 @@ __device__ __forceinline__ int exponent_to(uint32_t bits_of_abs, int top, int mo
 }
 constexpr int TOP = 13;                      // of a tile's largest number
 constexpr int LEAST = 112;                   // a tile's unit is 2^-LEAST at the least, and normal when P's scale divides it
-constexpr float LARGEST = 16384.f;           // and what that is below, 2^(TOP+1); P is scaled by it too
+constexpr float LARGEST = 16384.f;           // and what that is below, 2^(TOP+1); P is scaled by it too (sums of P v are not)
 
 // A tile of ROWS x D numbers in shared memory: the plane of the hi pieces, then that of the lo pieces; a plane is D / 64
 // chunks of [ROWS][64] halves whose rows of 128 bytes are swizzled (16-byte unit u of row r lies at u ^ (r & 7)).
@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(BLOCK, 1) attend(const Problem p) {
       l = l * factor + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
       m = top;
       before = factor;
-      v_unit = next_unit;
+      v_unit = next_unit * (1.f / LARGEST);
     }
     if (ok && tiles > 0) ok = add_tile(tiles - 1);
     // the halves' sums
@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(BLOCK, 1) attend(const Problem p) {
       l += shared_max[tiles & 1][half ^ 1][row];
       const int t = q0 + row;
       if (t < p.tq)
-        store_row(p.y + ((long long)n * p.tq + t) * q_row + (long long)h * p.d + half * OWN, acc, l != 0.f ? 1.f / l : 0.f, p.d - half * OWN,
+        store_row(p.y + ((long long)n * p.tq + t) * q_row + (long long)h * p.d + half * OWN, acc, l != 0.f ? LARGEST / l : 0.f, p.d - half * OWN,
                   p.vec);
       // (a row without keys, or behind the last one: exp2(S - inf) = 0 in the backward pass; l may be NaN)
       if (half == 0) p.lse[q_at * 128 + row] = l != 0.f && t < p.tq ? m - (TOP + 1) + log2f(l) : -NEG_INF;
