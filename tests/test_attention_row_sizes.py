@@ -36,6 +36,18 @@ def test_gradients_of_queries_beside_one_far_larger(power, most, tk, d):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e-9, 1e-14, 1e-16, 3e-18])
+def test_small_gradients_beside_one_far_larger(size):
+    """The same where all of them are small: 2^-22 of the neighbours is left by the pieces, and their dS is bounded by themselves."""
+    f = case(1, 100, 1500, 1, 1, 64, None, seed=1)
+    f["g"] *= np.float32(size)
+    f["g"][0, 7] *= np.float32(2.0) ** 16
+    _, dq, _ = evaluate(graph(False, None), f, ndarray.gpu(0))
+    want = definition(f["q"], f["kv"], None, 0.125, f["g"])[0][1]
+    assert (np.abs(dq - want).max(3) / np.abs(want).max(3)).max() <= 1e-5
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("size", [1e-28, 1e-32, 1e-35])
 @pytest.mark.parametrize("tq,d", [(100, 64), (100, 128), (1, 64)])
 def test_gradients_of_next_to_nothing(size, tq, d):

@@ -760,7 +760,8 @@ __device__ __forceinline__ void grad_of_queries(const Problem& p, const int bloc
     const float lse = load(p.lse + q_at * 128 + row), dot = load(p.dot + q_at * 128 + row);
     const float q_unit = load(p.qp.units + q_at).x;
     const float2 g_unit = load(p.gp.units + q_at);
-    const float own = load(p.lengths + q_at * 128 + row), length = own < 1e15f && own > 1e-15f ? own : g_unit.y;
+    // (a length whose squares are below 2^-126 is 0, from 1e-18 on it is too short by a factor of 1.6 at the most, and 2^15 has 2 to go)
+    const float own = load(p.lengths + q_at * 128 + row), length = own < 1e15f && own > 1e-18f ? own : g_unit.y;
     bool ok = true;
     auto add_tile = [&](int j) {
       if (!mbar_wait(&bar->dq_full, j & 1, p.status, 0x311)) return false;
