@@ -10,13 +10,13 @@
 // Products run on tcgen05 with the accuracy of fp32, of numbers that are not too far apart: an operand tile of 128 rows is scaled by
 // a power of two that brings its largest number to [2^13, 2^14) and split into two fp16 numbers, x = hi + lo, |x - hi - lo| <= 2^-22
 // |x|, or 2^-38 of the tile's largest, where fp16 ends (so a row down to 2^-16 of its tile keeps what fp32 keeps, one at 2^-20 7e-6 of
-// itself, at 2^-30 0.9 %); P ends at 2^-39, dS at 2^-39 of its bound.  A product is three: hi hi + hi lo + lo hi.  That takes 1.5 times the tensor time of one TF32
-// product, which keeps 2^-11, and the room of fp32, and 16-bit tiles can be read in both directions (K-major and MN-major)
-// from one copy in shared memory.  (Two bf16 numbers need no scale but keep 2^-17, three need six products.)  A kernel
-// before splits every operand once, in tiles of 128 rows that lie in memory as they will in shared memory, so the kernels
-// that multiply load them by bulk copies.  P and dS are split by the threads that compute them and go to tensor memory, from
-// where they are the A operand of the next product: P is at most 2^14, dS is scaled by a bound of its own.  What a tile adds
-// to y, dq, dk or dv is read from tensor memory and added in registers with the tile's scale.
+// itself, at 2^-30 0.9 %); P ends at 2^-39, dS at 2^-39 of its bound.  A product is three: hi hi + hi lo + lo hi.  That takes 1.5
+// times the tensor time of one TF32 product, which keeps 2^-11, and the room of fp32, and 16-bit tiles can be read in both directions
+// (K-major and MN-major) from one copy in shared memory.  (Two bf16 numbers need no scale but keep 2^-17, three need six products.)
+// A kernel before splits every operand once, in tiles of 128 rows that lie in memory as they will in shared memory, so the kernels
+// that multiply load them by bulk copies.  P and dS are split by the threads that compute them and go to tensor memory, from where
+// they are the A operand of the next product: P is at most 2^14, dS is scaled by a bound of its own.  What a tile adds to y, dq, dk
+// or dv is read from tensor memory and added in registers with the tile's scale.
 //
 // Scores are kept in units of log 2 (q is scaled by scale * log2(e) as it is loaded), so that an exponential is one ex2.
 #include <cuda_runtime.h>
